@@ -65,6 +65,13 @@ SIGNATURES = {
     "hydra_linear_fwd": [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I, _I, _P],
     "hydra_ce_rows": [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I, _P],
     "hydra_ce_grad_planes": [_P, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P],
+    "hydra_page_plan": [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P],
+    "hydra_page_plan_in_place": [_I64, _I64],
+    "hydra_page_release": [_P, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
+    "hydra_page_store": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I, _P],
+    "hydra_paged_attn": [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                         _I64P, _I64P, _I64P, _I64P, _F, _I, _P, _I64, _P],
+    "hydra_paged_attn_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I, _I64P],
     "hydra_ccgqa_prep_tiled_ok": [_I64, _I64, _I64, _I],
     "hydra_ccgqa_prep_faults": [_P],
     "hydra_ccgqa_prep_bwd": [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _P,

@@ -8,6 +8,7 @@ from .registry import (
 )
 from .backends.ccgqa.attention import CCGQAAttention
 from .factory import build_hybrid_attention_module
+from .paged import PagePlan, PagePool, paged_attention, plan_pages, release_pages, store_pages
 
 __all__ = [
     "HybridAttentionBackend",
@@ -16,4 +17,10 @@ __all__ = [
     "resolve_hybrid_attention_backend",
     "CCGQAAttention",
     "build_hybrid_attention_module",
+    "PagePlan",
+    "PagePool",
+    "paged_attention",
+    "plan_pages",
+    "release_pages",
+    "store_pages",
 ]

@@ -1,0 +1,336 @@
+// Pages of a key-value cache on gfx950: the page tables and slot maps of a
+// step from the lengths of its requests, the return of finished requests'
+// pages, and the store of key and value rows into their pages.
+//
+// A cache is a pool of pages, [pages, Hkv, page_size, hd] for keys and for
+// values; position t of request i lies in page table[i, t / page_size] at row
+// t % page_size, its slot is page * page_size + row.  Pages that nobody holds
+// lie on a stack (free_pages[0 .. free_count)).  Nothing here is read by the
+// host: a request that cannot get its pages is refused on the device.
+#include "common.h"
+#include "mod_keys.h"
+
+namespace hydra {
+namespace {
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanTokens = 4096;  // tokens of a request that one workgroup writes
+
+struct PlanArgs {
+  const int* lengths;  // may be lengths_out (see hydra_page_plan_in_place)
+  const int* fresh;  // tokens to add
+  int* table;
+  int64_t table_rs;
+  const int* free_pages;
+  const int* free_count;
+  int64_t* slots;
+  int* lengths_out;
+  int* seen;
+  uint8_t* granted;
+  int *positions, *free_out;
+  int N, P, F, width, shift, slice, from_empty;
+};
+
+struct Need {
+  int64_t len, add;
+  int have, need;
+  bool fits;
+};
+
+// What request i asks for: pages held, pages more, and whether its own table
+// row and the step's width hold it.
+__device__ __forceinline__ Need need_of(const PlanArgs& a, int i) {
+  Need r{0, 0, 0, 0, false};
+  if (i >= a.N) return r;
+  r.len = a.lengths[i];
+  r.add = a.fresh[i];
+  const int64_t page = int64_t(1) << a.shift;
+  r.fits = r.len >= 0 && r.add >= 0 && r.add <= a.width && r.len + r.add <= (static_cast<int64_t>(a.P) << a.shift) &&
+           (!a.from_empty || r.len == 0 || r.add == 0);
+  if (r.fits) {
+    r.have = static_cast<int>((r.len + page - 1) >> a.shift);
+    r.need = static_cast<int>((r.len + r.add + page - 1) >> a.shift) - r.have;
+  }
+  return r;
+}
+
+// Inclusive sum over the workgroup's 256 threads; `total` gets the whole sum.
+__device__ __forceinline__ int block_incl_sum(int x, int* part, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = wave_incl_sum(x);
+  __syncthreads();  // the last use of `part` is over
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) s += part[w];
+    all += part[w];
+  }
+  total = all;
+  return s;
+}
+
+// Workgroup (x, y) writes the results of the requests [x slice, (x+1) slice)
+// and, of each, the slots of the tokens [y kPlanTokens, ...).  Every workgroup
+// sums the needs of all requests before its own again (256 a step, 8 bytes
+// each, from L2): one launch, no exchange between workgroups.  New pages are
+// taken from the stack by index, so the table's new entries are written by one
+// workgroup and read by none.
+//
+// Bound by its launch and the chain of the sums at a decoding step, by the
+// slots' writes for prompts.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
+  __shared__ int part[kPlanThreads / 64];
+  __shared__ int s_first[kPlanThreads], s_have[kPlanThreads], s_need[kPlanThreads];
+  __shared__ int64_t s_len[kPlanThreads], s_add[kPlanThreads];  // add: -1 when refused
+  const int tid = threadIdx.x;
+  const int begin = blockIdx.x * a.slice, end = min(a.N, begin + a.slice);
+  int free = *a.free_count;
+  free = free < 0 ? 0 : (free > a.F ? a.F : free);
+  int before = 0;  // pages asked for by the requests before this step's 256
+  int taken = 0;   // pages granted in all (the last workgroup's alone is whole)
+  for (int i0 = 0; i0 < end; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    const Need r = need_of(a, i);
+    int step;
+    const int upto = before + block_incl_sum(r.need, part, step);
+    const bool granted = r.fits && (r.need == 0 || upto <= free);
+    // granted requests that need pages come first, so the last of them
+    // has the sum of all
+    taken = (granted && r.need > 0) ? upto : taken;
+    if (i >= begin && i < end) {
+      const int at = i - begin;
+      s_first[at] = free - 1 - (upto - r.need);
+      s_have[at] = r.have;
+      s_need[at] = r.need;
+      s_len[at] = r.len;
+      s_add[at] = granted ? r.add : -1;
+    }
+    before += step;
+  }
+  __syncthreads();
+  if (blockIdx.y == 0) {
+    for (int at = tid; at < end - begin; at += kPlanThreads) {
+      const int i = begin + at;
+      const bool granted = s_add[at] >= 0;
+      const int after = static_cast<int>(granted ? s_len[at] + s_add[at] : s_len[at]);
+      a.lengths_out[i] = after;
+      a.seen[i] = granted && s_add[at] > 0 ? after : 0;
+      a.granted[i] = granted;
+      a.positions[i] = static_cast<int>(s_len[at]);
+    }
+    for (int at = 0; at < end - begin; ++at) {
+      if (s_add[at] < 0) continue;
+      int* row = a.table + (begin + at) * a.table_rs;
+      for (int j = tid; j < s_need[at]; j += kPlanThreads) row[s_have[at] + j] = a.free_pages[s_first[at] - j];
+    }
+    if (blockIdx.x == gridDim.x - 1) {  // it went over every request
+      int most = taken;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+      if ((tid & 63) == 0) part[tid >> 6] = most;
+      __syncthreads();
+      if (tid == 0) {
+        for (int w = 1; w < kPlanThreads / 64; ++w) most = max(most, part[w]);
+        *a.free_out = free - most;
+      }
+    }
+  }
+  const int j0 = blockIdx.y * kPlanTokens, j1 = min(a.width, j0 + kPlanTokens);
+  const int64_t count = static_cast<int64_t>(end - begin) * (j1 - j0);
+  const int64_t low = (int64_t(1) << a.shift) - 1;
+  for (int64_t e = tid; e < count; e += kPlanThreads) {
+    const int at = static_cast<int>(e / (j1 - j0)), j = j0 + static_cast<int>(e - static_cast<int64_t>(at) * (j1 - j0));
+    int64_t slot = -1;
+    if (j < s_add[at]) {
+      const int64_t t = s_len[at] + j;
+      const int col = static_cast<int>(t >> a.shift);
+      const int page = col >= s_have[at] ? a.free_pages[s_first[at] - (col - s_have[at])]
+                                         : a.table[(begin + at) * a.table_rs + col];
+      if (page >= 0) slot = (static_cast<int64_t>(page) << a.shift) | (t & low);
+    }
+    a.slots[static_cast<int64_t>(begin + at) * a.width + j] = slot;
+  }
+}
+
+// The pages of the requests that are done go back on the stack, in the order
+// of the requests; their lengths become 0 and their table entries -1.  One
+// workgroup: the stack has one top.
+__global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* done, int* lengths, int* table,
+                                                               int64_t table_rs, int* free_pages, int* free_count,
+                                                               int N, int P, int F, int shift) {
+  __shared__ int part[kPlanThreads / 64];
+  __shared__ int s_first[kPlanThreads], s_count[kPlanThreads];
+  const int tid = threadIdx.x;
+  int free = *free_count;
+  free = free < 0 ? 0 : (free > F ? F : free);
+  for (int i0 = 0; i0 < N; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int count = 0;
+    if (i < N && done[i]) {
+      const int64_t len = lengths[i];
+      const int64_t pages = len <= 0 ? 0 : (len + (int64_t(1) << shift) - 1) >> shift;
+      count = static_cast<int>(pages < P ? pages : P);
+      lengths[i] = 0;
+    }
+    int step;
+    const int upto = block_incl_sum(count, part, step);
+    s_first[tid] = free + upto - count;
+    s_count[tid] = count;
+    __syncthreads();
+    for (int at = tid >> 6; at < kPlanThreads; at += kPlanThreads / 64) {
+      int* row = table + static_cast<int64_t>(i0 + at) * table_rs;
+      for (int j = tid & 63; j < s_count[at]; j += 64) {
+        const int to = s_first[at] + j;
+        if (to < F) free_pages[to] = row[j];
+        row[j] = -1;
+      }
+    }
+    free = min(F, free + step);
+    __syncthreads();
+  }
+  if (tid == 0) *free_count = free;
+}
+
+// Rows k, v [N, Hkv, S, hd] into their pages.  A thread moves one 16-byte
+// piece (VEC; one element else) of a key row and of the value row beside it;
+// neighbouring threads take a row's pieces, then the next position's, which
+// lie one after the other in the source and in the page.  Bound by HBM: each
+// row is read and written once.
+struct StoreArgs {
+  const char *k, *v;
+  char *kp, *vp;
+  const int64_t* slots;
+  int64_t ks[3], vs[3], kps[3], vps[3];  // strides in bytes: n/h/s, page/h/row
+  int64_t limit;                         // slots of the pool
+  int N, H, S, pieces, shift;
+};
+
+template <typename V>
+__global__ __launch_bounds__(256) void store_kernel(StoreArgs a) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t s = e / a.pieces;
+  if (s >= a.S) return;
+  const int64_t piece = (e - s * a.pieces) * static_cast<int64_t>(sizeof(V));
+  const int h = blockIdx.y;
+  for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
+    const int64_t slot = a.slots[static_cast<int64_t>(n) * a.S + s];
+    if (slot < 0 || slot >= a.limit) continue;
+    const int64_t page = slot >> a.shift, row = slot & ((int64_t(1) << a.shift) - 1);
+    const V k = *reinterpret_cast<const V*>(a.k + n * a.ks[0] + h * a.ks[1] + s * a.ks[2] + piece);
+    const V v = *reinterpret_cast<const V*>(a.v + n * a.vs[0] + h * a.vs[1] + s * a.vs[2] + piece);
+    *reinterpret_cast<V*>(a.kp + page * a.kps[0] + h * a.kps[1] + row * a.kps[2] + piece) = k;
+    *reinterpret_cast<V*>(a.vp + page * a.vps[0] + h * a.vps[1] + row * a.vps[2] + piece) = v;
+  }
+}
+
+// Requests of a workgroup: up to 256, fewer where their slots are many.
+int plan_slice(int64_t width) {
+  const int64_t slice = kPlanTokens / width;
+  return static_cast<int>(slice < 1 ? 1 : (slice > kPlanThreads ? kPlanThreads : slice));
+}
+
+int page_shift(int64_t page_size) {
+  for (int s = 4; s <= 12; ++s)
+    if (page_size == (int64_t(1) << s)) return s;
+  return -1;
+}
+
+}  // namespace
+}  // namespace hydra
+
+using namespace hydra;
+
+extern "C" int hydra_page_plan(const int* lengths, const int* new_tokens, int* table, int64_t table_rs,
+                               const int* free_pages, int64_t free_capacity, const int* free_count, int64_t* slots,
+                               int* lengths_out, int* seen, void* granted, int* positions, int* free_out,
+                               int64_t N, int64_t P, int64_t width, int64_t page_size, int from_empty, void* stream) {
+  HYDRA_REQUIRE(N >= 1 && P >= 1 && width >= 1 && free_capacity >= 0, "page_plan: bad size");
+  const int shift = page_shift(page_size);
+  HYDRA_REQUIRE(shift >= 0, "page_plan: page_size must be a power of two in [16, 4096]");
+  HYDRA_REQUIRE(table_rs >= P, "page_plan: table row stride < columns");
+  HYDRA_REQUIRE(N * P < (int64_t(1) << 31) && P * page_size < (int64_t(1) << 31) &&
+                    N * width < (int64_t(1) << 40) && N < (int64_t(1) << 31) && width < (int64_t(1) << 28) &&
+                    free_capacity < (int64_t(1) << 31),
+                "page_plan: too large");
+  HYDRA_REQUIRE(lengths && new_tokens && table && free_count && slots && lengths_out && seen && granted && positions &&
+                    free_out &&
+                    (free_pages || free_capacity == 0),
+                "page_plan: null pointer");
+  HYDRA_REQUIRE((lengths_out != lengths && free_out != free_count) || hydra_page_plan_in_place(N, width) == 1,
+                "page_plan: in place takes a step that one workgroup plans");
+  PlanArgs a{lengths, new_tokens, table, table_rs, free_pages, free_count, slots, lengths_out, seen,
+             static_cast<uint8_t*>(granted), positions, free_out, static_cast<int>(N), static_cast<int>(P),
+             static_cast<int>(free_capacity), static_cast<int>(width), shift, 0, from_empty ? 1 : 0};
+  a.slice = plan_slice(width);
+  const int64_t gx = (N + a.slice - 1) / a.slice, gy = (width + kPlanTokens - 1) / kPlanTokens;
+  HYDRA_REQUIRE(gx < (int64_t(1) << 31) && gy <= 65535, "page_plan: too large");
+  plan_kernel<<<dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), kPlanThreads, 0,
+                static_cast<hipStream_t>(stream)>>>(a);
+  return check_launch("page_plan");
+}
+
+// A lone workgroup has read every length, and the stack's height, before it
+// writes its first result.
+extern "C" int hydra_page_plan_in_place(int64_t N, int64_t width) {
+  return N >= 1 && width >= 1 && width <= kPlanTokens && N <= plan_slice(width) ? 1 : 0;
+}
+
+extern "C" int hydra_page_release(const void* done, int* lengths, int* table, int64_t table_rs, int* free_pages,
+                                  int64_t free_capacity, int* free_count, int64_t N, int64_t P, int64_t page_size,
+                                  void* stream) {
+  HYDRA_REQUIRE(N >= 1 && P >= 1 && free_capacity >= 1, "page_release: bad size");
+  const int shift = page_shift(page_size);
+  HYDRA_REQUIRE(shift >= 0, "page_release: page_size must be a power of two in [16, 4096]");
+  HYDRA_REQUIRE(table_rs >= P, "page_release: table row stride < columns");
+  HYDRA_REQUIRE(N * P < (int64_t(1) << 31) && free_capacity < (int64_t(1) << 31), "page_release: too large");
+  HYDRA_REQUIRE(done && lengths && table && free_pages && free_count, "page_release: null pointer");
+  release_kernel<<<1, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(done), lengths, table, table_rs, free_pages, free_count, static_cast<int>(N),
+      static_cast<int>(P), static_cast<int>(free_capacity), shift);
+  return check_launch("page_release");
+}
+
+extern "C" int hydra_page_store(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots,
+                                int64_t N, int64_t Hkv, int64_t S, int64_t hd, int64_t pages, int64_t page_size,
+                                const int64_t* k_st, const int64_t* v_st, const int64_t* kp_st, const int64_t* vp_st,
+                                int dtype, void* stream) {
+  HYDRA_REQUIRE(N >= 0 && S >= 0 && Hkv >= 1 && hd >= 1 && pages >= 1, "page_store: bad size");
+  const int shift = page_shift(page_size);
+  HYDRA_REQUIRE(shift >= 0, "page_store: page_size must be a power of two in [16, 4096]");
+  const int e = dtype_size(dtype);
+  HYDRA_REQUIRE(e > 0, "page_store: unknown dtype");
+  HYDRA_REQUIRE(N < (int64_t(1) << 31) && S < (int64_t(1) << 31) && Hkv <= 65535 && hd <= 65536, "page_store: too large");
+  if (N == 0 || S == 0) return HYDRA_OK;
+  HYDRA_REQUIRE(k && v && k_pages && v_pages && slots && k_st && v_st && kp_st && vp_st, "page_store: null pointer");
+  HYDRA_REQUIRE(k_st[3] == 1 && v_st[3] == 1 && kp_st[3] == 1 && vp_st[3] == 1, "page_store: rows need unit stride");
+  StoreArgs a{};
+  a.k = static_cast<const char*>(k);
+  a.v = static_cast<const char*>(v);
+  a.kp = static_cast<char*>(k_pages);
+  a.vp = static_cast<char*>(v_pages);
+  a.slots = slots;
+  a.limit = pages * page_size;
+  a.N = static_cast<int>(N);
+  a.H = static_cast<int>(Hkv);
+  a.S = static_cast<int>(S);
+  a.shift = shift;
+  bool vec = hd * e % 16 == 0 && aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages);
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = k_st[i] * e;
+    a.vs[i] = v_st[i] * e;
+    a.kps[i] = kp_st[i] * e;
+    a.vps[i] = vp_st[i] * e;
+    vec = vec && (a.ks[i] | a.vs[i] | a.kps[i] | a.vps[i]) % 16 == 0;
+  }
+  a.pieces = static_cast<int>(vec ? hd * e / 16 : hd);
+  const int64_t gx = (S * a.pieces + 255) / 256;
+  HYDRA_REQUIRE(gx < (int64_t(1) << 31), "page_store: too large");
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(Hkv), static_cast<unsigned>(N < 65535 ? N : 65535));
+  auto st = static_cast<hipStream_t>(stream);
+  if (vec) store_kernel<uint4><<<grid, 256, 0, st>>>(a);
+  else if (e == 4) store_kernel<uint32_t><<<grid, 256, 0, st>>>(a);
+  else store_kernel<uint16_t><<<grid, 256, 0, st>>>(a);
+  return check_launch("page_store");
+}

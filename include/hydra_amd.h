@@ -445,6 +445,69 @@ int hydra_ce_grad_planes(const float* logits, int64_t rows, int64_t vocab, int64
                          int64_t planes_rs, int64_t plane_stride, const float* grad_scale,
                          void* stream);
 
+/* ---- pages of a key-value cache (no counterpart in the reference, which
+ *      recomputes the whole sequence for every token) ---------------------- */
+
+/* A cache is a pool of pages, k and v [pages, Hkv, page_size, hd]; position t
+ * of request i lies in page table[i, t / page_size], row t % page_size; its
+ * slot is page * page_size + row.  page_size: a power of two in [16, 4096].
+ * Tables, lengths and counts are int32, slots int64.  What the device finds
+ * wrong (a request without room, an entry outside the pool) costs only the
+ * request it belongs to: no host synchronisation, no access out of bounds. */
+
+/* Plans a step that adds new_tokens[i] tokens to request i, which holds
+ * lengths[i].  Request i fits if 0 <= lengths[i], 0 <= new_tokens[i] <= width
+ * and their sum is at most P * page_size (with from_empty: and it holds none,
+ * or adds none).  Requests that fit take the pages they lack from the top of
+ * the stack free_pages[0 .. free_count[0]) in order; a request is granted if
+ * it fits and needs no page, or the stack holds what it and all fitting ones
+ * before it need.  Writes the new entries of table [N, P] (row stride
+ * table_rs), slots [N, width] (-1 where there is no token), lengths_out [N],
+ * seen [N] (the new length of a request that got tokens, else 0), granted [N]
+ * (bytes 0/1), positions [N] (the lengths as they were) and free_out [1].  The
+ * inputs stay as they are, so the call can be repeated; a step that one
+ * workgroup plans (hydra_page_plan_in_place) may take lengths_out = lengths and
+ * free_out = free_count and so commit itself. */
+int hydra_page_plan(const int* lengths, const int* new_tokens, int* table, int64_t table_rs,
+                    const int* free_pages, int64_t free_capacity, const int* free_count,
+                    int64_t* slots, int* lengths_out, int* seen, void* granted, int* positions,
+                    int* free_out, int64_t N, int64_t P, int64_t width, int64_t page_size,
+                    int from_empty, void* stream);
+/* 1 if a plan of N requests of up to width tokens may be made in place.  Host-only. */
+int hydra_page_plan_in_place(int64_t N, int64_t width);
+
+/* Puts the pages of the requests with done[i] != 0 (bytes) back on the stack,
+ * in order, in place: their lengths become 0, their table entries -1. */
+int hydra_page_release(const void* done, int* lengths, int* table, int64_t table_rs,
+                       int* free_pages, int64_t free_capacity, int* free_count, int64_t N,
+                       int64_t P, int64_t page_size, void* stream);
+
+/* Rows k, v [N, Hkv, S, hd] (element strides k_st[4], v_st[4]; unit last) to
+ * the slots [N, S] of k_pages, v_pages [pages, Hkv, page_size, hd] (strides
+ * kp_st[4], vp_st[4]; unit last).  A slot outside the pool takes nothing;
+ * slots must be distinct. */
+int hydra_page_store(const void* k, const void* v, void* k_pages, void* v_pages,
+                     const int64_t* slots, int64_t N, int64_t Hkv, int64_t S, int64_t hd,
+                     int64_t pages, int64_t page_size, const int64_t* k_st, const int64_t* v_st,
+                     const int64_t* kp_st, const int64_t* vp_st, int dtype, void* stream);
+
+/* Attention of one token per request over its pages:
+ *   out[n,h] = softmax_t(scale * q[n,h] . k[t]) v[t], t < lengths[n],
+ * key head h / (Hq / Hkv).  q, out: [N, Hq, hd] with strides q_st[3],
+ * o_st[3]; pages as above; hd <= 256.  Lengths are taken within
+ * [0, P * page_size]; keys on a page outside the pool are not seen; a request
+ * that sees no key gets zeros.  Scores, softmax and the products with v are
+ * fp32, one rounding into `dtype`.  Needs hydra_paged_attn_workspace bytes of
+ * device scratch (16-byte aligned). */
+int hydra_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* out,
+                     const int* table, int64_t table_rs, const int* lengths, int64_t N, int64_t Hq,
+                     int64_t Hkv, int64_t hd, int64_t P, int64_t page_size, int64_t pages,
+                     const int64_t* q_st, const int64_t* kp_st, const int64_t* vp_st,
+                     const int64_t* o_st, float scale, int dtype, void* workspace,
+                     int64_t workspace_size, void* stream);
+int hydra_paged_attn_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t hd, int64_t P,
+                               int64_t page_size, int dtype, int64_t* bytes);
+
 /* ---- block compositions (hydra/model/framework, hydra/layers) --------- */
 
 /* Token embedding: out[r, :] = table[clamp(ids[r], 0, vocab-1), :] * scale,
