@@ -72,6 +72,9 @@ SIGNATURES = {
     "hydra_paged_attn": [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                          _I64P, _I64P, _I64P, _I64P, _F, _I, _P, _I64, _P],
     "hydra_paged_attn_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I, _I64P],
+    "hydra_ccgqa_decode_prep": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P,
+                                _I64P, _I64P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P],
+    "hydra_ccgqa_ring_fill": [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _P],
     "hydra_ccgqa_prep_tiled_ok": [_I64, _I64, _I64, _I],
     "hydra_ccgqa_prep_faults": [_P],
     "hydra_ccgqa_prep_bwd": [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _P,

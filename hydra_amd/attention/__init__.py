@@ -6,7 +6,7 @@ from .registry import (
     is_hybrid_attention_backend_available,
     resolve_hybrid_attention_backend,
 )
-from .backends.ccgqa.attention import CCGQAAttention
+from .backends.ccgqa.attention import CCGQAAttention, CCGQACache
 from .factory import build_hybrid_attention_module
 from .paged import PagePlan, PagePool, paged_attention, plan_pages, release_pages, store_pages
 
@@ -16,6 +16,7 @@ __all__ = [
     "is_hybrid_attention_backend_available",
     "resolve_hybrid_attention_backend",
     "CCGQAAttention",
+    "CCGQACache",
     "build_hybrid_attention_module",
     "PagePlan",
     "PagePool",

@@ -20,6 +20,9 @@ whose backwards are the HIP prep backward (plus the convs' GEMMs) and the
 HIP attention backward; in eval() mode with grad-enabled parameters the
 inference kernels run and a backward recomputes the training path.
 
+prefill() and decode() are the forward of requests that keep their keys and
+values in a paged cache (new_cache()), whole prompts and one token each.
+
 The reference's precomputed [max_seq_len, max_seq_len] causal mask buffer is
 not kept: the kernel derives causality from indices.
 """
@@ -36,8 +39,10 @@ from ...._lib import CCGQA_V_TRANSPOSED, CCGQA_W_TILED, MASK_KEY_PADDING, MASK_R
 from .autograd import ccgqa_prep_train
 from .kernels.fused_attention import CCGQAAttentionFused, MaskedAttentionFunction
 from .kernels.fused_conv import OptimizedConvSequence
-from .ops import (PackedWeights, attention_forward, ccgqa_prep, linear_weight_ok, output_projection, pack_conv_weight,
-                  pack_conv_weights_tiled, pack_linear_weight, prep_flags, tiled_weights_ok)
+from ...paged import PagePlan, PagePool, paged_attention, store_pages
+from .ops import (PackedWeights, attention_forward, ccgqa_decode_prep, ccgqa_prep, ccgqa_ring_fill, decode_reach,
+                  linear_weight_ok, output_projection, pack_conv_weight, pack_conv_weights_tiled, pack_linear_weight,
+                  prep_flags, tiled_weights_ok)
 
 # Kept for callers that probe these names (attention.py:13-28).
 FUSED_KERNELS_AVAILABLE = True
@@ -87,6 +92,24 @@ class _EvalRecompute(torch.autograd.Function):
         dx = grads.pop(0) if xr.requires_grad else None
         dparams = [grads.pop(0) if p.requires_grad else None for p in params]
         return (None, dx, None, *dparams)
+
+
+class CCGQACache:
+    """A layer's keys and values in pages ([pages, Hkv, page_size, head_dim])
+    and the projected rows of each request's last tokens, which its next token
+    needs (ccgqa_decode_prep's ring).  The pool's table says which pages are
+    whose."""
+
+    def __init__(self, layer: "CCGQAAttention", pool: PagePool, dtype: torch.dtype):
+        device = pool.table.device
+        shape = (pool.pages, layer.n_kv_heads, pool.page_size, layer.head_dim)
+        self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
+        self.v_pages = torch.zeros(shape, dtype=dtype, device=device)
+        reach = decode_reach(layer._prep_args()[0], layer.conv_kernel_size)
+        self.ring = torch.zeros((pool.requests, reach + 1, layer.latent_dim + 2 * layer.kv_dim), dtype=dtype,
+                                device=device)
+        self.table = pool.table
+        self.max_length = pool.max_length
 
 
 class CCGQAAttention(nn.Module):
@@ -172,15 +195,19 @@ class CCGQAAttention(nn.Module):
                  if self.use_convs else ())
         return flags, convw
 
-    def _forward_infer(self, x, qkv, flags, convw, mask):
+    def _tiled(self, dtype: torch.dtype) -> bool:
+        """Whether the conv weights are taken in MFMA-fragment order."""
+        return (self.use_convs and self.conv_kernel_size == 3 and
+                tiled_weights_ok(self.n_heads, self.n_kv_heads, self.head_dim, dtype))
+
+    def _forward_infer(self, x, qkv, flags, convw, mask, keep=None):
         """The inference kernels: prep with V^T rows and MFMA-tiled conv
         weights, the attention kernel writing [B, S, L], o_proj in
-        hydra_linear_fwd."""
+        hydra_linear_fwd.  keep(k, v) gets the keys and values (V in rows)."""
         B, S, _ = x.shape
-        if x.dtype == torch.bfloat16 and S % 8 == 0 and self.head_dim in (16, 32, 64, 128):
+        if x.dtype == torch.bfloat16 and S % 8 == 0 and self.head_dim in (16, 32, 64, 128) and keep is None:
             flags |= CCGQA_V_TRANSPOSED  # V^T feeds the MFMA attention without a transpose
-        tiled = (self.use_convs and self.conv_kernel_size == 3 and
-                 tiled_weights_ok(self.n_heads, self.n_kv_heads, self.head_dim, x.dtype))
+        tiled = self._tiled(x.dtype)
         if tiled:
             flags |= CCGQA_W_TILED  # conv weights in MFMA-fragment order
         with torch.no_grad():
@@ -192,6 +219,8 @@ class CCGQAAttention(nn.Module):
                 cos=self.cos_cached if self.use_rope else None,
                 sin=self.sin_cached if self.use_rope else None, packed=True,
                 conv_ks=self.conv_kernel_size)
+            if keep is not None:
+                keep(k, v)
             out = torch.empty((B, S, self.latent_dim), dtype=x.dtype, device=x.device)
             o_view = out.view(B, S, self.n_heads, self.head_dim).transpose(1, 2)
             attention_forward(q, k, v, causal=True, scale=self.scale,
@@ -199,6 +228,90 @@ class CCGQAAttention(nn.Module):
                               out=o_view,
                               bound_temperature=self.key_temperature if self.use_qk_norm else None)
         out = output_projection(out, w_o, packed_o)
+        if self.output_scale != 1.0:
+            out = out * self.output_scale
+        return out
+
+    # ------------------------------------------------------------- serving
+    def new_cache(self, pool: PagePool, dtype: Optional[torch.dtype] = None) -> "CCGQACache":
+        """This layer's part of a paged cache for the requests of `pool` (which
+        all layers share), in the weights' dtype by default."""
+        w = self.qkv_proj.weight
+        if self.use_rope and pool.max_length > self.cos_cached.shape[2]:
+            raise ValueError(f"CCGQAAttention: requests of up to {pool.max_length} tokens exceed the RoPE cache "
+                             f"({self.cos_cached.shape[2]})")
+        if pool.table.device != w.device:
+            raise RuntimeError(f"CCGQAAttention: the pool is on {pool.table.device}, the layer on {w.device}")
+        return CCGQACache(self, pool, dtype or w.dtype)
+
+    def _check_cache(self, name: str, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan) -> None:
+        if cache.k_pages.shape[1] != self.n_kv_heads or cache.k_pages.shape[3] != self.head_dim or \
+                cache.ring.shape[2] != self.latent_dim + 2 * self.kv_dim:
+            raise ValueError(f"{name}: the cache is another layer's")
+        if x.dtype != cache.k_pages.dtype:
+            raise ValueError(f"{name}: x is {x.dtype}, the cache {cache.k_pages.dtype}")
+        if plan.slots.shape[0] != cache.ring.shape[0]:
+            raise ValueError(f"{name}: a plan of {plan.slots.shape[0]} requests, a cache of {cache.ring.shape[0]}")
+        if self.use_rope and cache.max_length > self.cos_cached.shape[2]:
+            raise ValueError(f"{name}: requests of up to {cache.max_length} tokens exceed the RoPE cache "
+                             f"({self.cos_cached.shape[2]})")
+
+    @torch.no_grad()
+    def prefill(self, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan,
+                rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """forward() of whole prompts x [M, S, dim], padded on the right, whose
+        keys and values go into the cache.  `plan`: pool.plan(new_tokens,
+        width=S, from_empty=True); rows: int64 [M], the requests that the
+        prompts belong to (distinct; default: prompt m is request m).  Output
+        rows past a prompt's end hold no result; a refused request's prompt is
+        computed but not kept."""
+        name = "CCGQAAttention.prefill"
+        M, S, _ = x.shape
+        self._check_cache(name, x, cache, plan)
+        if not plan.from_empty or plan.slots.shape[1] != S:
+            raise ValueError(f"{name}: needs a plan with from_empty=True and width {S} (got width "
+                             f"{plan.slots.shape[1]})")
+        slots, seen = plan.slots, plan.seen
+        if rows is not None:
+            if rows.dtype != torch.int64 or rows.shape != (M,):
+                raise ValueError(f"{name}: rows must be int64 [{M}], got {rows.dtype} {tuple(rows.shape)}")
+            slots, seen = slots.index_select(0, rows), seen.index_select(0, rows)
+        elif M != slots.shape[0]:
+            raise ValueError(f"{name}: {M} prompts for {slots.shape[0]} requests: say which (rows)")
+        if self.use_rope and S > self.cos_cached.shape[2]:
+            raise ValueError(f"{name}: sequence length {S} exceeds the RoPE cache ({self.cos_cached.shape[2]})")
+        qkv = F.linear(x, self.qkv_proj.weight)
+        flags, convw = self._prep_args()
+        ccgqa_ring_fill(qkv, cache.ring, seen, decode_reach(flags, self.conv_kernel_size), rows)
+        return self._forward_infer(x, qkv, flags, convw, None,
+                                   keep=lambda k, v: store_pages(k, v, cache.k_pages, cache.v_pages, slots))
+
+    @torch.no_grad()
+    def decode(self, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan) -> torch.Tensor:
+        """forward() of each request's newest token, x [N, dim] or [N, 1, dim],
+        on what the cache holds of it.  `plan`: pool.plan(new_tokens) of width
+        1; a request without a token (0 new, or refused) gets zeros and its
+        cache stays."""
+        name = "CCGQAAttention.decode"
+        self._check_cache(name, x, cache, plan)
+        N = cache.ring.shape[0]
+        if plan.slots.shape[1] != 1:
+            raise ValueError(f"{name}: needs a plan of width 1 (got {plan.slots.shape[1]})")
+        if x.numel() != N * self.dim or x.shape[0] != N or x.dim() not in (2, 3):
+            raise ValueError(f"{name}: x must be [{N}, {self.dim}], got {tuple(x.shape)}")
+        flags, convw = self._prep_args()
+        tiled = self._tiled(x.dtype)
+        w_o = self.o_proj.weight
+        packed, packed_o = self._packed(convw, w_o, x.dtype, tiled)
+        q = ccgqa_decode_prep(
+            F.linear(x.reshape(N, self.dim), self.qkv_proj.weight), cache.ring, plan.positions, plan.slots,
+            cache.k_pages, cache.v_pages, self.n_heads, self.n_kv_heads, self.head_dim,
+            flags | (CCGQA_W_TILED if tiled else 0), *packed,
+            temperature=self.key_temperature if self.use_qk_norm else None,
+            cos=self.cos_cached if self.use_rope else None, sin=self.sin_cached if self.use_rope else None,
+            packed=True, conv_ks=self.conv_kernel_size)
+        o = paged_attention(q, cache.k_pages, cache.v_pages, cache.table, plan.seen, scale=self.scale)
+        out = output_projection(o.view(N, self.latent_dim), w_o, packed_o).view(x.shape)
         if self.output_scale != 1.0:
             out = out * self.output_scale
         return out

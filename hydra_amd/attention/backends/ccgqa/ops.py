@@ -16,6 +16,7 @@ from ...._lib import (CCGQA_CONVS, CCGQA_QK_MEAN, CCGQA_QK_NORM, CCGQA_ROPE, CCG
                       CCGQA_V_TRANSPOSED, CCGQA_VALUE_SHIFT, CCGQA_W_TILED, MASK_KEY_PADDING, MASK_NONE,
                       MASK_REFERENCE_SDPA)
 from .... import _lib
+from ...paged import check_pages
 
 
 def prep_flags(use_convs: bool, use_qk_mean: bool, use_value_shift: bool,
@@ -259,6 +260,120 @@ def ccgqa_prep(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, 
                   _lib.ptr(sin), rope_rs, q.data_ptr(), k.data_ptr(), v.data_ptr(), B, S, n_heads, n_kv_heads,
                   head_dim, conv_ks, flags, _lib.dtype_code(qkv), _lib.stream(qkv))
     return q, k, (v.transpose(2, 3) if vt else v)
+
+
+def decode_reach(flags: int, conv_ks: int) -> int:
+    """Rows before its own that a token's q, k and v depend on."""
+    return max(2 * (conv_ks - 1) if flags & CCGQA_CONVS else 0, 1 if flags & CCGQA_VALUE_SHIFT else 0)
+
+
+def _check_ring(name: str, ring: torch.Tensor, W: int, dtype: torch.dtype) -> None:
+    if ring.dim() != 3 or ring.shape[2] != W or ring.dtype != dtype or not ring.is_contiguous():
+        raise ValueError(f"{name}: ring must be contiguous {dtype} [requests, rows, {W}], got {ring.dtype} "
+                         f"{tuple(ring.shape)}")
+
+
+def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                      k_pages: torch.Tensor, v_pages: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
+                      flags: int, wq1=None, wq2=None, wk1=None, wk2=None, temperature=None, cos=None, sin=None,
+                      packed: bool = False, conv_ks: int = 3) -> torch.Tensor:
+    """ccgqa_prep for the newest token of each of N requests: q [N, Hq, hd]
+    from its projected row qkv [N, L+2K] and the rows before it; k and v go
+    to the token's slot in the paged cache.
+
+    ring [N, R, L+2K] holds the projected rows of each request's last tokens,
+    row p at p % R, R more than decode_reach(flags, conv_ks); the new one is
+    kept in it.  positions: int32 [N], the tokens' own; slots: int64 of N
+    (PagePlan.slots of a step of width 1).  A request whose slot lies outside
+    the pool, or whose position is negative or past the RoPE tables, changes
+    nothing and gets zeros for q.  Weights, temperature, tables and flags as
+    ccgqa_prep takes them.  fp32 inside, one rounding.  Inference only."""
+    name = "ccgqa_decode_prep"
+    _lib.require_gpu(name, qkv, ring, positions, slots, k_pages, v_pages, wq1, wq2, wk1, wk2, temperature, cos, sin)
+    L, K = n_heads * head_dim, n_kv_heads * head_dim
+    W, dt = L + 2 * K, qkv.dtype
+    if qkv.dim() != 2 or qkv.shape[1] != W:
+        raise ValueError(f"{name}: qkv must be [N, L + 2K = {W}], got {tuple(qkv.shape)}")
+    N = qkv.shape[0]
+    _check_ring(name, ring, W, dt)
+    if ring.shape[0] != N or ring.shape[1] <= decode_reach(flags, conv_ks):
+        raise ValueError(f"{name}: ring must hold more than {decode_reach(flags, conv_ks)} rows of {N} requests, got "
+                         f"{tuple(ring.shape)}")
+    if positions.dtype != torch.int32 or positions.shape != (N,):
+        raise ValueError(f"{name}: positions must be int32 [{N}], got {positions.dtype} {tuple(positions.shape)}")
+    if slots.dtype != torch.int64 or slots.numel() != N:
+        raise ValueError(f"{name}: slots must be int64, one a request, got {slots.dtype} {tuple(slots.shape)}")
+    check_pages(name, k_pages, v_pages)
+    pages, _, page, _ = k_pages.shape
+    if k_pages.shape[1] != n_kv_heads or k_pages.shape[3] != head_dim or k_pages.dtype != dt:
+        raise ValueError(f"{name}: pages must be {dt} [pages, {n_kv_heads}, page_size, {head_dim}], got "
+                         f"{k_pages.dtype} {tuple(k_pages.shape)}")
+    if qkv.stride(1) != 1 or (N > 1 and qkv.stride(0) < W):
+        qkv = qkv.contiguous()
+    if flags & CCGQA_CONVS:
+        ws = (wq1, wq2, wk1, wk2)
+        tiled = bool(flags & CCGQA_W_TILED)
+        if packed:
+            ws = tuple(w.to(dt).contiguous() for w in ws)
+        elif tiled:
+            ws = pack_conv_weights_tiled(ws, dt, n_heads, n_kv_heads, head_dim)
+        else:
+            ws = tuple(pack_conv_weight(w, dt) for w in ws)
+        exp = [(conv_ks, L, head_dim), (conv_ks, L, L), (conv_ks, K, head_dim), (conv_ks, K, K)]
+        if tiled:
+            exp = [(conv_ks, o // 32, i // 16, 2, 32, 8) for _, o, i in exp]
+        for w, e in zip(ws, exp):
+            if tuple(w.shape) != e:
+                raise ValueError(f"{name}: packed conv weight shape {tuple(w.shape)} != {e}")
+        wq1, wq2, wk1, wk2 = ws
+    else:
+        wq1 = wq2 = wk1 = wk2 = None
+    temp = None
+    if flags & CCGQA_QK_NORM:
+        if temperature is None or temperature.numel() != 1:
+            raise ValueError(f"{name}: QK-norm needs a temperature of one element")
+        temp = temperature.detach().to(dt).contiguous()
+    rope_rs = rope_rows = 0
+    if flags & CCGQA_ROPE:
+        rope_rows = min(t.shape[-2] for t in (cos, sin))
+        if cos.shape[-1] != head_dim // 2:
+            raise ValueError(f"{name}: RoPE tables of {cos.shape[-1]} columns for head_dim {head_dim}")
+        cos, sin, rope_rs, rope16 = _rope_tables(cos, sin, rope_rows, True)
+        flags |= rope16
+    else:
+        cos = sin = None
+    positions, slots = positions.contiguous(), slots.contiguous()
+    q = torch.empty((N, n_heads, head_dim), dtype=dt, device=qkv.device)
+    with _lib.on_device(qkv):
+        _lib.call("hydra_ccgqa_decode_prep", qkv.data_ptr(), qkv.stride(0), ring.data_ptr(), ring.shape[1],
+                  positions.data_ptr(), slots.data_ptr(), _lib.ptr(wq1), _lib.ptr(wq2), _lib.ptr(wk1), _lib.ptr(wk2),
+                  _lib.ptr(temp), _lib.ptr(cos), _lib.ptr(sin), rope_rs, rope_rows, q.data_ptr(), k_pages.data_ptr(),
+                  v_pages.data_ptr(), _lib.strides(k_pages), _lib.strides(v_pages), pages, page, N, n_heads,
+                  n_kv_heads, head_dim, conv_ks, flags, _lib.dtype_code(qkv), _lib.stream(qkv))
+    return q
+
+
+def ccgqa_ring_fill(qkv: torch.Tensor, ring: torch.Tensor, lengths: torch.Tensor, keep: int,
+                    rows: Optional[torch.Tensor] = None) -> None:
+    """Keeps the last `keep` projected rows of prompts, qkv [M, S, W], in the
+    rings of their requests: prompt m has the length lengths[m] (int32; 0
+    leaves its ring as it is) and belongs to request rows[m] (int64, distinct;
+    None: m)."""
+    name = "ccgqa_ring_fill"
+    _lib.require_gpu(name, qkv, ring, lengths, rows)
+    M, S, W = qkv.shape
+    _check_ring(name, ring, W, qkv.dtype)
+    if lengths.dtype != torch.int32 or lengths.shape != (M,):
+        raise ValueError(f"{name}: lengths must be int32 [{M}], got {lengths.dtype} {tuple(lengths.shape)}")
+    if rows is not None and (rows.dtype != torch.int64 or rows.shape != (M,)):
+        raise ValueError(f"{name}: rows must be int64 [{M}], got {rows.dtype} {tuple(rows.shape)}")
+    if qkv.stride(-1) != 1:
+        qkv = qkv.contiguous()
+    lengths, rows = lengths.contiguous(), None if rows is None else rows.contiguous()
+    with _lib.on_device(qkv):
+        _lib.call("hydra_ccgqa_ring_fill", qkv.data_ptr(), qkv.stride(0), qkv.stride(1), ring.data_ptr(),
+                  _lib.ptr(rows), lengths.data_ptr(), M, S, W, ring.shape[0], ring.shape[1], int(keep),
+                  _lib.dtype_code(qkv), _lib.stream(qkv))
 
 
 def _mask_bytes(key_mask: torch.Tensor) -> torch.Tensor:

@@ -28,13 +28,15 @@ class PagePlan(NamedTuple):
     tokens (-1 beside them), `positions` int32 [N] of the first ones,
     `lengths` int32 [N] afterwards, `seen` int32 [N] (the new length of the
     requests that got tokens, 0 of the others: what paged_attention takes),
-    `granted` bool [N], `free_count` int32 [1] afterwards."""
+    `granted` bool [N], `free_count` int32 [1] afterwards; `from_empty`: as
+    the plan was asked for."""
     slots: torch.Tensor
     positions: torch.Tensor
     lengths: torch.Tensor
     seen: torch.Tensor
     granted: torch.Tensor
     free_count: torch.Tensor
+    from_empty: bool = False
 
 
 def _vector(name: str, what: str, t: torch.Tensor, dtype, n=None) -> torch.Tensor:
@@ -56,7 +58,7 @@ def _check_table(name: str, table: torch.Tensor, n: int) -> None:
         raise ValueError(f"{name}: table needs rows of unit stride that do not overlap")
 
 
-def _check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
+def check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
         raise ValueError(f"{name}: k_pages and v_pages must be alike, [pages, Hkv, page_size, hd], got "
                          f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
@@ -104,7 +106,7 @@ def _plan(name, lengths, new_tokens, table, free_pages, free_count, page_size, w
                   free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), slots.data_ptr(),
                   after.data_ptr(), seen.data_ptr(), granted.data_ptr(), positions.data_ptr(), left.data_ptr(),
                   N, table.shape[1], width, int(page_size), 1 if from_empty else 0, _lib.stream(lengths))
-    return PagePlan(slots, positions, after, seen, granted, left)
+    return PagePlan(slots, positions, after, seen, granted, left, bool(from_empty))
 
 
 def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
@@ -152,7 +154,7 @@ def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     distinct; -1, or any outside the pool, for rows that are not kept)."""
     name = "store_pages"
     _lib.require_gpu(name, k, v, k_pages, v_pages, slots)
-    _check_pages(name, k_pages, v_pages)
+    check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
     if k.dim() != 4 or k.shape[1] != K or k.shape[3] != hd or v.shape != k.shape:
         raise ValueError(f"{name}: k and v must be [N, {K}, S, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -182,7 +184,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     request that sees none gets zeros.  Inference only: no gradient."""
     name = "paged_attention"
     _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out)
-    _check_pages(name, k_pages, v_pages)
+    check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
     if q.dim() != 3 or q.shape[2] != hd:
         raise ValueError(f"{name}: q must be [N, Hq, {hd}], got {tuple(q.shape)}")

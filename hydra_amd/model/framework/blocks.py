@@ -16,6 +16,7 @@ import torch.nn as nn
 from ... import _lib
 from ...attention.backends.ccgqa.attention import CCGQAAttention
 from ...attention.factory import build_hybrid_attention_module
+from ...attention.paged import PagePlan, PagePool
 from ...layers import AdaRMSNorm, RMSNorm, SwiGLUMLPFused, residual_norm
 from ...routing.mixture_of_depths import MoDMLPWrapper, _own, _plain
 from ...routing.mixture_of_recursions import (MoRConfig, MoRExecutor, MoRRouter,
@@ -66,13 +67,32 @@ class HydraBlock(nn.Module):
         self.mlp = SwiGLUMLP(dim, hidden_dim)
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
-        a = self.attention(self.norm1(x), mask=mask)
+        return self._rest(x, self.attention(self.norm1(x), mask=mask))
+
+    def _rest(self, x: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
+        """The block after its attention's output a."""
         if _recording(x, a, *self.norm2.parameters(), *self.mlp.parameters()):
             h = x + a
             return h + self.mlp(self.norm2(h))
         h, y = residual_norm(x, r=a, weight=self.norm2.weight, eps=self.norm2.eps,
                              norm=_lib.NORM_RMS, want_h=True)
         return _mlp_residual(self.mlp, h, y)
+
+    def new_cache(self, pool: PagePool, dtype: Optional[torch.dtype] = None):
+        """The attention's cache for the requests of `pool`."""
+        return self.attention.new_cache(pool, dtype)
+
+    @torch.no_grad()
+    def prefill(self, x: torch.Tensor, cache, plan: PagePlan, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """forward() of whole prompts x [M, S, dim] into a paged cache
+        (CCGQAAttention.prefill)."""
+        return self._rest(x, self.attention.prefill(self.norm1(x), cache, plan, rows))
+
+    @torch.no_grad()
+    def decode(self, x: torch.Tensor, cache, plan: PagePlan) -> torch.Tensor:
+        """forward() of each request's newest token, x [N, dim] or [N, 1, dim]
+        (CCGQAAttention.decode)."""
+        return self._rest(x, self.attention.decode(self.norm1(x), cache, plan))
 
 
 class HydraMoRBlock(nn.Module):

@@ -508,6 +508,36 @@ int hydra_paged_attn(const void* q, const void* k_pages, const void* v_pages, vo
 int hydra_paged_attn_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t hd, int64_t P,
                                int64_t page_size, int dtype, int64_t* bytes);
 
+/* hydra_ccgqa_prep_fwd for the newest token of N requests that are decoded
+ * (attention.py:205-266, kernels/fused_conv.py:39-62).  qkv [N, L + 2K] (row
+ * stride qkv_rs) holds its projected row; ring [N, R, L + 2K] the rows before
+ * it, row p of request n at ring[n, p % R], R > the rows that a token looks back
+ * (2 (conv_ks - 1) with HYDRA_CCGQA_CONVS, 1 with the value shift).  positions
+ * [N]: the token's own (rows before position 0 count as zero); slots [N]: where
+ * k and v go in k_pages, v_pages [pages, Hkv, page_size, hd] (element strides
+ * kp_st[4], vp_st[4]).  q: contiguous [N, Hq, hd].  The new row is kept in the
+ * ring.  A request with a slot outside the pool, a negative position or one
+ * past the RoPE table's rope_rows changes nothing and gets zeros for q.
+ * Weights, temperature, cos/sin and flags as in hydra_ccgqa_prep_fwd
+ * (HYDRA_CCGQA_W_TILED: 16-bit, head_dim 16, 32, 64 or 128, three taps).  fp32
+ * inside, one rounding. */
+int hydra_ccgqa_decode_prep(const void* qkv, int64_t qkv_rs, void* ring, int64_t R,
+                            const int* positions, const int64_t* slots, const void* wq1,
+                            const void* wq2, const void* wk1, const void* wk2,
+                            const void* temperature, const void* cos, const void* sin,
+                            int64_t cs_rs, int64_t rope_rows, void* q, void* k_pages,
+                            void* v_pages, const int64_t* kp_st, const int64_t* vp_st,
+                            int64_t pages, int64_t page_size, int64_t N, int64_t Hq, int64_t Hkv,
+                            int64_t hd, int64_t conv_ks, int flags, int dtype, void* stream);
+
+/* The last `keep` rows of prompts into such a ring: of qkv [M, S, W] (strides
+ * qkv_bs, qkv_rs; unit columns) the rows s with lengths[m] - keep <= s <
+ * lengths[m] to ring[rows[m], s % R] (rows null: m).  A prompt with a length
+ * outside [0, S], or a row outside the ring, leaves it as it is. */
+int hydra_ccgqa_ring_fill(const void* qkv, int64_t qkv_bs, int64_t qkv_rs, void* ring,
+                          const int64_t* rows, const int* lengths, int64_t M, int64_t S,
+                          int64_t W, int64_t N, int64_t R, int64_t keep, int dtype, void* stream);
+
 /* ---- block compositions (hydra/model/framework, hydra/layers) --------- */
 
 /* Token embedding: out[r, :] = table[clamp(ids[r], 0, vocab-1), :] * scale,

@@ -103,4 +103,64 @@ def attention_bound(q, k_pages, weight, out, lengths, dtype, scale=None):
         torch.finfo(dtype).smallest_normal
 
 
-__all__ = ["plan", "release", "attention", "attention_bound"]
+
+def decode_bound(params, qkv, cfg, dtype):
+    """(q, k) bounds, [Hq, hd] and [Hkv, hd], of the error of the last row's q
+    and k of qkv [S, W] (fp64) when they are computed in fp32 and rounded once.
+
+    With |.| through both convs: y1 sums ks hd products, y2 ks C, each at most
+    u = 2^-24 a product and sum of the absolute values' result Y; a 16-bit
+    conv2 takes y1 as two rounded terms, 2^-8 of 2^-8 (bf16; fp16 less): 2^-16
+    of Y.  The mean sums at most Hq rows: (Hq + 4) u of its absolute value's.
+    The norm then moves z / |z| by at most (dz + |z_i| |dz| / |z|) / |z|, its own
+    sum and root by (hd + 8) u; the rotation mixes a pair's errors, 2 u more and
+    the table's fp32."""
+    u = 2.0 ** -24
+    L, K, hd, ks = cfg.latent_dim, cfg.kv_dim, cfg.head_dim, cfg.conv_kernel_size
+    S = qkv.shape[0]
+    x = qkv.abs()[None]
+    parts = {}
+    for name, a, b, heads, w in (("q", 0, L, cfg.n_heads, "q_conv"), ("k", L, L + K, cfg.n_kv_heads, "k_conv")):
+        C = b - a
+        raw = qkv[:, a:b]
+        if cfg.use_convs:
+            w1, w2 = (params[f"{w}.conv{i}.weight"].double() for i in (1, 2))
+            Y = _convs(x[..., a:b], w1.abs(), w2.abs(), heads)[0, -1]
+            z = _convs(raw[None], w1, w2, heads)[0, -1]
+            dz = (ks * (hd + C) + 8) * u * Y + (0 if dtype == torch.float32 else 2.0 ** -16) * Y
+        else:
+            z, dz = raw[-1], torch.zeros(C, dtype=torch.float64)
+        parts[name] = [z.view(heads, hd), dz.view(heads, hd), raw[-1].view(heads, hd)]
+    (zq, dq, q0), (zk, dk, k0) = parts["q"], parts["k"]
+    if cfg.use_qk_mean:
+        if cfg.n_groups == 1:
+            means = [(0.5 * (q0 + k0), 0.5 * (q0.abs() + k0.abs()))] * 2
+        else:
+            means = [(0.5 * k0.mean(0, True), 0.5 * k0.abs().mean(0, True)),
+                     (0.5 * q0.mean(0, True), 0.5 * q0.abs().mean(0, True))]
+        zq, zk = zq + means[0][0], zk + means[1][0]
+        dq, dk = (d + (cfg.n_heads + 4) * u * m[1] for d, m in zip((dq, dk), means))
+    bounds = []
+    for z, d, gain in ((zq, dq, 1.0), (zk, dk, float(params["key_temperature"].double()))):
+        d = d + 4 * u * z.abs()
+        if cfg.use_qk_norm:
+            norm = z.norm(dim=-1, keepdim=True)
+            d = (d + z.abs() * d.norm(dim=-1, keepdim=True) / norm) / norm * abs(gain)
+            z = z / norm * gain
+            d = d + (hd + 8) * u * z.abs()
+        if cfg.use_rope:
+            pair = lambda t: t.view(-1, hd // 2, 2).sum(-1, keepdim=True).expand(-1, -1, 2).reshape(-1, hd)  # noqa: E731
+            d = pair(d) + 4 * u * pair(z.abs())
+            z = pair(z.abs())
+        # z: at least the result's size; half a step of dtype
+        bounds.append(1.01 * d + torch.finfo(dtype).eps / 2 * (z.abs() + d) + torch.finfo(dtype).smallest_normal)
+    return bounds
+
+
+def _convs(x, w1, w2, groups):
+    from .ccgqa import causal_conv_seq
+
+    return causal_conv_seq(x, w1, w2, groups)
+
+
+__all__ = ["plan", "release", "attention", "attention_bound", "decode_bound"]
