@@ -21,6 +21,7 @@ from .fused_ops import (
     get_kernel_status,
     set_use_triton_kernels,
 )
+from .logprobs import TokenLogprobs, token_logprobs
 
 __all__ = [
     "chunked_cross_entropy",
@@ -41,4 +42,6 @@ __all__ = [
     "USE_FUSED_RMS_NORM",
     "set_use_triton_kernels",
     "get_kernel_status",
+    "TokenLogprobs",
+    "token_logprobs",
 ]

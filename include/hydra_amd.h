@@ -445,6 +445,30 @@ int hydra_ce_grad_planes(const float* logits, int64_t rows, int64_t vocab, int64
                          int64_t planes_rs, int64_t plane_stride, const float* grad_scale,
                          void* stream);
 
+/* Log probabilities of given tokens in their rows of logits x [rows, vocab]
+ * (unit column stride, row stride logits_rs), p = softmax(x / temperature):
+ * logprobs[r] = ln p[tokens[r]] (0 for a token outside [0, vocab)),
+ * entropy[r] = -sum p ln p, and the top_k (at most 64) largest logits of the
+ * row, the lowest index first among equals (NaN counts as the largest):
+ * top_tokens [rows, top_k] and ln p there, top_logprobs.  A row of -inf alone
+ * has log probabilities -inf and entropy 0; a row with a NaN or +inf has NaN.
+ * stats [rows, 2] (optional): what the backward takes.  fp32 results.  No
+ * counterpart in the reference, whose losses give mean cross-entropies. */
+int hydra_token_logprobs(const void* logits, int64_t rows, int64_t vocab, int64_t logits_rs,
+                         const int64_t* tokens, float temperature, int64_t top_k,
+                         float* logprobs, float* entropy, float* stats, float* top_logprobs,
+                         int64_t* top_tokens, int dtype, void* stream);
+
+/* Its gradient: grad [rows, vocab] (contiguous, `dtype`) of the logits from
+ * g_logprobs [rows], g_entropy [rows] and g_top [rows, top_k] (fp32; each may
+ * be null), the forward's stats and entropy and, with g_top, its top_tokens.
+ * Zero for a row of -inf alone; grad must not overlap the logits. */
+int hydra_token_logprobs_bwd(const void* logits, int64_t rows, int64_t vocab, int64_t logits_rs,
+                             const int64_t* tokens, float temperature, int64_t top_k,
+                             const float* stats, const float* entropy, const int64_t* top_tokens,
+                             const float* g_logprobs, const float* g_entropy, const float* g_top,
+                             void* grad, int dtype, void* stream);
+
 /* ---- pages of a key-value cache (no counterpart in the reference, which
  *      recomputes the whole sequence for every token) ---------------------- */
 
