@@ -75,7 +75,8 @@ SIGNATURES = {
                          _I64P, _I64P, _I64P, _I64P, _F, _I, _P, _I64, _P],
     "hydra_paged_attn_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I, _I64P],
     "hydra_ccgqa_decode_prep": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P,
-                                _I64P, _I64P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P],
+                                _I64P, _I64P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _P],
+    "hydra_ccgqa_decode_prep_workspace": [_I64, _I64, _I64, _I64, _I64, _I, _I],
     "hydra_ccgqa_ring_fill": [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _P],
     "hydra_ccgqa_prep_tiled_ok": [_I64, _I64, _I64, _I],
     "hydra_ccgqa_prep_faults": [_P],
@@ -103,7 +104,8 @@ SIGNATURES = {
 }
 
 # entry points that return a value (not a status) of type int64_t
-_RETURNS_INT64 = {"hydra_rms_norm_bwd_workspace", "hydra_ccgqa_prep_bwd_conv_workspace"}
+_RETURNS_INT64 = {"hydra_rms_norm_bwd_workspace", "hydra_ccgqa_prep_bwd_conv_workspace",
+                  "hydra_ccgqa_decode_prep_workspace"}
 
 _lib = None
 

@@ -552,7 +552,12 @@ int hydra_ccgqa_decode_prep(const void* qkv, int64_t qkv_rs, void* ring, int64_t
                             int64_t cs_rs, int64_t rope_rows, void* q, void* k_pages,
                             void* v_pages, const int64_t* kp_st, const int64_t* vp_st,
                             int64_t pages, int64_t page_size, int64_t N, int64_t Hq, int64_t Hkv,
-                            int64_t hd, int64_t conv_ks, int flags, int dtype, void* stream);
+                            int64_t hd, int64_t conv_ks, int flags, int dtype, void* workspace,
+                            int64_t workspace_size, void* stream);
+/* Device scratch bytes that takes (16-byte aligned; 0 where a head's convs are
+ * one workgroup's).  Host-only. */
+int64_t hydra_ccgqa_decode_prep_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t hd,
+                                          int64_t conv_ks, int flags, int dtype);
 
 /* The last `keep` rows of prompts into such a ring: of qkv [M, S, W] (strides
  * qkv_bs, qkv_rs; unit columns) the rows s with lengths[m] - keep <= s <

@@ -50,7 +50,7 @@ def test_greedy_generation(cuda):
         want = ol.forward(logits, out.top_tokens[n, :1].cpu(), TOP)
         # the logits are those of two fp32 evaluations: 1e-5 of the largest each
         tol = 4e-5 * float(logits.abs().max()) + 1e-5
-        assert abs(float(out.logprobs[n]) - float(want[0][0])) < tol
+        assert abs(float(out.logprobs[n].detach()) - float(want[0][0])) < tol
         assert abs(float(out.entropy[n]) - float(want[1][0])) < tol * math.log(VOCAB)
         assert (out.top_logprobs[n].cpu().double() - want[2][0]).abs().max() < tol
         assert float(out.logprobs[n]) == float(out.top_logprobs[n, 0])
