@@ -14,7 +14,7 @@
 //    of fp32 (16x16x4, full fp32 products);
 //  * the softmax keeps each head's running maximum (fp32, log2 units) in the
 //    lanes of its column; the sums of one lane's keys are added up at the end;
-//  * P goes through 4 KT GP bytes of LDS to the lanes that hold the rows of V,
+//  * P goes through KT GP floats of LDS to the lanes that hold the rows of V,
 //    which accumulate p v in fp32 with plain multiply-adds: P is never rounded,
 //    V needs no transposed copy, and G multiply-adds per value stay below the
 //    time its bytes take (G = 8: about a third).
@@ -25,7 +25,7 @@
 // most within their own page and stay out of both sums, whatever they hold.
 //
 // Split: the keys of all (request, key head, head block) items are laid end to
-// end in rounds of 4 KT keys (one tile per wave) and dealt out evenly to the
+// end in rounds of 8 KT keys (one tile per wave) and dealt out evenly to the
 // workgroups, whatever the lengths; an item that more than one of them works on
 // leaves (max, sum, unscaled output) per part in the workspace, and a second
 // kernel joins them in order.  No atomics: the same inputs give the same bits.
@@ -57,7 +57,7 @@ struct PagedArgs {
   int N, H, Hkv, hd, G, GB, P, shift, pages;
   float scale;                       // times log2(e)
   // split form: rounds of a workgroup at least, workgroups, results
-  int least, groups;
+  int least, groups, cus;
   int* plan;                         // [0] rounds per workgroup, [1 + n] prefix of rounds
   float* part;                       // [groups][2][GP (2 + hd)]
 };
@@ -98,12 +98,62 @@ __device__ __forceinline__ int seen_keys(const PagedArgs& a, int n) {
   return max(0, min(a.lengths[n], a.P << a.shift));
 }
 
-// Keys of a wave's step: 4 to 8 KB of keys and as much of values in flight.
-constexpr int tile_keys(int lpr) { return lpr <= 4 ? 64 : (lpr <= 16 ? 32 : 16); }
+// Most waves of a workgroup (a launch takes 4 or 8), and keys of a wave's step: 4 KB
+// of keys and as much of values in flight (64 keys of 128 bytes instead of 32 take
+// 150 registers: a workgroup less on each CU, 5% more time at long contexts).
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+__device__ __forceinline__ int waves() { return blockDim.x >> 6; }
+constexpr int tile_keys(int lpr) { return lpr < 4 ? 64 : (lpr <= 16 ? 32 : 16); }
 template <int LPR> struct Tile { static constexpr int KT = tile_keys(LPR); };
 
-// One item's keys [t0, t1) rounds -> per-head max, sum and output of the whole
-// workgroup in LDS (acc[GP][hdp], then m[GP], l[GP]).
+// One step of a sum over lanes that leaves each lane half of the values: lanes
+// without bit OFF keep v[0 .. N/2), the others v[N/2 .. N), to v[0 .. N/2).
+template <int OFF, int N>
+__device__ __forceinline__ void half_sum(float* v) {
+  const bool upper = threadIdx.x & OFF;
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    if constexpr (OFF == 32 || OFF == 16) {
+      // swaps a's upper lanes (of 64, of each 32) with b's lower ones: a + b is the sum
+      const auto r = OFF == 32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + N / 2]), false, false)
+                               : __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + N / 2]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+      const float keep = upper ? v[i + N / 2] : v[i], give = upper ? v[i] : v[i + N / 2];
+      v[i] = keep + __shfl_xor(give, OFF);
+    }
+  }
+}
+
+// v[N] of this lane summed over the lanes that differ from it in bits OFF ..
+// LPR (down); returns the index of the first value left, `left` of them.
+template <int OFF, int LPR, int N>
+__device__ __forceinline__ int scatter_sum(float* v) {
+  if constexpr (OFF < LPR) {
+    return 0;
+  } else if constexpr (N > 1) {
+    half_sum<OFF, N>(v);
+    return (threadIdx.x & OFF ? N / 2 : 0) + scatter_sum<OFF / 2, LPR, N / 2>(v);
+  } else {
+    v[0] += __shfl_xor(v[0], OFF);
+    return scatter_sum<OFF / 2, LPR, 1>(v);
+  }
+}
+
+// Pages of a wave's tile, one for each 16 keys, wave-uniform; -1: not there.
+template <int NB>
+__device__ __forceinline__ void tile_pages(const PagedArgs& a, const int* row, int key0, int len, int (&page)[NB]) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int key = __builtin_amdgcn_readfirstlane(key0 + 16 * b);
+    const int p = key < len ? row[key >> a.shift] : -1;
+    page[b] = static_cast<unsigned>(p) < static_cast<unsigned>(a.pages) ? p : -1;
+  }
+}
+
+// One item's keys, rounds [t0, t1) (a tile per wave each): every wave's per-head
+// max, sum and output in LDS, [kWaves][GP] twice and [kWaves][GP][HDP].
 template <typename T, int GP, int LPR, bool VEC>
 __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int gb, int t0, int t1, float* sm) {
   constexpr int KT = Tile<LPR>::KT, E = Vec<T>::N, NC = LPR < 4 ? 1 : LPR / 4;
@@ -113,8 +163,15 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g4 = lane >> 4;  // operand row / column, 16-byte piece
   const int heads = min(GP, a.G - gb * GP);
-  const int len = seen_keys(a, n);
+  const int len = seen_keys(a, n), rmask = (1 << a.shift) - 1;
+  const int* trow = a.table + n * a.table_rs;
+  const char *kbase = a.k + h * a.k_st[1], *vbase = a.v + h * a.v_st[1];
   float* plds = sm + wave * KT * GP;
+  int key0 = (t0 * waves() + wave) * KT;
+  const int last = min(t1 * waves() * KT, len);
+  int page[NB];
+  if (key0 < last) tile_pages<NB>(a, trow, key0, len, page);
+  const bool any = key0 < last;
 
   uint4 qf[NC];
   {
@@ -126,46 +183,42 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
     }
   }
   float m = -INFINITY, l = 0.f;
-  float acc[GP][E];
+  float acc[GP * E];
 #pragma unroll
-  for (int g = 0; g < GP; ++g)
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[g][e] = 0.f;
+  for (int i = 0; i < GP * E; ++i) acc[i] = 0.f;
 
-  const int* trow = a.table + n * a.table_rs;
   const int vrow = lane / LPR, vpiece = lane % LPR;
-  for (int t = t0; t < t1; ++t) {
-    const int key0 = (t * 4 + wave) * KT;
-    if (key0 >= len) break;
-    // page of each 16 keys, wave-uniform; -1: not there
-    int page[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int key = __builtin_amdgcn_readfirstlane(key0 + 16 * b);
-      int p = key < len ? trow[key >> a.shift] : -1;
-      page[b] = static_cast<unsigned>(p) < static_cast<unsigned>(a.pages) ? p : -1;
-    }
-    const int rmask = (1 << a.shift) - 1;
+  // a lane's place in a key block and in a value load, within a page
+  const uint32_t klane = col * static_cast<uint32_t>(a.k_st[2]);
+  const uint32_t vlane = (vrow & 15) * static_cast<uint32_t>(a.v_st[2]);
+  for (; key0 < last; key0 += waves() * KT) {
+    const bool tail = key0 + KT > len;
     uint4 kf[NB][NC];
+    bool whole = true;  // every page is there
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const char* base = a.k + max(page[b], 0) * a.k_st[0] + h * a.k_st[1] +
-                         static_cast<int64_t>(((key0 + 16 * b) & rmask) + col) * a.k_st[2];
+      whole = whole && page[b] >= 0;
+      const char* base = kbase + max(page[b], 0) * a.k_st[0] +
+                         static_cast<int64_t>((key0 + 16 * b) & rmask) * a.k_st[2];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) kf[b][c] = row_piece<T, VEC>(base, 4 * c + g4, a.hd);
+      for (int c = 0; c < NC; ++c) kf[b][c] = row_piece<T, VEC>(base + klane, 4 * c + g4, a.hd);
     }
     uint4 vf[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int row = i * RPI + vrow;
-      int p = page[i * RPI / 16];
-      if constexpr (RPI == 32) p = vrow < 16 ? p : page[i * RPI / 16 + 1];
-      const int key = key0 + row;
-      const bool seen = key < len && p >= 0;
-      const char* base = a.v + max(p, 0) * a.v_st[0] + h * a.v_st[1] + static_cast<int64_t>(key & rmask) * a.v_st[2];
-      vf[i] = row_piece<T, VEC>(base, vpiece, a.hd);
-      if (!seen) vf[i] = make_uint4(0, 0, 0, 0);  // 0 x whatever lies there must add nothing
+      const int b = i * RPI / 16;  // RPI = 32: the lower and the upper lanes' pages
+      const char* base = vbase + max(page[b], 0) * a.v_st[0] +
+                         static_cast<int64_t>((key0 + (RPI < 16 ? i * RPI : 16 * b)) & rmask) * a.v_st[2];
+      if constexpr (RPI == 32) {
+        const char* base1 = vbase + max(page[b + 1], 0) * a.v_st[0] +
+                            static_cast<int64_t>((key0 + 16 * b + 16) & rmask) * a.v_st[2];
+        base = vrow < 16 ? base : base1;
+      }
+      vf[i] = row_piece<T, VEC>(base + vlane, vpiece, a.hd);
     }
+    int next[NB];
+    const int key1 = key0 + waves() * KT;
+    if (key1 < last) tile_pages<NB>(a, trow, key1, len, next);
     f32x4_t s[NB];
     float top = -INFINITY;
 #pragma unroll
@@ -174,14 +227,31 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
 #pragma unroll
       for (int c = 0; c < NC; ++c) s[b] = mfma16<T>(kf[b][c], qf[c], s[b]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = key0 + 16 * b + 4 * g4 + r;
-        s[b][r] = key < len && page[b] >= 0 ? s[b][r] * a.scale : -INFINITY;
-        top = fmaxf(top, s[b][r]);
+      for (int r = 0; r < 4; ++r) s[b][r] *= a.scale;
+    }
+    if (tail || !whole) {  // what is not seen: out of the scores, and 0 in v (0 x whatever lies there)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (key0 + 16 * b + 4 * g4 + r >= len || page[b] < 0) s[b][r] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int b = i * RPI / 16;
+        bool there = page[b] >= 0;
+        if constexpr (RPI == 32) {
+          const bool upper = page[b + 1] >= 0;  // loaded before the choice: a chosen index would put the pages in memory
+          there = vrow < 16 ? there : upper;
+        }
+        if (key0 + i * RPI + vrow >= len || !there) vf[i] = make_uint4(0, 0, 0, 0);
       }
     }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[b][r]);
     top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = halves_max(top);
     if (__any(top > m)) {
       const float mn = fmaxf(m, top);
       const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -189,9 +259,9 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
       l *= alpha;
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
-        const float al = __shfl(alpha, g);
+        const float al = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(alpha), g));
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[g][e] *= al;
+        for (int e = 0; e < E; ++e) acc[g * E + e] *= al;
       }
     }
     const float ms = m == -INFINITY ? 0.f : m;
@@ -199,10 +269,15 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(s[b][r] - ms);
-        l += p;
-        if (col < GP) plds[(16 * b + 4 * g4 + r) * GP + col] = p;
+        s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - ms);
+        l += s[b][r];
       }
+    if (col < GP) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) plds[(16 * b + 4 * g4 + r) * GP + col] = s[b][r];
+    }
     // P is read by other lanes of this wave alone; its LDS operations keep their order.
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -215,58 +290,59 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
 #pragma unroll
       for (int g = 0; g < GP; ++g)
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[g][e] = fmaf(p[g], v[e], acc[g][e]);
+        for (int e = 0; e < E; ++e) acc[g * E + e] = fmaf(p[g], v[e], acc[g * E + e]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) page[b] = next[b];
   }
-  // The wave's own sums ...
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-#pragma unroll
-  for (int off = LPR; off < 64; off <<= 1)
-#pragma unroll
-    for (int g = 0; g < GP; ++g)
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[g][e] += __shfl_xor(acc[g][e], off);
-  // ... then the four waves', in order.
-  float* wm = sm;                 // [4][GP] max, [4][GP] sum, [4][GP][HDP] output
-  float* wl = sm + 4 * GP;
-  float* wa = sm + 8 * GP;
-  __syncthreads();                // P's memory is free
+  // The wave's own sums, each lane its share of the values.
+  float* wm = sm;
+  float* wl = sm + kWaves * GP;
+  float* wa = sm + 2 * kWaves * GP;
+  constexpr int ROWS = 64 / LPR, LEFT = GP * E > ROWS ? GP * E / ROWS : 1;
+  int first = 0;
+  if (any) {
+    l += __shfl_xor(l, 16);
+    l = halves_sum(l);
+    first = scatter_sum<32, LPR, GP * E>(acc);
+  }
+  __syncthreads();  // P's memory is free
   if (lane < GP) {
     wm[wave * GP + lane] = m;
     wl[wave * GP + lane] = l;
   }
-  if (lane < LPR) {
+  if (any) {  // a wave without keys leaves nothing: join_waves does not look at it
 #pragma unroll
-    for (int g = 0; g < GP; ++g)
-#pragma unroll
-      for (int e = 0; e < E; ++e) wa[(wave * GP + g) * HDP + lane * E + e] = acc[g][e];
+    for (int i = 0; i < LEFT; ++i) {
+      const int g = (first + i) / E, e = (first + i) % E;
+      wa[(wave * GP + g) * HDP + vpiece * E + e] = acc[i];
+    }
   }
   __syncthreads();
 }
 
-// The four waves' results of item_keys as (max, sum, output element) of head g.
+// The waves' results of item_keys as (max, sum, output element) of head g.
 template <int GP, int HDP>
 __device__ __forceinline__ void join_waves(const float* sm, int g, int d, float& m, float& l, float& o) {
   m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w * GP + g]);
+#pragma unroll 4
+  for (int w = 0; w < waves(); ++w) m = fmaxf(m, sm[w * GP + g]);
   const float ms = m == -INFINITY ? 0.f : m;
   l = 0.f;
   o = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float c = __builtin_amdgcn_exp2f(sm[w * GP + g] - ms);
-    l = fmaf(c, sm[4 * GP + w * GP + g], l);
-    o = fmaf(c, sm[8 * GP + (w * GP + g) * HDP + d], o);
+#pragma unroll 4
+  for (int w = 0; w < waves(); ++w) {
+    const float mw = sm[w * GP + g], c = __builtin_amdgcn_exp2f(mw - ms);
+    l = fmaf(c, sm[kWaves * GP + w * GP + g], l);
+    if (mw != -INFINITY) o = fmaf(c, sm[2 * kWaves * GP + (w * GP + g) * HDP + d], o);
   }
 }
 
 template <int GP, int LPR, typename T>
 constexpr int lds_floats() {
-  constexpr int p = 4 * Tile<LPR>::KT * GP, j = 8 * GP + 4 * GP * LPR * Vec<T>::N;
+  constexpr int p = kWaves * Tile<LPR>::KT * GP, j = 2 * kWaves * GP + kWaves * GP * LPR * Vec<T>::N;
   return p > j ? p : j;
 }
 
@@ -277,7 +353,7 @@ __device__ __forceinline__ T* out_row(const PagedArgs& a, int n, int head) {
 
 template <int LPR>
 __device__ __forceinline__ int rounds_of(int len) {
-  constexpr int R = 4 * Tile<LPR>::KT;
+  const int R = waves() * Tile<LPR>::KT;
   return len / R + (len % R != 0);
 }
 
@@ -285,7 +361,7 @@ __device__ __forceinline__ int rounds_of(int len) {
 template <typename T, int GP, int HDP>
 __device__ __forceinline__ void write_out(const PagedArgs& a, int n, int h, int gb, const float* sm) {
   const int heads = min(GP, a.G - gb * GP);
-  for (int e = threadIdx.x; e < heads * a.hd; e += 256) {
+  for (int e = threadIdx.x; e < heads * a.hd; e += static_cast<int>(blockDim.x)) {
     const int g = e / a.hd, d = e - g * a.hd;
     float m, l, o;
     join_waves<GP, HDP>(sm, g, d, m, l, o);
@@ -295,7 +371,7 @@ __device__ __forceinline__ void write_out(const PagedArgs& a, int n, int h, int 
 
 // One workgroup per item, no split.
 template <typename T, int GP, int LPR, bool VEC>
-__global__ __launch_bounds__(256) void paged_attn_whole_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kThreads) void paged_attn_whole_kernel(PagedArgs a) {
   constexpr int HDP = LPR * Vec<T>::N;
   __shared__ __attribute__((aligned(16))) float sm[lds_floats<GP, LPR, T>()];
   const int item = blockIdx.x, gb = item % a.GB, h = item / a.GB % a.Hkv, n = item / a.GB / a.Hkv;
@@ -303,25 +379,30 @@ __global__ __launch_bounds__(256) void paged_attn_whole_kernel(PagedArgs a) {
   write_out<T, GP, HDP>(a, n, h, gb, sm);
 }
 
+// A part of an item: per-head max at 0, sum at 8, output rows from 16 on, rounded
+// up to 16 bytes.
+__device__ __host__ __forceinline__ int row4(int hd) { return (hd + 3) & ~3; }
+template <int GP>
+__device__ __forceinline__ int part_floats(int hd) { return 16 + GP * row4(hd); }
+
 // Split form: workgroup w works on the rounds [w per, (w+1) per) of all items.
 template <typename T, int GP, int LPR, bool VEC>
-__global__ __launch_bounds__(256) void paged_attn_split_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kThreads) void paged_attn_split_kernel(PagedArgs a) {
   constexpr int HDP = LPR * Vec<T>::N;
   __shared__ __attribute__((aligned(16))) float sm[lds_floats<GP, LPR, T>()];
   __shared__ int pre[kMaxRequests + 1];
-  __shared__ int wsum[4];
+  __shared__ int wsum[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // prefix sums of the requests' rounds
   int base = 0;
   if (tid == 0) pre[0] = 0;
-  for (int i0 = 0; i0 < a.N; i0 += 256) {
+  for (int i0 = 0; i0 < a.N; i0 += static_cast<int>(blockDim.x)) {
     const int i = i0 + tid;
     int s = wave_incl_sum(i < a.N ? rounds_of<LPR>(seen_keys(a, i)) : 0);
     if (lane == 63) wsum[wave] = s;
     __syncthreads();
     int all = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < waves(); ++w) {
       if (w < wave) s += wsum[w];
       all += wsum[w];
     }
@@ -330,10 +411,12 @@ __global__ __launch_bounds__(256) void paged_attn_split_kernel(PagedArgs a) {
     __syncthreads();
   }
   const int HG = a.Hkv * a.GB, total = base * HG;
-  const int per = max(a.least, (total + a.groups - 1) / a.groups);
+  // two rounds and more, for the sake of each share's end, unless that left CUs idle
+  int per = (total + a.groups - 1) / a.groups;
+  per = max(max(per, min(2, (total + a.cus - 1) / a.cus)), a.least);
   if (blockIdx.x == 0) {  // for the joining kernel
     if (tid == 0) a.plan[0] = per;
-    for (int i = tid; i <= a.N; i += 256) a.plan[1 + i] = pre[i];
+    for (int i = tid; i <= a.N; i += static_cast<int>(blockDim.x)) a.plan[1 + i] = pre[i];
   }
   // the last workgroup's range may pass int only if the total does (checked on the host)
   const int begin = min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total));
@@ -354,15 +437,15 @@ __global__ __launch_bounds__(256) void paged_attn_split_kernel(PagedArgs a) {
     if (count == r) {
       write_out<T, GP, HDP>(a, n, h, gb, sm);
     } else {
-      float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * GP * (2 + a.hd);
-      for (int e = tid; e < GP * a.hd; e += 256) {
+      float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * part_floats<GP>(a.hd);
+      for (int e = tid; e < GP * a.hd; e += static_cast<int>(blockDim.x)) {
         const int g = e / a.hd, d = e - g * a.hd;
         float m, l, o;
         join_waves<GP, HDP>(sm, g, d, m, l, o);
-        part[2 * GP + e] = o;
+        part[16 + g * row4(a.hd) + d] = o;
         if (d == 0) {
           part[g] = m;
-          part[GP + g] = l;
+          part[8 + g] = l;
         }
       }
     }
@@ -373,51 +456,85 @@ __global__ __launch_bounds__(256) void paged_attn_split_kernel(PagedArgs a) {
 
 // Joins the parts of one item, in their order; writes the zeros of a request
 // without keys.  Items that one workgroup had whole are written already.
+// Four elements a thread, the parts dealt out over the threads left, eight loads
+// of 16 bytes in flight each.
 template <typename T, int GP>
 __global__ __launch_bounds__(1024) void paged_attn_join_kernel(PagedArgs a) {
+  constexpr int PL = kMaxParts / 64;
   __shared__ float weight[GP][kMaxParts];
-  __shared__ float sums[1024];
+  __shared__ float4 sums[1024];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int HG = a.Hkv * a.GB, n = blockIdx.x / HG, hg = blockIdx.x - n * HG, h = hg / a.GB, gb = hg - h * a.GB;
   const int per = a.plan[0], p0 = a.plan[1 + n], r = a.plan[2 + n] - p0;
   const int heads = min(GP, a.G - gb * GP);
   const int u0 = p0 * HG + hg * r, w0 = u0 / per, parts = r == 0 ? 0 : (u0 + r - 1) / per - w0 + 1;
   if (parts == 1) return;
-  const int size = GP * (2 + a.hd);
   auto part = [&](int p) {  // only the first one can begin inside its workgroup's range
-    return a.part + (static_cast<int64_t>(w0 + p) * 2 + (p == 0 && u0 != w0 * per ? 1 : 0)) * size;
+    return a.part + (static_cast<int64_t>(w0 + p) * 2 + (p == 0 && u0 != w0 * per ? 1 : 0)) * part_floats<GP>(a.hd);
   };
   for (int g = wave; g < GP; g += 16) {
-    float m = -INFINITY;
-    for (int p = lane; p < parts; p += 64) m = fmaxf(m, part(p)[g]);
-    m = wave_max(m);
-    const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int p = lane; p < parts; p += 64) l += __builtin_amdgcn_exp2f(part(p)[g] - ms) * part(p)[GP + g];
-    l = wave_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int p = lane; p < parts; p += 64) weight[g][p] = __builtin_amdgcn_exp2f(part(p)[g] - ms) * inv;
+    float m[PL], l[PL], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const int p = lane + 64 * i;
+      m[i] = p < parts ? part(p)[g] : -INFINITY;
+      l[i] = p < parts ? part(p)[8 + g] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < PL; ++i) top = fmaxf(top, m[i]);
+    top = wave_max(top);
+    const float ts = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      m[i] = __builtin_amdgcn_exp2f(m[i] - ts);
+      sum = fmaf(m[i], l[i], sum);
+    }
+    sum = wave_sum(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) weight[g][lane + 64 * i] = m[i] * inv;
   }
   __syncthreads();
-  // elements of the item side by side, the parts dealt out over what is left of the workgroup
-  const int elems = heads * a.hd;
-  int lanes = 1;  // threads of one element
-  while (lanes * 2 * elems <= 1024) lanes *= 2;
+  const int quads = row4(a.hd) / 4, elems = heads * quads;
+  int lanes = 1;  // threads of four elements
+  while (lanes < 64 && lanes * 2 * elems <= 1024) lanes *= 2;
   const int step = 1024 / lanes, sub = tid / step;
   for (int e0 = 0; e0 < elems; e0 += step) {
     const int e = e0 + tid - sub * step;
-    float o = 0.f;
+    const int g = e < elems ? e / quads : 0, d = 4 * (e - g * quads);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (e < elems) {
-      const int g = e / a.hd;
-#pragma unroll 8
-      for (int p = sub; p < parts; p += lanes) o = fmaf(weight[g][p], part(p)[2 * GP + e], o);
+      for (int p = sub; p < parts; p += 8 * lanes) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int q = min(p + j * lanes, parts - 1);
+          const float c = p + j * lanes < parts ? weight[g][q] : 0.f;
+          const float4 x = *reinterpret_cast<const float4*>(part(q) + 16 + g * row4(a.hd) + d);
+          // an output that a NaN or an infinity reached stays in its own part: c is not 0 there
+          if (c != 0.f) {
+            o.x = fmaf(c, x.x, o.x);
+            o.y = fmaf(c, x.y, o.y);
+            o.z = fmaf(c, x.z, o.z);
+            o.w = fmaf(c, x.w, o.w);
+          }
+        }
+      }
     }
     sums[tid] = o;
     __syncthreads();
     if (sub == 0 && e < elems) {
-      for (int i = 1; i < lanes; ++i) o += sums[i * step + tid];
-      const int g = e / a.hd;
-      out_row<T>(a, n, h * a.G + gb * GP + g)[e - g * a.hd] = from_f32<T>(o);
+      for (int i = 1; i < lanes; ++i) {
+        const float4 x = sums[i * step + tid];
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
+      }
+      T* out = out_row<T>(a, n, h * a.G + gb * GP + g) + d;
+      const float v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d + i < a.hd) out[i] = from_f32<T>(v[i]);
     }
     __syncthreads();
   }
@@ -447,18 +564,24 @@ inline Shape shape_of(int64_t N, int64_t H, int64_t Hkv, int64_t hd, int e) {
 
 struct Split {
   bool on;
-  int least, groups;
+  int least, waves;
 };
 
-// Split where the items alone would not fill the chip and a request may be
-// longer than one workgroup's least share.
+constexpr int kMaxResident = 4;  // workgroups of a CU that a split launch takes at most
+
+// Split where the items alone would not fill the chip and a request may be longer
+// than 1024 keys (of head_dim 64 they take one workgroup of 8 waves 5 us more than
+// 128 keys; the joining launch takes 3 to 5).  8 waves only for few short items:
+// where items or rounds are many, twice as many workgroups of 4 have more of the
+// chip's registers in use (256 requests of 20 keys, 28/4 heads of 64: 13.4
+// against 23 us).
 inline Split split_of(const Shape& s, int64_t N, int64_t capacity) {
-  const int64_t round = 4 * s.kt, most = (capacity + round - 1) / round;
   Split r{};
-  r.groups = 4 * device_cus();
-  const int64_t least = std::max<int64_t>(2, (most + kMaxParts - 2) / (kMaxParts - 1));
-  r.on = N <= kMaxRequests && s.items < 8 * device_cus() && most > least && most * s.items < (int64_t(1) << 31);
-  r.least = static_cast<int>(std::min<int64_t>(least, 1 << 30));
+  r.on = N <= kMaxRequests && s.items < 8 * device_cus() && capacity > 1024;
+  r.waves = r.on || s.items > device_cus() ? 4 : kWaves;
+  const int64_t most = (capacity + r.waves * s.kt - 1) / (r.waves * s.kt);
+  r.on = r.on && most * s.items < (int64_t(1) << 31);
+  r.least = static_cast<int>(std::max<int64_t>(1, (most + kMaxParts - 2) / (kMaxParts - 1)));
   return r;
 }
 
@@ -467,24 +590,30 @@ inline int64_t plan_ints(int64_t N) { return (N + 2 + 3) / 4 * 4; }
 
 inline int64_t workspace_bytes(const Split& p, int64_t N, int64_t hd) {
   if (!p.on) return 0;
-  return 4 * (plan_ints(N) + static_cast<int64_t>(p.groups) * 2 * 8 * (2 + hd));
+  return 4 * (plan_ints(N) + static_cast<int64_t>(kMaxResident) * device_cus() * 2 * (16 + 8 * row4(static_cast<int>(hd))));
+}
+
+template <typename T, int GP, int LPR, bool VEC>
+void launch_form(PagedArgs a, const Split& p, int64_t items, hipStream_t st) {
+  if (p.on) {
+    // as many workgroups as are resident at once, which the rounds are dealt to
+    const auto kernel = paged_attn_split_kernel<T, GP, LPR, VEC>;
+    a.cus = device_cus();
+    a.groups = a.cus * std::min(kMaxResident, blocks_per_cu(reinterpret_cast<const void*>(kernel), 64 * p.waves));
+    kernel<<<a.groups, 64 * p.waves, 0, st>>>(a);
+  } else {
+    paged_attn_whole_kernel<T, GP, LPR, VEC><<<static_cast<unsigned>(items), 64 * p.waves, 0, st>>>(a);
+  }
 }
 
 // Rows that 16-byte loads cannot take come through one form, of 8 heads.
 template <typename T, int GP, int LPR>
 int launch_paged(const PagedArgs& a, const Split& p, int64_t items, bool vec, hipStream_t st) {
   if constexpr (GP == 8) {
-    if (!vec) {
-      if (p.on) paged_attn_split_kernel<T, GP, LPR, false><<<p.groups, 256, 0, st>>>(a);
-      else paged_attn_whole_kernel<T, GP, LPR, false><<<static_cast<unsigned>(items), 256, 0, st>>>(a);
-    }
+    if (!vec) launch_form<T, GP, LPR, false>(a, p, items, st);
   }
-  if (p.on) {
-    if (vec) paged_attn_split_kernel<T, GP, LPR, true><<<p.groups, 256, 0, st>>>(a);
-    paged_attn_join_kernel<T, GP><<<static_cast<unsigned>(items), 1024, 0, st>>>(a);
-  } else if (vec) {
-    paged_attn_whole_kernel<T, GP, LPR, true><<<static_cast<unsigned>(items), 256, 0, st>>>(a);
-  }
+  if (vec) launch_form<T, GP, LPR, true>(a, p, items, st);
+  if (p.on) paged_attn_join_kernel<T, GP><<<static_cast<unsigned>(items), 1024, 0, st>>>(a);
   return check_launch("paged_attn");
 }
 

@@ -15,7 +15,7 @@ int check_paged(int64_t N, int64_t H, int64_t Hkv, int64_t hd, int64_t P, int64_
   HYDRA_REQUIRE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
                 "paged_attn: page_size must be a power of two in [16, 4096]");
   HYDRA_REQUIRE(dtype_size(dtype) > 0, "paged_attn: unknown dtype");
-  HYDRA_REQUIRE(P < (int64_t(1) << 31) / page_size && H < (1 << 20) && N < (int64_t(1) << 31) &&
+  HYDRA_REQUIRE(P <= (int64_t(1) << 30) / page_size && H < (1 << 20) && N < (int64_t(1) << 31) &&
                     N * H < (int64_t(1) << 31),
                 "paged_attn: too large");
   return HYDRA_OK;
@@ -72,6 +72,8 @@ extern "C" int hydra_paged_attn(const void* q, const void* k_pages, const void* 
     a.v_st[i] = vp_st[i] * e;
     vec = vec && (a.k_st[i] | a.v_st[i]) % 16 == 0;
   }
+  HYDRA_REQUIRE(kp_st[2] >= 0 && vp_st[2] >= 0 && std::max(kp_st[2], vp_st[2]) * e * page_size < (int64_t(1) << 31),
+                "paged_attn: rows of a page too far apart");
   a.table = table;
   a.lengths = lengths;
   a.table_rs = table_rs;
@@ -86,7 +88,6 @@ extern "C" int hydra_paged_attn(const void* q, const void* k_pages, const void* 
   a.pages = static_cast<int>(pages);
   a.scale = scale * kLog2e;
   a.least = p.least;
-  a.groups = p.groups;
   a.plan = static_cast<int*>(workspace);
   a.part = static_cast<float*>(workspace) + (p.on ? plan_ints(N) : 0);
   auto st = static_cast<hipStream_t>(stream);
