@@ -13,8 +13,8 @@
 // Both directions are bound by HBM: the forward reads a row once and keeps it
 // in registers between its maximum and its sums (16-bit values packed), the
 // backward reads it once and writes the gradient.  Rows start anywhere: a row
-// is taken in the 16-byte pieces of memory that it lies in, its first and last
-// piece element by element where they are not whole.
+// is taken in the 16-byte pieces of memory that it lies in, what is left at its
+// two ends element by element.
 #include "common.h"
 #include "mod_keys.h"
 
@@ -23,7 +23,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// exp2 of anything below is 0; keeps 0 * t_j a 0 where x_j is -inf.
+// exp2 of anything below is 0: keeps 0 * t_j a 0 where x_j is -inf.
 constexpr float kLowest = -2000.f;
 constexpr int kThreads = 512;
 constexpr int kMaxTop = 64;
@@ -40,27 +40,33 @@ struct LogpArgs {
   float c, inv_t;  // log2(e) / temperature, 1 / temperature
 };
 
-// A row as 16-byte pieces of memory: piece i holds the elements E i - shift + (0 .. E-1).
+// A row as 16-byte pieces of memory: piece i holds the elements E i - shift + (0 .. E-1);
+// pieces [first, last) are whole.  What is left of the row at its two ends, less
+// than E elements each, is one element of each of the first 2 E threads.
 template <typename T>
 struct Pieces {
   static constexpr int E = Vec<T>::N;
   const T* x;
-  int V, shift, count;
-  __device__ __forceinline__ Pieces(const T* row, int v) : x(row), V(v) {
+  int shift, first, last;
+  int own;  // this thread's element of the ends, or -1
+  __device__ __forceinline__ Pieces(const T* row, int V) : x(row) {
     shift = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-    count = (V + shift + E - 1) / E;
+    first = shift > 0 ? 1 : 0;
+    last = max((V + shift) / E, first);
+    const int head = min(first * E - shift, V);  // elements before the first whole piece
+    const int behind = max(last * E - shift, head), tid = threadIdx.x;
+    own = tid < E ? (tid < head ? tid : -1) : (tid < 2 * E && behind + tid - E < V ? behind + tid - E : -1);
   }
-  // Elements outside the row are -inf.
-  template <bool NT>
-  __device__ __forceinline__ uint4 load(int i) const {
-    const int e = i * E - shift;
-    if (e >= 0 && e + E <= V) return ld16raw<NT>(x + e);
-    float f[E];
-#pragma unroll
-    for (int k = 0; k < E; ++k) f[k] = e + k >= 0 && e + k < V ? to_f32(x[e + k]) : -INFINITY;
-    return pack16<T>(f);  // exact: T's own values
-  }
+  __device__ __forceinline__ int element(int piece) const { return piece * E - shift; }
+  __device__ __forceinline__ float end() const { return own >= 0 ? to_f32(x[own]) : -INFINITY; }
 };
+
+// Sixteen bytes of -inf.
+template <typename T>
+__device__ __forceinline__ uint4 low_piece() {
+  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, bf16>::value ? 0xff80ff80u : 0xfc00fc00u);
+  return make_uint4(w, w, w, w);
+}
 
 template <int N>
 __device__ __forceinline__ float max_of(const float* v) {
@@ -75,11 +81,15 @@ template <int N>
 __device__ __forceinline__ void add_sums(const float* v, float c, float M, float& s, float& w) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    // a NaN stays one: fmaxf would drop it
-    const float t = (v[i] - M) * c, u = t < kLowest ? kLowest : t, e = __builtin_amdgcn_exp2f(u);
+    const float t = (v[i] - M) * c, e = __builtin_amdgcn_exp2f(t);
     s += e;
-    w = fmaf(e, u, w);
+    w = fmaf(e, fmaxf(t, kLowest), w);  // a NaN stays one through e
   }
+}
+
+// score_key_asc's inverse (zero for both zeros).
+__device__ __forceinline__ float score_of_key(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
 // Order of the alternatives: value down, index up.
@@ -92,14 +102,27 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int off) {
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
+// The K-th largest of a wave's 64 keys, by their bits from the top: the largest
+// value that at least K of them reach.
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int K) {
+  uint32_t bound = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = bound | (1u << bit);
+    if (__popcll(__ballot(key >= t)) >= K) bound = t;
+  }
+  return bound;
+}
+
 // One row per workgroup.  NCH > 0: its pieces stay in registers, NCH of a
 // thread; NCH = 0: read again for the sums (rows of more than 16384 pieces).
 //
 // Alternatives: 64 groups of 8 lanes keep their maximum; the K-th largest of
 // these is a bound that at least K elements reach, and few more (about
-// 64 ln(64 / (64 - K)) of them where the order is random: 24 for K = 20).
-// They are listed in LDS and ranked against each other.  Where equal values
-// make them too many, the K best are taken one by one instead.
+// 64 ln(64 / (64 - K)) of them where the order is random: 24 for K = 20).  Only
+// threads whose own maximum reaches it look at their pieces again; what they
+// find is listed in LDS and ranked against each other.  Where equal values make
+// them too many, or a NaN leads the row, the K best are taken one by one.
 template <typename T, int NCH, bool TOP>
 __global__ __launch_bounds__(kThreads) void logp_kernel(LogpArgs a) {
   constexpr int E = Vec<T>::N, WAVES = kThreads / 64;
@@ -109,44 +132,40 @@ __global__ __launch_bounds__(kThreads) void logp_kernel(LogpArgs a) {
   const T* x = static_cast<const T*>(a.x) + row * a.rs;
   const Pieces<T> pieces(x, a.V);
   uint4 raw[NCH > 0 ? NCH : 1];
-  // every piece of this thread's: f(values, first element's index)
+  const int wave_first = __builtin_amdgcn_readfirstlane(pieces.first + (tid & ~63));
+  // every whole piece of this thread's
   auto each = [&](auto f) {
     if constexpr (NCH > 0) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         // the pieces stay packed between the passes: no widened copies kept
         asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
-        const int at = i * kThreads + tid;
-        if (at < pieces.count) {
-          float v[E];
-          unpack16<T>(raw[i], v);
-          f(v, at * E - pieces.shift);
-        }
+        if (wave_first + i * kThreads >= pieces.last) continue;  // the wave has none here
+        float v[E];
+        unpack16<T>(raw[i], v);
+        f(v);
       }
     } else {
-      for (int at = tid; at < pieces.count; at += kThreads) {
+#pragma unroll 4
+      for (int at = pieces.first + tid; at < pieces.last; at += kThreads) {
         float v[E];
-        unpack16<T>(pieces.template load<false>(at), v);
-        f(v, at * E - pieces.shift);
+        load16<T>(x + pieces.element(at), v);
+        f(v);
       }
     }
   };
   if constexpr (NCH > 0) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int at = i * kThreads + tid;
-      if (at < pieces.count) raw[i] = pieces.template load<true>(at);
+      const int at = pieces.first + i * kThreads + tid;
+      raw[i] = low_piece<T>();
+      if (at < pieces.last) raw[i] = ld16raw<!TOP>(x + pieces.element(at));  // alternatives are read again
     }
   }
   float m = -INFINITY;
-  bool nan = false;
-  each([&](const float* v, int) {
-    m = fmaxf(m, max_of<E>(v));
-    if constexpr (TOP) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) nan |= v[i] != v[i];
-    }
-  });
+  each([&](const float* v) { m = fmaxf(m, max_of<E>(v)); });
+  const float end = pieces.end();
+  m = fmaxf(m, end);
   const float mine = m;
   m = wave_max(m);
   if (lane == 0) red[0][wave] = m;
@@ -155,13 +174,24 @@ __global__ __launch_bounds__(kThreads) void logp_kernel(LogpArgs a) {
   const bool empty = m == -INFINITY;   // nothing is left (or NaN alone, which the sums keep)
   const float M = empty ? 0.f : m;
   float s = 0.f, w = 0.f;
-  each([&](const float* v, int) { add_sums<E>(v, a.c, M, s, w); });
+  each([&](const float* v) { add_sums<E>(v, a.c, M, s, w); });
+  add_sums<1>(&end, a.c, M, s, w);
   s = wave_sum(s);
   w = wave_sum(w);
   __syncthreads();
   if (lane == 0) {
     red[0][wave] = s;
     red[1][wave] = w;
+  }
+  __shared__ int count_s;
+  __shared__ uint32_t group[64];
+  if constexpr (TOP) {
+    uint32_t of = score_key_asc(mine);
+#pragma unroll
+    for (int off = 1; off < 8; off <<= 1) of = max(of, static_cast<uint32_t>(__shfl_xor(of, off)));
+    static_assert(kThreads == 8 * 64, "64 groups of 8 lanes");
+    if ((tid & 7) == 0) group[tid >> 3] = of;
+    if (tid == 0) count_s = 0;
   }
   __syncthreads();
   s = w = 0.f;
@@ -170,13 +200,12 @@ __global__ __launch_bounds__(kThreads) void logp_kernel(LogpArgs a) {
     s += red[0][i];
     w += red[1][i];
   }
-  // x = -inf alone: every 2^t is exp2(kLowest) = 0, s = 0
+  // x = -inf alone: every 2^t is 0, s = 0
   const float ls = __log2f(s);
   if (tid == 0) {
-    const int64_t t = a.tokens[row];
-    const bool given = t >= 0 && t < a.V;
+    const int64_t token = a.tokens[row];
     float lp = 0.f;
-    if (given) lp = s == 0.f ? -INFINITY : (to_f32(x[t]) - M) * a.inv_t - ls * kLn2;
+    if (token >= 0 && token < a.V) lp = s == 0.f ? -INFINITY : (to_f32(x[token]) - M) * a.inv_t - ls * kLn2;
     a.logp[row] = lp;
     a.entropy[row] = s == 0.f ? 0.f : (ls - w / s) * kLn2;
     if (a.stats) {
@@ -185,43 +214,60 @@ __global__ __launch_bounds__(kThreads) void logp_kernel(LogpArgs a) {
     }
   }
   if constexpr (TOP) {
-    __shared__ uint32_t bound_s;
-    __shared__ int count_s;
-    __shared__ uint32_t group[64];
     __shared__ uint64_t list[kCandidates];
-    uint32_t key = nan ? 0xffffffffu : score_key_asc(mine);
-#pragma unroll
-    for (int off = 1; off < kThreads / 64; off <<= 1) key = max(key, static_cast<uint32_t>(__shfl_xor(key, off)));
-    if (tid % (kThreads / 64) == 0) group[tid / (kThreads / 64)] = key;
-    if (tid == 0) count_s = 0;
-    __syncthreads();
-    if (wave == 0) {  // the K-th largest of the 64 (equal ones by their place)
-      const uint32_t g = group[lane];
-      int above = 0;
-#pragma unroll 8
-      for (int i = 0; i < 64; ++i) above += group[i] > g || (group[i] == g && i < lane);
-      if (above == a.K - 1) bound_s = g;
-    }
-    __syncthreads();
-    const uint32_t bound = bound_s;
-    each([&](const float* v, int e0) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int e = e0 + i;
-        if (score_key_asc(v[i]) >= bound && e >= 0 && e < a.V) {
-          const int at = atomicAdd(&count_s, 1);
-          if (at < kCandidates) list[at] = rank_key(v[i], e);
-        }
-      }
-    });
-    __syncthreads();
-    const int count = count_s;
     auto put = [&](int place, uint64_t k) {
       const int e = static_cast<int>(0xffffffffu - static_cast<uint32_t>(k));
       a.top_tokens[row * a.K + place] = e;
       a.top[row * a.K + place] = s == 0.f ? -INFINITY : (to_f32(x[e]) - M) * a.inv_t - ls * kLn2;
     };
-    if (count <= kCandidates) {
+    int count = kCandidates + 1;
+    if (s == s) {
+      const float bound = score_of_key(kth_of_wave(group[lane], a.K));
+      auto offer = [&](float v, int e) {
+        if (v >= bound) {
+          const int at = atomicAdd(&count_s, 1);
+          if (at < kCandidates) list[at] = rank_key(v, e);
+        }
+      };
+      auto offer_piece = [&](int at) {
+        float v[E];
+        load16<T>(x + pieces.element(at), v);
+#pragma unroll
+        for (int i = 0; i < E; ++i) offer(v[i], pieces.element(at) + i);
+      };
+      if (mine >= bound) {
+        if (pieces.own >= 0) offer(end, pieces.own);
+        if constexpr (NCH > 0) {
+          uint32_t hits = 0;  // pieces that reach the bound: few
+#pragma unroll
+          for (int i = 0; i < NCH; ++i) {
+            float v[E];
+            unpack16<T>(raw[i], v);
+            hits |= (max_of<E>(v) >= bound ? 1u : 0u) << i;
+          }
+          for (; hits != 0; hits &= hits - 1) {
+            const int at = pieces.first + (__ffs(hits) - 1) * kThreads + tid;
+            if (at < pieces.last) offer_piece(at);  // where the bound is -inf, what was never loaded reaches it
+          }
+        } else {
+          for (int at = pieces.first + tid; at < pieces.last; at += kThreads) offer_piece(at);
+        }
+      }
+      __syncthreads();
+      count = count_s;
+    }
+    if (count <= 64) {  // the usual case: one wave ranks them, a candidate in each lane
+      if (wave == 0) {
+        const uint64_t k = lane < count ? list[lane] : 0;
+        int above = 0;
+        for (int j = 0; j < count; ++j) {
+          const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(k >> 32), j);
+          const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(k), j);
+          above += ((static_cast<uint64_t>(hi) << 32) | lo) > k;
+        }
+        if (lane < count && above < a.K) put(above, k);
+      }
+    } else if (count <= kCandidates) {
       for (int i = tid; i < count; i += kThreads) {
         const uint64_t k = list[i];
         int above = 0;
@@ -290,21 +336,23 @@ __global__ __launch_bounds__(kGradThreads) void logp_grad_kernel(LogpGradArgs a)
   const float scale = none ? 0.f : -a.inv_t / s;
   const float A = scale * (g_all + (none ? 0.f : g_h * (a.entropy[row] - kLn2 * __log2f(s)))), B = scale * kLn2 * g_h;
   auto slope = [&](float v) {
-    const float t = (v - M) * a.c, u = t < kLowest ? kLowest : t;
-    return __builtin_amdgcn_exp2f(u) * fmaf(B, u, A);
+    const float t = (v - M) * a.c;
+    return __builtin_amdgcn_exp2f(t) * fmaf(B, fmaxf(t, kLowest), A);
   };
-  const int begin = part * kGradThreads * kGradPieces;
+  // whole pieces; the ends of the row are the last part's
+  const int begin = pieces.first + part * kGradThreads * kGradPieces;
   uint4 raw[kGradPieces];
 #pragma unroll
   for (int i = 0; i < kGradPieces; ++i) {
     const int at = begin + i * kGradThreads + tid;
-    if (at < pieces.count) raw[i] = pieces.template load<true>(at);
+    if (at < pieces.last) raw[i] = ld16raw<true>(x + pieces.element(at));
   }
+  auto value = [&](float v, int64_t e) { return slope(v) + (e == token && !none ? g_lp * a.inv_t : 0.f); };
   const int token_piece = given ? static_cast<int>((token + pieces.shift) / E) : -1;
 #pragma unroll
   for (int i = 0; i < kGradPieces; ++i) {
-    const int at = begin + i * kGradThreads + tid, e = at * E - pieces.shift;
-    if (at >= pieces.count) continue;
+    const int at = begin + i * kGradThreads + tid, e = pieces.element(at);
+    if (at >= pieces.last) continue;
     float v[E];
     unpack16<T>(raw[i], v);
 #pragma unroll
@@ -313,22 +361,24 @@ __global__ __launch_bounds__(kGradThreads) void logp_grad_kernel(LogpGradArgs a)
 #pragma unroll
       for (int k = 0; k < E; ++k) v[k] += e + k == token ? g_lp * a.inv_t : 0.f;
     }
-    if (VEC && e >= 0 && e + E <= a.V) {
+    if constexpr (VEC) {
       store16<T, true>(out + e, v);
     } else {
 #pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (e + k >= 0 && e + k < a.V) out[e + k] = from_f32<T>(v[k]);
+      for (int k = 0; k < E; ++k) out[e + k] = from_f32<T>(v[k]);
     }
   }
+  if (part == a.parts - 1 && pieces.own >= 0) out[pieces.own] = from_f32<T>(value(pieces.end(), pieces.own));
   if (a.g_top && !none) {  // the alternatives' own values once more, whole
     __syncthreads();
     for (int k = tid; k < a.K; k += kGradThreads) {
       const int64_t e = a.top_tokens[row * a.K + k];
+      if (e < 0 || e >= a.V) continue;
       const int64_t at = (e + pieces.shift) / E;
-      if (e < 0 || e >= a.V || at < begin || at >= begin + kGradThreads * kGradPieces) continue;
-      const float own = a.g_top[row * a.K + k] + (e == token ? g_lp : 0.f);
-      out[e] = from_f32<T>(slope(to_f32(x[e])) + own * a.inv_t);
+      // whose is it: a whole piece's part, or the last part's end of the row
+      const bool piece = at >= pieces.first && at < pieces.last;
+      if (piece ? at < begin || at >= begin + kGradThreads * kGradPieces : part != a.parts - 1) continue;
+      out[e] = from_f32<T>(value(to_f32(x[e]), e) + a.g_top[row * a.K + k] * a.inv_t);
     }
   }
 }
@@ -339,10 +389,11 @@ bool good_temperature(float t) { return t > 0.f && t < INFINITY && kLog2e / t < 
 template <typename T, bool TOP>
 int launch_logp(const LogpArgs& a, int64_t rows, hipStream_t st) {
   constexpr int E = Vec<T>::N;
-  const int64_t most = (static_cast<int64_t>(a.V) + 2 * E - 2) / E;  // pieces, wherever a row starts
+  const int64_t most = a.V / E;  // whole pieces
   const dim3 grid(static_cast<unsigned>(rows));
 #define HYDRA_LOGP(N) logp_kernel<T, N, TOP><<<grid, kThreads, 0, st>>>(a)
   if (most <= 2 * kThreads) HYDRA_LOGP(2);
+  else if (most <= 4 * kThreads) HYDRA_LOGP(4);
   else if (most <= 8 * kThreads) HYDRA_LOGP(8);
   else if (most <= 16 * kThreads) HYDRA_LOGP(16);
   else if (most <= 32 * kThreads) HYDRA_LOGP(32);
@@ -395,8 +446,8 @@ extern "C" int hydra_token_logprobs_bwd(const void* logits, int64_t rows, int64_
   HYDRA_REQUIRE(logits && tokens && stats && entropy && grad && (!g_top || top_tokens),
                 "token_logprobs_bwd: null pointer");
   HYDRA_REQUIRE(reinterpret_cast<uintptr_t>(logits) % e == 0, "token_logprobs_bwd: misaligned logits");
-  const int64_t most = (vocab + 2 * (16 / e) - 2) / (16 / e);
-  const int64_t parts = (most + kGradThreads * kGradPieces - 1) / (kGradThreads * kGradPieces);
+  const int64_t most = vocab / (16 / e);  // whole pieces
+  const int64_t parts = most == 0 ? 1 : (most + kGradThreads * kGradPieces - 1) / (kGradThreads * kGradPieces);
   HYDRA_REQUIRE(rows * parts < (int64_t(1) << 31), "token_logprobs_bwd: too large");
   const LogpGradArgs a{logits, logits_rs, tokens, stats, entropy, g_logprobs, g_entropy, g_top, top_tokens, grad,
                        static_cast<int>(vocab), static_cast<int>(top_k), static_cast<int>(parts),
