@@ -4,6 +4,7 @@ here; strides, pointers and the current stream go to the library."""
 from __future__ import annotations
 
 import ctypes
+import functools
 import operator
 import threading
 import weakref
@@ -273,6 +274,18 @@ def _check_ring(name: str, ring: torch.Tensor, W: int, dtype: torch.dtype) -> No
                          f"{tuple(ring.shape)}")
 
 
+@functools.lru_cache(maxsize=256)
+def _packed_shapes(conv_ks: int, L: int, K: int, head_dim: int, tiled: bool):
+    """Shapes of the packed conv weights (wq1, wq2, wk1, wk2)."""
+    exp = [(conv_ks, L, head_dim), (conv_ks, L, L), (conv_ks, K, head_dim), (conv_ks, K, K)]
+    return [(conv_ks, o // 32, i // 16, 2, 32, 8) for _, o, i in exp] if tiled else exp
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_workspace(*sizes) -> int:
+    return _lib.query("hydra_ccgqa_decode_prep_workspace", *sizes)
+
+
 def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                       k_pages: torch.Tensor, v_pages: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
                       flags: int, wq1=None, wq2=None, wk1=None, wk2=None, temperature=None, cos=None, sin=None,
@@ -314,16 +327,13 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
         ws = (wq1, wq2, wk1, wk2)
         tiled = bool(flags & CCGQA_W_TILED)
         if packed:
-            ws = tuple(w.to(dt).contiguous() for w in ws)
+            ws = tuple(w if w.dtype == dt and w.is_contiguous() else w.to(dt).contiguous() for w in ws)
         elif tiled:
             ws = pack_conv_weights_tiled(ws, dt, n_heads, n_kv_heads, head_dim)
         else:
             ws = tuple(pack_conv_weight(w, dt) for w in ws)
-        exp = [(conv_ks, L, head_dim), (conv_ks, L, L), (conv_ks, K, head_dim), (conv_ks, K, K)]
-        if tiled:
-            exp = [(conv_ks, o // 32, i // 16, 2, 32, 8) for _, o, i in exp]
-        for w, e in zip(ws, exp):
-            if tuple(w.shape) != e:
+        for w, e in zip(ws, _packed_shapes(conv_ks, L, K, head_dim, tiled)):
+            if w.shape != e:
                 raise ValueError(f"{name}: packed conv weight shape {tuple(w.shape)} != {e}")
         wq1, wq2, wk1, wk2 = ws
     else:
@@ -332,7 +342,7 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     if flags & CCGQA_QK_NORM:
         if temperature is None or temperature.numel() != 1:
             raise ValueError(f"{name}: QK-norm needs a temperature of one element")
-        temp = temperature.detach().to(dt).contiguous()
+        temp = temperature if temperature.dtype == dt else temperature.detach().to(dt)
     rope_rs = rope_rows = 0
     if flags & CCGQA_ROPE:
         rope_rows = min(t.shape[-2] for t in (cos, sin))
@@ -343,9 +353,8 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     else:
         cos = sin = None
     positions, slots = positions.contiguous(), slots.contiguous()
-    q = torch.empty((N, n_heads, head_dim), dtype=dt, device=qkv.device)
-    need = _lib.query("hydra_ccgqa_decode_prep_workspace", N, n_heads, n_kv_heads, head_dim, conv_ks, flags,
-                      _lib.dtype_code(qkv))
+    q = qkv.new_empty((N, n_heads, head_dim))
+    need = _decode_workspace(N, n_heads, n_kv_heads, head_dim, conv_ks, flags, _lib.dtype_code(qkv))
     ws = _lib.scratch(need, qkv) if need else None
     with _lib.on_device(qkv):
         _lib.call("hydra_ccgqa_decode_prep", qkv.data_ptr(), qkv.stride(0), ring.data_ptr(), ring.shape[1],

@@ -16,6 +16,7 @@ The reference has no cache (it recomputes the sequence for every token).
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -92,13 +93,10 @@ def _plan(name, lengths, new_tokens, table, free_pages, free_count, page_size, w
     width = int(width)
     if N == 0 or table.shape[1] == 0 or width < 1:
         raise ValueError(f"{name}: {N} requests, {table.shape[1]} pages each, width {width}")
-    lengths, new_tokens, free_pages = (t.contiguous() for t in (lengths, new_tokens, free_pages))
-    dev = lengths.device
-    slots = torch.empty((N, width), dtype=torch.int64, device=dev)
-    bytes_ = torch.empty(13 * N + 4, dtype=torch.uint8, device=dev)
-    ints = bytes_[:12 * N + 4].view(torch.int32)
-    granted = bytes_[12 * N + 4:].view(torch.bool)
-    after, seen, positions, left = ints[:N], ints[N:2 * N], ints[2 * N:3 * N], ints[3 * N:]
+    lengths, new_tokens, free_pages = lengths.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
+    slots = lengths.new_empty((N, width), dtype=torch.int64)
+    granted = lengths.new_empty((N,), dtype=torch.bool)
+    after, seen, positions, left = lengths.new_empty((3 * N + 1,)).split((N, N, N, 1))
     if in_place:
         after, left = lengths, free_count
     with _lib.on_device(lengths):
@@ -171,6 +169,14 @@ def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
                   _strides(v_pages), _lib.dtype_code(k), _lib.stream(k))
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(device: int, *sizes) -> int:
+    """Scratch bytes of these sizes on a device, which is current."""
+    need = ctypes.c_int64(0)
+    _lib.call("hydra_paged_attn_workspace", *sizes, ctypes.byref(need))
+    return need.value
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                     lengths: torch.Tensor, scale: Optional[float] = None,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -202,19 +208,18 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.stride(-1) != 1 and hd > 1:
         q = q.contiguous()
     if out is None:
-        out = torch.empty((N, H, hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((N, H, hd))
     elif out.shape != q.shape or out.dtype != q.dtype or (out.stride(-1) != 1 and hd > 1):
         raise ValueError(f"{name}: out must be {q.dtype} {tuple(q.shape)} with a unit last stride")
     lengths = lengths.contiguous()
     P, code = table.shape[1], _lib.dtype_code(q)
     with _lib.on_device(q):
-        need = ctypes.c_int64(0)
-        _lib.call("hydra_paged_attn_workspace", N, H, K, hd, P, page, code, ctypes.byref(need))
-        ws = _lib.scratch(need.value, q) if need.value else None
+        need = _attention_workspace(q.device.index, N, H, K, hd, P, page, code)
+        ws = _lib.scratch(need, q) if need else None
         _lib.call("hydra_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
                   table.data_ptr(), table.stride(0), lengths.data_ptr(), N, H, K, hd, P, page, pages, _strides(q),
                   _strides(k_pages), _strides(v_pages), _strides(out), hd ** -0.5 if scale is None else float(scale),
-                  code, _lib.ptr(ws), need.value, _lib.stream(q))
+                  code, _lib.ptr(ws), need, _lib.stream(q))
     return out
 
 

@@ -24,18 +24,23 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor
 
 
-def _forward(x, rows, stride, tokens, top_k, temperature, want_stats):
-    V, dev = x.shape[-1], x.device
-    out = torch.empty((4 if want_stats else 2, rows), dtype=torch.float32, device=dev)
-    logp, entropy = out[0], out[1]
-    stats = out[2:] if want_stats else None
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+def _forward(logits, tokens, top_k, temperature, want_stats):
+    """(logits as rows, their number and stride, tokens in rows, the four
+    results, stats)."""
+    x, (rows, stride) = _as_rows(logits)
+    if x.dim() > 1 and stride < x.shape[-1] and rows > 1:  # rows that overlap: broadcast ones
+        x, (rows, stride) = _as_rows(logits.contiguous())
+    tokens = tokens.reshape(-1)
+    lead = logits.shape[:-1]
+    logp, entropy = (x.new_empty(lead, dtype=torch.float32) for _ in range(2))
+    top = x.new_empty((*lead, top_k), dtype=torch.float32)
+    ids = x.new_empty((*lead, top_k), dtype=torch.int64)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     with _lib.on_device(x):
-        _lib.call("hydra_token_logprobs", x.data_ptr(), rows, V, stride, tokens.data_ptr(), temperature, top_k,
-                  logp.data_ptr(), entropy.data_ptr(), _lib.ptr(stats), top.data_ptr(), ids.data_ptr(),
+        _lib.call("hydra_token_logprobs", x.data_ptr(), rows, x.shape[-1], stride, tokens.data_ptr(), temperature,
+                  top_k, logp.data_ptr(), entropy.data_ptr(), _lib.ptr(stats), top.data_ptr(), ids.data_ptr(),
                   _lib.dtype_code(x), _lib.stream(x))
-    return logp, entropy, top, ids, stats
+    return x, rows, stride, tokens, (logp, entropy, top, ids), stats
 
 
 class _TokenLogprobsFunction(torch.autograd.Function):
@@ -44,15 +49,11 @@ class _TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature):
         ctx.set_materialize_grads(False)
-        x, (rows, stride) = _as_rows(logits)
-        tokens = tokens.reshape(-1)
-        logp, entropy, top, ids, stats = _forward(x, rows, stride, tokens, top_k, temperature, True)
-        ctx.save_for_backward(x, tokens, stats, entropy, ids)
+        x, _, _, tokens, out, stats = _forward(logits, tokens, top_k, temperature, True)
+        ctx.save_for_backward(x, tokens, stats, out[1], out[3])
         ctx.meta = (top_k, temperature)
-        lead = logits.shape[:-1]
-        ids = ids.view(*lead, top_k)
-        ctx.mark_non_differentiable(ids)
-        return logp.view(lead), entropy.view(lead), top.view(*lead, top_k), ids
+        ctx.mark_non_differentiable(out[3])
+        return out
 
     @staticmethod
     @once_differentiable
@@ -98,7 +99,4 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
         raise ValueError(f"{name}: temperature must be positive and finite, got {temperature}")
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobsFunction.apply(logits, tokens, top_k, temperature))
-    x, (rows, stride) = _as_rows(logits.detach())
-    lead = logits.shape[:-1]
-    logp, entropy, top, ids, _ = _forward(x, rows, stride, tokens.reshape(-1), top_k, temperature, False)
-    return TokenLogprobs(logp.view(lead), entropy.view(lead), top.view(*lead, top_k), ids.view(*lead, top_k))
+    return TokenLogprobs(*_forward(logits, tokens, top_k, temperature, False)[4])
