@@ -120,10 +120,12 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
       a.granted[i] = granted;
       a.positions[i] = static_cast<int>(s_len[at]);
     }
-    for (int at = 0; at < end - begin; ++at) {
-      if (s_add[at] < 0) continue;
-      int* row = a.table + (begin + at) * a.table_rs;
-      for (int j = tid; j < s_need[at]; j += kPlanThreads) row[s_have[at] + j] = a.free_pages[s_first[at] - j];
+    // new pages: at most this many a request
+    const unsigned most = (a.width >> a.shift) + 2, all = (end - begin) * most;
+    for (unsigned e = tid; e < all; e += kPlanThreads) {
+      const int at = e / most, j = e - at * most;
+      if (s_add[at] >= 0 && j < s_need[at])
+        a.table[(begin + at) * a.table_rs + s_have[at] + j] = a.free_pages[s_first[at] - j];
     }
     if (blockIdx.x == gridDim.x - 1) {  // it went over every request
       int most = taken;
@@ -138,19 +140,26 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
     }
   }
   const int j0 = blockIdx.y * kPlanTokens, j1 = min(a.width, j0 + kPlanTokens);
-  const int64_t count = static_cast<int64_t>(end - begin) * (j1 - j0);
   const int64_t low = (int64_t(1) << a.shift) - 1;
-  for (int64_t e = tid; e < count; e += kPlanThreads) {
-    const int at = static_cast<int>(e / (j1 - j0)), j = j0 + static_cast<int>(e - static_cast<int64_t>(at) * (j1 - j0));
-    int64_t slot = -1;
-    if (j < s_add[at]) {
-      const int64_t t = s_len[at] + j;
-      const int col = static_cast<int>(t >> a.shift);
-      const int page = col >= s_have[at] ? a.free_pages[s_first[at] - (col - s_have[at])]
-                                         : a.table[(begin + at) * a.table_rs + col];
-      if (page >= 0) slot = (static_cast<int64_t>(page) << a.shift) | (t & low);
+  auto slot_of = [&](int at, int j) -> int64_t {
+    if (j >= s_add[at]) return -1;
+    const int64_t t = s_len[at] + j;
+    const int col = static_cast<int>(t >> a.shift);
+    const int page = col >= s_have[at] ? a.free_pages[s_first[at] - (col - s_have[at])]
+                                       : a.table[(begin + at) * a.table_rs + col];
+    return page >= 0 ? (static_cast<int64_t>(page) << a.shift) | (t & low) : -1;
+  };
+  if (a.slice == 1) {
+    int64_t* row = a.slots + static_cast<int64_t>(begin) * a.width;
+#pragma unroll 4
+    for (int j = j0 + tid; j < j1; j += kPlanThreads) row[j] = slot_of(0, j);
+  } else {  // whole rows of several requests, one after the other
+    const unsigned width = a.width, count = (end - begin) * width;
+    int64_t* rows = a.slots + static_cast<int64_t>(begin) * a.width;
+    for (unsigned e = tid; e < count; e += kPlanThreads) {
+      const unsigned at = e / width;
+      rows[e] = slot_of(at, e - at * width);
     }
-    a.slots[static_cast<int64_t>(begin + at) * a.width + j] = slot;
   }
 }
 
