@@ -393,36 +393,55 @@ __global__ __launch_bounds__(kThreads) void paged_attn_split_kernel(PagedArgs a)
   __shared__ int pre[kMaxRequests + 1];
   __shared__ int wsum[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // prefix sums of the requests' rounds
-  int base = 0;
-  if (tid == 0) pre[0] = 0;
-  for (int i0 = 0; i0 < a.N; i0 += static_cast<int>(blockDim.x)) {
-    const int i = i0 + tid;
-    int s = wave_incl_sum(i < a.N ? rounds_of<LPR>(seen_keys(a, i)) : 0);
-    if (lane == 63) wsum[wave] = s;
-    __syncthreads();
-    int all = 0;
-    for (int w = 0; w < waves(); ++w) {
-      if (w < wave) s += wsum[w];
-      all += wsum[w];
+  // prefix sums of the requests' rounds: of up to 64 requests in each wave's lanes,
+  // of more in LDS
+  const bool few = a.N <= 64;
+  int base = 0, incl = 0;
+  if (few) {
+    incl = wave_incl_sum(lane < a.N ? rounds_of<LPR>(seen_keys(a, lane)) : 0);
+    base = __builtin_amdgcn_readlane(incl, 63);
+  } else {
+    if (tid == 0) pre[0] = 0;
+    for (int i0 = 0; i0 < a.N; i0 += static_cast<int>(blockDim.x)) {
+      const int i = i0 + tid;
+      int s = wave_incl_sum(i < a.N ? rounds_of<LPR>(seen_keys(a, i)) : 0);
+      if (lane == 63) wsum[wave] = s;
+      __syncthreads();
+      int all = 0;
+      for (int w = 0; w < waves(); ++w) {
+        if (w < wave) s += wsum[w];
+        all += wsum[w];
+      }
+      if (i < a.N) pre[i + 1] = base + s;
+      base += all;
+      __syncthreads();
     }
-    if (i < a.N) pre[i + 1] = base + s;
-    base += all;
-    __syncthreads();
   }
+  auto before = [&](int i) {  // rounds of the requests before i, wave-uniform
+    if (!few) return pre[i];
+    const int s = __builtin_amdgcn_readlane(incl, max(i - 1, 0));
+    return i == 0 ? 0 : s;
+  };
   const int HG = a.Hkv * a.GB, total = base * HG;
   // two rounds and more, for the sake of each share's end, unless that left CUs idle
   int per = (total + a.groups - 1) / a.groups;
   per = max(max(per, min(2, (total + a.cus - 1) / a.cus)), a.least);
   if (blockIdx.x == 0) {  // for the joining kernel
     if (tid == 0) a.plan[0] = per;
-    for (int i = tid; i <= a.N; i += static_cast<int>(blockDim.x)) a.plan[1 + i] = pre[i];
+    if (few) {
+      if (tid < a.N) a.plan[2 + tid] = incl;
+      if (tid == 0) a.plan[1] = 0;
+    } else {
+      for (int i = tid; i <= a.N; i += static_cast<int>(blockDim.x)) a.plan[1 + i] = pre[i];
+    }
   }
   // the last workgroup's range may pass int only if the total does (checked on the host)
   const int begin = min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total));
   const int end = min(static_cast<int64_t>(begin) + per, static_cast<int64_t>(total));
   int n = 0;
-  if (begin < end) {  // the last n with pre[n] HG <= begin
+  if (few) {  // requests that end before it
+    n = __popcll(__ballot(lane < a.N && incl * HG <= begin));
+  } else if (begin < end) {  // the last n with pre[n] HG <= begin
     int hi = a.N;
     while (hi - n > 1) {
       const int mid = (n + hi) >> 1;
@@ -430,8 +449,8 @@ __global__ __launch_bounds__(kThreads) void paged_attn_split_kernel(PagedArgs a)
     }
   }
   for (int u = begin; u < end;) {
-    while (pre[n + 1] * HG <= u) ++n;
-    const int r = pre[n + 1] - pre[n], at = u - pre[n] * HG, hg = at / r, t0 = at - hg * r;
+    while (before(n + 1) * HG <= u) ++n;
+    const int r = before(n + 1) - before(n), at = u - before(n) * HG, hg = at / r, t0 = at - hg * r;
     const int count = min(r - t0, end - u), h = hg / a.GB, gb = hg - h * a.GB;
     item_keys<T, GP, LPR, VEC>(a, n, h, gb, t0, t0 + count, sm);
     if (count == r) {
@@ -542,7 +561,7 @@ __global__ __launch_bounds__(1024) void paged_attn_join_kernel(PagedArgs a) {
 
 // ------------------------------------------------------------------- launch
 struct Shape {
-  int gp, lpr, kt;
+  int gp, lpr, kt, row;  // row: bytes of a key
   int64_t gb, items;
 };
 
@@ -558,6 +577,7 @@ inline Shape shape_of(int64_t N, int64_t H, int64_t Hkv, int64_t hd, int e) {
   s.lpr = 2;
   while (s.lpr * 16 < hd * e) s.lpr *= 2;
   s.kt = tile_keys(s.lpr);
+  s.row = static_cast<int>(hd) * e;
   s.items = N * Hkv * s.gb;
   return s;
 }
@@ -570,14 +590,14 @@ struct Split {
 constexpr int kMaxResident = 4;  // workgroups of a CU that a split launch takes at most
 
 // Split where the items alone would not fill the chip and a request may be longer
-// than 1024 keys (of head_dim 64 they take one workgroup of 8 waves 5 us more than
-// 128 keys; the joining launch takes 3 to 5).  8 waves only for few short items:
+// than 128 KB of keys or 2048 of them (1024 keys of 128 bytes take one workgroup of
+// 8 waves 5 us more than 128 of them; the joining launch takes 5).  8 waves only for few short items:
 // where items or rounds are many, twice as many workgroups of 4 have more of the
 // chip's registers in use (256 requests of 20 keys, 28/4 heads of 64: 13.4
 // against 23 us).
 inline Split split_of(const Shape& s, int64_t N, int64_t capacity) {
   Split r{};
-  r.on = N <= kMaxRequests && s.items < 8 * device_cus() && capacity > 1024;
+  r.on = N <= kMaxRequests && s.items < 8 * device_cus() && capacity > std::min<int64_t>(2048, (128 << 10) / s.row);
   r.waves = r.on || s.items > device_cus() ? 4 : kWaves;
   const int64_t most = (capacity + r.waves * s.kt - 1) / (r.waves * s.kt);
   r.on = r.on && most * s.items < (int64_t(1) << 31);
