@@ -240,6 +240,8 @@ class CCGQAAttention(nn.Module):
         if self.use_rope and pool.max_length > self.cos_cached.shape[2]:
             raise ValueError(f"CCGQAAttention: requests of up to {pool.max_length} tokens exceed the RoPE cache "
                              f"({self.cos_cached.shape[2]})")
+        if self.head_dim > 256:
+            raise ValueError(f"CCGQAAttention: a cache takes head_dim up to 256, not {self.head_dim}")
         if pool.table.device != w.device:
             raise RuntimeError(f"CCGQAAttention: the pool is on {pool.table.device}, the layer on {w.device}")
         return CCGQACache(self, pool, dtype or w.dtype)
@@ -271,20 +273,18 @@ class CCGQAAttention(nn.Module):
         if not plan.from_empty or plan.slots.shape[1] != S:
             raise ValueError(f"{name}: needs a plan with from_empty=True and width {S} (got width "
                              f"{plan.slots.shape[1]})")
-        slots, seen = plan.slots, plan.seen
         if rows is not None:
             if rows.dtype != torch.int64 or rows.shape != (M,):
                 raise ValueError(f"{name}: rows must be int64 [{M}], got {rows.dtype} {tuple(rows.shape)}")
-            slots, seen = slots.index_select(0, rows), seen.index_select(0, rows)
-        elif M != slots.shape[0]:
-            raise ValueError(f"{name}: {M} prompts for {slots.shape[0]} requests: say which (rows)")
+        elif M != plan.slots.shape[0]:
+            raise ValueError(f"{name}: {M} prompts for {plan.slots.shape[0]} requests: say which (rows)")
         if self.use_rope and S > self.cos_cached.shape[2]:
             raise ValueError(f"{name}: sequence length {S} exceeds the RoPE cache ({self.cos_cached.shape[2]})")
         qkv = F.linear(x, self.qkv_proj.weight)
         flags, convw = self._prep_args()
-        ccgqa_ring_fill(qkv, cache.ring, seen, decode_reach(flags, self.conv_kernel_size), rows)
+        ccgqa_ring_fill(qkv, cache.ring, plan.seen, decode_reach(flags, self.conv_kernel_size), rows)
         return self._forward_infer(x, qkv, flags, convw, None,
-                                   keep=lambda k, v: store_pages(k, v, cache.k_pages, cache.v_pages, slots))
+                                   keep=lambda k, v: store_pages(k, v, cache.k_pages, cache.v_pages, plan.slots, rows))
 
     @torch.no_grad()
     def decode(self, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan) -> torch.Tensor:
@@ -297,7 +297,7 @@ class CCGQAAttention(nn.Module):
         N = cache.ring.shape[0]
         if plan.slots.shape[1] != 1:
             raise ValueError(f"{name}: needs a plan of width 1 (got {plan.slots.shape[1]})")
-        if x.numel() != N * self.dim or x.shape[0] != N or x.dim() not in (2, 3):
+        if x.shape not in ((N, self.dim), (N, 1, self.dim)):
             raise ValueError(f"{name}: x must be [{N}, {self.dim}], got {tuple(x.shape)}")
         flags, convw = self._prep_args()
         tiled = self._tiled(x.dtype)

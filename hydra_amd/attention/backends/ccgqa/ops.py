@@ -17,7 +17,7 @@ from ...._lib import (CCGQA_CONVS, CCGQA_QK_MEAN, CCGQA_QK_NORM, CCGQA_ROPE, CCG
                       CCGQA_V_TRANSPOSED, CCGQA_VALUE_SHIFT, CCGQA_W_TILED, MASK_KEY_PADDING, MASK_NONE,
                       MASK_REFERENCE_SDPA)
 from .... import _lib
-from ...paged import check_pages
+from ...paged import check_no_gradient, check_pages
 
 
 def prep_flags(use_convs: bool, use_qk_mean: bool, use_value_shift: bool,
@@ -300,7 +300,8 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     (PagePlan.slots of a step of width 1).  A request whose slot lies outside
     the pool, or whose position is negative or past the RoPE tables, changes
     nothing and gets zeros for q.  Weights, temperature, tables and flags as
-    ccgqa_prep takes them.  fp32 inside, one rounding.  Inference only."""
+    ccgqa_prep takes them.  fp32 inside, one rounding.  Inference only: no
+    gradient."""
     name = "ccgqa_decode_prep"
     _lib.require_gpu(name, qkv, ring, positions, slots, k_pages, v_pages, wq1, wq2, wk1, wk2, temperature, cos, sin)
     L, K = n_heads * head_dim, n_kv_heads * head_dim
@@ -317,6 +318,7 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     if slots.dtype != torch.int64 or slots.numel() != N:
         raise ValueError(f"{name}: slots must be int64, one a request, got {slots.dtype} {tuple(slots.shape)}")
     check_pages(name, k_pages, v_pages)
+    check_no_gradient(name, qkv, ring, k_pages, v_pages)
     pages, _, page, _ = k_pages.shape
     if k_pages.shape[1] != n_kv_heads or k_pages.shape[3] != head_dim or k_pages.dtype != dt:
         raise ValueError(f"{name}: pages must be {dt} [pages, {n_kv_heads}, page_size, {head_dim}], got "
@@ -357,8 +359,8 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     need = _decode_workspace(N, n_heads, n_kv_heads, head_dim, conv_ks, flags, _lib.dtype_code(qkv))
     ws = _lib.scratch(need, qkv) if need else None
     with _lib.on_device(qkv):
-        _lib.call("hydra_ccgqa_decode_prep", qkv.data_ptr(), qkv.stride(0), ring.data_ptr(), ring.shape[1],
-                  positions.data_ptr(), slots.data_ptr(), _lib.ptr(wq1), _lib.ptr(wq2), _lib.ptr(wk1), _lib.ptr(wk2),
+        _lib.call("hydra_ccgqa_decode_prep", qkv.data_ptr(), qkv.stride(0) if N > 1 else W, ring.data_ptr(),
+                  ring.shape[1], positions.data_ptr(), slots.data_ptr(), _lib.ptr(wq1), _lib.ptr(wq2), _lib.ptr(wk1), _lib.ptr(wk2),
                   _lib.ptr(temp), _lib.ptr(cos), _lib.ptr(sin), rope_rs, rope_rows, q.data_ptr(), k_pages.data_ptr(),
                   v_pages.data_ptr(), _lib.strides(k_pages), _lib.strides(v_pages), pages, page, N, n_heads,
                   n_kv_heads, head_dim, conv_ks, flags, _lib.dtype_code(qkv), _lib.ptr(ws), need, _lib.stream(qkv))
@@ -368,15 +370,17 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
 def ccgqa_ring_fill(qkv: torch.Tensor, ring: torch.Tensor, lengths: torch.Tensor, keep: int,
                     rows: Optional[torch.Tensor] = None) -> None:
     """Keeps the last `keep` projected rows of prompts, qkv [M, S, W], in the
-    rings of their requests: prompt m has the length lengths[m] (int32; 0
-    leaves its ring as it is) and belongs to request rows[m] (int64, distinct;
-    None: m)."""
+    rings of their requests, ring [N, R, W].  Prompt m is request rows[m]
+    (int64, distinct; None: m) and lengths[request] (int32 [N]) tokens long; a
+    length of 0, one past S, or a row outside the ring leaves it as it is."""
     name = "ccgqa_ring_fill"
     _lib.require_gpu(name, qkv, ring, lengths, rows)
     M, S, W = qkv.shape
     _check_ring(name, ring, W, qkv.dtype)
-    if lengths.dtype != torch.int32 or lengths.shape != (M,):
-        raise ValueError(f"{name}: lengths must be int32 [{M}], got {lengths.dtype} {tuple(lengths.shape)}")
+    check_no_gradient(name, qkv, ring)
+    N = ring.shape[0]
+    if lengths.dtype != torch.int32 or lengths.shape != (N,):
+        raise ValueError(f"{name}: lengths must be int32 [{N}], got {lengths.dtype} {tuple(lengths.shape)}")
     if rows is not None and (rows.dtype != torch.int64 or rows.shape != (M,)):
         raise ValueError(f"{name}: rows must be int64 [{M}], got {rows.dtype} {tuple(rows.shape)}")
     if qkv.stride(-1) != 1:
@@ -384,8 +388,8 @@ def ccgqa_ring_fill(qkv: torch.Tensor, ring: torch.Tensor, lengths: torch.Tensor
     lengths, rows = lengths.contiguous(), None if rows is None else rows.contiguous()
     with _lib.on_device(qkv):
         _lib.call("hydra_ccgqa_ring_fill", qkv.data_ptr(), qkv.stride(0), qkv.stride(1), ring.data_ptr(),
-                  _lib.ptr(rows), lengths.data_ptr(), M, S, W, ring.shape[0], ring.shape[1], int(keep),
-                  _lib.dtype_code(qkv), _lib.stream(qkv))
+                  _lib.ptr(rows), lengths.data_ptr(), M, S, W, N, ring.shape[1], int(keep), _lib.dtype_code(qkv),
+                  _lib.stream(qkv))
 
 
 def _mask_bytes(key_mask: torch.Tensor) -> torch.Tensor:

@@ -66,15 +66,24 @@ def check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None
     if 0 in k_pages.shape:
         raise ValueError(f"{name}: an empty pool {tuple(k_pages.shape)}")
     for t in (k_pages, v_pages):
-        if t.is_contiguous():
-            continue
-        reach = 1  # elements that the dimensions up to here span
-        for size, stride in sorted(zip(t.shape, t.stride()), key=lambda d: d[1]):
-            if size > 1 and stride < reach:
-                raise ValueError(f"{name}: pages of strides {t.stride()} overlap")
-            reach += (size - 1) * stride
-        if t.stride(3) != 1 and t.shape[3] > 1:
-            raise ValueError(f"{name}: pages need rows of unit stride")
+        if not t.is_contiguous():
+            _check_distinct(name, "pages", t)
+
+
+def check_no_gradient(name: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name}: no gradient (call it under torch.no_grad())")
+
+
+def _check_distinct(name: str, what: str, t: torch.Tensor) -> None:
+    """A unit last stride, and no memory that two elements share."""
+    reach = 1  # elements that the dimensions up to here span
+    for size, stride in sorted(zip(t.shape, t.stride()), key=lambda d: d[1]):
+        if size > 1 and stride < reach:
+            raise ValueError(f"{name}: {what} of strides {t.stride()} overlap")
+        reach += (size - 1) * stride
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: {what} need rows of unit stride")
 
 
 def _strides(t: torch.Tensor):
@@ -127,7 +136,9 @@ def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Ten
 def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
                   free_count: torch.Tensor, page_size: int) -> None:
     """Puts the pages of the requests with `done` (bool [N]) back on the
-    stack, in place: their lengths become 0, their table entries -1."""
+    stack, in place: their lengths become 0, their table entries -1.  A page
+    belongs to one request: one that several tables name would come back more
+    than once."""
     name = "release_pages"
     _lib.require_gpu(name, done, lengths, table, free_pages, free_count)
     N = _vector(name, "lengths", lengths, torch.int32).shape[0]
@@ -147,26 +158,33 @@ def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
 
 
 def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                slots: torch.Tensor) -> None:
-    """Writes the rows k, v [N, Hkv, S, hd] to their slots (int64 [N, S];
-    distinct; -1, or any outside the pool, for rows that are not kept)."""
+                slots: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
+    """Writes the rows k, v [N, Hkv, S, hd] to their slots in the pool:
+    prompt n's are `slots[n]`, or `slots[rows[n]]`, of int64 [R, S] (distinct;
+    -1, or any outside the pool, for rows that are not kept).  rows: int64 [N],
+    distinct; a row outside the slots stores nothing.  The pages are none of
+    k's and v's memory.  Inference only: no gradient."""
     name = "store_pages"
-    _lib.require_gpu(name, k, v, k_pages, v_pages, slots)
+    _lib.require_gpu(name, k, v, k_pages, v_pages, slots, rows)
     check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
     if k.dim() != 4 or k.shape[1] != K or k.shape[3] != hd or v.shape != k.shape:
         raise ValueError(f"{name}: k and v must be [N, {K}, S, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
     if not k.dtype == v.dtype == k_pages.dtype:
         raise ValueError(f"{name}: k, v and the pages must share a dtype")
+    check_no_gradient(name, k, v, k_pages, v_pages)
     N, S = k.shape[0], k.shape[2]
-    if slots.dtype != torch.int64 or slots.shape != (N, S):
-        raise ValueError(f"{name}: slots must be int64 [{N}, {S}], got {slots.dtype} {tuple(slots.shape)}")
+    if slots.dtype != torch.int64 or slots.dim() != 2 or slots.shape[1] != S or (rows is None and slots.shape[0] != N):
+        raise ValueError(f"{name}: slots must be int64 [{'R' if rows is not None else N}, {S}], got {slots.dtype} "
+                         f"{tuple(slots.shape)}")
+    if rows is not None:
+        rows = _vector(name, "rows", rows, torch.int64, N).contiguous()
     k, v = (t if t.stride(-1) == 1 or hd == 1 else t.contiguous() for t in (k, v))
     slots = slots.contiguous()
     with _lib.on_device(k):
         _lib.call("hydra_page_store", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                  slots.data_ptr(), N, K, S, hd, pages, page, _strides(k), _strides(v), _strides(k_pages),
-                  _strides(v_pages), _lib.dtype_code(k), _lib.stream(k))
+                  slots.data_ptr(), slots.shape[0], _lib.ptr(rows), N, K, S, hd, pages, page, _strides(k), _strides(v),
+                  _strides(k_pages), _strides(v_pages), _lib.dtype_code(k), _lib.stream(k))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -183,7 +201,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """softmax(scale * q k^T) v of one query token per request, q [N, Hq, hd],
     over the first `lengths[i]` (int32) positions of its pages; query head h
     reads key head h // (Hq / Hkv).  scale: hd ** -0.5 by default.  `out`: a
-    [N, Hq, hd] tensor with a unit last stride to write to.
+    [N, Hq, hd] tensor with a unit last stride to write to (q itself is one).
 
     fp32 scores, softmax and sums, one rounding.  Lengths count within
     [0, P * page_size]; keys on a page outside the pool are not seen; a
@@ -199,8 +217,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"{name}: {H} query heads are no multiple of {K} key heads")
     if q.dtype != k_pages.dtype:
         raise ValueError(f"{name}: q and the pages must share a dtype")
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
-        raise RuntimeError(f"{name}: no gradient (call it under torch.no_grad())")
+    check_no_gradient(name, q, k_pages, v_pages)
     _vector(name, "lengths", lengths, torch.int32, N)
     _check_table(name, table, N)
     if table.shape[1] == 0:
@@ -209,8 +226,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         q = q.contiguous()
     if out is None:
         out = q.new_empty((N, H, hd))
-    elif out.shape != q.shape or out.dtype != q.dtype or (out.stride(-1) != 1 and hd > 1):
-        raise ValueError(f"{name}: out must be {q.dtype} {tuple(q.shape)} with a unit last stride")
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"{name}: out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+    elif not out.is_contiguous():
+        _check_distinct(name, "rows of out", out)
     lengths = lengths.contiguous()
     P, code = table.shape[1], _lib.dtype_code(q)
     with _lib.on_device(q):

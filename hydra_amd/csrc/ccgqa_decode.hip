@@ -639,17 +639,18 @@ int launch_decode(DecodeArgs a, hipStream_t st) {
   return check_launch("ccgqa_decode_prep");
 }
 
-// The last `keep` rows of prompts into the ring: qkv [M, S, W] (strides qs),
-// row s of prompt m, if lengths[m] - keep <= s < lengths[m], to
-// ring[rows[m]][s % R]; prompts with a length outside [0, S] or a row outside
-// the ring leave it as it is.
+// The last `keep` rows of prompts into the ring: qkv [M, S, W], prompt m being
+// request r = rows[m], row s if lengths[r] - keep <= s < lengths[r] to
+// ring[r][s % R].
 template <typename T>
 __global__ __launch_bounds__(256) void ring_fill_kernel(const T* qkv, int64_t bs, int64_t rs, T* ring,
                                                         const int64_t* rows, const int* lengths, int N, int R, int W,
-                                                        int S, int keep) {
-  const int m = blockIdx.y, len = lengths[m], s = len - 1 - static_cast<int>(blockIdx.x);
+                                                        int S) {
+  const int m = blockIdx.y;
   const int64_t row = rows ? rows[m] : m;
-  if (len > S || s < 0 || row < 0 || row >= N) return;
+  if (row < 0 || row >= N) return;
+  const int len = lengths[row], s = len - 1 - static_cast<int>(blockIdx.x);
+  if (len > S || s < 0) return;
   const T* from = qkv + m * bs + s * rs;
   T* to = ring + (row * R + s % R) * W;
   for (int c = threadIdx.x; c < W; c += 256) to[c] = from[c];
@@ -756,7 +757,7 @@ extern "C" int hydra_ccgqa_ring_fill(const void* qkv, int64_t qkv_bs, int64_t qk
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     ring_fill_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(qkv), qkv_bs, qkv_rs, static_cast<T*>(ring), rows,
                                               lengths, static_cast<int>(N), static_cast<int>(R), static_cast<int>(W),
-                                              static_cast<int>(S), static_cast<int>(keep));
+                                              static_cast<int>(S));
     return check_launch("ccgqa_ring_fill");
   });
 }

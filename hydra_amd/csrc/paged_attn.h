@@ -600,7 +600,7 @@ inline Split split_of(const Shape& s, int64_t N, int64_t capacity) {
   r.on = N <= kMaxRequests && s.items < 8 * device_cus() && capacity > std::min<int64_t>(2048, (128 << 10) / s.row);
   r.waves = r.on || s.items > device_cus() ? 4 : kWaves;
   const int64_t most = (capacity + r.waves * s.kt - 1) / (r.waves * s.kt);
-  r.on = r.on && most * s.items < (int64_t(1) << 31);
+  r.on = r.on && most * s.items < (int64_t(1) << 31) - (1 << 20);  // all rounds, and the workgroups, in an int
   r.least = static_cast<int>(std::max<int64_t>(1, (most + kMaxParts - 2) / (kMaxParts - 1)));
   return r;
 }

@@ -210,10 +210,10 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
 struct StoreArgs {
   const char *k, *v;
   char *kp, *vp;
-  const int64_t* slots;
+  const int64_t *slots, *rows;  // rows: n -> row of slots (null: n)
   int64_t ks[3], vs[3], kps[3], vps[3];  // strides in bytes: n/h/s, page/h/row
   int64_t limit;                         // slots of the pool
-  int N, H, S, pieces, shift;
+  int N, H, S, R, pieces, shift;
 };
 
 template <typename V>
@@ -224,7 +224,9 @@ __global__ __launch_bounds__(256) void store_kernel(StoreArgs a) {
   const int64_t piece = (e - s * a.pieces) * static_cast<int64_t>(sizeof(V));
   const int h = blockIdx.y;
   for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
-    const int64_t slot = a.slots[static_cast<int64_t>(n) * a.S + s];
+    const int64_t r = a.rows ? a.rows[n] : n;
+    if (r < 0 || r >= a.R) continue;
+    const int64_t slot = a.slots[r * a.S + s];
     if (slot < 0 || slot >= a.limit) continue;
     const int64_t page = slot >> a.shift, row = slot & ((int64_t(1) << a.shift) - 1);
     const V k = *reinterpret_cast<const V*>(a.k + n * a.ks[0] + h * a.ks[1] + s * a.ks[2] + piece);
@@ -302,15 +304,18 @@ extern "C" int hydra_page_release(const void* done, int* lengths, int* table, in
 }
 
 extern "C" int hydra_page_store(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots,
-                                int64_t N, int64_t Hkv, int64_t S, int64_t hd, int64_t pages, int64_t page_size,
-                                const int64_t* k_st, const int64_t* v_st, const int64_t* kp_st, const int64_t* vp_st,
+                                int64_t R, const int64_t* rows, int64_t N, int64_t Hkv, int64_t S, int64_t hd,
+                                int64_t pages, int64_t page_size, const int64_t* k_st, const int64_t* v_st, const int64_t* kp_st, const int64_t* vp_st,
                                 int dtype, void* stream) {
-  HYDRA_REQUIRE(N >= 0 && S >= 0 && Hkv >= 1 && hd >= 1 && pages >= 1, "page_store: bad size");
+  HYDRA_REQUIRE(N >= 0 && S >= 0 && R >= 0 && Hkv >= 1 && hd >= 1 && pages >= 1, "page_store: bad size");
+  HYDRA_REQUIRE(rows || R >= N, "page_store: fewer rows of slots than prompts");
   const int shift = page_shift(page_size);
   HYDRA_REQUIRE(shift >= 0, "page_store: page_size must be a power of two in [16, 4096]");
   const int e = dtype_size(dtype);
   HYDRA_REQUIRE(e > 0, "page_store: unknown dtype");
-  HYDRA_REQUIRE(N < (int64_t(1) << 31) && S < (int64_t(1) << 31) && Hkv <= 65535 && hd <= 65536, "page_store: too large");
+  HYDRA_REQUIRE(N < (int64_t(1) << 31) && R < (int64_t(1) << 31) && S < (int64_t(1) << 31) && Hkv <= 65535 &&
+                    hd <= 65536,
+                "page_store: too large");
   if (N == 0 || S == 0) return HYDRA_OK;
   HYDRA_REQUIRE(k && v && k_pages && v_pages && slots && k_st && v_st && kp_st && vp_st, "page_store: null pointer");
   HYDRA_REQUIRE(k_st[3] == 1 && v_st[3] == 1 && kp_st[3] == 1 && vp_st[3] == 1, "page_store: rows need unit stride");
@@ -320,6 +325,8 @@ extern "C" int hydra_page_store(const void* k, const void* v, void* k_pages, voi
   a.kp = static_cast<char*>(k_pages);
   a.vp = static_cast<char*>(v_pages);
   a.slots = slots;
+  a.rows = rows;
+  a.R = static_cast<int>(R);
   a.limit = pages * page_size;
   a.N = static_cast<int>(N);
   a.H = static_cast<int>(Hkv);

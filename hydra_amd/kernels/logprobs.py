@@ -85,7 +85,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     first.  Masked logits may be -inf or the type's lowest value; a row of -inf
     alone has log probabilities -inf, entropy 0 and no gradient; a row with a
     NaN or +inf has NaN.  The gradient covers logprobs, entropy and
-    top_logprobs (once differentiable)."""
+    top_logprobs (once differentiable); a captured backward belongs to a
+    captured forward, through torch.autograd.grad or leaves that no eager graph
+    shares."""
     name = "token_logprobs"
     _lib.require_gpu(name, logits, tokens)
     if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:

@@ -507,19 +507,21 @@ int hydra_page_release(const void* done, int* lengths, int* table, int64_t table
                        int64_t P, int64_t page_size, void* stream);
 
 /* Rows k, v [N, Hkv, S, hd] (element strides k_st[4], v_st[4]; unit last) to
- * the slots [N, S] of k_pages, v_pages [pages, Hkv, page_size, hd] (strides
- * kp_st[4], vp_st[4]; unit last).  A slot outside the pool takes nothing;
- * slots must be distinct. */
+ * their slots in k_pages, v_pages [pages, Hkv, page_size, hd] (strides kp_st[4],
+ * vp_st[4]; unit last): prompt n's are slots[rows[n]] of slots [R, S] (rows
+ * null: slots[n]).  A row outside [0, R) or a slot outside the pool stores
+ * nothing; slots must be distinct and the pages none of k's and v's memory. */
 int hydra_page_store(const void* k, const void* v, void* k_pages, void* v_pages,
-                     const int64_t* slots, int64_t N, int64_t Hkv, int64_t S, int64_t hd,
-                     int64_t pages, int64_t page_size, const int64_t* k_st, const int64_t* v_st,
-                     const int64_t* kp_st, const int64_t* vp_st, int dtype, void* stream);
+                     const int64_t* slots, int64_t R, const int64_t* rows, int64_t N, int64_t Hkv,
+                     int64_t S, int64_t hd, int64_t pages, int64_t page_size, const int64_t* k_st,
+                     const int64_t* v_st, const int64_t* kp_st, const int64_t* vp_st, int dtype,
+                     void* stream);
 
 /* Attention of one token per request over its pages:
  *   out[n,h] = softmax_t(scale * q[n,h] . k[t]) v[t], t < lengths[n],
  * key head h / (Hq / Hkv).  q, out: [N, Hq, hd] with strides q_st[3],
- * o_st[3]; pages as above; hd <= 256.  Lengths are taken within
- * [0, P * page_size]; keys on a page outside the pool are not seen; a request
+ * o_st[3]; pages as above; hd <= 256, P * page_size <= 2^30, a page's rows within
+ * 2 GiB.  Lengths are taken within [0, P * page_size]; keys on a page outside the pool are not seen; a request
  * that sees no key gets zeros.  Scores, softmax and the products with v are
  * fp32, one rounding into `dtype`.  Needs hydra_paged_attn_workspace bytes of
  * device scratch (16-byte aligned). */
@@ -543,8 +545,8 @@ int hydra_paged_attn_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t hd, i
  * ring.  A request with a slot outside the pool, a negative position or one
  * past the RoPE table's rope_rows changes nothing and gets zeros for q.
  * Weights, temperature, cos/sin and flags as in hydra_ccgqa_prep_fwd
- * (HYDRA_CCGQA_W_TILED: 16-bit, head_dim 16, 32, 64 or 128, three taps).  fp32
- * inside, one rounding. */
+ * (HYDRA_CCGQA_W_TILED: 16-bit, head_dim 16, 32, 64 or 128, three taps).  At most
+ * 65535 requests.  fp32 inside, one rounding. */
 int hydra_ccgqa_decode_prep(const void* qkv, int64_t qkv_rs, void* ring, int64_t R,
                             const int* positions, const int64_t* slots, const void* wq1,
                             const void* wq2, const void* wk1, const void* wk2,
@@ -560,9 +562,10 @@ int64_t hydra_ccgqa_decode_prep_workspace(int64_t N, int64_t Hq, int64_t Hkv, in
                                           int64_t conv_ks, int flags, int dtype);
 
 /* The last `keep` rows of prompts into such a ring: of qkv [M, S, W] (strides
- * qkv_bs, qkv_rs; unit columns) the rows s with lengths[m] - keep <= s <
- * lengths[m] to ring[rows[m], s % R] (rows null: m).  A prompt with a length
- * outside [0, S], or a row outside the ring, leaves it as it is. */
+ * qkv_bs, qkv_rs; unit columns), prompt m being request r = rows[m] (rows null:
+ * m) of the ring's N, the rows s with lengths[r] - keep <= s < lengths[r] to
+ * ring[r, s % R].  A request outside [0, N) or of a length outside [0, S]
+ * leaves the ring as it is. */
 int hydra_ccgqa_ring_fill(const void* qkv, int64_t qkv_bs, int64_t qkv_rs, void* ring,
                           const int64_t* rows, const int* lengths, int64_t M, int64_t S,
                           int64_t W, int64_t N, int64_t R, int64_t keep, int dtype, void* stream);

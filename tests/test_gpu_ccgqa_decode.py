@@ -176,19 +176,19 @@ def test_ring_fill(cuda, dtype):
 
     g = torch.Generator().manual_seed(0)
     qkv = torch.randn(5, 11, 48, generator=g).to(dtype)
-    lengths, rows = [0, 1, 3, 11, 12], [4, 0, 6, 2, 1]
+    lengths, rows = [1, 12, 11, 3, 0, 7, 2], [4, 0, 6, 2, 1]
+    lens = torch.tensor(lengths, dtype=torch.int32, device=cuda)
     for order in (None, rows):
         ring = torch.full((7, 6, 48), 3.0, dtype=dtype)
         got = ring.to(cuda)
-        ccgqa_ring_fill(qkv.to(cuda), got, torch.tensor(lengths, dtype=torch.int32, device=cuda), 4,
-                        None if order is None else torch.tensor(order, device=cuda))
-        for m, n in enumerate(lengths):
+        ccgqa_ring_fill(qkv.to(cuda), got, lens, 4, None if order is None else torch.tensor(order, device=cuda))
+        for m in range(5):
+            r = m if order is None else order[m]
+            n = lengths[r]
             for s in range(max(0, n - 4), n if n <= 11 else 0):
-                ring[m if order is None else order[m], s % 6] = qkv[m, s]
+                ring[r, s % 6] = qkv[m, s]
         assert torch.equal(got.cpu(), ring)
-    got = ring.to(cuda)
-    ccgqa_ring_fill(qkv.to(cuda), got, torch.full((5,), 3, dtype=torch.int32, device=cuda), 4,
-                    torch.tensor([-1, 7, 2**40, -2**40, 7], device=cuda))
+    ccgqa_ring_fill(qkv.to(cuda), got, lens, 4, torch.tensor([-1, 7, 2**40, -2**40, 7], device=cuda))
     assert torch.equal(got.cpu(), ring)
 
 
@@ -268,6 +268,9 @@ def test_prompts_join_a_running_batch(cuda):
     assert max_rel_err(out[0], want[2, :33]) < 1e-5
     plan = pool.plan(i32(5, 0, 0), width=5, from_empty=True)  # no page left
     assert plan.granted.tolist() == [False, True, True]
+    before = [t.clone() for t in (cache.k_pages, cache.v_pages, cache.ring)]
+    m.prefill(x[:3, :5].to(cuda), cache, plan, rows=torch.tensor([0, -1, 3], device=cuda))  # refused, no requests
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.k_pages, cache.v_pages, cache.ring)))
     for step in range(2):
         plan = pool.plan(i32(1, 1, 1))
         out = m.decode(torch.stack([x[3, 0], x[1, 30 + step], x[2, 33 + step]]).to(cuda), cache, plan)
@@ -349,7 +352,7 @@ def test_block_generates(cuda, dtype, tol):
 
 def test_refusals(cuda):
     from hydra_amd.attention import PagePool
-    from hydra_amd.attention.backends.ccgqa.ops import ccgqa_decode_prep
+    from hydra_amd.attention.backends.ccgqa.ops import ccgqa_decode_prep, ccgqa_ring_fill
 
     cfg, dtype = oc.CCGQAConfig(**CONFIGS["debug"]), torch.bfloat16
     m, params = layer(cuda, cfg, dtype, seed=1, max_seq_len=64)
@@ -370,8 +373,9 @@ def test_refusals(cuda):
         m.prefill(x, cache, empty, rows=i32(0, 1))
     with pytest.raises(ValueError, match="width 1"):
         m.decode(x[:, 0], cache, wide)
-    with pytest.raises(ValueError, match="x must be"):
-        m.decode(x[:1, 0], cache, one)
+    for bad in (x[:1, 0], x[:, :2], x[:, 0].view(2, 2, -1)):
+        with pytest.raises(ValueError, match="x must be"):
+            m.decode(bad, cache, one)
     with pytest.raises(ValueError, match="the cache"):
         m.decode(x[:, 0].float(), cache, one)
     with pytest.raises(ValueError, match="RoPE cache"):
@@ -397,3 +401,10 @@ def test_refusals(cuda):
                          (dict(conv_ks=5), "more than 8"), (dict(n_heads=7), "qkv must be")):
         with pytest.raises(ValueError, match=text):
             ccgqa_decode_prep(**{**good, **change})
+    for key in ("qkv", "ring", "k_pages"):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ccgqa_decode_prep(**{**good, key: good[key].clone().requires_grad_()})
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ccgqa_ring_fill(x[:, :, :1].expand(2, 8, cache.ring.shape[2]).clone().requires_grad_(), cache.ring, one.seen, 4)
+    none = m.prefill(x[:0], cache, empty, rows=torch.zeros(0, dtype=torch.long, device=cuda))
+    assert none.shape == (0, 8, cfg.dim)

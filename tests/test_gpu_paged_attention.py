@@ -142,6 +142,9 @@ def test_strides(cuda, dtype):
     buf = torch.full((6, 3, 40), 7.0, dtype=dtype, device=cuda)
     check(case, cuda, out=buf.transpose(0, 1)[..., 4:36])
     assert (buf[..., :4] == 7).all() and (buf[..., 36:] == 7).all()
+    inside = case[0].to(cuda)
+    got = check((inside.cpu(), *case[1:]), cuda, form=lambda q, k, v, t: (inside, k, v, t), out=inside)
+    assert got.data_ptr() == inside.data_ptr()
 
 
 def test_same_bits_again_and_on_another_stream(cuda):
@@ -214,7 +217,9 @@ def test_refusals(cuda):
                        ((q, kp, vp, table, lengths.long()), "lengths"), ((q, kp, vp, table, lengths[:1]), "lengths"),
                        ((q, kp, vp, table[:, :0], lengths), "without pages"),
                        ((q, kp[:, :, :8], vp[:, :, :8], table, lengths), "power of two"),
-                       ((q, kp, vp, table, lengths, None, q[:, :2]), "out must be")):
+                       ((q, kp, vp, table, lengths, None, q[:, :2]), "out must be"),
+                       ((q, kp, vp, table, lengths, None, q[:1].expand(2, 4, 16)), "overlap"),
+                       ((q, kp, vp, table, lengths, None, q.mT.contiguous().mT), "unit stride")):
         with pytest.raises(ValueError, match=text):
             paged_attention(*args)
     with pytest.raises(TypeError, match="dtype"):

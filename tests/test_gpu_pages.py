@@ -173,6 +173,29 @@ def test_store(cuda, dtype, N, K, S, hd, page):
         assert torch.equal(got[0].cpu(), kp) and torch.equal(got[1].cpu(), vp), name
 
 
+def test_store_by_rows(cuda):
+    """Prompts that belong to some of the requests, in any order; rows outside
+    the slots store nothing."""
+    from hydra_amd.attention import store_pages
+
+    g = torch.Generator().manual_seed(3)
+    slots = torch.randperm(160, generator=g)[:70].view(7, 10)
+    k, v = (torch.randn(5, 2, 10, 8, generator=g) for _ in range(2))
+    kp, vp = (torch.zeros(10, 2, 16, 8) for _ in range(2))
+    got = kp.to(cuda), vp.to(cuda)
+    rows = [6, -1, 2, 7, 0]
+    store_pages(k.to(cuda), v.to(cuda), *got, slots.to(cuda), rows=torch.tensor(rows, device=cuda))
+    for n, r in enumerate(rows):
+        for s in range(10 if 0 <= r < 7 else 0):
+            slot = int(slots[r, s])
+            kp[slot // 16, :, slot % 16] = k[n, :, s]
+            vp[slot // 16, :, slot % 16] = v[n, :, s]
+    assert torch.equal(got[0].cpu(), kp) and torch.equal(got[1].cpu(), vp)
+    for bad in (torch.zeros(4, dtype=torch.long, device=cuda), torch.zeros(5, dtype=torch.int32, device=cuda)):
+        with pytest.raises(ValueError, match="rows"):
+            store_pages(k.to(cuda), v.to(cuda), *got, slots.to(cuda), rows=bad)
+
+
 def test_refusals(cuda):
     from hydra_amd.attention import plan_pages, release_pages, store_pages
 
@@ -201,3 +224,8 @@ def test_refusals(cuda):
                          kv[:, :, :12].transpose(2, 3)[..., :6], slots), "must be|unit stride")):
         with pytest.raises(ValueError, match=text):
             store_pages(*args)
+    for i in range(4):
+        args = [rows, rows, kv, kv]
+        args[i] = args[i].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            store_pages(*args, slots)

@@ -31,7 +31,7 @@ def test_page_size_is_a_power_of_two_in_range(page):
         _lib.call("hydra_page_release", FAKE, FAKE, FAKE, 4, FAKE, 8, FAKE, 2, 4, page, None)
     s = st(1, 1, 1, 1)
     with pytest.raises(ValueError, match="power of two"):
-        _lib.call("hydra_page_store", FAKE, FAKE, FAKE, FAKE, FAKE, 1, 1, 1, 16, 4, page, s, s, s, s, 1, None)
+        _lib.call("hydra_page_store", FAKE, FAKE, FAKE, FAKE, FAKE, 1, None, 1, 1, 1, 16, 4, page, s, s, s, s, 1, None)
     need = ctypes.c_int64(0)
     with pytest.raises(ValueError, match="power of two"):
         _lib.call("hydra_paged_attn_workspace", 1, 1, 1, 16, 4, page, 1, ctypes.byref(need))
