@@ -78,8 +78,9 @@ __device__ __forceinline__ int block_incl_sum(int x, int* part, int& total) {
 // taken from the stack by index, so the table's new entries are written by one
 // workgroup and read by none.
 //
-// Bound by its launch and the chain of the sums at a decoding step, by the
-// slots' writes for prompts.
+// Bound by its launch and the chain lengths -> sums -> stack -> slots at a decoding
+// step (32 requests: 3.6 us), by the slots' writes for prompts (256 of 4096
+// tokens, 8 MB: 7.2 us).
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
   __shared__ int part[kPlanThreads / 64];
   __shared__ int s_first[kPlanThreads], s_have[kPlanThreads], s_need[kPlanThreads];
@@ -165,12 +166,15 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 
 // The pages of the requests that are done go back on the stack, in the order
 // of the requests; their lengths become 0 and their table entries -1.  One
-// workgroup: the stack has one top.
+// workgroup: the stack has one top.  Its threads take the pages of 256 requests
+// in their order on the stack and look up whose each is; bound by the launch and
+// the chain lengths -> sums -> table -> stack: 2 us
+// behind another kernel for 32 of 256 requests with 16 pages each.
 __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* done, int* lengths, int* table,
                                                                int64_t table_rs, int* free_pages, int* free_count,
                                                                int N, int P, int F, int shift) {
   __shared__ int part[kPlanThreads / 64];
-  __shared__ int s_first[kPlanThreads], s_count[kPlanThreads];
+  __shared__ int s_upto[kPlanThreads];
   const int tid = threadIdx.x;
   int free = *free_count;
   free = free < 0 ? 0 : (free > F ? F : free);
@@ -185,16 +189,16 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
     }
     int step;
     const int upto = block_incl_sum(count, part, step);
-    s_first[tid] = free + upto - count;
-    s_count[tid] = count;
+    s_upto[tid] = upto;
     __syncthreads();
-    for (int at = tid >> 6; at < kPlanThreads; at += kPlanThreads / 64) {
-      int* row = table + static_cast<int64_t>(i0 + at) * table_rs;
-      for (int j = tid & 63; j < s_count[at]; j += 64) {
-        const int to = s_first[at] + j;
-        if (to < F) free_pages[to] = row[j];
-        row[j] = -1;
-      }
+    for (int e = tid; e < step; e += kPlanThreads) {
+      int at = 0;  // the first request with s_upto > e
+#pragma unroll
+      for (int half = kPlanThreads / 2; half > 0; half >>= 1)
+        if (s_upto[at + half - 1] <= e) at += half;
+      int* entry = table + static_cast<int64_t>(i0 + at) * table_rs + (e - (at > 0 ? s_upto[at - 1] : 0));
+      if (free + e < F) free_pages[free + e] = *entry;
+      *entry = -1;
     }
     free = min(F, free + step);
     __syncthreads();
@@ -202,37 +206,64 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
   if (tid == 0) *free_count = free;
 }
 
-// Rows k, v [N, Hkv, S, hd] into their pages.  A thread moves one 16-byte
-// piece (VEC; one element else) of a key row and of the value row beside it;
-// neighbouring threads take a row's pieces, then the next position's, which
-// lie one after the other in the source and in the page.  Bound by HBM: each
-// row is read and written once.
+// Rows k, v [N, Hkv, S, hd] into their pages.  A thread moves kStorePieces 16-byte
+// pieces (elements where rows are not made of such) of key rows and of the value
+// rows beside them; neighbouring threads take a row's pieces, then the next
+// position's, which lie one after the other in the source and in the page.
+// Bound by HBM: each row is read and written once, and not read again soon (so
+// past the L2).  64 prompts of up to 4096 tokens, 8 heads of 128, bf16 (262 MB
+// moved): 50 us, 5.3 TB/s with three pieces a thread; 3.1 with one, 4.4 with
+// two, 4.7 with four (workgroups of 12 KB spread their addresses best).  Fewer
+// than 20 MB: 3 to 6 us, the launch.
+constexpr int kStorePieces = 3;
+
 struct StoreArgs {
   const char *k, *v;
   char *kp, *vp;
   const int64_t *slots, *rows;  // rows: n -> row of slots (null: n)
-  int64_t ks[3], vs[3], kps[3], vps[3];  // strides in bytes: n/h/s, page/h/row
+  int64_t ks[2], vs[2], kps[2], vps[2];  // strides in bytes: n/h, page/h
+  uint32_t k_row, v_row, kp_row, vp_row;
   int64_t limit;                         // slots of the pool
-  int N, H, S, R, pieces, shift;
+  int N, R, log, shift;                  // log: of pieces, or -1
+  uint32_t S, pieces, total;             // total: pieces of a head's rows
 };
 
 template <typename V>
 __global__ __launch_bounds__(256) void store_kernel(StoreArgs a) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t s = e / a.pieces;
-  if (s >= a.S) return;
-  const int64_t piece = (e - s * a.pieces) * static_cast<int64_t>(sizeof(V));
+  constexpr int U = kStorePieces;
+  const uint32_t e0 = blockIdx.x * (256 * U) + threadIdx.x;
   const int h = blockIdx.y;
   for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
     const int64_t r = a.rows ? a.rows[n] : n;
     if (r < 0 || r >= a.R) continue;
-    const int64_t slot = a.slots[r * a.S + s];
-    if (slot < 0 || slot >= a.limit) continue;
-    const int64_t page = slot >> a.shift, row = slot & ((int64_t(1) << a.shift) - 1);
-    const V k = *reinterpret_cast<const V*>(a.k + n * a.ks[0] + h * a.ks[1] + s * a.ks[2] + piece);
-    const V v = *reinterpret_cast<const V*>(a.v + n * a.vs[0] + h * a.vs[1] + s * a.vs[2] + piece);
-    *reinterpret_cast<V*>(a.kp + page * a.kps[0] + h * a.kps[1] + row * a.kps[2] + piece) = k;
-    *reinterpret_cast<V*>(a.vp + page * a.vps[0] + h * a.vps[1] + row * a.vps[2] + piece) = v;
+    const int64_t* slots = a.slots + r * a.S;
+    const char *k = a.k + n * a.ks[0] + h * a.ks[1], *v = a.v + n * a.vs[0] + h * a.vs[1];
+    int64_t slot[U];
+    uint32_t s[U], piece[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t e = min(e0 + 256 * u, a.total - 1);
+      s[u] = a.log >= 0 ? e >> a.log : e / a.pieces;
+      piece[u] = (e - s[u] * a.pieces) * static_cast<uint32_t>(sizeof(V));
+      slot[u] = e0 + 256 * u < a.total ? slots[s[u]] : -1;
+    }
+    V kv[U], vv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (slot[u] < 0 || slot[u] >= a.limit) continue;
+      kv[u] = *reinterpret_cast<const V*>(k + (static_cast<uint64_t>(s[u]) * a.k_row + piece[u]));
+      vv[u] = *reinterpret_cast<const V*>(v + (static_cast<uint64_t>(s[u]) * a.v_row + piece[u]));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (slot[u] < 0 || slot[u] >= a.limit) continue;
+      const int64_t page = slot[u] >> a.shift;
+      const uint32_t row = static_cast<uint32_t>(slot[u]) & ((1u << a.shift) - 1);
+      char* kp = a.kp + page * a.kps[0] + h * a.kps[1] + (static_cast<uint64_t>(row) * a.kp_row + piece[u]);
+      char* vp = a.vp + page * a.vps[0] + h * a.vps[1] + (static_cast<uint64_t>(row) * a.vp_row + piece[u]);
+      __builtin_nontemporal_store(kv[u], reinterpret_cast<V*>(kp));
+      __builtin_nontemporal_store(vv[u], reinterpret_cast<V*>(vp));
+    }
   }
 }
 
@@ -329,23 +360,32 @@ extern "C" int hydra_page_store(const void* k, const void* v, void* k_pages, voi
   a.R = static_cast<int>(R);
   a.limit = pages * page_size;
   a.N = static_cast<int>(N);
-  a.H = static_cast<int>(Hkv);
-  a.S = static_cast<int>(S);
+  a.S = static_cast<uint32_t>(S);
   a.shift = shift;
   bool vec = hd * e % 16 == 0 && aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages);
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < 2; ++i) {
     a.ks[i] = k_st[i] * e;
     a.vs[i] = v_st[i] * e;
     a.kps[i] = kp_st[i] * e;
     a.vps[i] = vp_st[i] * e;
     vec = vec && (a.ks[i] | a.vs[i] | a.kps[i] | a.vps[i]) % 16 == 0;
   }
-  a.pieces = static_cast<int>(vec ? hd * e / 16 : hd);
-  const int64_t gx = (S * a.pieces + 255) / 256;
-  HYDRA_REQUIRE(gx < (int64_t(1) << 31), "page_store: too large");
-  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(Hkv), static_cast<unsigned>(N < 65535 ? N : 65535));
+  uint32_t* const row[4] = {&a.k_row, &a.v_row, &a.kp_row, &a.vp_row};
+  for (int i = 0; i < 4; ++i) {
+    const int64_t st = (i == 0 ? k_st : i == 1 ? v_st : i == 2 ? kp_st : vp_st)[2] * e;
+    HYDRA_REQUIRE(st >= 0 && st < (int64_t(1) << 32), "page_store: rows too far apart");
+    *row[i] = static_cast<uint32_t>(st);
+    vec = vec && st % 16 == 0;
+  }
+  a.pieces = static_cast<uint32_t>(vec ? hd * e / 16 : hd);
+  a.log = (a.pieces & (a.pieces - 1)) == 0 ? __builtin_ctz(a.pieces) : -1;
+  HYDRA_REQUIRE(S * a.pieces < (int64_t(1) << 31), "page_store: too large");
+  a.total = a.S * a.pieces;
+  const int64_t z = N < 65535 ? N : 65535;
+  const unsigned span = 256 * kStorePieces;
+  const dim3 grid((a.total + span - 1) / span, static_cast<unsigned>(Hkv), static_cast<unsigned>(z));
   auto st = static_cast<hipStream_t>(stream);
-  if (vec) store_kernel<uint4><<<grid, 256, 0, st>>>(a);
+  if (vec) store_kernel<u32x4_nt><<<grid, 256, 0, st>>>(a);
   else if (e == 4) store_kernel<uint32_t><<<grid, 256, 0, st>>>(a);
   else store_kernel<uint16_t><<<grid, 256, 0, st>>>(a);
   return check_launch("page_store");
