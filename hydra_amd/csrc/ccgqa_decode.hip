@@ -171,11 +171,36 @@ __device__ __forceinline__ void keep_row16(const DecodeArgs& a, int n, int p, in
   for (int c = lane; c < bytes / 16; c += 64) to[c] = from[c];
 }
 
+constexpr int kGenericThreads = 1024;
+
+// s plus the product of n elements of a and b, in 16-byte pieces where VEC.
+template <typename T, bool VEC>
+__device__ __forceinline__ float dot(const T* a, const T* b, int n, float s) {
+  if constexpr (VEC) {
+    constexpr int E = Vec<T>::N;
+#pragma unroll 4
+    for (int i = 0; i < n; i += E) {
+      float x[E], y[E];
+      load16<T>(a + i, x);
+      load16<T>(b + i, y);
+#pragma unroll
+      for (int k = 0; k < E; ++k) s = fmaf(x[k], y[k], s);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) s = fmaf(to_f32(a[i]), to_f32(b[i]), s);
+  }
+  return s;
+}
+
 // Any head_dim, taps and flags: one workgroup per request and head on the
-// VALU, y1 in LDS as [ks][C] floats, then y2 [hd].
-template <typename T>
-__global__ __launch_bounds__(256) void decode_prep_generic_kernel(DecodeArgs a) {
-  extern __shared__ float sm[];
+// VALU, y1 in LDS as [ks][C] floats, then y2 [hd].  Every workgroup computes all
+// of conv1 for itself, ks^2 hd products a channel, and a lane's weights are rows
+// of their own, so the cache's lines bound it: 8/2 heads of 48, three taps, 17 us
+// for one request and 33 us for 32; heads of 64 with five taps, 32 requests, 150 us.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kGenericThreads) void decode_prep_generic_kernel(DecodeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float sm[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int hh = blockIdx.x, n = blockIdx.y;
   const bool is_k = hh >= a.Hq;
@@ -186,35 +211,43 @@ __global__ __launch_bounds__(256) void decode_prep_generic_kernel(DecodeArgs a) 
   float* y2 = sm + (convs ? a.ks * C : 0);
   if (p >= 0 && convs) {
     const T *w1 = static_cast<const T*>(a.w[is_k ? 2 : 0]), *w2 = static_cast<const T*>(a.w[is_k ? 3 : 1]);
-    for (int i = tid; i < a.ks * C; i += 256) {
+    for (int i = tid; i < a.ks * C; i += kGenericThreads) {
       const int j = i / C, c = i - j * C, g0 = c / hd * hd;
       float s = 0.f;
       for (int t = 0; t < a.ks; ++t) {
         const int back = 2 * (a.ks - 1) - j - t;
         if (back > p) continue;
-        const T* x = row_at<T>(a, n, p, back) + col0 + g0;
-        const T* w = w1 + (static_cast<int64_t>(t) * C + c) * hd;
-        for (int e = 0; e < hd; ++e) s = fmaf(to_f32(w[e]), to_f32(x[e]), s);
+        s = dot<T, VEC>(w1 + (static_cast<int64_t>(t) * C + c) * hd, row_at<T>(a, n, p, back) + col0 + g0, hd, s);
       }
       sm[i] = s;
     }
     __syncthreads();
-    for (int d = wave; d < hd; d += 4) {
+    for (int d = wave; d < hd; d += kGenericThreads / 64) {
       float s = 0.f;
       for (int j = 0; j < a.ks; ++j) {
         const T* w = w2 + (static_cast<int64_t>(j) * C + head * hd + d) * C;
-        for (int c = lane; c < C; c += 64) s = fmaf(to_f32(w[c]), sm[j * C + c], s);
+        if constexpr (VEC) {
+          constexpr int E = Vec<T>::N;
+          for (int c = lane * E; c < C; c += 64 * E) {
+            float x[E];
+            load16<T>(w + c, x);
+#pragma unroll
+            for (int k = 0; k < E; ++k) s = fmaf(x[k], sm[j * C + c + k], s);
+          }
+        } else {
+          for (int c = lane; c < C; c += 64) s = fmaf(to_f32(w[c]), sm[j * C + c], s);
+        }
       }
       s = wave_sum(s);
       if (lane == 0) y2[d] = s;
     }
   } else if (p >= 0) {
     const T* x = row_at<T>(a, n, p, 0) + col0 + head * hd;
-    for (int d = tid; d < hd; d += 256) y2[d] = to_f32(x[d]);
+    for (int d = tid; d < hd; d += kGenericThreads) y2[d] = to_f32(x[d]);
   }
   __syncthreads();
   if (wave == 0) finish<T>(a, n, p, hh, lane, [&](int d) { return y2[d]; });
-  if (hh == 0) keep_row<T>(a, n, p, tid, 256);
+  if (hh == 0) keep_row<T>(a, n, p, tid, kGenericThreads);
 }
 
 // ---- matrix-core form: three taps, head_dim 16, 32, 64 or 128 ---------------
@@ -460,8 +493,9 @@ struct Tail {
 // conv1's channels there and their share of conv2 at once, and the waves' y2 are
 // added up in LDS.  Parts leave their sums in `part` [split][head][tile][16][HD],
 // which decode_join_kernel adds in order.  Weights come from L2 (each head
-// reads all of conv1's); bound by the chain position -> rows -> convs -> norm,
-// and for many requests by the rows' and weights' way from L2.
+// reads all of conv1's); bound by the chain position -> rows -> convs -> norm
+// (one request, 4/1 heads of 64: 7.9 us), and for many requests by the rows' and
+// weights' way from L2 (256, 8/2 heads of 64, 65 MB of it: 19.6 us).
 template <typename T, int HB, bool TILED>
 __global__ __launch_bounds__(64 * decode_waves(HB, sizeof(T))) void decode_prep_mfma_kernel(DecodeArgs a) {
   constexpr int HD = HB * 16;
@@ -600,10 +634,10 @@ template <typename T>
 int launch_decode(DecodeArgs a, hipStream_t st) {
   const int L = a.Hq * a.hd, W = L + 2 * a.Hkv * a.hd;
   const int need = 16 / static_cast<int>(sizeof(T));
-  // the operands are loaded four values at a time: rows and weights aligned to that
-  bool mfma = decode_mfma_size(a.hd, a.ks, a.flags) && a.qkv_rs % need == 0 && W % need == 0 &&
-              aligned16(a.qkv) && aligned16(a.ring);
-  for (const void* w : a.w) mfma = mfma && aligned16(w);
+  // rows and weights that 16-byte loads take
+  bool vec = a.qkv_rs % need == 0 && W % need == 0 && aligned16(a.qkv) && aligned16(a.ring);
+  for (const void* w : a.w) vec = vec && aligned16(w);
+  bool mfma = vec && decode_mfma_size(a.hd, a.ks, a.flags);
   // 32-bit byte offsets of rows
   mfma = mfma && static_cast<int64_t>(a.N) * a.R * W * sizeof(T) < (int64_t(1) << 32) &&
          a.N * a.qkv_rs * static_cast<int64_t>(sizeof(T)) < (int64_t(1) << 32);
@@ -632,8 +666,9 @@ int launch_decode(DecodeArgs a, hipStream_t st) {
     if (lds > 64 * 1024)
       return fail(HYDRA_ERR_UNSUPPORTED, "ccgqa_decode_prep: conv taps times channels above 16384 need head_dim 16, "
                                          "32, 64 or 128 and three taps");
-    decode_prep_generic_kernel<T><<<dim3(static_cast<unsigned>(a.Hq + a.Hkv), static_cast<unsigned>(a.N)), 256, lds,
-                                    st>>>(a);
+    const dim3 grid(tiles.x, static_cast<unsigned>(a.N));
+    if (vec && a.hd % need == 0) decode_prep_generic_kernel<T, true><<<grid, kGenericThreads, lds, st>>>(a);
+    else decode_prep_generic_kernel<T, false><<<grid, kGenericThreads, lds, st>>>(a);
   }
 #undef HYDRA_DECODE
   return check_launch("ccgqa_decode_prep");
