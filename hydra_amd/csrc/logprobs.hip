@@ -12,7 +12,10 @@
 //
 // Both directions are bound by HBM: the forward reads a row once and keeps it
 // in registers between its maximum and its sums (16-bit values packed), the
-// backward reads it once and writes the gradient.  Rows start anywhere: a row
+// backward reads it once and writes the gradient.  8192 rows of 32000, bf16:
+// 108 us, 4.9 TB/s, forward (135 with 20 alternatives) and 190 us, 5.5 TB/s,
+// backward.  A few rows take the chain row -> maximum -> sums (-> bound ->
+// candidates -> ranks): 16 of 50257, 20 alternatives, 12.4 us.  Rows start anywhere: a row
 // is taken in the 16-byte pieces of memory that it lies in, what is left at its
 // two ends element by element.
 #include "common.h"

@@ -3,8 +3,13 @@
 //   o[n,h] = sum_t p_t v[t, h/G],  p = softmax_t(scale q[n,h] . k[t, h/G]),
 //   t < lengths[n], position t in page table[n, t / page_size].
 //
-// A step reads each key and value once and does 4 G flops per element pair:
-// HBM-bound at every group size up to 16.  A wave walks its keys KT at a time:
+// A step reads each key and value once and does 4 G flops per element pair.
+// 64 requests of 16384 keys, 8/2 heads of 64, bf16 (537 MB): 104 to 110 us, 4.9
+// to 5.2 TB/s, a large copy's rate.  Short rows shared by many heads do not
+// reach it (48 requests of up to 8192 keys, 28/4 heads of 16: 18 us, 0.6 TB/s):
+// exponentials and products of 8 heads for 32 bytes of key take longer.  A few
+// keys take the launch and the chain table -> keys -> softmax -> output, 5 us.
+// A wave walks its keys KT at a time:
 //
 //  * scores S^T = K Q^T on the matrix cores: keys are the rows of the A operand,
 //    loaded from the pages in the operand's own layout (16 bytes a lane), the up
@@ -17,7 +22,7 @@
 //  * P goes through KT GP floats of LDS to the lanes that hold the rows of V,
 //    which accumulate p v in fp32 with plain multiply-adds: P is never rounded,
 //    V needs no transposed copy, and G multiply-adds per value stay below the
-//    time its bytes take (G = 8: about a third).
+//    time its bytes take while rows are long.
 //
 // Pages hold 16 rows or more, so the 16 keys of an operand lie in one page and
 // page ids are wave-uniform scalar loads.  An entry outside the pool counts as
@@ -25,7 +30,7 @@
 // most within their own page and stay out of both sums, whatever they hold.
 //
 // Split: the keys of all (request, key head, head block) items are laid end to
-// end in rounds of 8 KT keys (one tile per wave) and dealt out evenly to the
+// end in rounds (one tile of KT keys per wave) and dealt out evenly to the
 // workgroups, whatever the lengths; an item that more than one of them works on
 // leaves (max, sum, unscaled output) per part in the workspace, and a second
 // kernel joins them in order.  No atomics: the same inputs give the same bits.
@@ -99,8 +104,9 @@ __device__ __forceinline__ int seen_keys(const PagedArgs& a, int n) {
 }
 
 // Most waves of a workgroup (a launch takes 4 or 8), and keys of a wave's step: 4 KB
-// of keys and as much of values in flight (64 keys of 128 bytes instead of 32 take
-// 150 registers: a workgroup less on each CU, 5% more time at long contexts).
+// of keys and as much of values in flight.  Of 128-byte keys 32: with 16, 4 requests
+// of 16384 keys take 18.8 us instead of 17.3, 32 of 3001 with 28/4 heads 31.9
+// instead of 28.9; with 64, 16 of 16384 take 34.0 instead of 32.0.
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 __device__ __forceinline__ int waves() { return blockDim.x >> 6; }
@@ -424,6 +430,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_split_kernel(PagedArgs a)
   };
   const int HG = a.Hkv * a.GB, total = base * HG;
   // two rounds and more, for the sake of each share's end, unless that left CUs idle
+  // (4 requests of 16384 keys, 8/2 heads of 64: 17.3 us, 18.7 with single rounds)
   int per = (total + a.groups - 1) / a.groups;
   per = max(max(per, min(2, (total + a.cus - 1) / a.cus)), a.least);
   if (blockIdx.x == 0) {  // for the joining kernel
@@ -587,14 +594,15 @@ struct Split {
   int least, waves;
 };
 
-constexpr int kMaxResident = 4;  // workgroups of a CU that a split launch takes at most
+constexpr int kMaxResident = 4;  // workgroups of a CU that a split launch takes at most (8: the same times)
 
 // Split where the items alone would not fill the chip and a request may be longer
-// than 128 KB of keys or 2048 of them (1024 keys of 128 bytes take one workgroup of
-// 8 waves 5 us more than 128 of them; the joining launch takes 5).  8 waves only for few short items:
-// where items or rounds are many, twice as many workgroups of 4 have more of the
-// chip's registers in use (256 requests of 20 keys, 28/4 heads of 64: 13.4
-// against 23 us).
+// than 128 KB of keys or 2048 of them, whole and split: of 128-byte keys 512 take
+// 8.0 and 10.3 us, 1000 10.5 and 10.6, 2000 15.6 and 10.8; of 32-byte keys 2000 take
+// 9.9 and 11.0, 4000 15.1 and 11.1.  8 waves for few short items (one request of
+// 500 keys, 28/4 heads of 64: 9.4 us, 11.4 with 4); where items or rounds are many,
+// twice as many workgroups of 4 have more of the chip's registers in use (256
+// requests of 20 keys, 28/4 heads of 64: 8.0 us, 11.8 with 8).
 inline Split split_of(const Shape& s, int64_t N, int64_t capacity) {
   Split r{};
   r.on = N <= kMaxRequests && s.items < 8 * device_cus() && capacity > std::min<int64_t>(2048, (128 << 10) / s.row);
