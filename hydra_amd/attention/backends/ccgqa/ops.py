@@ -360,10 +360,11 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     ws = _lib.scratch(need, qkv) if need else None
     with _lib.on_device(qkv):
         _lib.call("hydra_ccgqa_decode_prep", qkv.data_ptr(), qkv.stride(0) if N > 1 else W, ring.data_ptr(),
-                  ring.shape[1], positions.data_ptr(), slots.data_ptr(), _lib.ptr(wq1), _lib.ptr(wq2), _lib.ptr(wk1), _lib.ptr(wk2),
-                  _lib.ptr(temp), _lib.ptr(cos), _lib.ptr(sin), rope_rs, rope_rows, q.data_ptr(), k_pages.data_ptr(),
-                  v_pages.data_ptr(), _lib.strides(k_pages), _lib.strides(v_pages), pages, page, N, n_heads,
-                  n_kv_heads, head_dim, conv_ks, flags, _lib.dtype_code(qkv), _lib.ptr(ws), need, _lib.stream(qkv))
+                  ring.shape[1], positions.data_ptr(), slots.data_ptr(), _lib.ptr(wq1), _lib.ptr(wq2), _lib.ptr(wk1),
+                  _lib.ptr(wk2), _lib.ptr(temp), _lib.ptr(cos), _lib.ptr(sin), rope_rs, rope_rows, q.data_ptr(),
+                  k_pages.data_ptr(), v_pages.data_ptr(), _lib.strides(k_pages), _lib.strides(v_pages), pages, page, N,
+                  n_heads, n_kv_heads, head_dim, conv_ks, flags, _lib.dtype_code(qkv), _lib.ptr(ws), need,
+                  _lib.stream(qkv))
     return q
 
 

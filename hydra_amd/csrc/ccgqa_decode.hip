@@ -552,7 +552,8 @@ __global__ __launch_bounds__(64 * decode_waves(HB, sizeof(T))) void decode_prep_
         for (int t = 0; t < 3; ++t) w1f[i][t] = w1(t, cb, i0 + i);
 #pragma unroll
         for (int o = 0; o < 5; ++o)
-          xf[i][o] = *reinterpret_cast<const Frag<T, K>*>(static_cast<const char*>(o == 4 ? a.qkv : a.ring) + in_group + xo[o]);
+          xf[i][o] = *reinterpret_cast<const Frag<T, K>*>(static_cast<const char*>(o == 4 ? a.qkv : a.ring) + in_group +
+                                                          xo[o]);
       }
       if (young) {
 #pragma unroll
@@ -646,14 +647,18 @@ int launch_decode(DecodeArgs a, hipStream_t st) {
   a.span = plan.span;
   const dim3 tiles(static_cast<unsigned>(a.Hq + a.Hkv), static_cast<unsigned>((a.N + 15) / 16));
   const dim3 parts(tiles.x, tiles.y, static_cast<unsigned>(plan.splits));
-  const int threads = 64 * plan.waves;
+  // More workgroups than CUs: of half as many waves two share a CU (512 requests,
+  // 8/8 heads of 32: 15.8 us with 16 waves, 13.9 with 8; no more than CUs, 256
+  // requests, 4/1 heads of 64: 12.1 and 13.4).
+  const bool shared = static_cast<int64_t>(tiles.x) * tiles.y > device_cus();
+  const int threads = 64 * (shared && plan.waves > 8 ? 8 : plan.waves);
 #define HYDRA_DECODE(HB)                                                                          \
   {                                                                                               \
     if constexpr (sizeof(T) == 2) {                                                               \
       if (tiled) decode_prep_mfma_kernel<T, HB, true><<<parts, threads, 0, st>>>(a);              \
     }                                                                                             \
     if (!tiled) decode_prep_mfma_kernel<T, HB, false><<<parts, threads, 0, st>>>(a);              \
-    if (plan.splits > 1) decode_join_kernel<T, HB><<<tiles, 1024, 0, st>>>(a);                          \
+    if (plan.splits > 1) decode_join_kernel<T, HB><<<tiles, 1024, 0, st>>>(a);                    \
   }
   if (mfma && a.hd == 16) HYDRA_DECODE(1)
   else if (mfma && a.hd == 32) HYDRA_DECODE(2)
@@ -662,7 +667,8 @@ int launch_decode(DecodeArgs a, hipStream_t st) {
   else {
     if (tiled)
       return fail(HYDRA_ERR_UNSUPPORTED, "ccgqa_decode_prep: tiled weights need the matrix-core form");
-    const size_t lds = sizeof(float) * ((a.flags & HYDRA_CCGQA_CONVS ? static_cast<size_t>(a.ks) * std::max(a.Hq, a.Hkv) * a.hd : 0) + a.hd);
+    const size_t y1 = a.flags & HYDRA_CCGQA_CONVS ? static_cast<size_t>(a.ks) * std::max(a.Hq, a.Hkv) * a.hd : 0;
+    const size_t lds = sizeof(float) * (y1 + a.hd);
     if (lds > 64 * 1024)
       return fail(HYDRA_ERR_UNSUPPORTED, "ccgqa_decode_prep: conv taps times channels above 16384 need head_dim 16, "
                                          "32, 64 or 128 and three taps");
@@ -781,7 +787,8 @@ extern "C" int hydra_ccgqa_ring_fill(const void* qkv, int64_t qkv_bs, int64_t qk
                                      int64_t keep, int dtype, void* stream) {
   HYDRA_REQUIRE(M >= 0 && S >= 1 && W >= 1 && N >= 1 && R >= 1 && keep >= 0, "ccgqa_ring_fill: bad size");
   HYDRA_REQUIRE(keep <= R, "ccgqa_ring_fill: more rows than the ring holds");
-  HYDRA_REQUIRE(M <= 65535 && S < (int64_t(1) << 31) && W < (int64_t(1) << 31) && N < (int64_t(1) << 31) && R < (1 << 20),
+  HYDRA_REQUIRE(M <= 65535 && S < (int64_t(1) << 31) && W < (int64_t(1) << 31) && N < (int64_t(1) << 31) &&
+                    R < (1 << 20),
                 "ccgqa_ring_fill: too large");
   HYDRA_REQUIRE(dtype_size(dtype) > 0, "ccgqa_ring_fill: unknown dtype");
   if (M == 0 || keep == 0) return HYDRA_OK;

@@ -122,8 +122,9 @@ __device__ __forceinline__ void half_sum(float* v) {
   for (int i = 0; i < N / 2; ++i) {
     if constexpr (OFF == 32 || OFF == 16) {
       // swaps a's upper lanes (of 64, of each 32) with b's lower ones: a + b is the sum
-      const auto r = OFF == 32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + N / 2]), false, false)
-                               : __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + N / 2]), false, false);
+      const uint32_t lo = __float_as_uint(v[i]), hi = __float_as_uint(v[i + N / 2]);
+      const auto r = OFF == 32 ? __builtin_amdgcn_permlane32_swap(lo, hi, false, false)
+                               : __builtin_amdgcn_permlane16_swap(lo, hi, false, false);
       v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     } else {
       const float keep = upper ? v[i + N / 2] : v[i], give = upper ? v[i] : v[i + N / 2];
@@ -181,7 +182,8 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
 
   uint4 qf[NC];
   {
-    const char* qrow = a.q + n * a.q_st[0] + static_cast<int64_t>(h * a.G + gb * GP + (col < heads ? col : 0)) * a.q_st[1];
+    const int head = h * a.G + gb * GP + (col < heads ? col : 0);
+    const char* qrow = a.q + n * a.q_st[0] + static_cast<int64_t>(head) * a.q_st[1];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       qf[c] = row_piece<T, VEC>(qrow, 4 * c + g4, a.hd);
@@ -246,7 +248,8 @@ __device__ __forceinline__ void item_keys(const PagedArgs& a, int n, int h, int 
         const int b = i * RPI / 16;
         bool there = page[b] >= 0;
         if constexpr (RPI == 32) {
-          const bool upper = page[b + 1] >= 0;  // loaded before the choice: a chosen index would put the pages in memory
+          // loaded before the choice: a chosen index would put the pages in memory
+          const bool upper = page[b + 1] >= 0;
           there = vrow < 16 ? there : upper;
         }
         if (key0 + i * RPI + vrow >= len || !there) vf[i] = make_uint4(0, 0, 0, 0);
@@ -608,7 +611,7 @@ inline Split split_of(const Shape& s, int64_t N, int64_t capacity) {
   r.on = N <= kMaxRequests && s.items < 8 * device_cus() && capacity > std::min<int64_t>(2048, (128 << 10) / s.row);
   r.waves = r.on || s.items > device_cus() ? 4 : kWaves;
   const int64_t most = (capacity + r.waves * s.kt - 1) / (r.waves * s.kt);
-  r.on = r.on && most * s.items < (int64_t(1) << 31) - (1 << 20);  // all rounds, and the workgroups, in an int
+  r.on = r.on && most * s.items < (int64_t(1) << 31) - (1 << 20);  // rounds and workgroups in an int
   r.least = static_cast<int>(std::max<int64_t>(1, (most + kMaxParts - 2) / (kMaxParts - 1)));
   return r;
 }
@@ -618,7 +621,8 @@ inline int64_t plan_ints(int64_t N) { return (N + 2 + 3) / 4 * 4; }
 
 inline int64_t workspace_bytes(const Split& p, int64_t N, int64_t hd) {
   if (!p.on) return 0;
-  return 4 * (plan_ints(N) + static_cast<int64_t>(kMaxResident) * device_cus() * 2 * (16 + 8 * row4(static_cast<int>(hd))));
+  const int64_t parts = static_cast<int64_t>(kMaxResident) * device_cus() * 2;
+  return 4 * (plan_ints(N) + parts * (16 + 8 * row4(static_cast<int>(hd))));
 }
 
 template <typename T, int GP, int LPR, bool VEC>

@@ -336,8 +336,8 @@ extern "C" int hydra_page_release(const void* done, int* lengths, int* table, in
 
 extern "C" int hydra_page_store(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots,
                                 int64_t R, const int64_t* rows, int64_t N, int64_t Hkv, int64_t S, int64_t hd,
-                                int64_t pages, int64_t page_size, const int64_t* k_st, const int64_t* v_st, const int64_t* kp_st, const int64_t* vp_st,
-                                int dtype, void* stream) {
+                                int64_t pages, int64_t page_size, const int64_t* k_st, const int64_t* v_st,
+                                const int64_t* kp_st, const int64_t* vp_st, int dtype, void* stream) {
   HYDRA_REQUIRE(N >= 0 && S >= 0 && R >= 0 && Hkv >= 1 && hd >= 1 && pages >= 1, "page_store: bad size");
   HYDRA_REQUIRE(rows || R >= N, "page_store: fewer rows of slots than prompts");
   const int shift = page_shift(page_size);

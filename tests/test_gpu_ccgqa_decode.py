@@ -133,6 +133,18 @@ def test_tiled_weights_and_longer_rings(cuda, name, N):
     check(cfg, torch.bfloat16, params, rows, ring, positions, slots, 64, got)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_workgroups_than_units(cuda, dtype):
+    """Heads times tiles of 16 requests past 256: workgroups of fewer waves."""
+    cfg, N = oc.CCGQAConfig(**CONFIGS["seven"]), 133
+    assert (cfg.n_heads + cfg.n_kv_heads) * -(-N // 16) > torch.cuda.get_device_properties(0).multi_processor_count
+    positions = [n % 7 for n in range(N)]
+    slots = [n * 16 + n % 16 for n in range(N)]
+    params, rows, ring = case(cfg, positions, dtype, seed=3)
+    got = run(cuda, cfg, dtype, params, rows, ring, positions, slots, N, 16)
+    check(cfg, dtype, params, rows, ring, positions, slots, 16, got)
+
+
 @pytest.mark.parametrize("name", ["debug", "hd48"])
 def test_idle_requests_change_nothing(cuda, name):
     """No slot, one outside the pool, a position below 0 or past the rotation's
