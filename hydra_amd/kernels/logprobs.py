@@ -30,7 +30,7 @@ def _forward(logits, tokens, top_k, temperature, want_stats):
     x, (rows, stride) = _as_rows(logits)
     if x.dim() > 1 and stride < x.shape[-1] and rows > 1:  # rows that overlap: broadcast ones
         x, (rows, stride) = _as_rows(logits.contiguous())
-    tokens = tokens.reshape(-1)
+    tokens = tokens.reshape(-1).contiguous()  # a reshaped view may keep its stride
     lead = logits.shape[:-1]
     logp, entropy = (x.new_empty(lead, dtype=torch.float32) for _ in range(2))
     top = x.new_empty((*lead, top_k), dtype=torch.float32)

@@ -66,6 +66,30 @@ def test_strides_and_shapes(cuda, dtype):
     check(x[:1].repeat(4, 1), t[:4], cuda, 1, 1.0, form=lambda x: x[:1].expand(4, -1))
 
 
+def test_strides_of_tokens(cuda):
+    """A column of a wider tensor, every second of a vector, one for all rows, a
+    transposed batch: the tokens' own strides, forward and backward."""
+    from hydra_amd.kernels import token_logprobs
+
+    x, t, g = make(6, 300, torch.float32, seed=4)
+    wide = torch.randint(0, 300, (2, 3, 2), generator=g)
+    wide[..., 1] = t.view(2, 3)
+    spread = torch.full((11,), 7)
+    spread[::2] = t
+    for rows, tokens in ((x.view(2, 3, 300), wide.to(cuda)[..., 1]), (x, spread.to(cuda)[::2]),
+                         (x, torch.tensor([5], device=cuda).expand(6)),
+                         (x.view(2, 3, 300), t.view(2, 3).t().contiguous().to(cuda).t())):
+        leaf, flat = rows.to(cuda).requires_grad_(), x.to(cuda).requires_grad_()
+        same = tokens.cpu().contiguous().view(-1).to(cuda)
+        got, want = token_logprobs(leaf, tokens, top_k=3), token_logprobs(flat, same, top_k=3)
+        assert all(torch.equal(a.reshape(b.shape), b) for a, b in zip(got, want))
+        got.logprobs.sum().backward()
+        want.logprobs.sum().backward()
+        assert torch.equal(leaf.grad.view(6, 300), flat.grad)
+        with torch.no_grad():
+            assert torch.equal(token_logprobs(leaf, tokens).logprobs.view(-1), want.logprobs)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [40, 5000, 50257])
 def test_equal_logits_take_the_lowest_index(cuda, dtype, V):
