@@ -78,7 +78,7 @@ SIGNATURES = {
     "hydra_ccgqa_decode_prep": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P,
                                 _I64P, _I64P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _P],
     "hydra_ccgqa_decode_prep_workspace": [_I64, _I64, _I64, _I64, _I64, _I, _I],
-    "hydra_ccgqa_ring_fill": [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _P],
+    "hydra_ccgqa_ring_fill": [_P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P],
     "hydra_ccgqa_prep_tiled_ok": [_I64, _I64, _I64, _I],
     "hydra_ccgqa_prep_faults": [_P],
     "hydra_ccgqa_prep_bwd": [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _P,

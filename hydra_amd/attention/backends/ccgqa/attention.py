@@ -264,9 +264,9 @@ class CCGQAAttention(nn.Module):
         """forward() of whole prompts x [M, S, dim], padded on the right, whose
         keys and values go into the cache.  `plan`: pool.plan(new_tokens,
         width=S, from_empty=True); rows: int64 [M], the requests that the
-        prompts belong to (distinct; default: prompt m is request m).  Output
-        rows past a prompt's end hold no result; a refused request's prompt is
-        computed but not kept."""
+        prompts belong to (distinct; default: prompt m is request m).  The
+        padding may hold anything.  Output rows past a prompt's end, and all of
+        a refused request's, hold no result."""
         name = "CCGQAAttention.prefill"
         M, S, _ = x.shape
         self._check_cache(name, x, cache, plan)
@@ -282,7 +282,8 @@ class CCGQAAttention(nn.Module):
             raise ValueError(f"{name}: sequence length {S} exceeds the RoPE cache ({self.cos_cached.shape[2]})")
         qkv = F.linear(x, self.qkv_proj.weight)
         flags, convw = self._prep_args()
-        ccgqa_ring_fill(qkv, cache.ring, plan.seen, decode_reach(flags, self.conv_kernel_size), rows)
+        # padding may hold anything, and the attention's tiles would take it up
+        ccgqa_ring_fill(qkv, cache.ring, plan.seen, decode_reach(flags, self.conv_kernel_size), rows, clear=True)
         return self._forward_infer(x, qkv, flags, convw, None,
                                    keep=lambda k, v: store_pages(k, v, cache.k_pages, cache.v_pages, plan.slots, rows))
 

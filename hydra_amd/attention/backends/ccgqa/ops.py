@@ -17,7 +17,7 @@ from ...._lib import (CCGQA_CONVS, CCGQA_QK_MEAN, CCGQA_QK_NORM, CCGQA_ROPE, CCG
                       CCGQA_V_TRANSPOSED, CCGQA_VALUE_SHIFT, CCGQA_W_TILED, MASK_KEY_PADDING, MASK_NONE,
                       MASK_REFERENCE_SDPA)
 from .... import _lib
-from ...paged import check_no_gradient, check_pages
+from ...paged import check_distinct, check_no_gradient, check_pages
 
 
 def prep_flags(use_convs: bool, use_qk_mean: bool, use_value_shift: bool,
@@ -369,11 +369,13 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
 
 
 def ccgqa_ring_fill(qkv: torch.Tensor, ring: torch.Tensor, lengths: torch.Tensor, keep: int,
-                    rows: Optional[torch.Tensor] = None) -> None:
+                    rows: Optional[torch.Tensor] = None, clear: bool = False) -> None:
     """Keeps the last `keep` projected rows of prompts, qkv [M, S, W], in the
     rings of their requests, ring [N, R, W].  Prompt m is request rows[m]
-    (int64, distinct; None: m) and lengths[request] (int32 [N]) tokens long; a
-    length of 0, one past S, or a row outside the ring leaves it as it is."""
+    (int64, distinct; None: m) and lengths[request] (int32 [N]) tokens long.
+    clear: also sets qkv's rows past each prompt's end to zero, whatever they
+    hold.  A length of 0, one past S, or a row outside the ring changes
+    nothing.  Inference only: no gradient."""
     name = "ccgqa_ring_fill"
     _lib.require_gpu(name, qkv, ring, lengths, rows)
     M, S, W = qkv.shape
@@ -384,13 +386,15 @@ def ccgqa_ring_fill(qkv: torch.Tensor, ring: torch.Tensor, lengths: torch.Tensor
         raise ValueError(f"{name}: lengths must be int32 [{N}], got {lengths.dtype} {tuple(lengths.shape)}")
     if rows is not None and (rows.dtype != torch.int64 or rows.shape != (M,)):
         raise ValueError(f"{name}: rows must be int64 [{M}], got {rows.dtype} {tuple(rows.shape)}")
-    if qkv.stride(-1) != 1:
+    if clear and not qkv.is_contiguous():
+        check_distinct(name, "rows of qkv", qkv)
+    elif qkv.stride(-1) != 1:
         qkv = qkv.contiguous()
     lengths, rows = lengths.contiguous(), None if rows is None else rows.contiguous()
     with _lib.on_device(qkv):
         _lib.call("hydra_ccgqa_ring_fill", qkv.data_ptr(), qkv.stride(0), qkv.stride(1), ring.data_ptr(),
-                  _lib.ptr(rows), lengths.data_ptr(), M, S, W, N, ring.shape[1], int(keep), _lib.dtype_code(qkv),
-                  _lib.stream(qkv))
+                  _lib.ptr(rows), lengths.data_ptr(), M, S, W, N, ring.shape[1], int(keep), 1 if clear else 0,
+                  _lib.dtype_code(qkv), _lib.stream(qkv))
 
 
 def _mask_bytes(key_mask: torch.Tensor) -> torch.Tensor:

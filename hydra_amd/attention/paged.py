@@ -67,7 +67,7 @@ def check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None
         raise ValueError(f"{name}: an empty pool {tuple(k_pages.shape)}")
     for t in (k_pages, v_pages):
         if not t.is_contiguous():
-            _check_distinct(name, "pages", t)
+            check_distinct(name, "pages", t)
 
 
 def check_no_gradient(name: str, *tensors: torch.Tensor) -> None:
@@ -75,7 +75,7 @@ def check_no_gradient(name: str, *tensors: torch.Tensor) -> None:
         raise RuntimeError(f"{name}: no gradient (call it under torch.no_grad())")
 
 
-def _check_distinct(name: str, what: str, t: torch.Tensor) -> None:
+def check_distinct(name: str, what: str, t: torch.Tensor) -> None:
     """A unit last stride, and no memory that two elements share."""
     reach = 1  # elements that the dimensions up to here span
     for size, stride in sorted(zip(t.shape, t.stride()), key=lambda d: d[1]):
@@ -229,7 +229,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError(f"{name}: out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
     elif not out.is_contiguous():
-        _check_distinct(name, "rows of out", out)
+        check_distinct(name, "rows of out", out)
     lengths = lengths.contiguous()
     P, code = table.shape[1], _lib.dtype_code(q)
     with _lib.on_device(q):

@@ -682,19 +682,28 @@ int launch_decode(DecodeArgs a, hipStream_t st) {
 
 // The last `keep` rows of prompts into the ring: qkv [M, S, W], prompt m being
 // request r = rows[m], row s if lengths[r] - keep <= s < lengths[r] to
-// ring[r][s % R].
+// ring[r][s % R].  The workgroups from `keep` on set the rows past the prompt's
+// end to zero (none of them is kept): a matrix product over a tile would
+// multiply what lies there by a weight of 0, and 0 * inf is NaN.
 template <typename T>
-__global__ __launch_bounds__(256) void ring_fill_kernel(const T* qkv, int64_t bs, int64_t rs, T* ring,
-                                                        const int64_t* rows, const int* lengths, int N, int R, int W,
-                                                        int S) {
-  const int m = blockIdx.y;
+__global__ __launch_bounds__(256) void ring_fill_kernel(T* qkv, int64_t bs, int64_t rs, T* ring, const int64_t* rows,
+                                                        const int* lengths, int N, int R, int W, int S, int keep) {
+  const int m = blockIdx.y, b = blockIdx.x;
   const int64_t row = rows ? rows[m] : m;
   if (row < 0 || row >= N) return;
-  const int len = lengths[row], s = len - 1 - static_cast<int>(blockIdx.x);
-  if (len > S || s < 0) return;
-  const T* from = qkv + m * bs + s * rs;
-  T* to = ring + (row * R + s % R) * W;
-  for (int c = threadIdx.x; c < W; c += 256) to[c] = from[c];
+  const int len = lengths[row];
+  if (len <= 0 || len > S) return;
+  T* x = qkv + m * bs;
+  if (b < keep) {
+    const int s = len - 1 - b;
+    if (s < 0) return;
+    T* to = ring + (row * R + s % R) * W;
+    for (int c = threadIdx.x; c < W; c += 256) to[c] = x[s * rs + c];
+  } else {
+    const int step = gridDim.x - keep;
+    for (int64_t s = static_cast<int64_t>(len) + b - keep; s < S; s += step)
+      for (int c = threadIdx.x; c < W; c += 256) x[s * rs + c] = from_f32<T>(0.f);
+  }
 }
 
 }  // namespace
@@ -782,24 +791,26 @@ extern "C" int hydra_ccgqa_decode_prep(const void* qkv, int64_t qkv_rs, void* ri
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int { return launch_decode<T>(a, st); });
 }
 
-extern "C" int hydra_ccgqa_ring_fill(const void* qkv, int64_t qkv_bs, int64_t qkv_rs, void* ring, const int64_t* rows,
+extern "C" int hydra_ccgqa_ring_fill(void* qkv, int64_t qkv_bs, int64_t qkv_rs, void* ring, const int64_t* rows,
                                      const int* lengths, int64_t M, int64_t S, int64_t W, int64_t N, int64_t R,
-                                     int64_t keep, int dtype, void* stream) {
+                                     int64_t keep, int clear, int dtype, void* stream) {
   HYDRA_REQUIRE(M >= 0 && S >= 1 && W >= 1 && N >= 1 && R >= 1 && keep >= 0, "ccgqa_ring_fill: bad size");
   HYDRA_REQUIRE(keep <= R, "ccgqa_ring_fill: more rows than the ring holds");
   HYDRA_REQUIRE(M <= 65535 && S < (int64_t(1) << 31) && W < (int64_t(1) << 31) && N < (int64_t(1) << 31) &&
                     R < (1 << 20),
                 "ccgqa_ring_fill: too large");
   HYDRA_REQUIRE(dtype_size(dtype) > 0, "ccgqa_ring_fill: unknown dtype");
-  if (M == 0 || keep == 0) return HYDRA_OK;
+  // workgroups of a prompt that clear: one a row, up to 128
+  const int64_t past = clear ? std::min<int64_t>(S, 128) : 0;
+  if (M == 0 || keep + past == 0) return HYDRA_OK;
   HYDRA_REQUIRE(qkv && ring && lengths, "ccgqa_ring_fill: null pointer");
   HYDRA_REQUIRE(rows || M <= N, "ccgqa_ring_fill: more prompts than rows");
-  const dim3 grid(static_cast<unsigned>(keep), static_cast<unsigned>(M));
+  const dim3 grid(static_cast<unsigned>(keep + past), static_cast<unsigned>(M));
   auto st = static_cast<hipStream_t>(stream);
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
-    ring_fill_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(qkv), qkv_bs, qkv_rs, static_cast<T*>(ring), rows,
+    ring_fill_kernel<T><<<grid, 256, 0, st>>>(static_cast<T*>(qkv), qkv_bs, qkv_rs, static_cast<T*>(ring), rows,
                                               lengths, static_cast<int>(N), static_cast<int>(R), static_cast<int>(W),
-                                              static_cast<int>(S));
+                                              static_cast<int>(S), static_cast<int>(keep));
     return check_launch("ccgqa_ring_fill");
   });
 }

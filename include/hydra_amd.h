@@ -564,11 +564,12 @@ int64_t hydra_ccgqa_decode_prep_workspace(int64_t N, int64_t Hq, int64_t Hkv, in
 /* The last `keep` rows of prompts into such a ring: of qkv [M, S, W] (strides
  * qkv_bs, qkv_rs; unit columns), prompt m being request r = rows[m] (rows null:
  * m) of the ring's N, the rows s with lengths[r] - keep <= s < lengths[r] to
- * ring[r, s % R].  A request outside [0, N) or of a length outside [0, S]
- * leaves the ring as it is. */
-int hydra_ccgqa_ring_fill(const void* qkv, int64_t qkv_bs, int64_t qkv_rs, void* ring,
+ * ring[r, s % R].  With clear != 0 the rows s >= lengths[r] of qkv become zeros.  A
+ * request outside [0, N) or of a length outside [1, S] changes nothing. */
+int hydra_ccgqa_ring_fill(void* qkv, int64_t qkv_bs, int64_t qkv_rs, void* ring,
                           const int64_t* rows, const int* lengths, int64_t M, int64_t S,
-                          int64_t W, int64_t N, int64_t R, int64_t keep, int dtype, void* stream);
+                          int64_t W, int64_t N, int64_t R, int64_t keep, int clear, int dtype,
+                          void* stream);
 
 /* ---- block compositions (hydra/model/framework, hydra/layers) --------- */
 

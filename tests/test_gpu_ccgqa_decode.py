@@ -200,8 +200,23 @@ def test_ring_fill(cuda, dtype):
             for s in range(max(0, n - 4), n if n <= 11 else 0):
                 ring[r, s % 6] = qkv[m, s]
         assert torch.equal(got.cpu(), ring)
-    ccgqa_ring_fill(qkv.to(cuda), got, lens, 4, torch.tensor([-1, 7, 2**40, -2**40, 7], device=cuda))
+    ccgqa_ring_fill(qkv.to(cuda), got, lens, 4, torch.tensor([-1, 7, 2**40, -2**40, 7], device=cuda), clear=True)
     assert torch.equal(got.cpu(), ring)
+    # the rows past a prompt's end, in place, of requests alone and also without a row to keep
+    for keep in (4, 0):
+        for order in (None, rows, [7, 0, -1, 2, 1]):
+            x = qkv.clone()
+            wide = torch.full((5, 11, 50), 2.0, dtype=dtype, device=cuda)
+            wide[..., 1:49] = qkv.to(cuda)
+            ccgqa_ring_fill(wide[..., 1:49], got.clone(), lens, keep,
+                            None if order is None else torch.tensor(order, device=cuda), clear=True)
+            for m in range(5):
+                r = m if order is None else order[m]
+                if 0 <= r < 7 and 0 < lengths[r] <= 11:
+                    x[m, lengths[r]:] = 0
+            assert torch.equal(wide[..., 1:49].cpu(), x) and (wide[..., ::49] == 2).all()
+    with pytest.raises(ValueError, match="overlap"):
+        ccgqa_ring_fill(qkv.to(cuda)[:1].expand(5, 11, 48), got, lens, 4, clear=True)
 
 
 def layer(cuda, cfg, dtype, seed, max_seq_len=256):
@@ -252,6 +267,34 @@ def test_layer_prefill_and_decode(cuda, name, dtype, tol):
             else:
                 assert not out[n].any()
     assert pool.lengths.tolist() == at
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["debug", "hd64", "mha", "hd48", "noconv"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_padding_stays_out_whatever_it_holds(cuda, name, dtype, bad):
+    from hydra_amd.attention import PagePool
+
+    cfg = oc.CCGQAConfig(**CONFIGS[name])
+    m, _ = layer(cuda, cfg, dtype, seed=1)
+    prompts, S = [50, 64, 1, 33, 0], 64
+    x = torch.randn(5, S, cfg.dim, generator=torch.Generator().manual_seed(8)).to(cuda, dtype)
+    new = torch.tensor(prompts, dtype=torch.int32, device=cuda)
+    outs = []
+    for fill in (0.0, bad):
+        pool = PagePool(5, 96, 30, 16, device=cuda)
+        cache = m.new_cache(pool)
+        for n, p in enumerate(prompts):
+            x[n, p:] = fill
+        out = m.prefill(x, cache, pool.plan(new, width=S, from_empty=True))
+        step = m.decode(x[:, 0], cache, pool.plan((new > 0).int()))
+        assert not step[4].any()  # idle, its row of x padding
+        outs.append(([out[n, :p].clone() for n, p in enumerate(prompts)], step[:4], cache.ring[:4], cache.k_pages,
+                     cache.v_pages))
+    for a, b in zip(outs[0][0], outs[1][0]):
+        assert torch.equal(a, b)
+    assert all(torch.equal(a, b) for a, b in zip(outs[0][1:], outs[1][1:]))
+    assert all(t.isfinite().all() for t in (*outs[1][0], *outs[1][1:]))
 
 
 def test_prompts_join_a_running_batch(cuda):
