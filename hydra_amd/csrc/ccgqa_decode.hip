@@ -738,7 +738,8 @@ extern "C" int hydra_ccgqa_decode_prep(const void* qkv, int64_t qkv_rs, void* ri
   HYDRA_REQUIRE(!convs || (conv_ks >= 1 && conv_ks <= 16), "ccgqa_decode_prep: conv taps must be in [1, 16]");
   const int64_t back = std::max<int64_t>(convs ? 2 * (conv_ks - 1) : 0, flags & HYDRA_CCGQA_VALUE_SHIFT ? 1 : 0);
   HYDRA_REQUIRE(R > back && R < (1 << 20), "ccgqa_decode_prep: the ring must hold more rows than a token looks back");
-  HYDRA_REQUIRE(N <= 65535 && Hq <= 4096 && hd <= 4096, "ccgqa_decode_prep: too large");
+  HYDRA_REQUIRE(N <= 65535 && Hq <= 4096 && hd <= 4096 && pages < (int64_t(1) << 31),
+                "ccgqa_decode_prep: too large");
   const int64_t W = (Hq + 2 * Hkv) * hd;
   HYDRA_REQUIRE(qkv_rs >= W || N <= 1, "ccgqa_decode_prep: row stride < L + 2K");
   HYDRA_REQUIRE(dtype_size(dtype) > 0, "ccgqa_decode_prep: unknown dtype");

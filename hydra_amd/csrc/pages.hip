@@ -292,9 +292,9 @@ extern "C" int hydra_page_plan(const int* lengths, const int* new_tokens, int* t
   const int shift = page_shift(page_size);
   HYDRA_REQUIRE(shift >= 0, "page_plan: page_size must be a power of two in [16, 4096]");
   HYDRA_REQUIRE(table_rs >= P, "page_plan: table row stride < columns");
-  HYDRA_REQUIRE(N * P < (int64_t(1) << 31) && P * page_size < (int64_t(1) << 31) &&
-                    N * width < (int64_t(1) << 40) && N < (int64_t(1) << 31) && width < (int64_t(1) << 28) &&
-                    free_capacity < (int64_t(1) << 31),
+  HYDRA_REQUIRE(N < (int64_t(1) << 31) && P < (int64_t(1) << 31) && width < (int64_t(1) << 28) &&
+                    N * P < (int64_t(1) << 31) && P * page_size < (int64_t(1) << 31) &&
+                    N * width < (int64_t(1) << 40) && free_capacity < (int64_t(1) << 31),
                 "page_plan: too large");
   HYDRA_REQUIRE(lengths && new_tokens && table && free_count && slots && lengths_out && seen && granted && positions &&
                     free_out &&
@@ -326,7 +326,9 @@ extern "C" int hydra_page_release(const void* done, int* lengths, int* table, in
   const int shift = page_shift(page_size);
   HYDRA_REQUIRE(shift >= 0, "page_release: page_size must be a power of two in [16, 4096]");
   HYDRA_REQUIRE(table_rs >= P, "page_release: table row stride < columns");
-  HYDRA_REQUIRE(N * P < (int64_t(1) << 31) && free_capacity < (int64_t(1) << 31), "page_release: too large");
+  HYDRA_REQUIRE(N < (int64_t(1) << 31) && P < (int64_t(1) << 31) && N * P < (int64_t(1) << 31) &&
+                    free_capacity < (int64_t(1) << 31),
+                "page_release: too large");
   HYDRA_REQUIRE(done && lengths && table && free_pages && free_count, "page_release: null pointer");
   release_kernel<<<1, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(
       static_cast<const uint8_t*>(done), lengths, table, table_rs, free_pages, free_count, static_cast<int>(N),
@@ -345,7 +347,7 @@ extern "C" int hydra_page_store(const void* k, const void* v, void* k_pages, voi
   const int e = dtype_size(dtype);
   HYDRA_REQUIRE(e > 0, "page_store: unknown dtype");
   HYDRA_REQUIRE(N < (int64_t(1) << 31) && R < (int64_t(1) << 31) && S < (int64_t(1) << 31) && Hkv <= 65535 &&
-                    hd <= 65536,
+                    hd <= 65536 && pages < (int64_t(1) << 31),
                 "page_store: too large");
   if (N == 0 || S == 0) return HYDRA_OK;
   HYDRA_REQUIRE(k && v && k_pages && v_pages && slots && k_st && v_st && kp_st && vp_st, "page_store: null pointer");

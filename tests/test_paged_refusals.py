@@ -99,3 +99,77 @@ def test_python_entry_points_take_gpu_tensors_only():
     for kw in (dict(requests=0), dict(max_length=0), dict(pages=0), dict(page_size=24)):
         with pytest.raises(ValueError, match="PagePool"):
             PagePool(**{**dict(requests=2, max_length=64, pages=4, page_size=16, device="cpu"), **kw})
+
+
+def test_sizes_whose_products_overflow():
+    from hydra_amd import _lib
+
+    huge = 1 << 32
+    s = st(1, 1, 1, 1)
+    with pytest.raises(ValueError, match="too large"):
+        plan(N=huge, P=huge, rs=huge)
+    with pytest.raises(ValueError, match="too large"):
+        plan(N=16, P=1 << 60, rs=1 << 60)
+    with pytest.raises(ValueError, match="too large"):
+        _lib.call("hydra_page_release", FAKE, FAKE, FAKE, huge, FAKE, 8, FAKE, huge, huge, 16, None)
+    with pytest.raises(ValueError, match="too large"):
+        _lib.call("hydra_page_store", FAKE, FAKE, FAKE, FAKE, FAKE, 1, None, 1, 1, 1, 16, 1 << 60, 16, s, s, s, s, 1, None)
+    far = st(1, 1, 1 << 40, 1)
+    with pytest.raises(ValueError, match="too far apart"):
+        _lib.call("hydra_page_store", FAKE, FAKE, FAKE, FAKE, FAKE, 1, None, 1, 1, 1, 16, 4, 16, s, s, far, s, 1, None)
+    with pytest.raises(ValueError, match="too large"):
+        _lib.call("hydra_page_store", FAKE, FAKE, FAKE, FAKE, FAKE, 1, None, 1, 1, (1 << 31) - 1, 16, 4, 16, s, s, s, s, 1,
+                  None)
+
+
+def test_decode_prep_refusals():
+    from hydra_amd import _lib
+    from hydra_amd.attention.backends.ccgqa.ops import CCGQA_CONVS, CCGQA_QK_NORM, CCGQA_ROPE
+
+    def call(N=1, Hq=4, Hkv=2, hd=16, ks=3, flags=CCGQA_CONVS, R=5, rs=128, pages=4, page=16, w=FAKE, temp=FAKE,
+             cos=FAKE, last=1, dtype=1, q=FAKE):
+        p = st(1, 1, 1, last)
+        _lib.call("hydra_ccgqa_decode_prep", FAKE, rs, FAKE, R, FAKE, FAKE, w, w, w, w, temp, cos, cos, hd // 2, 64, q,
+                  FAKE, FAKE, p, p, pages, page, N, Hq, Hkv, hd, ks, flags, dtype, FAKE, 1 << 40, None)
+
+    for kw, text in ((dict(Hkv=3), "multiple"), (dict(hd=15), "even"), (dict(hd=0), "bad size"), (dict(R=4), "looks back"),
+                     (dict(ks=5), "looks back"), (dict(ks=17), "taps"), (dict(page=8), "power of two"),
+                     (dict(flags=1 << 20), "unknown flag"), (dict(N=2, rs=127), "row stride"), (dict(N=65536), "too large"),
+                     (dict(pages=1 << 60), "too large"), (dict(dtype=9), "unknown dtype"), (dict(w=None), "four weights"),
+                     (dict(flags=CCGQA_QK_NORM, temp=None), "temperature"), (dict(flags=CCGQA_ROPE, cos=None), "cos"),
+                     (dict(last=2), "unit stride"), (dict(q=None), "null"),
+                     (dict(flags=CCGQA_CONVS | _lib.CCGQA_W_TILED, dtype=0), "16-bit")):
+        with pytest.raises(ValueError, match=text):
+            call(**kw)
+    call(N=0)  # nothing to do
+
+    def fill(M=1, S=4, W=8, N=2, R=5, keep=4, rows=None, dtype=1, qkv=FAKE):
+        _lib.call("hydra_ccgqa_ring_fill", qkv, S * W, W, FAKE, rows, FAKE, M, S, W, N, R, keep, 1, dtype, None)
+
+    for kw, text in ((dict(keep=6), "more rows"), (dict(M=3), "more prompts"), (dict(S=0), "bad size"), (dict(N=0), "bad size"),
+                     (dict(M=65536, N=65536), "too large"), (dict(dtype=5), "unknown dtype"), (dict(qkv=None), "null")):
+        with pytest.raises(ValueError, match=text):
+            fill(**kw)
+    fill(M=0)
+
+
+def test_token_logprobs_refusals():
+    from hydra_amd import _lib
+
+    def call(rows=2, V=100, rs=100, top=4, T=1.0, dtype=1, x=FAKE, ids=FAKE):
+        _lib.call("hydra_token_logprobs", x, rows, V, rs, FAKE, T, top, FAKE, FAKE, None, FAKE, ids, dtype, None)
+
+    def grad(rows=2, V=100, rs=100, top=4, T=1.0, dtype=1, x=FAKE, ids=FAKE):
+        _lib.call("hydra_token_logprobs_bwd", x, rows, V, rs, FAKE, T, top, FAKE, FAKE, ids, FAKE, FAKE, FAKE, FAKE, dtype,
+                  None)
+
+    for kw, text in ((dict(V=0), "bad size"), (dict(rows=-1), "bad size"), (dict(V=1 << 30), "too large"),
+                     (dict(rows=1 << 31), "too large"), (dict(rs=-1), "negative"), (dict(top=65), "top_k"),
+                     (dict(V=3), "top_k"), (dict(T=0.0), "temperature"), (dict(T=float("nan")), "temperature"),
+                     (dict(dtype=4), "unknown dtype"), (dict(x=None), "null"), (dict(ids=None), "null"),
+                     (dict(x=FAKE + 1), "misaligned")):
+        for entry in (call, grad):
+            with pytest.raises(ValueError, match=text):
+                entry(**kw)
+    call(rows=0)
+    grad(rows=0)
