@@ -91,6 +91,16 @@ def test_many_requests(cuda, N):
     check(make(lengths, 8, 4, 16, 16, torch.bfloat16, seed=N, P=64), cuda)
 
 
+@pytest.mark.parametrize("N", [63, 64, 65, 300, 1000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_requests_are_split(cuda, N, dtype):
+    """Prefix sums of the requests' rounds in a wave's lanes (64 and fewer) and
+    in LDS; runs of requests without keys, a long one among short ones."""
+    lengths = [0 if i % 5 == 2 or 20 < i < 40 else (i * 61) % 170 for i in range(N)]
+    lengths[N // 2] = 2500
+    check(make(lengths, 4, 2, 32, 16, dtype, seed=N, P=160), cuda)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
 def test_scale(cuda, scale):
     check(make([40, 600], 4, 2, 32, 32, torch.bfloat16, seed=3), cuda, scale=scale)
