@@ -242,6 +242,10 @@ class CCGQAAttention(nn.Module):
                              f"({self.cos_cached.shape[2]})")
         if self.head_dim > 256:
             raise ValueError(f"CCGQAAttention: a cache takes head_dim up to 256, not {self.head_dim}")
+        if self.use_convs and not (self.conv_kernel_size == 3 and self.head_dim in (16, 32, 64, 128)) and \
+                self.conv_kernel_size * self.latent_dim + self.head_dim > 16384:
+            raise ValueError(f"CCGQAAttention: a cache takes {self.conv_kernel_size} taps of {self.latent_dim} "
+                             f"channels only at three taps and head_dim 16, 32, 64 or 128")
         if pool.table.device != w.device:
             raise RuntimeError(f"CCGQAAttention: the pool is on {pool.table.device}, the layer on {w.device}")
         return CCGQACache(self, pool, dtype or w.dtype)

@@ -173,3 +173,22 @@ def test_token_logprobs_refusals():
                 entry(**kw)
     call(rows=0)
     grad(rows=0)
+
+
+def test_layers_that_have_no_cache():
+    """What the one-token kernels do not take is refused before a prompt enters."""
+    from hydra_amd.attention import CCGQAAttention, PagePool
+
+    pool = PagePool(2, 64, 4, 16, device="cpu")
+    for kw, text in ((dict(dim=4096, n_heads=64, n_kv_heads=2, conv_kernel_size=5), "5 taps of 4096"),
+                     (dict(dim=6144, n_heads=128, n_kv_heads=2), "3 taps of 6144"),
+                     (dict(dim=1024, n_heads=2, n_kv_heads=1), "up to 256"),
+                     (dict(dim=256, n_heads=4, n_kv_heads=2, max_seq_len=63), "RoPE cache")):
+        with torch.device("meta"):
+            m = CCGQAAttention(compression_factor=1, **{**dict(max_seq_len=64), **kw})
+        with pytest.raises(ValueError, match=text):
+            m.new_cache(pool)
+    with torch.device("meta"):
+        m = CCGQAAttention(dim=256, n_heads=4, n_kv_heads=2, max_seq_len=64)
+    with pytest.raises(RuntimeError, match="the pool is on cpu"):
+        m.new_cache(pool)
