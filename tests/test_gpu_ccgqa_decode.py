@@ -159,6 +159,29 @@ def test_idle_requests_change_nothing(cuda, name):
     check(cfg, dtype, params, rows[:1], ring[:1], positions[:1], slots[:1], page, (q[:1], kp, vp, kept[:1], tables))
 
 
+@pytest.mark.parametrize("name", ["hd128", "hd48"])
+def test_pages_past_32_bits(cuda, name):
+    """A slot in the last page of a pool of more than 2^32 bytes is written like
+    one of a small pool."""
+    from hydra_amd.attention.backends.ccgqa.ops import ccgqa_decode_prep
+    from oracle.fused_ops import rope_cache
+
+    cfg, dtype, page = oc.CCGQAConfig(**CONFIGS[name]), torch.bfloat16, 4096
+    params, rows, ring = case(cfg, [9], dtype, seed=4)
+    cos, sin = (t.to(cuda) for t in rope_cache(cfg.head_dim, 16))
+    many = (1 << 32) // (page * cfg.kv_dim * 2) + 2
+    outs = []
+    for pages in (2, many):
+        kp, vp = (torch.zeros(pages, cfg.n_kv_heads, page, cfg.head_dim, dtype=dtype, device=cuda) for _ in range(2))
+        q = ccgqa_decode_prep(rows[0][-1:].to(cuda), ring.to(cuda), torch.tensor([9], dtype=torch.int32, device=cuda),
+                              torch.tensor([pages * page - 5], device=cuda), kp, vp, cfg.n_heads, cfg.n_kv_heads,
+                              cfg.head_dim, flags_of(cfg), *weights_of(params, cfg, cuda, dtype),
+                              temperature=params["key_temperature"].to(cuda), cos=cos, sin=sin)
+        outs.append((q, kp[-1].clone(), vp[-1].clone()))
+        assert kp[-1, :, -5].any() and not kp[:-1].any() and not vp[:-1].any()
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 def test_bf16_tables_and_strided_rows(cuda):
     from hydra_amd.attention.backends.ccgqa.ops import ccgqa_decode_prep
     from oracle.fused_ops import rope_cache

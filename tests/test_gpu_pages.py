@@ -196,6 +196,22 @@ def test_store_by_rows(cuda):
             store_pages(k.to(cuda), v.to(cuda), *got, slots.to(cuda), rows=bad)
 
 
+def test_store_past_32_bits(cuda):
+    """The last page of a pool of more than 2^32 bytes and 2^31 elements."""
+    from hydra_amd.attention import store_pages
+
+    page, K, hd = 4096, 8, 128
+    pages = (1 << 32) // (page * K * hd * 2) + 8
+    kp, vp = (torch.zeros(pages, K, page, hd, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    assert kp.numel() > 2**31
+    k, v = (torch.randn(1, K, 3, hd, generator=torch.Generator().manual_seed(i)).to(cuda, torch.bfloat16) for i in (1, 2))
+    last = pages * page - 1
+    store_pages(k, v, kp, vp, torch.tensor([[last, last + 1, last - page]], device=cuda))
+    for pool, x in ((kp, k), (vp, v)):
+        assert torch.equal(pool[-1, :, -1], x[0, :, 0]) and torch.equal(pool[-2, :, -1], x[0, :, 2])
+        assert not pool[:-2].any() and not pool[-2:, :, :-1].any()
+
+
 def test_refusals(cuda):
     from hydra_amd.attention import plan_pages, release_pages, store_pages
 
