@@ -987,7 +987,7 @@ static int rms_norm_bwd_check(const void* x, const void* w, const void* grad_y, 
   HYDRA_REQUIRE(rows >= 0 && dim >= 1, "rms_norm_bwd: rows must be >= 0 and dim >= 1");
   HYDRA_REQUIRE(dim <= (int64_t(1) << 24), "rms_norm_bwd: dim too large");
   HYDRA_REQUIRE(x_rs >= dim && gy_rs >= dim && gx_rs >= dim, "rms_norm_bwd: row stride smaller than dim");
-  HYDRA_REQUIRE(x && w && grad_y && grad_x && grad_w, "rms_norm_bwd: null pointer");
+  HYDRA_REQUIRE(w && grad_w && (rows == 0 || (x && grad_y && grad_x)), "rms_norm_bwd: null pointer");
   HYDRA_REQUIRE(dtype_size(dtype) > 0, "rms_norm_bwd: unknown dtype code");
   HYDRA_REQUIRE(w_dtype == dtype || w_dtype == HYDRA_F32,
                 "rms_norm_bwd: the weight must be of x's dtype or fp32");
