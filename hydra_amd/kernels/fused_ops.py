@@ -14,6 +14,7 @@ the GPU.
 """
 from __future__ import annotations
 
+import math
 import os
 from typing import Tuple
 
@@ -215,19 +216,25 @@ def fused_qk_norm(q: torch.Tensor, k: torch.Tensor, scale: float,
 # ---------------------------------------------------------------------------
 def _rows_view(t: torch.Tensor):
     """(rows, row_stride) when t is a 2-D-collapsible view with unit stride on
-    the last dim (e.g. one half of a gate_up.chunk(2)); else None."""
-    if t.dim() == 0 or t.stride(-1) != 1:
+    the last dim (e.g. one half of a gate_up.chunk(2)); else None.  The strides
+    of dimensions of one element say nothing and are not looked at; a
+    contiguous tensor always has rows."""
+    if t.dim() == 0:
         return None
-    if t.dim() == 1:
-        return 1, t.shape[-1]
-    rs = t.stride(-2)
-    rows = 1
-    expect = rs
-    for d in range(t.dim() - 2, -1, -1):
-        if t.shape[d] != 1 and t.stride(d) != expect:
+    if 0 in t.shape:  # nothing to walk
+        return math.prod(t.shape[:-1]), t.shape[-1]
+    if t.shape[-1] != 1 and t.stride(-1) != 1:
+        return None
+    rows, rs, expect = 1, t.shape[-1], None
+    for n, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if expect is None:
+            rs = stride
+        elif stride != expect:
             return None
-        rows *= t.shape[d]
-        expect = expect * t.shape[d]
+        rows *= n
+        expect = stride * n
     return rows, rs
 
 
