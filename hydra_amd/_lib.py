@@ -70,6 +70,7 @@ SIGNATURES = {
     "hydra_page_plan": [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P],
     "hydra_page_plan_in_place": [_I64, _I64],
     "hydra_page_release": [_P, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
+    "hydra_pool_release": [_P, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P],
     "hydra_page_store": [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
                          _I64P, _I, _P],
     "hydra_paged_attn": [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,

@@ -134,11 +134,12 @@ def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Ten
 
 
 def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
-                  free_count: torch.Tensor, page_size: int) -> None:
+                  free_count: torch.Tensor, page_size: int, pages: Optional[int] = None) -> None:
     """Puts the pages of the requests with `done` (bool [N]) back on the
-    stack, in place: their lengths become 0, their table entries -1.  A page
-    belongs to one request: one that several tables name would come back more
-    than once."""
+    stack, in place: their lengths become 0, their table entries -1.  Entries
+    that are no page (negative, or not below `pages`, where that is given) do
+    not come back.  A page belongs to one request: one that several tables name
+    would come back more than once."""
     name = "release_pages"
     _lib.require_gpu(name, done, lengths, table, free_pages, free_count)
     N = _vector(name, "lengths", lengths, torch.int32).shape[0]
@@ -151,10 +152,11 @@ def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     if N == 0 or table.shape[1] == 0 or free_pages.numel() == 0:
         return
     done = done.contiguous()
+    within = () if pages is None else (int(pages),)
     with _lib.on_device(lengths):
-        _lib.call("hydra_page_release", done.data_ptr(), lengths.data_ptr(), table.data_ptr(), table.stride(0),
-                  free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), N, table.shape[1],
-                  int(page_size), _lib.stream(lengths))
+        _lib.call("hydra_pool_release" if within else "hydra_page_release", done.data_ptr(), lengths.data_ptr(),
+                  table.data_ptr(), table.stride(0), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+                  N, table.shape[1], int(page_size), *within, _lib.stream(lengths))
 
 
 def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -279,4 +281,4 @@ class PagePool:
         return plan
 
     def release(self, done: torch.Tensor) -> None:
-        release_pages(done, self.lengths, self.table, self.free_pages, self.free_count, self.page_size)
+        release_pages(done, self.lengths, self.table, self.free_pages, self.free_count, self.page_size, self.pages)

@@ -165,14 +165,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 }
 
 // The pages of the requests that are done go back on the stack, in the order
-// of the requests; their lengths become 0 and their table entries -1.  One
-// workgroup: the stack has one top.  Its threads take the pages of 256 requests
-// in their order on the stack and look up whose each is; bound by the launch and
-// the chain lengths -> sums -> table -> stack: 2 us
-// behind another kernel for 32 of 256 requests with 16 pages each.
+// of the requests; their lengths become 0 and their table entries -1.  Entries
+// that are no page (outside [0, pages)) do not come back: the next plan would
+// hand them to another request.  One workgroup: the stack has one top.  Its
+// threads take the entries of 256 requests in their order, four neighbouring
+// ones each, look up whose they are and count the pages among them; bound by the
+// launch and the chain lengths -> sums -> table -> sums -> stack.
+constexpr int kReleaseEntries = 4;
+
 __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* done, int* lengths, int* table,
                                                                int64_t table_rs, int* free_pages, int* free_count,
-                                                               int N, int P, int F, int shift) {
+                                                               int N, int P, int F, int pages, int shift) {
+  constexpr int U = kReleaseEntries;
   __shared__ int part[kPlanThreads / 64];
   __shared__ int s_upto[kPlanThreads];
   const int tid = threadIdx.x;
@@ -183,24 +187,40 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
     int count = 0;
     if (i < N && done[i]) {
       const int64_t len = lengths[i];
-      const int64_t pages = len <= 0 ? 0 : (len + (int64_t(1) << shift) - 1) >> shift;
-      count = static_cast<int>(pages < P ? pages : P);
+      const int64_t held = len <= 0 ? 0 : (len + (int64_t(1) << shift) - 1) >> shift;
+      count = static_cast<int>(held < P ? held : P);
       lengths[i] = 0;
     }
     int step;
     const int upto = block_incl_sum(count, part, step);
     s_upto[tid] = upto;
     __syncthreads();
-    for (int e = tid; e < step; e += kPlanThreads) {
-      int at = 0;  // the first request with s_upto > e
+    for (int e0 = 0; e0 < step; e0 += kPlanThreads * U) {
+      int page[U], mine = 0;
 #pragma unroll
-      for (int half = kPlanThreads / 2; half > 0; half >>= 1)
-        if (s_upto[at + half - 1] <= e) at += half;
-      int* entry = table + static_cast<int64_t>(i0 + at) * table_rs + (e - (at > 0 ? s_upto[at - 1] : 0));
-      if (free + e < F) free_pages[free + e] = *entry;
-      *entry = -1;
+      for (int u = 0; u < U; ++u) {
+        const int e = e0 + tid * U + u;
+        page[u] = -1;
+        if (e >= step) continue;
+        int at = 0;  // the first request with s_upto > e
+#pragma unroll
+        for (int half = kPlanThreads / 2; half > 0; half >>= 1)
+          if (s_upto[at + half - 1] <= e) at += half;
+        int* entry = table + static_cast<int64_t>(i0 + at) * table_rs + (e - (at > 0 ? s_upto[at - 1] : 0));
+        page[u] = *entry < pages ? *entry : -1;
+        mine += page[u] >= 0;
+        *entry = -1;
+      }
+      int all;
+      int to = free + block_incl_sum(mine, part, all) - mine;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (page[u] < 0) continue;
+        if (to < F) free_pages[to] = page[u];
+        ++to;
+      }
+      free = min(F, free + all);
     }
-    free = min(F, free + step);
     __syncthreads();
   }
   if (tid == 0) *free_count = free;
@@ -322,17 +342,24 @@ extern "C" int hydra_page_plan_in_place(int64_t N, int64_t width) {
 extern "C" int hydra_page_release(const void* done, int* lengths, int* table, int64_t table_rs, int* free_pages,
                                   int64_t free_capacity, int* free_count, int64_t N, int64_t P, int64_t page_size,
                                   void* stream) {
-  HYDRA_REQUIRE(N >= 1 && P >= 1 && free_capacity >= 1, "page_release: bad size");
+  return hydra_pool_release(done, lengths, table, table_rs, free_pages, free_capacity, free_count, N, P, page_size,
+                            INT32_MAX, stream);
+}
+
+extern "C" int hydra_pool_release(const void* done, int* lengths, int* table, int64_t table_rs, int* free_pages,
+                                  int64_t free_capacity, int* free_count, int64_t N, int64_t P, int64_t page_size,
+                                  int64_t pages, void* stream) {
+  HYDRA_REQUIRE(N >= 1 && P >= 1 && free_capacity >= 1 && pages >= 1, "page_release: bad size");
   const int shift = page_shift(page_size);
   HYDRA_REQUIRE(shift >= 0, "page_release: page_size must be a power of two in [16, 4096]");
   HYDRA_REQUIRE(table_rs >= P, "page_release: table row stride < columns");
   HYDRA_REQUIRE(N < (int64_t(1) << 31) && P < (int64_t(1) << 31) && N * P < (int64_t(1) << 31) &&
-                    free_capacity < (int64_t(1) << 31),
+                    free_capacity < (int64_t(1) << 31) && pages < (int64_t(1) << 31),
                 "page_release: too large");
   HYDRA_REQUIRE(done && lengths && table && free_pages && free_count, "page_release: null pointer");
   release_kernel<<<1, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(
       static_cast<const uint8_t*>(done), lengths, table, table_rs, free_pages, free_count, static_cast<int>(N),
-      static_cast<int>(P), static_cast<int>(free_capacity), shift);
+      static_cast<int>(P), static_cast<int>(free_capacity), static_cast<int>(pages), shift);
   return check_launch("page_release");
 }
 

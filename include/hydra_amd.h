@@ -501,10 +501,15 @@ int hydra_page_plan(const int* lengths, const int* new_tokens, int* table, int64
 int hydra_page_plan_in_place(int64_t N, int64_t width);
 
 /* Puts the pages of the requests with done[i] != 0 (bytes) back on the stack,
- * in order, in place: their lengths become 0, their table entries -1. */
+ * in order, in place: their lengths become 0, their table entries -1.  Negative
+ * entries are no pages and do not come back. */
 int hydra_page_release(const void* done, int* lengths, int* table, int64_t table_rs,
                        int* free_pages, int64_t free_capacity, int* free_count, int64_t N,
                        int64_t P, int64_t page_size, void* stream);
+/* The same for a pool of `pages` pages: entries from there on are none either. */
+int hydra_pool_release(const void* done, int* lengths, int* table, int64_t table_rs,
+                       int* free_pages, int64_t free_capacity, int* free_count, int64_t N,
+                       int64_t P, int64_t page_size, int64_t pages, void* stream);
 
 /* Rows k, v [N, Hkv, S, hd] (element strides k_st[4], v_st[4]; unit last) to
  * their slots in k_pages, v_pages [pages, Hkv, page_size, hd] (strides kp_st[4],

@@ -39,16 +39,17 @@ def plan(lengths, new_tokens, table, free_pages, free_count, page_size, width, f
     return slots, after, seen, granted, left, table
 
 
-def release(done, lengths, table, free_pages, free_count, page_size):
+def release(done, lengths, table, free_pages, free_count, page_size, pages=None):
     """(lengths, table, free_pages, free_count) after the requests with `done`
-    have given their pages back."""
+    have given their pages back; entries that are no page (negative, or not
+    below `pages`) do not come back."""
     lengths, table, free_pages = list(lengths), [list(r) for r in table], list(free_pages)
     top = max(0, min(free_count, len(free_pages)))
     for i, d in enumerate(done):
         if not d:
             continue
         for c in range(min(len(table[i]), max(0, -(-lengths[i] // page_size)))):
-            if top < len(free_pages):
+            if table[i][c] >= 0 and (pages is None or table[i][c] < pages) and top < len(free_pages):
                 free_pages[top] = table[i][c]
                 top += 1
             table[i][c] = -1
