@@ -195,31 +195,32 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
     const int upto = block_incl_sum(count, part, step);
     s_upto[tid] = upto;
     __syncthreads();
-    for (int e0 = 0; e0 < step; e0 += kPlanThreads * U) {
+    // the last trip's indexes, and a full stack's, may pass an int
+    for (int64_t e0 = 0; e0 < step; e0 += kPlanThreads * U) {
       int page[U], mine = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int e = e0 + tid * U + u;
+        const int64_t e = e0 + tid * U + u;
         page[u] = -1;
         if (e >= step) continue;
         int at = 0;  // the first request with s_upto > e
 #pragma unroll
         for (int half = kPlanThreads / 2; half > 0; half >>= 1)
           if (s_upto[at + half - 1] <= e) at += half;
-        int* entry = table + static_cast<int64_t>(i0 + at) * table_rs + (e - (at > 0 ? s_upto[at - 1] : 0));
+        int* entry = table + (i0 + at) * table_rs + (e - (at > 0 ? s_upto[at - 1] : 0));
         page[u] = *entry < pages ? *entry : -1;
         mine += page[u] >= 0;
         *entry = -1;
       }
       int all;
-      int to = free + block_incl_sum(mine, part, all) - mine;
+      int64_t to = static_cast<int64_t>(free) + block_incl_sum(mine, part, all) - mine;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (page[u] < 0) continue;
         if (to < F) free_pages[to] = page[u];
         ++to;
       }
-      free = min(F, free + all);
+      free = static_cast<int>(min(static_cast<int64_t>(F), static_cast<int64_t>(free) + all));
     }
     __syncthreads();
   }

@@ -1,4 +1,5 @@
-"""GPU tests of what bounds a pool of pages: entries that are no page."""
+"""GPU tests of what bounds a pool of pages: entries that are no page,
+stacks near the reach of an int."""
 from __future__ import annotations
 
 import random
@@ -56,3 +57,25 @@ def test_a_damaged_entry_costs_its_own_request_alone(cuda):
     assert plan.granted.all()
     held = plan.slots[1].tolist() + plan.slots[2, :32].tolist()
     assert all(0 <= s < 8 * 16 for s in held) and len(set(held)) == 96
+
+
+def test_release_onto_a_full_stack_of_the_largest_size(cuda):
+    """What finds no room is dropped, also where the stack's height and the
+    pages together pass an int."""
+    from hydra_amd.attention import release_pages
+
+    cap = 2**31 - 1
+    stack = torch.empty(cap, dtype=torch.int32, device=cuda)
+    stack[-100:] = 7
+    for free in (cap, cap - 2, cap - 40, cap - 90):
+        table = torch.arange(80, dtype=torch.int32, device=cuda).view(2, 40)
+        lengths, height = ints([640, 600], cuda), ints([free], cuda)
+        release_pages(torch.tensor([True, True], device=cuda), lengths, table, stack, height, 16)
+        assert height.tolist() == [min(cap, free + 78)] and lengths.tolist() == [0, 0]
+        want = [7] * 100
+        for j, page in enumerate([*range(40), *range(40, 78)]):
+            if free + j < cap:
+                want[100 - (cap - free) + j] = page
+        assert stack[-100:].tolist() == want
+        assert table.tolist() == [[-1] * 40, [-1] * 38 + [78, 79]]
+        stack[-100:] = 7
