@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kPlanThreads = 256;
 constexpr int kPlanTokens = 4096;  // tokens of a request that one workgroup writes
+constexpr int64_t kMaxPlanned = int64_t(1) << 24;  // requests: each workgroup of a plan goes over those before it
 
 struct PlanArgs {
   const int* lengths;  // may be lengths_out (see hydra_page_plan_in_place)
@@ -313,7 +314,7 @@ extern "C" int hydra_page_plan(const int* lengths, const int* new_tokens, int* t
   const int shift = page_shift(page_size);
   HYDRA_REQUIRE(shift >= 0, "page_plan: page_size must be a power of two in [16, 4096]");
   HYDRA_REQUIRE(table_rs >= P, "page_plan: table row stride < columns");
-  HYDRA_REQUIRE(N < (int64_t(1) << 31) && P < (int64_t(1) << 31) && width < (int64_t(1) << 28) &&
+  HYDRA_REQUIRE(N <= kMaxPlanned && P < (int64_t(1) << 31) && width < (int64_t(1) << 28) &&
                     N * P < (int64_t(1) << 31) && P * page_size < (int64_t(1) << 31) &&
                     N * width < (int64_t(1) << 40) && free_capacity < (int64_t(1) << 31),
                 "page_plan: too large");
@@ -354,7 +355,7 @@ extern "C" int hydra_pool_release(const void* done, int* lengths, int* table, in
   const int shift = page_shift(page_size);
   HYDRA_REQUIRE(shift >= 0, "page_release: page_size must be a power of two in [16, 4096]");
   HYDRA_REQUIRE(table_rs >= P, "page_release: table row stride < columns");
-  HYDRA_REQUIRE(N < (int64_t(1) << 31) && P < (int64_t(1) << 31) && N * P < (int64_t(1) << 31) &&
+  HYDRA_REQUIRE(N <= kMaxPlanned && P < (int64_t(1) << 31) && N * P < (int64_t(1) << 31) &&
                     free_capacity < (int64_t(1) << 31) && pages < (int64_t(1) << 31),
                 "page_release: too large");
   HYDRA_REQUIRE(done && lengths && table && free_pages && free_count, "page_release: null pointer");

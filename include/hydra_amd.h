@@ -475,9 +475,10 @@ int hydra_token_logprobs_bwd(const void* logits, int64_t rows, int64_t vocab, in
 /* A cache is a pool of pages, k and v [pages, Hkv, page_size, hd]; position t
  * of request i lies in page table[i, t / page_size], row t % page_size; its
  * slot is page * page_size + row.  page_size: a power of two in [16, 4096].
- * Tables, lengths and counts are int32, slots int64.  What the device finds
- * wrong (a request without room, an entry outside the pool) costs only the
- * request it belongs to: no host synchronisation, no access out of bounds. */
+ * Tables, lengths and counts are int32, slots int64; at most 2^24 requests are
+ * planned or released at once.  What the device finds wrong (a request without
+ * room, an entry outside the pool) costs only the request it belongs to: no host
+ * synchronisation, no access out of bounds. */
 
 /* Plans a step that adds new_tokens[i] tokens to request i, which holds
  * lengths[i].  Request i fits if 0 <= lengths[i], 0 <= new_tokens[i] <= width
