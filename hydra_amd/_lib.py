@@ -68,6 +68,7 @@ SIGNATURES = {
     "hydra_token_logprobs": [_P, _I64, _I64, _I64, _P, _F, _I64, _P, _P, _P, _P, _P, _I, _P],
     "hydra_token_logprobs_bwd": [_P, _I64, _I64, _I64, _P, _F, _I64, _P, _P, _P, _P, _P, _P, _P, _I, _P],
     "hydra_page_plan": [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P],
+    "hydra_pool_plan": [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P],
     "hydra_page_plan_in_place": [_I64, _I64],
     "hydra_page_release": [_P, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
     "hydra_pool_release": [_P, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P],

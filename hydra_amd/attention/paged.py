@@ -92,7 +92,8 @@ def _strides(t: torch.Tensor):
     return _lib._stride_array((*t.stride()[:-1], 1)) if t.shape[-1] == 1 else _lib.strides(t)
 
 
-def _plan(name, lengths, new_tokens, table, free_pages, free_count, page_size, width, from_empty, in_place):
+def _plan(name, lengths, new_tokens, table, free_pages, free_count, page_size, width, from_empty,
+          max_length=None, in_place=False):
     _lib.require_gpu(name, lengths, new_tokens, table, free_pages, free_count)
     N = _vector(name, "lengths", lengths, torch.int32).shape[0]
     _vector(name, "new_tokens", new_tokens, torch.int32, N)
@@ -108,11 +109,13 @@ def _plan(name, lengths, new_tokens, table, free_pages, free_count, page_size, w
     after, seen, positions, left = lengths.new_empty((3 * N + 1,)).split((N, N, N, 1))
     if in_place:
         after, left = lengths, free_count
+    within = () if max_length is None else (max_length,)
     with _lib.on_device(lengths):
-        _lib.call("hydra_page_plan", lengths.data_ptr(), new_tokens.data_ptr(), table.data_ptr(), table.stride(0),
-                  free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), slots.data_ptr(),
-                  after.data_ptr(), seen.data_ptr(), granted.data_ptr(), positions.data_ptr(), left.data_ptr(),
-                  N, table.shape[1], width, int(page_size), 1 if from_empty else 0, _lib.stream(lengths))
+        _lib.call("hydra_pool_plan" if within else "hydra_page_plan", lengths.data_ptr(), new_tokens.data_ptr(),
+                  table.data_ptr(), table.stride(0), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+                  slots.data_ptr(), after.data_ptr(), seen.data_ptr(), granted.data_ptr(), positions.data_ptr(),
+                  left.data_ptr(), N, table.shape[1], width, int(page_size), *within, 1 if from_empty else 0,
+                  _lib.stream(lengths))
     return PagePlan(slots, positions, after, seen, granted, left, bool(from_empty))
 
 
@@ -130,7 +133,7 @@ def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Ten
     tokens and counts are int32 on the GPU, and stay as they are: copy
     `plan.lengths` and `plan.free_count` over them when the step is taken
     (PagePool does)."""
-    return _plan("plan_pages", lengths, new_tokens, table, free_pages, free_count, page_size, width, from_empty, False)
+    return _plan("plan_pages", lengths, new_tokens, table, free_pages, free_count, page_size, width, from_empty)
 
 
 def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
@@ -245,9 +248,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 class PagePool:
-    """The pages of up to `requests` requests of up to `max_length` tokens:
-    which pages each holds and which nobody does.  Layers keep their keys and
-    values in pools of `pages` pages of their own and share this.
+    """The pages of up to `requests` requests of up to `max_length` tokens
+    (whatever the page size: a plan refuses what goes past it): which pages each
+    holds and which nobody does.  Layers keep their keys and values in pools of
+    `pages` pages of their own and share this.
 
     `plan(new_tokens, width)` takes a step's pages and moves the lengths on;
     `release(done)` returns finished requests' pages.  All of it runs on the
@@ -260,9 +264,9 @@ class PagePool:
         if page_size not in (16, 32, 64, 128, 256, 512, 1024, 2048, 4096):
             raise ValueError(f"PagePool: page_size {page_size} is no power of two in [16, 4096]")
         self.requests, self.pages, self.page_size = int(requests), int(pages), int(page_size)
-        self.max_length = -(-int(max_length) // self.page_size) * self.page_size
+        self.max_length = int(max_length)
         self.lengths = torch.zeros(self.requests, dtype=torch.int32, device=device)
-        self.table = torch.full((self.requests, self.max_length // self.page_size), -1, dtype=torch.int32,
+        self.table = torch.full((self.requests, -(-self.max_length // self.page_size)), -1, dtype=torch.int32,
                                 device=device)
         self.free_pages = torch.arange(self.pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), self.pages, dtype=torch.int32, device=device)
@@ -273,7 +277,7 @@ class PagePool:
         width = int(width)
         in_place = _lib.query("hydra_page_plan_in_place", self.requests, width) == 1
         plan = _plan("PagePool.plan", self.lengths, new_tokens, self.table, self.free_pages, self.free_count,
-                     self.page_size, width, from_empty, in_place)
+                     self.page_size, width, from_empty, self.max_length, in_place)
         if not in_place:
             self.lengths.copy_(plan.lengths)
             self.free_count.copy_(plan.free_count)

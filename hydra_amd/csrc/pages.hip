@@ -29,7 +29,8 @@ struct PlanArgs {
   int* seen;
   uint8_t* granted;
   int *positions, *free_out;
-  int N, P, F, width, shift, slice, from_empty;
+  int64_t limit;  // tokens of a request at most
+  int N, F, width, shift, slice, from_empty;
 };
 
 struct Need {
@@ -38,15 +39,15 @@ struct Need {
   bool fits;
 };
 
-// What request i asks for: pages held, pages more, and whether its own table
-// row and the step's width hold it.
+// What request i asks for: pages held, pages more, and whether the longest
+// request and the step's width allow it.
 __device__ __forceinline__ Need need_of(const PlanArgs& a, int i) {
   Need r{0, 0, 0, 0, false};
   if (i >= a.N) return r;
   r.len = a.lengths[i];
   r.add = a.fresh[i];
   const int64_t page = int64_t(1) << a.shift;
-  r.fits = r.len >= 0 && r.add >= 0 && r.add <= a.width && r.len + r.add <= (static_cast<int64_t>(a.P) << a.shift) &&
+  r.fits = r.len >= 0 && r.add >= 0 && r.add <= a.width && r.len + r.add <= a.limit &&
            (!a.from_empty || r.len == 0 || r.add == 0);
   if (r.fits) {
     r.have = static_cast<int>((r.len + page - 1) >> a.shift);
@@ -310,7 +311,17 @@ extern "C" int hydra_page_plan(const int* lengths, const int* new_tokens, int* t
                                const int* free_pages, int64_t free_capacity, const int* free_count, int64_t* slots,
                                int* lengths_out, int* seen, void* granted, int* positions, int* free_out,
                                int64_t N, int64_t P, int64_t width, int64_t page_size, int from_empty, void* stream) {
-  HYDRA_REQUIRE(N >= 1 && P >= 1 && width >= 1 && free_capacity >= 0, "page_plan: bad size");
+  return hydra_pool_plan(lengths, new_tokens, table, table_rs, free_pages, free_capacity, free_count, slots,
+                         lengths_out, seen, granted, positions, free_out, N, P, width, page_size, INT64_MAX, from_empty,
+                         stream);
+}
+
+extern "C" int hydra_pool_plan(const int* lengths, const int* new_tokens, int* table, int64_t table_rs,
+                               const int* free_pages, int64_t free_capacity, const int* free_count, int64_t* slots,
+                               int* lengths_out, int* seen, void* granted, int* positions, int* free_out,
+                               int64_t N, int64_t P, int64_t width, int64_t page_size, int64_t max_length,
+                               int from_empty, void* stream) {
+  HYDRA_REQUIRE(N >= 1 && P >= 1 && width >= 1 && free_capacity >= 0 && max_length >= 0, "page_plan: bad size");
   const int shift = page_shift(page_size);
   HYDRA_REQUIRE(shift >= 0, "page_plan: page_size must be a power of two in [16, 4096]");
   HYDRA_REQUIRE(table_rs >= P, "page_plan: table row stride < columns");
@@ -325,8 +336,9 @@ extern "C" int hydra_page_plan(const int* lengths, const int* new_tokens, int* t
   HYDRA_REQUIRE((lengths_out != lengths && free_out != free_count) || hydra_page_plan_in_place(N, width) == 1,
                 "page_plan: in place takes a step that one workgroup plans");
   PlanArgs a{lengths, new_tokens, table, table_rs, free_pages, free_count, slots, lengths_out, seen,
-             static_cast<uint8_t*>(granted), positions, free_out, static_cast<int>(N), static_cast<int>(P),
-             static_cast<int>(free_capacity), static_cast<int>(width), shift, 0, from_empty ? 1 : 0};
+             static_cast<uint8_t*>(granted), positions, free_out, P * page_size < max_length ? P * page_size : max_length,
+             static_cast<int>(N), static_cast<int>(free_capacity), static_cast<int>(width), shift, 0,
+             from_empty ? 1 : 0};
   a.slice = plan_slice(width);
   const int64_t gx = (N + a.slice - 1) / a.slice, gy = (width + kPlanTokens - 1) / kPlanTokens;
   HYDRA_REQUIRE(gx < (int64_t(1) << 31) && gy <= 65535, "page_plan: too large");

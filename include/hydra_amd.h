@@ -498,6 +498,13 @@ int hydra_page_plan(const int* lengths, const int* new_tokens, int* table, int64
                     int64_t* slots, int* lengths_out, int* seen, void* granted, int* positions,
                     int* free_out, int64_t N, int64_t P, int64_t width, int64_t page_size,
                     int from_empty, void* stream);
+/* The same for requests of at most max_length tokens, where that is less than
+ * P * page_size. */
+int hydra_pool_plan(const int* lengths, const int* new_tokens, int* table, int64_t table_rs,
+                    const int* free_pages, int64_t free_capacity, const int* free_count,
+                    int64_t* slots, int* lengths_out, int* seen, void* granted, int* positions,
+                    int* free_out, int64_t N, int64_t P, int64_t width, int64_t page_size,
+                    int64_t max_length, int from_empty, void* stream);
 /* 1 if a plan of N requests of up to width tokens may be made in place.  Host-only. */
 int hydra_page_plan_in_place(int64_t N, int64_t width);
 

@@ -1,5 +1,5 @@
 """GPU tests of what bounds a pool of pages: entries that are no page,
-stacks near the reach of an int."""
+stacks near the reach of an int, the longest request."""
 from __future__ import annotations
 
 import random
@@ -79,3 +79,47 @@ def test_release_onto_a_full_stack_of_the_largest_size(cuda):
         assert stack[-100:].tolist() == want
         assert table.tolist() == [[-1] * 40, [-1] * 38 + [78, 79]]
         stack[-100:] = 7
+
+
+def test_requests_end_at_max_length(cuda):
+    """A length that is no whole number of pages."""
+    from hydra_amd.attention import PagePool
+
+    for N in (2, 300):  # planned in place, and by several workgroups
+        pool = PagePool(N, 20, 2 * N, 16, device=cuda)
+        assert pool.max_length == 20 and pool.table.shape == (N, 2)
+        plan = pool.plan(ints([21] + [20] * (N - 1), cuda), width=32, from_empty=True)
+        assert plan.granted.tolist() == [False] + [True] * (N - 1)
+        assert pool.lengths.tolist() == [0] + [20] * (N - 1) and pool.free_count.tolist() == [2]
+        plan = pool.plan(ints([19] + [0] * (N - 1), cuda), width=32, from_empty=True)
+        assert plan.granted.all()
+        plan = pool.plan(ints([1] * N, cuda))
+        assert plan.granted.tolist() == [True] + [False] * (N - 1) and plan.slots[1:].eq(-1).all()
+        assert not pool.plan(ints([1] * N, cuda)).granted.any()
+        assert pool.lengths.tolist() == [20] * N
+
+
+def test_layer_at_its_full_length(cuda):
+    """A layer whose rotation table ends inside a page, served up to its end."""
+    from hydra_amd.attention import CCGQAAttention, PagePool
+    from oracle import ccgqa as oc
+
+    cfg = oc.CCGQAConfig(dim=256, n_heads=4, n_kv_heads=2, max_seq_len=20)
+    params = oc.init_params(cfg, torch.Generator().manual_seed(1), std=0.05)
+    m = CCGQAAttention(dim=256, n_heads=4, n_kv_heads=2, max_seq_len=20)
+    m.load_state_dict(params)
+    m = m.to(cuda).eval()
+    pool = PagePool(2, 20, 4, 16, device=cuda)
+    cache = m.new_cache(pool)
+    x = torch.randn(2, 20, 256, generator=torch.Generator().manual_seed(2))
+    want = oc.forward(params, x, cfg)
+    plan = pool.plan(ints([18, 20], cuda), width=20, from_empty=True)
+    out = m.prefill(x.to(cuda), cache, plan)
+    top = want.abs().max()
+    assert (out[1].cpu() - want[1]).abs().max() / top < 1e-5  # the layer's own tolerance in fp32
+    for s in (18, 19):
+        plan = pool.plan(ints([1, 1], cuda))
+        assert plan.granted.tolist() == [True, False]
+        out = m.decode(x[:, s].to(cuda), cache, plan)
+        assert (out[0].cpu() - want[0, s]).abs().max() / top < 1e-5 and not out[1].any()
+    assert not pool.plan(ints([1, 1], cuda)).granted.any()
