@@ -537,10 +537,10 @@ __global__ __launch_bounds__(1024) void paged_attn_join_kernel(PagedArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int q = min(p + j * lanes, parts - 1);
-          const float c = p + j * lanes < parts ? weight[g][q] : 0.f;
+          const float c = weight[g][q];
           const float4 x = *reinterpret_cast<const float4*>(part(q) + 16 + g * row4(a.hd) + d);
-          // an output that a NaN or an infinity reached stays in its own part: c is not 0 there
-          if (c != 0.f) {
+          // by its number, not by its weight: 0 x NaN of a part whose weight vanishes is NaN
+          if (p + j * lanes < parts) {
             o.x = fmaf(c, x.x, o.x);
             o.y = fmaf(c, x.y, o.y);
             o.z = fmaf(c, x.z, o.z);
