@@ -16,6 +16,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(os.environ.get("HYDRA_AMD_LIB", Path(__file__).with_name("libhydra_amd.so")))
 
@@ -253,3 +254,11 @@ def require_gpu(name: str, *tensors) -> None:
                 dev = t.device
             elif t.device != dev:
                 raise RuntimeError(f"{name}: tensors on different devices ({dev}, {t.device})")
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """A kernel knows nothing of forward-mode tangents: they would be lost
+    without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise RuntimeError(f"{name}: no forward-mode derivative")

@@ -301,7 +301,8 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     the pool, or whose position is negative or past the RoPE tables, changes
     nothing and gets zeros for q.  Weights, temperature, tables and flags as
     ccgqa_prep takes them.  fp32 inside, one rounding.  Inference only: no
-    gradient."""
+    gradient, and refused where the row, the ring, the pages or the conv weights
+    record one; the temperature and the tables count as constants."""
     name = "ccgqa_decode_prep"
     _lib.require_gpu(name, qkv, ring, positions, slots, k_pages, v_pages, wq1, wq2, wk1, wk2, temperature, cos, sin)
     L, K = n_heads * head_dim, n_kv_heads * head_dim
@@ -318,7 +319,8 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     if slots.dtype != torch.int64 or slots.numel() != N:
         raise ValueError(f"{name}: slots must be int64, one a request, got {slots.dtype} {tuple(slots.shape)}")
     check_pages(name, k_pages, v_pages)
-    check_no_gradient(name, qkv, ring, k_pages, v_pages)
+    check_no_gradient(name, qkv, ring, k_pages, v_pages, wq1, wq2, wk1, wk2)
+    _lib.refuse_tangents(name, temperature, cos, sin)
     pages, _, page, _ = k_pages.shape
     if k_pages.shape[1] != n_kv_heads or k_pages.shape[3] != head_dim or k_pages.dtype != dt:
         raise ValueError(f"{name}: pages must be {dt} [pages, {n_kv_heads}, page_size, {head_dim}], got "

@@ -70,9 +70,10 @@ def check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None
             check_distinct(name, "pages", t)
 
 
-def check_no_gradient(name: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def check_no_gradient(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name}: no gradient (call it under torch.no_grad())")
+    _lib.refuse_tangents(name, *tensors)
 
 
 def check_distinct(name: str, what: str, t: torch.Tensor) -> None:
@@ -222,7 +223,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"{name}: {H} query heads are no multiple of {K} key heads")
     if q.dtype != k_pages.dtype:
         raise ValueError(f"{name}: q and the pages must share a dtype")
-    check_no_gradient(name, q, k_pages, v_pages)
+    check_no_gradient(name, q, k_pages, v_pages, out)
     _vector(name, "lengths", lengths, torch.int32, N)
     _check_table(name, table, N)
     if table.shape[1] == 0:

@@ -60,6 +60,7 @@ class _TokenLogprobsFunction(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy, g_top, _):
         x, tokens, stats, entropy, ids = ctx.saved_tensors
         top_k, temperature = ctx.meta
+        _lib.refuse_tangents("token_logprobs", g_logp, g_entropy, g_top)
         _, (rows, stride) = _as_rows(x)
         if g_top is not None and top_k == 0:
             g_top = None
@@ -85,11 +86,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     first.  Masked logits may be -inf or the type's lowest value; a row of -inf
     alone has log probabilities -inf, entropy 0 and no gradient; a row with a
     NaN or +inf has NaN.  The gradient covers logprobs, entropy and
-    top_logprobs (once differentiable); a captured backward belongs to a
-    captured forward, through torch.autograd.grad or leaves that no eager graph
-    shares."""
+    top_logprobs (once differentiable; forward-mode tangents are refused); a
+    captured backward belongs to a captured forward, through
+    torch.autograd.grad or leaves that no eager graph shares."""
     name = "token_logprobs"
     _lib.require_gpu(name, logits, tokens)
+    _lib.refuse_tangents(name, logits)
     if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"{name}: tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     if tokens.dtype != torch.int64:

@@ -32,3 +32,76 @@ def test_bad_values_behind_vanishing_weights(cuda, dtype, length, columns, bad):
     rest = [c for c in range(hd) if c != 3]
     assert not got[..., 3].isfinite().any()
     assert (got[..., rest] == 1).all()
+
+
+class Step(torch.nn.Module):
+    def __init__(self, layer):
+        super().__init__()
+        self.layer = layer
+
+    def forward(self, *args):
+        return self.layer.decode(*args)
+
+
+def test_derivatives_that_nothing_gives_are_refused(cuda):
+    """A recorded gradient of a weight or of `out`, and forward-mode tangents
+    of anything, are an error and not lost."""
+    import torch.autograd.forward_ad as fwad
+
+    from hydra_amd.attention import CCGQAAttention, PagePool, paged_attention, store_pages
+    from hydra_amd.attention.backends.ccgqa.ops import CCGQA_CONVS, CCGQA_QK_NORM, ccgqa_decode_prep, ccgqa_ring_fill
+    from hydra_amd.kernels import token_logprobs
+
+    new = lambda *s: torch.ones(*s, device=cuda)  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    kp, vp, q, table = new(4, 1, 16, 16), new(4, 1, 16, 16), new(1, 2, 16), i32(0, 1, 2)[None]
+    ring, row, slot = new(1, 5, 64), new(1, 64), torch.zeros(1, 1, dtype=torch.long, device=cuda)
+    w = [new(3, 32, 16), new(3, 32, 32), new(3, 16, 16), new(3, 16, 16)]
+    tokens = torch.zeros(3, dtype=torch.long, device=cuda)
+
+    def prep(row=row, ring=ring, w=w, temperature=new(1)):
+        return ccgqa_decode_prep(row, ring, i32(5), slot, kp, vp, 2, 1, 16, CCGQA_CONVS | CCGQA_QK_NORM, *w,
+                                 temperature=temperature, packed=True)
+
+    prep()
+    for i in range(4):
+        recorded = [t.clone().requires_grad_() if j == i else t for j, t in enumerate(w)]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            prep(w=recorded)
+        with torch.no_grad():
+            prep(w=recorded)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged_attention(q, kp, vp, table, i32(40), out=q.clone().requires_grad_())
+
+    torch.manual_seed(0)
+    m = CCGQAAttention(dim=256, n_heads=4, n_kv_heads=2, max_seq_len=32).to(cuda).eval()
+    pool = PagePool(2, 32, 4, 16, device=cuda)
+    cache = m.new_cache(pool)
+    plans = pool.plan(i32(4, 4), width=4, from_empty=True), pool.plan(i32(1, 1))
+    x = new(2, 4, 256)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: token_logprobs(dual(new(3, 8)), tokens), lambda: token_logprobs(dual(new(3, 8).requires_grad_()), tokens),
+                 lambda: prep(row=dual(row)), lambda: prep(ring=dual(ring)), lambda: prep(w=[dual(t) for t in w]),
+                 lambda: prep(temperature=dual(new(1))), lambda: paged_attention(dual(q), kp, vp, table, i32(40)),
+                 lambda: paged_attention(q, kp, dual(vp), table, i32(40)),
+                 lambda: store_pages(dual(new(1, 1, 1, 16)), new(1, 1, 1, 16), kp, vp, slot),
+                 lambda: ccgqa_ring_fill(dual(new(1, 4, 64)), ring, i32(4), 4),
+                 lambda: m.prefill(dual(x), cache, plans[0]), lambda: m.decode(dual(x[:, 0]), cache, plans[1])]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        logits = new(3, 8).requires_grad_()
+        out = token_logprobs(logits, tokens)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out.logprobs, logits, dual(new(3)))
+        token_logprobs(new(3, 8), tokens), prep(), m.prefill(x, cache, plans[0])  # no tangents: as ever
+        step = Step(m)
+        params = {k: v.detach() for k, v in step.named_parameters()}
+        torch.func.functional_call(step, params, (x[:, 0], cache, plans[1]))
+        for name in ("q_conv.conv1.weight", "key_temperature", "o_proj.weight"):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.func.functional_call(step, {**params, f"layer.{name}": dual(params[f"layer.{name}"])},
+                                           (x[:, 0], cache, plans[1]))
