@@ -244,13 +244,22 @@ class CCGQAAttention(nn.Module):
                              f"({self.cos_cached.shape[2]})")
         if self.head_dim > 256:
             raise ValueError(f"CCGQAAttention: a cache takes head_dim up to 256, not {self.head_dim}")
-        if self.use_convs and not (self.conv_kernel_size == 3 and self.head_dim in (16, 32, 64, 128)) and \
-                self.conv_kernel_size * self.latent_dim + self.head_dim > 16384:
+        # what decode's kernels take, so that no prompt enters in vain
+        if pool.requests > 65535:
+            raise ValueError(f"CCGQAAttention: a cache takes up to 65535 requests, not {pool.requests}")
+        if pool.table.shape[1] * pool.page_size > 1 << 30:
+            raise ValueError(f"CCGQAAttention: requests of up to {pool.max_length} tokens, where a cache takes 2^30")
+        dtype = dtype or w.dtype
+        reach = decode_reach(self._prep_args()[0], self.conv_kernel_size)
+        ring = pool.requests * (reach + 1) * (self.latent_dim + 2 * self.kv_dim) * dtype.itemsize
+        matrix = self.conv_kernel_size == 3 and self.head_dim in (16, 32, 64, 128) and ring < 1 << 32
+        if self.use_convs and not matrix and self.conv_kernel_size * self.latent_dim + self.head_dim > 16384:
             raise ValueError(f"CCGQAAttention: a cache takes {self.conv_kernel_size} taps of {self.latent_dim} "
-                             f"channels only at three taps and head_dim 16, 32, 64 or 128")
+                             f"channels only at three taps, head_dim 16, 32, 64 or 128 and less than 4 GiB of rows "
+                             f"to look back at ({ring} bytes)")
         if pool.table.device != w.device:
             raise RuntimeError(f"CCGQAAttention: the pool is on {pool.table.device}, the layer on {w.device}")
-        return CCGQACache(self, pool, dtype or w.dtype)
+        return CCGQACache(self, pool, dtype)
 
     def _check_cache(self, name: str, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan) -> None:
         if forward_ad._current_level >= 0:

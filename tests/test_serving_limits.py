@@ -21,3 +21,26 @@ def test_requests_of_a_plan_and_a_release():
             _lib.call("hydra_page_release", FAKE, FAKE, FAKE, 1, FAKE, 8, FAKE, N, 1, 16, None)
         with pytest.raises(ValueError, match="too large"):
             _lib.call("hydra_pool_release", FAKE, FAKE, FAKE, 1, FAKE, 8, FAKE, N, 1, 16, 4, None)
+
+
+def test_pools_that_no_layer_decodes():
+    """A pool whose requests decode would refuse is refused by new_cache."""
+    from hydra_amd.attention import CCGQAAttention, PagePool
+
+    with torch.device("meta"):
+        narrow = CCGQAAttention(dim=256, n_heads=4, n_kv_heads=2, max_seq_len=64)
+        wide = CCGQAAttention(dim=32768, n_heads=64, n_kv_heads=2, max_seq_len=64)
+        endless = CCGQAAttention(dim=256, n_heads=4, n_kv_heads=2, use_rope=False)
+    many = PagePool(65536, 16, 4, 16, device="cpu")
+    with pytest.raises(ValueError, match="65535 requests"):
+        narrow.new_cache(many)
+    with pytest.raises(ValueError, match="2\\^30"):
+        endless.new_cache(PagePool(1, (1 << 30) + 1, 4, 4096, device="cpu"))
+    # rings of 8192 + 512 channels in fp32: 5 rows of 34816 bytes a request
+    assert 24672 * 5 * 34816 < 1 << 32 <= 24673 * 5 * 34816
+    with pytest.raises(ValueError, match="4 GiB"):
+        wide.new_cache(PagePool(24673, 16, 4, 16, device="cpu"))
+    for layer, pool in ((narrow, PagePool(65535, 16, 4, 16, device="cpu")), (wide, PagePool(24672, 16, 4, 16, device="cpu")),
+                        (endless, PagePool(1, 1 << 30, 4, 4096, device="cpu"))):
+        with pytest.raises(RuntimeError, match="the pool is on cpu"):  # nothing else against them
+            layer.new_cache(pool)
