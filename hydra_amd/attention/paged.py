@@ -55,8 +55,13 @@ def _in_place(name: str, what: str, t: torch.Tensor, unit: bool = True) -> None:
 def _check_table(name: str, table: torch.Tensor, n: int) -> None:
     if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != n:
         raise ValueError(f"{name}: table must be int32 [{n}, P], got {table.dtype} {tuple(table.shape)}")
-    if table.stride(1) != 1 or (n > 1 and table.stride(0) < table.shape[1]):
+    if (table.shape[1] > 1 and table.stride(1) != 1) or (n > 1 and table.stride(0) < table.shape[1]):
         raise ValueError(f"{name}: table needs rows of unit stride that do not overlap")
+
+
+def _row_stride(table: torch.Tensor) -> int:
+    """A lone row's stride says nothing."""
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
 
 
 def check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
@@ -113,7 +118,7 @@ def _plan(name, lengths, new_tokens, table, free_pages, free_count, page_size, w
     within = () if max_length is None else (max_length,)
     with _lib.on_device(lengths):
         _lib.call("hydra_pool_plan" if within else "hydra_page_plan", lengths.data_ptr(), new_tokens.data_ptr(),
-                  table.data_ptr(), table.stride(0), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+                  table.data_ptr(), _row_stride(table), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
                   slots.data_ptr(), after.data_ptr(), seen.data_ptr(), granted.data_ptr(), positions.data_ptr(),
                   left.data_ptr(), N, table.shape[1], width, int(page_size), *within, 1 if from_empty else 0,
                   _lib.stream(lengths))
@@ -159,7 +164,7 @@ def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     within = () if pages is None else (int(pages),)
     with _lib.on_device(lengths):
         _lib.call("hydra_pool_release" if within else "hydra_page_release", done.data_ptr(), lengths.data_ptr(),
-                  table.data_ptr(), table.stride(0), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+                  table.data_ptr(), _row_stride(table), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
                   N, table.shape[1], int(page_size), *within, _lib.stream(lengths))
 
 
@@ -242,7 +247,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         need = _attention_workspace(q.device.index, N, H, K, hd, P, page, code)
         ws = _lib.scratch(need, q) if need else None
         _lib.call("hydra_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
-                  table.data_ptr(), table.stride(0), lengths.data_ptr(), N, H, K, hd, P, page, pages, _strides(q),
+                  table.data_ptr(), _row_stride(table), lengths.data_ptr(), N, H, K, hd, P, page, pages, _strides(q),
                   _strides(k_pages), _strides(v_pages), _strides(out), hd ** -0.5 if scale is None else float(scale),
                   code, _lib.ptr(ws), need, _lib.stream(q))
     return out

@@ -1,5 +1,5 @@
 """GPU tests of what bounds a pool of pages: entries that are no page,
-stacks near the reach of an int, the longest request."""
+stacks near the reach of an int, the longest request, tables of one row or column."""
 from __future__ import annotations
 
 import random
@@ -123,3 +123,27 @@ def test_layer_at_its_full_length(cuda):
         out = m.decode(x[:, s].to(cuda), cache, plan)
         assert (out[0].cpu() - want[0, s]).abs().max() / top < 1e-5 and not out[1].any()
     assert not pool.plan(ints([1, 1], cuda)).granted.any()
+
+
+@pytest.mark.parametrize("N,P", [(3, 1), (1, 4), (1, 1)])
+def test_tables_of_one_row_or_column(cuda, N, P):
+    """The stride of a dimension of one element says nothing."""
+    from hydra_amd.attention import paged_attention, plan_pages, release_pages
+
+    g = torch.Generator().manual_seed(1)
+    kp, vp = (torch.randn(8, 1, 16, 16, generator=g).to(cuda) for _ in range(2))
+    q = torch.randn(N, 2, 16, generator=g).to(cuda)
+    outs = []
+    for table in (ints([[-1] * P] * N, cuda), ints([[-1] * N] * P, cuda).t(),
+                  torch.empty_strided((N, P), (1, 5) if P == 1 else (0, 1), dtype=torch.int32, device=cuda).fill_(-1)):
+        stack, height, lengths = ints(range(8), cuda), ints([8], cuda), ints([0] * N, cuda)
+        plan = plan_pages(lengths, ints([P * 16 - 3] * N, cuda), table, stack, height, 16, width=P * 16)
+        out = paged_attention(q, kp, vp, table, plan.seen)
+        assert plan.granted.all()
+        held = table.clone()
+        after, count = plan.lengths.clone(), plan.free_count.clone()
+        release_pages(torch.ones(N, dtype=torch.bool, device=cuda), after, table, stack, count, 16)
+        assert table.eq(-1).all() and count.tolist() == [8] and not after.any()
+        outs.append((out, plan.slots, held, stack))
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
