@@ -389,20 +389,61 @@ __global__ __launch_bounds__(kGradThreads) void logp_grad_kernel(LogpGradArgs a)
 // Positive, finite, and its inverse too.
 bool good_temperature(float t) { return t > 0.f && t < INFINITY && kLog2e / t < INFINITY; }
 
+// Workgroups of a launch: HIP counts its threads in 32 bits.
+constexpr int64_t kMaxGroups = int64_t(1) << 22;
+
+template <typename T>
+T* at_row(T* p, int64_t at) { return p ? p + at : nullptr; }
+
 template <typename T, bool TOP>
-int launch_logp(const LogpArgs& a, int64_t rows, hipStream_t st) {
+int launch_logp(LogpArgs a, int64_t rows, hipStream_t st) {
   constexpr int E = Vec<T>::N;
   const int64_t most = a.V / E;  // whole pieces
-  const dim3 grid(static_cast<unsigned>(rows));
+  for (int64_t row = 0; row < rows; row += kMaxGroups) {
+    const int64_t here = rows - row < kMaxGroups ? rows - row : kMaxGroups;
+    const dim3 grid(static_cast<unsigned>(here));
 #define HYDRA_LOGP(N) logp_kernel<T, N, TOP><<<grid, kThreads, 0, st>>>(a)
-  if (most <= 2 * kThreads) HYDRA_LOGP(2);
-  else if (most <= 4 * kThreads) HYDRA_LOGP(4);
-  else if (most <= 8 * kThreads) HYDRA_LOGP(8);
-  else if (most <= 16 * kThreads) HYDRA_LOGP(16);
-  else if (most <= 32 * kThreads) HYDRA_LOGP(32);
-  else HYDRA_LOGP(0);
+    if (most <= 2 * kThreads) HYDRA_LOGP(2);
+    else if (most <= 4 * kThreads) HYDRA_LOGP(4);
+    else if (most <= 8 * kThreads) HYDRA_LOGP(8);
+    else if (most <= 16 * kThreads) HYDRA_LOGP(16);
+    else if (most <= 32 * kThreads) HYDRA_LOGP(32);
+    else HYDRA_LOGP(0);
+    const int rc = check_launch("token_logprobs");
+    if (rc != HYDRA_OK) return rc;
+    a.x = static_cast<const T*>(a.x) + here * a.rs;
+    a.tokens += here;
+    a.logp += here;
+    a.entropy += here;
+    a.stats = at_row(a.stats, 2 * here);
+    a.top = at_row(a.top, here * a.K);
+    a.top_tokens = at_row(a.top_tokens, here * a.K);
+  }
 #undef HYDRA_LOGP
-  return check_launch("token_logprobs");
+  return HYDRA_OK;
+}
+
+template <typename T>
+int launch_grad(LogpGradArgs a, int64_t rows, bool vec, hipStream_t st) {
+  const int64_t most = kMaxGroups / a.parts;  // parts <= 2^17
+  for (int64_t row = 0; row < rows; row += most) {
+    const int64_t here = rows - row < most ? rows - row : most;
+    const dim3 grid(static_cast<unsigned>(here * a.parts));
+    if (vec) logp_grad_kernel<T, true><<<grid, kGradThreads, 0, st>>>(a);
+    else logp_grad_kernel<T, false><<<grid, kGradThreads, 0, st>>>(a);
+    const int rc = check_launch("token_logprobs_bwd");
+    if (rc != HYDRA_OK) return rc;
+    a.x = static_cast<const T*>(a.x) + here * a.rs;
+    a.grad = static_cast<T*>(a.grad) + here * a.V;
+    a.tokens += here;
+    a.stats += 2 * here;
+    a.entropy += here;
+    a.g_logp = at_row(a.g_logp, here);
+    a.g_entropy = at_row(a.g_entropy, here);
+    a.g_top = at_row(a.g_top, here * a.K);
+    a.top_tokens = at_row(a.top_tokens, here * a.K);
+  }
+  return HYDRA_OK;
 }
 
 }  // namespace
@@ -451,7 +492,6 @@ extern "C" int hydra_token_logprobs_bwd(const void* logits, int64_t rows, int64_
   HYDRA_REQUIRE(reinterpret_cast<uintptr_t>(logits) % e == 0, "token_logprobs_bwd: misaligned logits");
   const int64_t most = vocab / (16 / e);  // whole pieces
   const int64_t parts = most == 0 ? 1 : (most + kGradThreads * kGradPieces - 1) / (kGradThreads * kGradPieces);
-  HYDRA_REQUIRE(rows * parts < (int64_t(1) << 31), "token_logprobs_bwd: too large");
   const LogpGradArgs a{logits, logits_rs, tokens, stats, entropy, g_logprobs, g_entropy, g_top, top_tokens, grad,
                        static_cast<int>(vocab), static_cast<int>(top_k), static_cast<int>(parts),
                        kLog2e / temperature, 1.f / temperature};
@@ -459,10 +499,5 @@ extern "C" int hydra_token_logprobs_bwd(const void* logits, int64_t rows, int64_
   const bool vec = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(grad)) % 16 == 0 &&
                    (rows <= 1 || (logits_rs - vocab) * e % 16 == 0);
   auto st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(rows * parts));
-  return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
-    if (vec) logp_grad_kernel<T, true><<<grid, kGradThreads, 0, st>>>(a);
-    else logp_grad_kernel<T, false><<<grid, kGradThreads, 0, st>>>(a);
-    return check_launch("token_logprobs_bwd");
-  });
+  return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int { return launch_grad<T>(a, rows, vec, st); });
 }

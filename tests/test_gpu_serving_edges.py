@@ -105,3 +105,27 @@ def test_derivatives_that_nothing_gives_are_refused(cuda):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.func.functional_call(step, {**params, f"layer.{name}": dual(params[f"layer.{name}"])},
                                            (x[:, 0], cache, plans[1]))
+
+
+@pytest.mark.parametrize("rows", [(1 << 22) + 1, (1 << 23) + 3])
+def test_log_probabilities_of_more_rows_than_a_grid(cuda, rows):
+    """HIP counts a launch's threads in 32 bits; rows past them are worked on
+    like the first ones."""
+    from hydra_amd.kernels import token_logprobs
+
+    V, K = 12, 2
+    x = torch.randn(rows, V, generator=torch.Generator(device=cuda).manual_seed(1), device=cuda).to(torch.bfloat16)
+    tokens = torch.arange(rows, device=cuda) % V
+
+    def step(x, tokens):
+        x = x.clone().requires_grad_()
+        out = token_logprobs(x, tokens, top_k=K)
+        grad, = torch.autograd.grad([out.logprobs.sum() + 0.5 * out.entropy.sum() + out.top_logprobs.sum()], [x])
+        return (*(t.detach() for t in out), grad)
+
+    whole = step(x, tokens)
+    for begin in range(0, rows, 1 << 20):
+        part = slice(begin, begin + (1 << 20))
+        for a, b in zip(whole, step(x[part], tokens[part])):
+            assert torch.equal(a[part], b), begin
+    assert torch.equal(token_logprobs(x, tokens).logprobs, whole[0])
