@@ -61,6 +61,7 @@ struct PagedArgs {
   int64_t table_rs;
   int N, H, Hkv, hd, G, GB, P, shift, pages;
   float scale;                       // times log2(e)
+  int first;                         // item of the launch's first workgroup (whole form)
   // split form: rounds of a workgroup at least, workgroups, results
   int least, groups, cus;
   int* plan;                         // [0] rounds per workgroup, [1 + n] prefix of rounds
@@ -383,7 +384,7 @@ template <typename T, int GP, int LPR, bool VEC>
 __global__ __launch_bounds__(kThreads) void paged_attn_whole_kernel(PagedArgs a) {
   constexpr int HDP = LPR * Vec<T>::N;
   __shared__ __attribute__((aligned(16))) float sm[lds_floats<GP, LPR, T>()];
-  const int item = blockIdx.x, gb = item % a.GB, h = item / a.GB % a.Hkv, n = item / a.GB / a.Hkv;
+  const int item = a.first + blockIdx.x, gb = item % a.GB, h = item / a.GB % a.Hkv, n = item / a.GB / a.Hkv;
   item_keys<T, GP, LPR, VEC>(a, n, h, gb, 0, rounds_of<LPR>(seen_keys(a, n)), sm);
   write_out<T, GP, HDP>(a, n, h, gb, sm);
 }
@@ -634,7 +635,13 @@ void launch_form(PagedArgs a, const Split& p, int64_t items, hipStream_t st) {
     a.groups = a.cus * std::min(kMaxResident, blocks_per_cu(reinterpret_cast<const void*>(kernel), 64 * p.waves));
     kernel<<<a.groups, 64 * p.waves, 0, st>>>(a);
   } else {
-    paged_attn_whole_kernel<T, GP, LPR, VEC><<<static_cast<unsigned>(items), 64 * p.waves, 0, st>>>(a);
+    // HIP counts a launch's threads in 32 bits
+    constexpr int64_t most = int64_t(1) << 22;
+    for (int64_t first = 0; first < items; first += most) {
+      a.first = static_cast<int>(first);
+      paged_attn_whole_kernel<T, GP, LPR, VEC>
+          <<<static_cast<unsigned>(std::min(most, items - first)), 64 * p.waves, 0, st>>>(a);
+    }
   }
 }
 

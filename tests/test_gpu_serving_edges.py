@@ -129,3 +129,19 @@ def test_log_probabilities_of_more_rows_than_a_grid(cuda, rows):
         for a, b in zip(whole, step(x[part], tokens[part])):
             assert torch.equal(a[part], b), begin
     assert torch.equal(token_logprobs(x, tokens).logprobs, whole[0])
+
+
+def test_attention_of_more_items_than_a_grid(cuda):
+    """Requests times key heads past what one launch's threads count."""
+    from hydra_amd.attention import paged_attention
+
+    N, K, hd, pages = (1 << 23) + 5, 2, 8, 64
+    g = torch.Generator(device=cuda).manual_seed(1)
+    rand = lambda *s: torch.randn(*s, generator=g, device=cuda).to(torch.bfloat16)  # noqa: E731
+    q, kp, vp = rand(N, K, hd), rand(pages, K, 16, hd), rand(pages, K, 16, hd)
+    table = torch.randint(pages, (N, 1), generator=g, device=cuda, dtype=torch.int32)
+    lengths = torch.randint(17, (N,), generator=g, device=cuda, dtype=torch.int32)
+    whole = paged_attention(q, kp, vp, table, lengths, out=torch.full_like(q, 9.0))
+    for begin in range(0, N, 1 << 20):
+        part = slice(begin, begin + (1 << 20))
+        assert torch.equal(whole[part], paged_attention(q[part], kp, vp, table[part], lengths[part])), begin
