@@ -85,13 +85,15 @@ class HydraBlock(nn.Module):
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, cache, plan: PagePlan, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward() of whole prompts x [M, S, dim] into a paged cache
-        (CCGQAAttention.prefill)."""
+        (CCGQAAttention.prefill, which rows hold results)."""
         return self._rest(x, self.attention.prefill(self.norm1(x), cache, plan, rows))
 
     @torch.no_grad()
     def decode(self, x: torch.Tensor, cache, plan: PagePlan) -> torch.Tensor:
         """forward() of each request's newest token, x [N, dim] or [N, 1, dim]
-        (CCGQAAttention.decode)."""
+        (CCGQAAttention.decode).  The row of a request without a token
+        (plan.seen 0) holds no result: it is x and the MLP's part of it, without
+        attention."""
         return self._rest(x, self.attention.decode(self.norm1(x), cache, plan))
 
 

@@ -145,3 +145,56 @@ def test_attention_of_more_items_than_a_grid(cuda):
     for begin in range(0, N, 1 << 20):
         part = slice(begin, begin + (1 << 20))
         assert torch.equal(whole[part], paged_attention(q[part], kp, vp, table[part], lengths[part])), begin
+
+
+def test_blocks_with_idle_and_refused_requests(cuda):
+    """Blocks over one pool, one request idle at every step and one refused in
+    the end: the others' rows are those of blocks that serve them alone, an idle
+    request's caches stay, and its own row is what the block makes of an
+    attention of zeros: no result."""
+    from hydra_amd.attention import PagePool
+    from hydra_amd.model.framework import HydraBlock
+
+    torch.manual_seed(0)
+    dim, N, S = 256, 3, 12
+    blocks = [HydraBlock(dim, n_heads=4, n_kv_heads=2, max_seq_len=64).to(cuda).eval() for _ in range(2)]
+    x = torch.randn(N, 40, dim, generator=torch.Generator().manual_seed(1)).to(cuda)
+    lens = [12, 5, 9]
+
+    def serve(idle):
+        """Rows [step][n]; request `idle(step)` has no token then."""
+        pool = PagePool(N, 16, 3, 16, device=cuda)
+        caches = [b.new_cache(pool) for b in blocks]
+        h = x[:, :S]
+        plan = pool.plan(torch.tensor(lens, dtype=torch.int32, device=cuda), width=S, from_empty=True)
+        for b, c in zip(blocks, caches):
+            h = b.prefill(h, c, plan)
+        rows, at = [], list(lens)
+        for step in range(6):
+            who = idle(step)
+            new = torch.tensor([int(n != who) for n in range(N)], dtype=torch.int32, device=cuda)
+            before = [(c.ring[who].clone(), c.k_pages.clone()) for c in caches] if who is not None else None
+            plan = pool.plan(new)
+            h = token = torch.stack([x[n, at[n]] for n in range(N)])
+            for b, c in zip(blocks, caches):
+                h = b.decode(h, c, plan)
+            rows.append(h)
+            at = pool.lengths.tolist()
+            if who is not None:
+                page = int(pool.table[who, 0])
+                for c, (ring, kp) in zip(caches, before):
+                    assert torch.equal(c.ring[who], ring) and torch.equal(c.k_pages[page], kp[page])
+                alone = token[who:who + 1]
+                for b in blocks:
+                    with torch.no_grad():
+                        alone = b._rest(alone, torch.zeros_like(alone))
+                assert plan.seen[who] == 0 and alone.any()
+                assert (h[who] - alone[0]).abs().max() <= 1e-5 * alone.abs().max()
+        return rows, plan
+
+    whole, plan = serve(lambda step: None)
+    assert plan.granted.tolist() == [False, True, True]  # 12 + 4 tokens fill the page: the last two are refused
+    turns, _ = serve(lambda step: 1)
+    for step in range(6):
+        for n in (0, 2):
+            assert torch.equal(turns[step][n], whole[step][n]), (step, n)
