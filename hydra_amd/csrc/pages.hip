@@ -170,10 +170,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 // of the requests; their lengths become 0 and their table entries -1.  Entries
 // that are no page (outside [0, pages)) do not come back: the next plan would
 // hand them to another request.  One workgroup: the stack has one top.  Its
-// threads take the entries of 256 requests in their order, four neighbouring
-// ones each, look up whose they are and count the pages among them; bound by the
-// launch and the chain lengths -> sums -> table -> sums -> stack.
-constexpr int kReleaseEntries = 4;
+// threads take the entries of 256 requests in their order on the stack, twice
+// 256 at once, and look up whose each is; those that are pages are counted only
+// where one of them is none.  Bound by the launch and the chain lengths ->
+// sums -> table -> stack.
+constexpr int kReleaseEntries = 2;
 
 __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* done, int* lengths, int* table,
                                                                int64_t table_rs, int* free_pages, int* free_count,
@@ -197,32 +198,45 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
     const int upto = block_incl_sum(count, part, step);
     s_upto[tid] = upto;
     __syncthreads();
-    // the last trip's indexes, and a full stack's, may pass an int
-    for (int64_t e0 = 0; e0 < step; e0 += kPlanThreads * U) {
-      int page[U], mine = 0;
+    const unsigned entries = step;
+    // unsigned: the last trip's indexes, and a full stack's, may pass an int
+    for (unsigned e0 = 0; e0 < entries; e0 += kPlanThreads * U) {
+      int at[U], page[U];  // at: the first request with s_upto > e
+      int* entry[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) at[u] = 0;
+#pragma unroll
+      for (int half = kPlanThreads / 2; half > 0; half >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (static_cast<unsigned>(s_upto[at[u] + half - 1]) <= min(e0 + u * kPlanThreads + tid, entries - 1)) at[u] += half;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t e = e0 + tid * U + u;
-        page[u] = -1;
-        if (e >= step) continue;
-        int at = 0;  // the first request with s_upto > e
-#pragma unroll
-        for (int half = kPlanThreads / 2; half > 0; half >>= 1)
-          if (s_upto[at + half - 1] <= e) at += half;
-        int* entry = table + (i0 + at) * table_rs + (e - (at > 0 ? s_upto[at - 1] : 0));
-        page[u] = *entry < pages ? *entry : -1;
-        mine += page[u] >= 0;
-        *entry = -1;
+        const unsigned e = min(e0 + u * kPlanThreads + tid, entries - 1);
+        entry[u] = table + (i0 + at[u]) * table_rs + (e - (at[u] > 0 ? s_upto[at[u] - 1] : 0));
+        page[u] = *entry[u];
       }
-      int all;
-      int64_t to = static_cast<int64_t>(free) + block_incl_sum(mine, part, all) - mine;
+      bool wrong = false;  // any that is no page
+#pragma unroll
+      for (int u = 0; u < U; ++u) wrong = wrong || page[u] < 0 || page[u] >= pages;
+      const bool all_pages = !__syncthreads_or(wrong);
+      unsigned below = free;  // the height of the stack below the next 256
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (page[u] < 0) continue;
-        if (to < F) free_pages[to] = page[u];
-        ++to;
+        const unsigned e = e0 + u * kPlanThreads + tid;
+        bool back = e < entries;
+        if (back) *entry[u] = -1;
+        unsigned to = below + tid;
+        int more = kPlanThreads;
+        if (!all_pages) {
+          back = back && page[u] >= 0 && page[u] < pages;
+          to = below + block_incl_sum(back, part, more) - 1;
+        }
+        if (back && to < static_cast<unsigned>(F)) free_pages[to] = page[u];
+        below += more;
       }
-      free = static_cast<int>(min(static_cast<int64_t>(F), static_cast<int64_t>(free) + all));
+      if (all_pages) below = min(below, free + (entries - e0));
+      free = min(below, static_cast<unsigned>(F));
     }
     __syncthreads();
   }
