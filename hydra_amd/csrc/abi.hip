@@ -110,7 +110,7 @@ extern "C" int hydra_stream_copy(const void* src, void* dst, int64_t bytes, void
   HYDRA_REQUIRE(src && dst, "stream_copy: null pointer");
   HYDRA_REQUIRE(aligned16(src) && aligned16(dst), "stream_copy: pointers must be 16-byte aligned");
   const int64_t n = bytes / 16;
-  HYDRA_REQUIRE((n + 255) / 256 < (int64_t(1) << 31), "stream_copy: too large");
+  HYDRA_REQUIRE(grid_fits((n + 255) / 256, 256), "stream_copy: too large");
   stream_copy_kernel<<<dim3(static_cast<unsigned>((n + 255) / 256)), 256, 0, static_cast<hipStream_t>(stream)>>>(
       static_cast<const uint4*>(src), static_cast<uint4*>(dst), n);
   return check_launch("stream_copy_kernel");

@@ -1057,7 +1057,7 @@ int launch_fwd(const AttnF32Args& a) {
   const int vec = (a.hd == HDP && vec_ok(a.k, a.ks, E) && vec_ok(a.v, a.vs, E) ? 1 : 0) |
                   (a.hd == HDP && vec_ok(a.q, a.qs, E) ? 2 : 0);
   const int64_t blocks = static_cast<int64_t>(items) * a.B * a.Hkv;
-  if (blocks >= (int64_t(1) << 31)) return fail(HYDRA_ERR_ARG, "attn_fwd: too many rows");
+  if (!grid_fits(blocks, kThreads)) return fail(HYDRA_ERR_ARG, "attn_fwd: too many rows");
   // Key groups when the items are fewer than two per resident workgroup
   // (registers: 3 per CU at head_dim 64): the longest walk sets the time then.
   // Two groups at head_dim 128 (LDS), else four.  fp16 B2 8/2 x 64, S 1500
@@ -1082,7 +1082,7 @@ int launch_bwd(const AttnF32Args& a, float* part, size_t part_bytes) {
   const bool qv = a.hd == HDP && vec_ok(a.q, a.qs, E) && vec_ok(a.dout, a.dos, E);
   const bool kv = a.hd == HDP && vec_ok(a.k, a.ks, E) && vec_ok(a.v, a.vs, E);
   const float sl2 = a.scale * kLog2eF;
-  if (p.wg_kv >= (int64_t(1) << 31) || p.wg_q >= (int64_t(1) << 31)) return fail(HYDRA_ERR_ARG, "attn_bwd: problem too large");
+  if (!grid_fits(p.wg_kv, kThreads) || !grid_fits(p.wg_q, kThreads)) return fail(HYDRA_ERR_ARG, "attn_bwd: problem too large");
   const T* q = static_cast<const T*>(a.q);
   const T* k = static_cast<const T*>(a.k);
   const T* v = static_cast<const T*>(a.v);
@@ -1105,7 +1105,7 @@ int launch_bwd(const AttnF32Args& a, float* part, size_t part_bytes) {
   const int first = p.max_kv > 1 ? 0 : 2, count = (p.max_kv > 1 ? 2 : 0) + (p.max_q > 1 ? 1 : 0);
   const int64_t rows = static_cast<int64_t>(p.BHkv) * 64 * std::max(p.max_kv > 1 ? p.nkg : 0, p.max_q > 1 ? p.items : 0);
   const int64_t blocks = (rows * (HDP / 4) + 255) / 256;
-  if (blocks >= (int64_t(1) << 31)) return fail(HYDRA_ERR_ARG, "attn_bwd: problem too large");
+  if (!grid_fits(blocks, 256)) return fail(HYDRA_ERR_ARG, "attn_bwd: problem too large");
   attn_bwd_f32_reduce_kernel<T, HDP><<<dim3(static_cast<unsigned>(blocks), count), 256, 0, a.st>>>(r, first);
   return check_launch("attn_bwd: f32 reduce");
 }

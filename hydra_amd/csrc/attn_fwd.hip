@@ -1456,6 +1456,7 @@ static int launch_mfma(const void* q, const void* k, const void* v, void* o, flo
       *need = wb;
       return HYDRA_OK;
     }
+    if (!grid_fits(P, 64 * NW)) return fail(HYDRA_ERR_ARG, "attn_fwd: too many rows");
     if (wb > 0) {
       if (ws_ptr == nullptr || ws_bytes < wb)
         return fail(HYDRA_ERR_ARG, "attn_fwd: workspace of " + std::to_string(wb) +
@@ -1499,6 +1500,7 @@ static int launch_generic(const void* q, const void* k, const void* v, void* o, 
                           const int64_t* ks, const int64_t* vs, const int64_t* os,
                           bool causal, float scale, hipStream_t st) {
   const int64_t total = B * Hq * S;
+  HYDRA_REQUIRE(grid_fits((total + 255) / 256, 256), "attn_fwd: too many rows");
   const dim3 grid(static_cast<unsigned>((total + 255) / 256));
   auto Q = static_cast<const T*>(q);
   auto K = static_cast<const T*>(k);

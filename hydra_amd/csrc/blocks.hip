@@ -288,6 +288,7 @@ template <typename T, typename WT, int LPR, int CPL, int NORM>
 int launch_resnorm_vec(const ResNormArgs& a, hipStream_t st) {
   constexpr int RI = CPL >= 3 ? 1 : (CPL >= 2 ? 2 : 4);
   constexpr int RPB = (kBlk / 64) * (64 / LPR) * RI;
+  HYDRA_REQUIRE(grid_fits((a.rows + RPB - 1) / RPB, kBlk), "residual_norm: too many rows");
   const dim3 grid(static_cast<unsigned>((a.rows + RPB - 1) / RPB));
   resnorm_vec_kernel<T, WT, LPR, CPL, RI, NORM><<<grid, kBlk, 0, st>>>(a);
   return check_launch("resnorm_vec_kernel");
@@ -317,6 +318,7 @@ int launch_resnorm(ResNormArgs a, bool vec_ok, hipStream_t st) {
 #undef HYDRA_RN_CASE
   }
   (void)E;
+  HYDRA_REQUIRE(grid_fits((a.rows + 3) / 4, kBlk), "residual_norm: too many rows");
   const dim3 grid(static_cast<unsigned>((a.rows + 3) / 4));
   resnorm_scalar_kernel<T, WT, NORM><<<grid, kBlk, 0, st>>>(a);
   return check_launch("resnorm_scalar_kernel");
@@ -426,6 +428,7 @@ extern "C" int hydra_embedding_fwd(const int64_t* ids, int64_t n, const void* ta
       return check_launch("embed_vec_kernel");
     }
     const int64_t tot = n * dim;
+    HYDRA_REQUIRE(grid_fits((tot + kBlk - 1) / kBlk, kBlk), "embedding: too large");
     embed_scalar_kernel<T><<<dim3(static_cast<unsigned>((tot + kBlk - 1) / kBlk)), kBlk, 0, st>>>(
         ids, static_cast<const T*>(table), static_cast<T*>(out), tot, dim, vocab, table_rs, out_rs,
         scale);
@@ -500,6 +503,7 @@ extern "C" int hydra_mor_update(void* current, int64_t c_rs, const void* delta, 
       return check_launch("mor_update_vec_kernel");
     }
     const int64_t tot = rows * dim;
+    HYDRA_REQUIRE(grid_fits((tot + kBlk - 1) / kBlk, kBlk), "mor_update: too large");
     mor_update_scalar_kernel<T><<<dim3(static_cast<unsigned>((tot + kBlk - 1) / kBlk)), kBlk, 0, st>>>(
         static_cast<T*>(current), static_cast<const T*>(delta), static_cast<T*>(output), depth, tot,
         dim, c_rs, d_rs, o_rs, recursion);
@@ -510,7 +514,7 @@ extern "C" int hydra_mor_update(void* current, int64_t c_rs, const void* delta, 
 extern "C" int hydra_mor_route(const void* logits, int64_t n, void* probs, void* logits_out,
                                int64_t* depth, int64_t n_recursions, int64_t min_depth, int dtype,
                                void* stream) {
-  HYDRA_REQUIRE(n >= 0 && n < (int64_t(1) << 40), "mor_route: bad size");
+  HYDRA_REQUIRE(n >= 0 && grid_fits((n + kBlk - 1) / kBlk, kBlk), "mor_route: bad size");
   HYDRA_REQUIRE(n_recursions >= 1 && n_recursions < (int64_t(1) << 20), "mor_route: bad n_recursions");
   HYDRA_REQUIRE(min_depth >= 0 && min_depth <= n_recursions - 1, "mor_route: min_depth out of range");
   if (n == 0) return HYDRA_OK;

@@ -454,6 +454,7 @@ int launch_prep_bwd(const PrepBwdArgs& a) {
       ptr_ok = ptr_ok && aligned16(p);
     if (hd_ok && rows_ok && ptr_ok && CW <= 2048) {
       const int tpb = 256 / (CW / 8);
+      HYDRA_REQUIRE(grid_fits((ntok + tpb - 1) / tpb, 256), "ccgqa_prep_bwd: too many tokens");
       ccgqa_prep_bwd_vec_kernel<T><<<dim3(static_cast<unsigned>((ntok + tpb - 1) / tpb)), 256, 0, a.st>>>(a, tpb);
       return check_launch("ccgqa_prep_bwd_vec_kernel");
     }
@@ -516,7 +517,8 @@ extern "C" int hydra_causal_im2col(const void* x, int64_t x_rs, void* out, int64
   const int64_t total = G * B * S * taps * cg;
   if (total == 0) return HYDRA_OK;
   HYDRA_REQUIRE(x && out, "causal_im2col: null pointer");
-  HYDRA_REQUIRE(S < (int64_t(1) << 31) && G * cg < (int64_t(1) << 31), "causal_im2col: too large");
+  HYDRA_REQUIRE(S < (int64_t(1) << 31) && G * cg < (int64_t(1) << 31) &&
+                    grid_fits((total + 255) / 256, 256), "causal_im2col: too large");
   auto st = static_cast<hipStream_t>(stream);
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&] {
     causal_im2col_kernel<T><<<static_cast<unsigned>((total + 255) / 256), 256, 0, st>>>(
@@ -535,7 +537,8 @@ extern "C" int hydra_causal_col2im(const void* in, void* out, int64_t out_rs, in
   const int64_t total = B * S * G * cg;
   if (total == 0) return HYDRA_OK;
   HYDRA_REQUIRE(in && out, "causal_col2im: null pointer");
-  HYDRA_REQUIRE(S < (int64_t(1) << 31) && G * cg < (int64_t(1) << 31), "causal_col2im: too large");
+  HYDRA_REQUIRE(S < (int64_t(1) << 31) && G * cg < (int64_t(1) << 31) &&
+                    grid_fits((total + 255) / 256, 256), "causal_col2im: too large");
   auto st = static_cast<hipStream_t>(stream);
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&] {
     causal_col2im_kernel<T><<<static_cast<unsigned>((total + 255) / 256), 256, 0, st>>>(

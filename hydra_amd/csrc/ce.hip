@@ -383,7 +383,7 @@ extern "C" int hydra_ce_rows(const void* logits, int64_t rows, int64_t vocab, in
                              float* lse, void* grad, int64_t grad_rs, const float* grad_scale,
                              int dtype, void* stream) {
   HYDRA_REQUIRE(rows >= 0 && vocab >= 1, "ce_rows: bad size");
-  HYDRA_REQUIRE(vocab < (int64_t(1) << 31) && rows < (int64_t(1) << 31), "ce_rows: too large");
+  HYDRA_REQUIRE(vocab < (int64_t(1) << 31) && grid_fits(rows, 256), "ce_rows: too large");
   HYDRA_REQUIRE(logits_rs >= vocab && (!grad || grad_rs >= vocab), "ce_rows: row stride < vocab");
   HYDRA_REQUIRE(dtype == HYDRA_F32 || dtype == HYDRA_BF16 || dtype == HYDRA_F16,
                 "ce_rows: unknown dtype");
@@ -410,7 +410,7 @@ extern "C" int hydra_ce_grad_planes(const float* logits, int64_t rows, int64_t v
                                     int64_t planes_rs, int64_t plane_stride, const float* grad_scale,
                                     void* stream) {
   HYDRA_REQUIRE(rows >= 0 && vocab >= 1, "ce_grad_planes: bad size");
-  HYDRA_REQUIRE(vocab < (int64_t(1) << 31) && rows < (int64_t(1) << 31), "ce_grad_planes: too large");
+  HYDRA_REQUIRE(vocab < (int64_t(1) << 31) && grid_fits(rows, 256), "ce_grad_planes: too large");
   HYDRA_REQUIRE(logits_rs >= vocab && planes_rs >= vocab, "ce_grad_planes: row stride < vocab");
   const bool in_place = planes == logits;
   if (in_place)

@@ -154,6 +154,9 @@ __device__ __forceinline__ float halves_sum(float x) {
 void set_error(const std::string& msg);
 int fail(int code, const std::string& msg);
 int check_launch(const char* what);
+// Whether a launch's first dimension runs whole: HIP counts its threads in 32
+// bits and runs what is left modulo 2^32, without an error, where they pass it.
+inline bool grid_fits(int64_t groups, int threads) { return groups * threads < (int64_t(1) << 32); }
 bool aligned16(const void* p);
 int dtype_size(int dtype);
 // Compute units of the current device (cached per device).

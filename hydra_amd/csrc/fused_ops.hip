@@ -97,6 +97,7 @@ static int launch_rms_vec(const T* X, const T* W, T* Y, int64_t rows, int nvec, 
                           int64_t x_rs, int64_t y_rs, float eps, hipStream_t st) {
   constexpr int RI = CPL >= 4 ? 1 : (CPL >= 2 ? 2 : 4);
   constexpr int RPB = (kBlock / 64) * (64 / LPR) * RI;
+  HYDRA_REQUIRE(grid_fits((rows + RPB - 1) / RPB, kBlock), "rms_norm: too many rows");
   const dim3 grid(static_cast<unsigned>((rows + RPB - 1) / RPB));
   rms_norm_vec_kernel<T, LPR, CPL, RI><<<grid, kBlock, 0, st>>>(X, W, Y, rows, nvec, (int)dim,
                                                                x_rs, y_rs, eps);
@@ -131,6 +132,7 @@ static int launch_rms_norm(const void* x, const void* w, void* y, int64_t rows,
     HYDRA_RMS_CASE(64, 1) HYDRA_RMS_CASE(64, 2) HYDRA_RMS_CASE(64, 3) HYDRA_RMS_CASE(64, 4) HYDRA_RMS_CASE(64, 6) HYDRA_RMS_CASE(64, 8)
 #undef HYDRA_RMS_CASE
   }
+  HYDRA_REQUIRE(grid_fits((rows + 3) / 4, kBlock), "rms_norm: too many rows");
   const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
   rms_norm_scalar_kernel<T><<<grid, kBlock, 0, st>>>(X, W, Y, rows, (int)dim, x_rs, y_rs, eps);
   return check_launch("rms_norm_scalar_kernel");
@@ -349,6 +351,7 @@ static int launch_swiglu(const void* g, const void* u, void* o, int64_t rows,
     return check_launch("swiglu_vec_kernel");
   }
   const int64_t total = rows * hidden;
+  HYDRA_REQUIRE(grid_fits((total + kBlock - 1) / kBlock, kBlock), "swiglu: tensor too large");
   const dim3 grid(static_cast<unsigned>((total + kBlock - 1) / kBlock));
   swiglu_scalar_kernel<T><<<grid, kBlock, 0, st>>>(G, Up, O, total, hidden, g_rs,
                                                    u_rs, o_rs);
@@ -424,6 +427,7 @@ static int launch_qk_norm(const void* q, const void* k, void* qo, void* ko,
                       aligned16(q) && aligned16(k) && aligned16(qo) && aligned16(ko);
   if (vec_ok) {
     const int64_t threads = (q_rows + k_rows) * lpr;
+    HYDRA_REQUIRE(grid_fits((threads + kBlock - 1) / kBlock, kBlock), "qk_norm: tensor too large");
     const dim3 grid(static_cast<unsigned>((threads + kBlock - 1) / kBlock));
 #define HYDRA_QKN_CASE(L)                                                      \
   case L:                                                                      \
@@ -437,6 +441,7 @@ static int launch_qk_norm(const void* q, const void* k, void* qo, void* ko,
     }
 #undef HYDRA_QKN_CASE
   }
+  HYDRA_REQUIRE(grid_fits((q_rows + k_rows + kBlock - 1) / kBlock, kBlock), "qk_norm: tensor too large");
   const dim3 grid(static_cast<unsigned>((q_rows + k_rows + kBlock - 1) / kBlock));
   qk_norm_scalar_kernel<T><<<grid, kBlock, 0, st>>>(Q, K, QO, KO, q_rows, k_rows,
                                                     (int)hd, scale, temp);
@@ -778,6 +783,7 @@ static int launch_swiglu_bwd(const void* g, const void* u, const void* gy, void*
     return check_launch("swiglu_bwd_vec_kernel");
   }
   const int64_t total = rows * hidden;
+  HYDRA_REQUIRE(grid_fits((total + kBlock - 1) / kBlock, kBlock), "swiglu_bwd: tensor too large");
   const dim3 grid(static_cast<unsigned>((total + kBlock - 1) / kBlock));
   swiglu_bwd_scalar_kernel<T><<<grid, kBlock, 0, st>>>(G, Up, GY, GG, GU, total, hidden, g_rs, u_rs, gy_rs,
                                                        gg_rs, gu_rs);
@@ -863,6 +869,7 @@ static int launch_qk_norm_bwd(const void* q, const void* k, const void* gqo, con
                       aligned16(k) && aligned16(gqo) && aligned16(gko) && aligned16(gq) && aligned16(gk);
   if (vec_ok) {
     const int64_t threads = (q_rows + k_rows) * lpr;
+    HYDRA_REQUIRE(grid_fits((threads + kBlock - 1) / kBlock, kBlock), "qk_norm_bwd: tensor too large");
     const dim3 grid(static_cast<unsigned>((threads + kBlock - 1) / kBlock));
 #define HYDRA_QKNB_CASE(L)                                                                              \
   case L:                                                                                               \
@@ -876,6 +883,7 @@ static int launch_qk_norm_bwd(const void* q, const void* k, const void* gqo, con
     }
 #undef HYDRA_QKNB_CASE
   }
+  HYDRA_REQUIRE(grid_fits((q_rows + k_rows + kBlock - 1) / kBlock, kBlock), "qk_norm_bwd: tensor too large");
   const dim3 grid(static_cast<unsigned>((q_rows + k_rows + kBlock - 1) / kBlock));
   qk_norm_bwd_scalar_kernel<T><<<grid, kBlock, 0, st>>>(Q, K, GQO, GKO, GQ, GK, q_rows, k_rows, (int)hd, scale,
                                                         temp);

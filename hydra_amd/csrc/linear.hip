@@ -154,7 +154,7 @@ extern "C" int hydra_linear_fwd(const void* x, int64_t x_rs, const void* w, int6
   auto st = static_cast<hipStream_t>(stream);
   const int64_t ncg = (N + kLinCols - 1) / kLinCols;
   const int64_t nrg = ((M + kLinRows - 1) / kLinRows + 7) / 8 * 8;
-  HYDRA_REQUIRE(ncg * nrg < (int64_t(1) << 31), "linear: too large");
+  HYDRA_REQUIRE(grid_fits(ncg * nrg, 64 * kLinWaves), "linear: too large");
   const dim3 grid(static_cast<unsigned>(ncg * nrg));
   auto X = static_cast<const bf16*>(x);
   auto W = static_cast<const bf16*>(w);

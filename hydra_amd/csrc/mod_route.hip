@@ -704,6 +704,7 @@ static int launch_gather(const void* x, const int64_t* idx, void* xs, int64_t B,
     return check_launch("mod_gather_kernel");
   }
   const int64_t total = B * k * D;
+  HYDRA_REQUIRE(grid_fits((total + 255) / 256, 256), "mod_gather: too large");
   const dim3 grid(static_cast<unsigned>((total + 255) / 256));
   mod_gather_scalar_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(x), idx,
                                                      static_cast<T*>(xs), total, D, k, L,
@@ -890,6 +891,7 @@ static int launch_scatter(void* out, const void* y, const int64_t* idx, const fl
   auto O = static_cast<T*>(out);
   auto Y = static_cast<const T*>(y);
   if (mode == HYDRA_SCATTER_ADD_SEQ) {
+    HYDRA_REQUIRE(grid_fits((B * D + 255) / 256, 256), "mod_scatter: too large");
     const dim3 grid(static_cast<unsigned>((B * D + 255) / 256));
     mod_scatter_seq_kernel<T><<<grid, 256, 0, st>>>(O, Y, idx, B, D, k, L, o_bs, o_ls);
     return check_launch("mod_scatter_seq_kernel");
@@ -909,6 +911,7 @@ static int launch_scatter(void* out, const void* y, const int64_t* idx, const fl
     return check_launch("mod_scatter_kernel");
   }
   const int64_t total = B * k * D;
+  HYDRA_REQUIRE(grid_fits((total + 255) / 256, 256), "mod_scatter: too large");
   const dim3 grid(static_cast<unsigned>((total + 255) / 256));
   if (mode == HYDRA_SCATTER_ADD)
     mod_scatter_scalar_kernel<T, HYDRA_SCATTER_ADD><<<grid, 256, 0, st>>>(
@@ -951,7 +954,7 @@ extern "C" int hydra_mod_scatter_bwd(const void* grad, const void* y, const int6
   HYDRA_REQUIRE(D > 0, "mod_scatter_bwd: empty rows");
   HYDRA_REQUIRE(grad && y && idx && w, "mod_scatter_bwd: null pointer");
   HYDRA_REQUIRE(g_ls >= D, "mod_scatter_bwd: row stride smaller than D");
-  HYDRA_REQUIRE((B * k + 3) / 4 < (int64_t(1) << 31), "mod_scatter_bwd: too large");
+  HYDRA_REQUIRE(grid_fits((B * k + 3) / 4, 256), "mod_scatter_bwd: too large");
   auto st = static_cast<hipStream_t>(stream);
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&] {
     constexpr int E = Vec<T>::N;
