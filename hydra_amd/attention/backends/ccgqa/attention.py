@@ -34,7 +34,6 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd import forward_ad
 
 from .... import _lib
 from ...._lib import CCGQA_V_TRANSPOSED, CCGQA_W_TILED, MASK_KEY_PADDING, MASK_REFERENCE_SDPA
@@ -262,7 +261,7 @@ class CCGQAAttention(nn.Module):
         return CCGQACache(self, pool, dtype)
 
     def _check_cache(self, name: str, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan) -> None:
-        if forward_ad._current_level >= 0:
+        if _lib.forward_ad._current_level >= 0:
             _lib.refuse_tangents(name, x, *self.parameters())
         if cache.k_pages.shape[1] != self.n_kv_heads or cache.k_pages.shape[3] != self.head_dim or \
                 cache.ring.shape[2] != self.latent_dim + 2 * self.kv_dim:

@@ -320,7 +320,8 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
         raise ValueError(f"{name}: slots must be int64, one a request, got {slots.dtype} {tuple(slots.shape)}")
     check_pages(name, k_pages, v_pages)
     check_no_gradient(name, qkv, ring, k_pages, v_pages, wq1, wq2, wk1, wk2)
-    _lib.refuse_tangents(name, temperature, cos, sin)
+    if _lib.forward_ad._current_level >= 0:
+        _lib.refuse_tangents(name, temperature, cos, sin)
     pages, _, page, _ = k_pages.shape
     if k_pages.shape[1] != n_kv_heads or k_pages.shape[3] != head_dim or k_pages.dtype != dt:
         raise ValueError(f"{name}: pages must be {dt} [pages, {n_kv_heads}, page_size, {head_dim}], got "

@@ -76,9 +76,12 @@ def check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None
 
 
 def check_no_gradient(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name}: no gradient (call it under torch.no_grad())")
-    _lib.refuse_tangents(name, *tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name}: no gradient (call it under torch.no_grad())")
+    if _lib.forward_ad._current_level >= 0:
+        _lib.refuse_tangents(name, *tensors)
 
 
 def check_distinct(name: str, what: str, t: torch.Tensor) -> None:
