@@ -300,8 +300,11 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     (PagePlan.slots of a step of width 1).  A request whose slot lies outside
     the pool, or whose position is negative or past the RoPE tables, changes
     nothing and gets zeros for q.  Weights, temperature, tables and flags as
-    ccgqa_prep takes them.  fp32 inside, one rounding.  Inference only: no
-    gradient, and refused where the row, the ring, the pages or the conv weights
+    ccgqa_prep takes them.  fp32 inside, one rounding at the end; with three taps
+    and head_dim 16, 32, 64 or 128 a 16-bit type carries what lies between the two
+    convs as two terms of its own (16 significant bits for bf16; for fp16 22 from
+    1/8 on, to within 2^-25 below, infinity beyond its range), where ccgqa_prep
+    rounds it to one.  Inference only: no gradient, and refused where the row, the ring, the pages or the conv weights
     record one; the temperature and the tables count as constants."""
     name = "ccgqa_decode_prep"
     _lib.require_gpu(name, qkv, ring, positions, slots, k_pages, v_pages, wq1, wq2, wk1, wk2, temperature, cos, sin)

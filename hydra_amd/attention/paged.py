@@ -215,11 +215,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """softmax(scale * q k^T) v of one query token per request, q [N, Hq, hd],
     over the first `lengths[i]` (int32) positions of its pages; query head h
     reads key head h // (Hq / Hkv).  scale: hd ** -0.5 by default.  `out`: a
-    [N, Hq, hd] tensor with a unit last stride to write to (q itself is one).
+    [N, Hq, hd] tensor with a unit last stride to write to (q itself is one;
+    otherwise none of the memory that is read).
 
     fp32 scores, softmax and sums, one rounding.  Lengths count within
     [0, P * page_size]; keys on a page outside the pool are not seen; a
-    request that sees none gets zeros.  Inference only: no gradient."""
+    request that sees none (or whose scores are all -inf) gets zeros.  Inference only: no gradient."""
     name = "paged_attention"
     _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out)
     check_pages(name, k_pages, v_pages)

@@ -10,8 +10,10 @@
 //   q, k  = rope(normalize(y2 + QK-mean) (* temperature)), v = v_curr | v_prev.
 // y1 is computed again at its ks positions: that is ks^2 hd products a channel
 // beside the ks C of conv2, and leaves one launch and a state of plain rows.
-// fp32 throughout, one rounding at the end; the MFMA form carries y1 into conv2 as
-// two 16-bit terms (16 significant bits for bf16, 22 for fp16).
+// fp32 throughout, one rounding at the end, but that the matrix form of a 16-bit
+// type carries y1 into conv2 as two terms of it: 16 significant bits for bf16; for
+// fp16 22 from 1/8 on, to within 2^-25 below, and infinity beyond fp16's range.
+// The prompts' kernels keep one such term.
 //
 // The ring holds each request's last R projected rows, row p at p % R.  A step
 // reads rows p - 2(ks-1) .. p-1 and writes row p, which is none of them as R >
@@ -196,8 +198,8 @@ __device__ __forceinline__ float dot(const T* a, const T* b, int n, float s) {
 // Any head_dim, taps and flags: one workgroup per request and head on the
 // VALU, y1 in LDS as [ks][C] floats, then y2 [hd].  Every workgroup computes all
 // of conv1 for itself, ks^2 hd products a channel, and a lane's weights are rows
-// of their own, so the cache's lines bound it: 8/2 heads of 48, three taps, 17 us
-// for one request and 33 us for 32; heads of 64 with five taps, 32 requests, 150 us.
+// of their own, so the cache's lines bound it: 8/2 heads of 48, three taps, 18 us
+// for one request and 34 us for 32; heads of 64 with five taps, 32 requests, 156 us.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kGenericThreads) void decode_prep_generic_kernel(DecodeArgs a) {
   extern __shared__ __attribute__((aligned(16))) float sm[];
@@ -344,8 +346,9 @@ constexpr int decode_waves(int hb, int size) { return hb * size <= 8 ? 16 : 8; }
 // few of them run, so a head whose weights (conv1's of all its channels, its own
 // of conv2) are large is dealt out to workgroups of 4 waves and 4 blocks, and a
 // second launch (4 us, what 200 KB take, or 100 KB of tap-major weights, whose
-// operands are 32-byte pieces of rows) adds them up and ends the chain; not where
-// the heads of many requests fill the chip as they are.
+// operands are 32-byte pieces of rows) adds them up and ends the chain; not from
+// 128 workgroups on (128 requests, 8/2 heads of 64, 80 workgroups split in 8: 14.0 +
+// 4.0 us; 256, 160 of them whole: 19.3).
 struct DecodePlan {
   int span, waves, splits;
 };
@@ -493,9 +496,10 @@ struct Tail {
 // conv1's channels there and their share of conv2 at once, and the waves' y2 are
 // added up in LDS.  Parts leave their sums in `part` [split][head][tile][16][HD],
 // which decode_join_kernel adds in order.  Weights come from L2 (each head
-// reads all of conv1's); bound by the chain position -> rows -> convs -> norm
-// (one request, 4/1 heads of 64: 7.9 us), and for many requests by the rows' and
-// weights' way from L2 (256, 8/2 heads of 64, 65 MB of it: 19.6 us).
+// reads all of conv1's); bound by the chain position -> rows -> convs -> norm:
+// one request, 4/1 heads of 64, 7.6 us; 256, 8/2 heads of 64, 19.3 us, where 160
+// workgroups on 256 CUs go through two channel blocks a wave and draw 65 MB from
+// L2, 0.4 MB each at 21 GB/s, less than a CU can.
 template <typename T, int HB, bool TILED>
 __global__ __launch_bounds__(64 * decode_waves(HB, sizeof(T))) void decode_prep_mfma_kernel(DecodeArgs a) {
   constexpr int HD = HB * 16;

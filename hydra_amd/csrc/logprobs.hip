@@ -15,9 +15,12 @@
 // backward reads it once and writes the gradient.  8192 rows of 32000, bf16:
 // 108 us, 4.9 TB/s, forward (135 with 20 alternatives) and 190 us, 5.5 TB/s,
 // backward.  A few rows take the chain row -> maximum -> sums (-> bound ->
-// candidates -> ranks): 16 of 50257, 20 alternatives, 12.4 us.  Rows start anywhere: a row
-// is taken in the 16-byte pieces of memory that it lies in, what is left at its
-// two ends element by element.
+// candidates -> ranks): 16 of 50257, 20 alternatives, 12.1 us.  Where fewer than
+// K of 64 groups of lanes hold an allowed logit, or equal ones lead the row, the
+// alternatives are taken one by one (see logp_kernel): such rows (12 allowed of
+// 50257, or all equal) take 367 us, and a launch with one among them as long.
+// Rows start anywhere: a row is taken in the 16-byte pieces of memory that it lies
+// in, what is left at its two ends element by element.
 #include "common.h"
 #include "mod_keys.h"
 
@@ -125,7 +128,9 @@ __device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int K) {
 // 64 ln(64 / (64 - K)) of them where the order is random: 24 for K = 20).  Only
 // threads whose own maximum reaches it look at their pieces again; what they
 // find is listed in LDS and ranked against each other.  Where equal values make
-// them too many, or a NaN leads the row, the K best are taken one by one.
+// them more than 1024 (masked ones too, where they are the bound), or a NaN leads
+// the row, the K best are taken one by one, each by a scan of the row that waits
+// for the last one.
 template <typename T, int NCH, bool TOP>
 __global__ __launch_bounds__(kThreads) void logp_kernel(LogpArgs a) {
   constexpr int E = Vec<T>::N, WAVES = kThreads / 64;

@@ -4,11 +4,14 @@
 //   t < lengths[n], position t in page table[n, t / page_size].
 //
 // A step reads each key and value once and does 4 G flops per element pair.
-// 64 requests of 16384 keys, 8/2 heads of 64, bf16 (537 MB): 104 to 110 us, 4.9
-// to 5.2 TB/s, a large copy's rate.  Short rows shared by many heads do not
-// reach it (48 requests of up to 8192 keys, 28/4 heads of 16: 18 us, 0.6 TB/s):
-// exponentials and products of 8 heads for 32 bytes of key take longer.  A few
-// keys take the launch and the chain table -> keys -> softmax -> output, 5 us.
+// 64 requests of 16384 keys, 8/2 heads of 64, bf16 (537 MB): 100 us and 5 for the
+// join, 5.1 TB/s, a large copy's rate; 8 heads to a key head of 128, 16 requests
+// of 16384 keys (134 MB): 32 + 6.5 us, 3.5 TB/s, and of 256, 8 requests: 33 + 15.
+// Little work does not reach it.  48 requests of up to 8192 keys, 28/4 heads of
+// 16 (11 MB), take 13.6 + 4.5 us: their 828 rounds are dealt out two at a time,
+// so that 414 of 768 workgroups go through two chains of table, keys, softmax
+// and values, one after the other, and 354 have none; then the join is launched.
+// A few keys take the launch and one such chain, 5 us.
 // A wave walks its keys KT at a time:
 //
 //  * scores S^T = K Q^T on the matrix cores: keys are the rows of the A operand,
@@ -104,13 +107,15 @@ __device__ __forceinline__ int seen_keys(const PagedArgs& a, int n) {
   return max(0, min(a.lengths[n], a.P << a.shift));
 }
 
-// Most waves of a workgroup (a launch takes 4 or 8), and keys of a wave's step: 4 KB
-// of keys and as much of values in flight.  Of 128-byte keys 32: with 16, 4 requests
+// Most waves of a workgroup (a launch takes 4 or 8, LDS is sized for 8), and keys
+// of a wave's step: 4 KB of keys and as much of values in flight.  Of 128-byte keys 32: with 16, 4 requests
 // of 16384 keys take 18.8 us instead of 17.3, 32 of 3001 with 28/4 heads 31.9
 // instead of 28.9; with 64, 16 of 16384 take 34.0 instead of 32.0.
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 __device__ __forceinline__ int waves() { return blockDim.x >> 6; }
+// Registers: 190 with 8 heads of 256-byte keys, 215 of 512, two waves a SIMD; in
+// fp32 keys above 512 bytes spill 7 (2 heads) to 54 (8 heads, whole form) of 256.
 constexpr int tile_keys(int lpr) { return lpr < 4 ? 64 : (lpr <= 16 ? 32 : 16); }
 template <int LPR> struct Tile { static constexpr int KT = tile_keys(LPR); };
 
@@ -601,9 +606,9 @@ struct Split {
 constexpr int kMaxResident = 4;  // workgroups of a CU that a split launch takes at most (8: the same times)
 
 // Split where the items alone would not fill the chip and a request may be longer
-// than 128 KB of keys or 2048 of them, whole and split: of 128-byte keys 512 take
-// 8.0 and 10.3 us, 1000 10.5 and 10.6, 2000 15.6 and 10.8; of 32-byte keys 2000 take
-// 9.9 and 11.0, 4000 15.1 and 11.1.  8 waves for few short items (one request of
+// than 128 KB of keys or 2048 of them, whole and split with its join: of 128-byte
+// keys 512 take 8.0 and 10.3 us, 1000 10.5 and 10.6, 2000 15.6 and 10.8; of 32-byte
+// keys 2000 take 9.9 and 11.0, 4000 15.1 and 11.1.  8 waves for few short items (one request of
 // 500 keys, 28/4 heads of 64: 9.4 us, 11.4 with 4); where items or rounds are many,
 // twice as many workgroups of 4 have more of the chip's registers in use (256
 // requests of 20 keys, 28/4 heads of 64: 8.0 us, 11.8 with 8).

@@ -81,8 +81,10 @@ __device__ __forceinline__ int block_incl_sum(int x, int* part, int& total) {
 // workgroup and read by none.
 //
 // Bound by its launch and the chain lengths -> sums -> stack -> slots at a decoding
-// step (32 requests: 3.6 us), by the slots' writes for prompts (256 of 4096
-// tokens, 8 MB: 7.2 us).
+// step (32 requests: 2.7 us).  For prompts (256 of up to 4096 tokens: 7.0 us, 8 MB
+// written at 1.3 TB/s, far below what the memory takes) by the sixteen trips of a
+// thread, each a look into the table or the stack for its one token and a store of
+// 8 bytes, although the tokens of a page share what is looked up.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
   __shared__ int part[kPlanThreads / 64];
   __shared__ int s_first[kPlanThreads], s_have[kPlanThreads], s_need[kPlanThreads];
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 // threads take the entries of 256 requests in their order on the stack, twice
 // 256 at once, and look up whose each is; those that are pages are counted only
 // where one of them is none.  Bound by the launch and the chain lengths ->
-// sums -> table -> stack.
+// sums -> table -> stack: 32 of 256 requests with 16 pages each, 3.0 us.
 constexpr int kReleaseEntries = 2;
 
 __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* done, int* lengths, int* table,
@@ -249,7 +251,8 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
 // position's, which lie one after the other in the source and in the page.
 // Bound by HBM: each row is read and written once, and not read again soon (so
 // past the L2).  64 prompts of up to 4096 tokens, 8 heads of 128, bf16 (262 MB
-// moved): 50 us, 5.3 TB/s with three pieces a thread; 3.1 with one, 4.4 with
+// moved): 49 us, 5.3 TB/s with three pieces a thread (60 us where the pages lie
+// in no order); 3.1 with one, 4.4 with
 // two, 4.7 with four (workgroups of 12 KB spread their addresses best).  Fewer
 // than 20 MB: 3 to 6 us, the launch.
 constexpr int kStorePieces = 3;

@@ -79,14 +79,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     """ln softmax(logits / temperature) at `tokens`, its entropy, and its
     `top_k` (at most 64) largest entries.
 
-    logits [..., V] (bf16, fp16 or fp32; rows may start anywhere), tokens [...]
-    int64.  A token outside [0, V) (an ignored position's -100) has the log
-    probability 0 and no gradient through it; its row's entropy and
-    alternatives are given as ever.  Among equal logits the lowest index comes
-    first.  Masked logits may be -inf or the type's lowest value; a row of -inf
-    alone has log probabilities -inf, entropy 0 and no gradient; a row with a
-    NaN or +inf has NaN.  The gradient covers logprobs, entropy and
-    top_logprobs (once differentiable; forward-mode tangents are refused); a
+    logits [..., V] (bf16, fp16 or fp32), tokens [...] int64.  Rows may start
+    anywhere, at one stride from each other; others (a batch's logits[:, :-1])
+    are copied first, and the copy is kept for the backward.  A token outside
+    [0, V) (an ignored position's -100) has the log probability 0 and no
+    gradient through it; its row's entropy and alternatives are given as ever.
+    Among equal logits the lowest index comes first.  Masked logits may be -inf
+    or the type's lowest value; a row of -inf alone has log probabilities -inf,
+    entropy 0 and no gradient; a row with a NaN or +inf has NaN.  A row that has
+    masked or equal logits among its alternatives, and more than 1024 of them,
+    takes a scan for each alternative.  The gradient covers logprobs, entropy
+    and top_logprobs (once differentiable; forward-mode tangents are refused); a
     captured backward belongs to a captured forward, through
     torch.autograd.grad or leaves that no eager graph shares."""
     name = "token_logprobs"

@@ -450,7 +450,8 @@ int hydra_ce_grad_planes(const float* logits, int64_t rows, int64_t vocab, int64
  * logprobs[r] = ln p[tokens[r]] (0 for a token outside [0, vocab)),
  * entropy[r] = -sum p ln p, and the top_k (at most 64) largest logits of the
  * row, the lowest index first among equals (NaN counts as the largest):
- * top_tokens [rows, top_k] and ln p there, top_logprobs.  A row of -inf alone
+ * top_tokens [rows, top_k] and ln p there, top_logprobs (by a scan of the row each
+ * where masked or equal logits are among them and more than 1024 in number).  A row of -inf alone
  * has log probabilities -inf and entropy 0; a row with a NaN or +inf has NaN.
  * stats [rows, 2] (optional): what the backward takes.  fp32 results.  No
  * counterpart in the reference, whose losses give mean cross-entropies. */
@@ -534,9 +535,10 @@ int hydra_page_store(const void* k, const void* v, void* k_pages, void* v_pages,
  *   out[n,h] = softmax_t(scale * q[n,h] . k[t]) v[t], t < lengths[n],
  * key head h / (Hq / Hkv).  q, out: [N, Hq, hd] with strides q_st[3],
  * o_st[3]; pages as above; hd <= 256, P * page_size <= 2^30, a page's rows within
- * 2 GiB.  Lengths are taken within [0, P * page_size]; keys on a page outside the pool are not seen; a request
- * that sees no key gets zeros.  Scores, softmax and the products with v are
- * fp32, one rounding into `dtype`.  Needs hydra_paged_attn_workspace bytes of
+ * 2 GiB.  Lengths are taken within [0, P * page_size]; keys on a page outside the
+ * pool are not seen; a request that sees no key (or whose scores are all -inf) gets
+ * zeros.  out may be q; it shares no other memory with what is read.  Scores,
+ * softmax and the products with v are fp32, one rounding into `dtype`.  Needs hydra_paged_attn_workspace bytes of
  * device scratch (16-byte aligned). */
 int hydra_paged_attn(const void* q, const void* k_pages, const void* v_pages, void* out,
                      const int* table, int64_t table_rs, const int* lengths, int64_t N, int64_t Hq,
@@ -559,7 +561,10 @@ int hydra_paged_attn_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t hd, i
  * past the RoPE table's rope_rows changes nothing and gets zeros for q.
  * Weights, temperature, cos/sin and flags as in hydra_ccgqa_prep_fwd
  * (HYDRA_CCGQA_W_TILED: 16-bit, head_dim 16, 32, 64 or 128, three taps).  At most
- * 65535 requests.  fp32 inside, one rounding. */
+ * 65535 requests.  fp32 inside, one rounding at the end; with three taps and those
+ * head_dims a 16-bit type carries what lies between the convs as two terms of its
+ * own: 16 significant bits for bf16; for fp16 22 from 1/8 on, to within 2^-25
+ * below, infinity beyond its range. */
 int hydra_ccgqa_decode_prep(const void* qkv, int64_t qkv_rs, void* ring, int64_t R,
                             const int* positions, const int64_t* slots, const void* wq1,
                             const void* wq2, const void* wk1, const void* wk2,
