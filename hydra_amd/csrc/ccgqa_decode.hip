@@ -647,7 +647,8 @@ int launch_decode(DecodeArgs a, hipStream_t st) {
   mfma = mfma && static_cast<int64_t>(a.N) * a.R * W * sizeof(T) < (int64_t(1) << 32) &&
          a.N * a.qkv_rs * static_cast<int64_t>(sizeof(T)) < (int64_t(1) << 32);
   const bool tiled = a.flags & HYDRA_CCGQA_W_TILED;
-  const DecodePlan plan = decode_plan(a.N, a.Hq, a.Hkv, a.hd, sizeof(T), tiled);
+  // the matrix form's: other sizes may have no block of 16 channels
+  const DecodePlan plan = mfma ? decode_plan(a.N, a.Hq, a.Hkv, a.hd, sizeof(T), tiled) : DecodePlan{};
   a.span = plan.span;
   const dim3 tiles(static_cast<unsigned>(a.Hq + a.Hkv), static_cast<unsigned>((a.N + 15) / 16));
   const dim3 parts(tiles.x, tiles.y, static_cast<unsigned>(plan.splits));

@@ -198,3 +198,21 @@ def test_blocks_with_idle_and_refused_requests(cuda):
     for step in range(6):
         for n in (0, 2):
             assert torch.equal(turns[step][n], whole[step][n]), (step, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,taps", [(1, 1, 2, 4), (1, 1, 2, 3), (2, 1, 2, 1), (1, 1, 14, 3),
+                                                          (7, 7, 2, 2), (3, 1, 4, 5), (1, 1, 16, 3)])
+def test_layers_of_few_channels(cuda, dtype, heads, kv_heads, head_dim, taps):
+    """Fewer channels than a block of the matrix form (16): one token against
+    the oracle's whole sequence."""
+    import test_gpu_ccgqa_decode as td
+
+    from oracle import ccgqa as oc
+
+    cfg = oc.CCGQAConfig(dim=4 * heads * head_dim, n_heads=heads, n_kv_heads=kv_heads, conv_kernel_size=taps)
+    positions = [0, 3, 9, 1]
+    slots = [5, 17, 40, 33]
+    params, rows, ring = td.case(cfg, positions, dtype, seed=heads * head_dim + taps)
+    got = td.run(cuda, cfg, dtype, params, rows, ring, positions, slots, 3, 16)
+    td.check(cfg, dtype, params, rows, ring, positions, slots, 16, got)
