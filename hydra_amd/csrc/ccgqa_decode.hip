@@ -631,6 +631,8 @@ __global__ __launch_bounds__(1024) void decode_join_kernel(DecodeArgs a) {
     tail.store(a, n, hh, tid & 15, [&](int d) { return sum[d][r]; }, [&](int d) { return mean[d][r]; });
 }
 
+constexpr int64_t kDecodeRequests = 65535, kDecodeHeads = 4096;  // of a call
+
 bool decode_mfma_size(int64_t hd, int64_t ks, int flags) {
   return (flags & HYDRA_CCGQA_CONVS) && ks == 3 && (hd == 16 || hd == 32 || hd == 64 || hd == 128);
 }
@@ -721,6 +723,7 @@ extern "C" int64_t hydra_ccgqa_decode_prep_workspace(int64_t N, int64_t Hq, int6
                                                      int flags, int dtype) {
   const int e = dtype_size(dtype);
   if (N <= 0 || Hq <= 0 || Hkv <= 0 || e == 0 || !decode_mfma_size(hd, conv_ks, flags)) return 0;
+  if (N > kDecodeRequests || Hq > kDecodeHeads || Hkv > Hq) return 0;  // which hydra_ccgqa_decode_prep refuses
   const int splits = decode_plan(N, Hq, Hkv, hd, e, flags & HYDRA_CCGQA_W_TILED).splits;
   return splits == 1 ? 0 : 4 * static_cast<int64_t>(splits) * (Hq + Hkv) * ((N + 15) / 16) * 16 * hd;
 }
@@ -744,7 +747,7 @@ extern "C" int hydra_ccgqa_decode_prep(const void* qkv, int64_t qkv_rs, void* ri
   HYDRA_REQUIRE(!convs || (conv_ks >= 1 && conv_ks <= 16), "ccgqa_decode_prep: conv taps must be in [1, 16]");
   const int64_t back = std::max<int64_t>(convs ? 2 * (conv_ks - 1) : 0, flags & HYDRA_CCGQA_VALUE_SHIFT ? 1 : 0);
   HYDRA_REQUIRE(R > back && R < (1 << 20), "ccgqa_decode_prep: the ring must hold more rows than a token looks back");
-  HYDRA_REQUIRE(N <= 65535 && Hq <= 4096 && hd <= 4096 && pages < (int64_t(1) << 31),
+  HYDRA_REQUIRE(N <= kDecodeRequests && Hq <= kDecodeHeads && hd <= 4096 && pages < (int64_t(1) << 31),
                 "ccgqa_decode_prep: too large");
   const int64_t W = (Hq + 2 * Hkv) * hd;
   HYDRA_REQUIRE(qkv_rs >= W || N <= 1, "ccgqa_decode_prep: row stride < L + 2K");

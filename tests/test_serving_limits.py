@@ -44,3 +44,13 @@ def test_pools_that_no_layer_decodes():
                         (endless, PagePool(1, 1 << 30, 4, 4096, device="cpu"))):
         with pytest.raises(RuntimeError, match="the pool is on cpu"):  # nothing else against them
             layer.new_cache(pool)
+
+
+def test_workspace_of_sizes_that_are_refused():
+    """A query of heads whose channels pass 64 bits ended the process in a
+    division by zero."""
+    from hydra_amd import _lib
+
+    for N, Hq, Hkv in ((1024, 1 << 62, 1), (1 << 62, 8, 2), (1, 4097, 1), (65536, 8, 2), (1, 2, 4)):
+        assert _lib.query("hydra_ccgqa_decode_prep_workspace", N, Hq, Hkv, 32, 3, 1, 1) == 0
+    assert _lib.query("hydra_ccgqa_decode_prep_workspace", 16, 16, 4, 64, 3, 1, 1) > 0
