@@ -1367,6 +1367,7 @@ extern "C" int hydra_ccgqa_prep_fwd(const void* qkv, int64_t qkv_rs, const void*
   HYDRA_REQUIRE(Hq % Hkv == 0, "ccgqa_prep: n_heads must be a multiple of n_kv_heads");
   HYDRA_REQUIRE(hd % 2 == 0, "ccgqa_prep: head_dim must be even");
   HYDRA_REQUIRE((flags & ~(127 | HYDRA_CCGQA_ROPE_BF16)) == 0, "ccgqa_prep: unknown flag bits");
+  HYDRA_REQUIRE(dtype_size(dtype) > 0, "ccgqa_prep: unknown dtype code");
   const int64_t L = Hq * hd, K = Hkv * hd;
   HYDRA_REQUIRE(!(flags & HYDRA_CCGQA_VALUE_SHIFT) || K % 2 == 0,
                 "ccgqa_prep: kv_dim must be even for the value shift");

@@ -54,3 +54,13 @@ def test_workspace_of_sizes_that_are_refused():
     for N, Hq, Hkv in ((1024, 1 << 62, 1), (1 << 62, 8, 2), (1, 4097, 1), (65536, 8, 2), (1, 2, 4)):
         assert _lib.query("hydra_ccgqa_decode_prep_workspace", N, Hq, Hkv, 32, 3, 1, 1) == 0
     assert _lib.query("hydra_ccgqa_decode_prep_workspace", 16, 16, 4, 64, 3, 1, 1) > 0
+
+
+def test_prep_of_an_unknown_type():
+    """It took the alignment of weights by a size of 0."""
+    from hydra_amd import _lib
+
+    for dtype in (-1, 3, 7):
+        with pytest.raises(ValueError, match="unknown dtype"):
+            _lib.call("hydra_ccgqa_prep_fwd", FAKE, 192, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 16, FAKE, FAKE, FAKE, 3,
+                      128, 8, 2, 16, 3, 1, dtype, None)
