@@ -304,8 +304,9 @@ def ccgqa_decode_prep(qkv: torch.Tensor, ring: torch.Tensor, positions: torch.Te
     and head_dim 16, 32, 64 or 128 a 16-bit type carries what lies between the two
     convs as two terms of its own (16 significant bits for bf16; for fp16 22 from
     1/8 on, to within 2^-25 below, infinity beyond its range), where ccgqa_prep
-    rounds it to one.  Inference only: no gradient, and refused where the row, the ring, the pages or the conv weights
-    record one; the temperature and the tables count as constants."""
+    rounds it to one.  Inference only: no gradient, and refused where the row,
+    the ring, the pages or the conv weights record one; the temperature and the
+    tables count as constants."""
     name = "ccgqa_decode_prep"
     _lib.require_gpu(name, qkv, ring, positions, slots, k_pages, v_pages, wq1, wq2, wk1, wk2, temperature, cos, sin)
     L, K = n_heads * head_dim, n_kv_heads * head_dim

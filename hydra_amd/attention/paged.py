@@ -121,10 +121,10 @@ def _plan(name, lengths, new_tokens, table, free_pages, free_count, page_size, w
     within = () if max_length is None else (max_length,)
     with _lib.on_device(lengths):
         _lib.call("hydra_pool_plan" if within else "hydra_page_plan", lengths.data_ptr(), new_tokens.data_ptr(),
-                  table.data_ptr(), _row_stride(table), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
-                  slots.data_ptr(), after.data_ptr(), seen.data_ptr(), granted.data_ptr(), positions.data_ptr(),
-                  left.data_ptr(), N, table.shape[1], width, int(page_size), *within, 1 if from_empty else 0,
-                  _lib.stream(lengths))
+                  table.data_ptr(), _row_stride(table), free_pages.data_ptr(), free_pages.numel(),
+                  free_count.data_ptr(), slots.data_ptr(), after.data_ptr(), seen.data_ptr(), granted.data_ptr(),
+                  positions.data_ptr(), left.data_ptr(), N, table.shape[1], width, int(page_size), *within,
+                  1 if from_empty else 0, _lib.stream(lengths))
     return PagePlan(slots, positions, after, seen, granted, left, bool(from_empty))
 
 
@@ -167,8 +167,8 @@ def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     within = () if pages is None else (int(pages),)
     with _lib.on_device(lengths):
         _lib.call("hydra_pool_release" if within else "hydra_page_release", done.data_ptr(), lengths.data_ptr(),
-                  table.data_ptr(), _row_stride(table), free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
-                  N, table.shape[1], int(page_size), *within, _lib.stream(lengths))
+                  table.data_ptr(), _row_stride(table), free_pages.data_ptr(), free_pages.numel(),
+                  free_count.data_ptr(), N, table.shape[1], int(page_size), *within, _lib.stream(lengths))
 
 
 def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -220,7 +220,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     fp32 scores, softmax and sums, one rounding.  Lengths count within
     [0, P * page_size]; keys on a page outside the pool are not seen; a
-    request that sees none (or whose scores are all -inf) gets zeros.  Inference only: no gradient."""
+    request that sees none (or whose scores are all -inf) gets zeros.  Inference
+    only: no gradient."""
     name = "paged_attention"
     _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out)
     check_pages(name, k_pages, v_pages)

@@ -211,7 +211,8 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const uint8_t* do
       for (int half = kPlanThreads / 2; half > 0; half >>= 1)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (static_cast<unsigned>(s_upto[at[u] + half - 1]) <= min(e0 + u * kPlanThreads + tid, entries - 1)) at[u] += half;
+          if (static_cast<unsigned>(s_upto[at[u] + half - 1]) <= min(e0 + u * kPlanThreads + tid, entries - 1))
+            at[u] += half;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const unsigned e = min(e0 + u * kPlanThreads + tid, entries - 1);
