@@ -23,6 +23,7 @@ LIB_PATH = Path(os.environ.get("HYDRA_AMD_LIB", Path(__file__).with_name("libhyd
 # status / dtype / flag codes (include/hydra_amd.h)
 OK, ERR_ARG, ERR_LAUNCH, ERR_UNSUPPORTED = 0, 1, 2, 3
 F32, BF16, F16 = 0, 1, 2
+PAGE_I8, PAGE_E4M3 = 16, 17
 CCGQA_CONVS, CCGQA_QK_MEAN, CCGQA_VALUE_SHIFT, CCGQA_QK_NORM, CCGQA_ROPE = 1, 2, 4, 8, 16
 CCGQA_V_TRANSPOSED = 32
 CCGQA_W_TILED = 64
@@ -33,6 +34,7 @@ NORM_NONE, NORM_RMS, NORM_ADA = 0, 1, 2
 LINEAR_W_TILED = 1
 
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+PAGE_CODE = {torch.int8: PAGE_I8, torch.float8_e4m3fn: PAGE_E4M3}  # of pages of 8 bits
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -78,6 +80,9 @@ SIGNATURES = {
     "hydra_paged_attn": [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                          _I64P, _I64P, _I64P, _I64P, _F, _I, _P, _I64, _P],
     "hydra_paged_attn_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I, _I64P],
+    "hydra_prefix_attn": [_P, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                          _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _F, _I, _I, _P, _I64, _P],
+    "hydra_prefix_attn_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _I64P],
     "hydra_ccgqa_decode_prep": [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P,
                                 _I64P, _I64P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _P],
     "hydra_ccgqa_decode_prep_workspace": [_I64, _I64, _I64, _I64, _I64, _I, _I],

@@ -201,6 +201,33 @@ def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
                   _strides(k_pages), _strides(v_pages), _lib.dtype_code(k), _lib.stream(k))
 
 
+def check_scales(name: str, pages: torch.Tensor, scales):
+    """(k_scales, v_scales) of pages of 8 bits; None for others, which have none."""
+    eight = pages.dtype in _lib.PAGE_CODE
+    if scales is None:
+        if eight:
+            raise ValueError(f"{name}: pages of {str(pages.dtype)[6:]} need scales")
+        return None
+    k, v = scales
+    if not eight:
+        raise ValueError(f"{name}: scales are of pages of 8 bits, these are {str(pages.dtype)[6:]}")
+    _lib.require_gpu(name, pages, k, v)
+    for t in (k, v):
+        if t.dtype != torch.float32 or t.shape != pages.shape[:3]:
+            raise ValueError(f"{name}: scales must be float32 {list(pages.shape[:3])}, got {t.dtype} {tuple(t.shape)}")
+        if not t.is_contiguous():
+            check_distinct(name, "scales", t)
+    return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefix_workspace(device: int, *sizes) -> int:
+    """Scratch bytes of these sizes on a device, which is current."""
+    need = ctypes.c_int64(0)
+    _lib.call("hydra_prefix_attn_workspace", *sizes, ctypes.byref(need))
+    return need.value
+
+
 @functools.lru_cache(maxsize=1024)
 def _attention_workspace(device: int, *sizes) -> int:
     """Scratch bytes of these sizes on a device, which is current."""
@@ -210,20 +237,28 @@ def _attention_workspace(device: int, *sizes) -> int:
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
-                    lengths: torch.Tensor, scale: Optional[float] = None,
-                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    lengths: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    scales=None, shared: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(scale * q k^T) v of one query token per request, q [N, Hq, hd],
     over the first `lengths[i]` (int32) positions of its pages; query head h
     reads key head h // (Hq / Hkv).  scale: hd ** -0.5 by default.  `out`: a
     [N, Hq, hd] tensor with a unit last stride to write to (q itself is one;
     otherwise none of the memory that is read).
 
-    fp32 scores, softmax and sums, one rounding.  Lengths count within
+    `scales`: (k_scales, v_scales) of pages of 8 bits (store_pages).  `shared`:
+    int32 [groups]; the N / groups requests from g N / groups on hold the same
+    in their first shared[g] positions, which are read once for all of them,
+    from the pages of the first one that is as long.  A request that is shorter
+    is answered from its own pages alone.
+
+    fp32 scores, softmax and sums, one rounding (with scales or shared a weight
+    enters its product as two 16-bit terms, to 2^-16 of it, and an infinity among
+    the values seen may come out as NaN).  Lengths count within
     [0, P * page_size]; keys on a page outside the pool are not seen; a
     request that sees none (or whose scores are all -inf) gets zeros.  Inference
     only: no gradient."""
     name = "paged_attention"
-    _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out)
+    _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out, shared)
     check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
     if q.dim() != 3 or q.shape[2] != hd:
@@ -231,7 +266,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     N, H, _ = q.shape
     if H == 0 or H % K != 0:
         raise ValueError(f"{name}: {H} query heads are no multiple of {K} key heads")
-    if q.dtype != k_pages.dtype:
+    scales = check_scales(name, k_pages, scales)
+    if scales is None and q.dtype != k_pages.dtype:
         raise ValueError(f"{name}: q and the pages must share a dtype")
     check_no_gradient(name, q, k_pages, v_pages, out)
     _vector(name, "lengths", lengths, torch.int32, N)
@@ -248,12 +284,33 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         check_distinct(name, "rows of out", out)
     lengths = lengths.contiguous()
     P, code = table.shape[1], _lib.dtype_code(q)
+    scale = hd ** -0.5 if scale is None else float(scale)
+    groups = 0
+    if shared is not None:
+        groups = _vector(name, "shared", shared, torch.int32).shape[0]
+        if groups == 0 or N % groups != 0:
+            raise ValueError(f"{name}: {N} requests are no multiple of {groups} groups")
+        if groups == N:  # nobody shares anything
+            groups = 0
+        shared = shared.contiguous()
     with _lib.on_device(q):
+        if groups or scales is not None:
+            of = code if scales is None else _lib.PAGE_CODE[k_pages.dtype]
+            ks, vs = scales or (None, None)
+            need = _prefix_workspace(q.device.index, groups, N, H, K, hd, P, page, code, of)
+            ws = _lib.scratch(need, q) if need else None
+            _lib.call("hydra_prefix_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks),
+                      _lib.ptr(vs), out.data_ptr(), table.data_ptr(), _row_stride(table), lengths.data_ptr(),
+                      shared.data_ptr() if groups else None, groups, N, H, K, hd, P, page, pages, _strides(q),
+                      _strides(k_pages), _strides(v_pages), None if ks is None else _strides(ks),
+                      None if vs is None else _strides(vs), _strides(out), scale, code, of, _lib.ptr(ws), need,
+                      _lib.stream(q))
+            return out
         need = _attention_workspace(q.device.index, N, H, K, hd, P, page, code)
         ws = _lib.scratch(need, q) if need else None
         _lib.call("hydra_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
                   table.data_ptr(), _row_stride(table), lengths.data_ptr(), N, H, K, hd, P, page, pages, _strides(q),
-                  _strides(k_pages), _strides(v_pages), _strides(out), hd ** -0.5 if scale is None else float(scale),
+                  _strides(k_pages), _strides(v_pages), _strides(out), scale,
                   code, _lib.ptr(ws), need, _lib.stream(q))
     return out
 

@@ -1,0 +1,10 @@
+// Attention over shared prefixes and 8-bit pages: the kernels of bf16 queries over e4m3 pages.
+#include "prefix_attn.h"
+
+namespace hydra {
+namespace prefix {
+
+template int launch_pages<bf16, e4m3>(const PrefixArgs&, const Shape&, hipStream_t);
+
+}  // namespace prefix
+}  // namespace hydra

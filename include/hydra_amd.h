@@ -31,6 +31,11 @@ extern "C" {
 #define HYDRA_BF16 1
 #define HYDRA_F16  2
 
+/* Element types of 8-bit pages: whole numbers in [-127, 127], and e4m3 (OCP, no
+ * infinities); each row has a scale. */
+#define HYDRA_PAGE_I8   16
+#define HYDRA_PAGE_E4M3 17
+
 /* Message of the last failure on this thread ("" if none). */
 const char* hydra_last_error(void);
 /* ABI version (major*10000 + minor*100 + patch). */
@@ -548,6 +553,29 @@ int hydra_paged_attn(const void* q, const void* k_pages, const void* v_pages, vo
                      int64_t workspace_size, void* stream);
 int hydra_paged_attn_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t hd, int64_t P,
                                int64_t page_size, int dtype, int64_t* bytes);
+
+/* hydra_paged_attn over pages of 8 bits, for requests that share prefixes, or both.
+ * page_dtype: dtype itself, HYDRA_PAGE_I8 or HYDRA_PAGE_E4M3; in 8 bits row r of
+ * a page stands for its values times k_scales, v_scales [pages, Hkv, page_size]
+ * (fp32, element strides ks_st[3], vs_st[3], unit last).  groups > 0: requests [g W,
+ * (g+1) W), W = N / groups, hold the same in their first shared[g] positions (counted
+ * within [0, P * page_size]); those of them that are as long get what they see there
+ * from the pages of the first such request's table row, read once for all of them,
+ * and the others from their own.  groups 0: shared is not used, and pages are of 8
+ * bits.  Scores, softmax and sums are fp32; a weight (times its value's scale) enters
+ * the product with v as two 16-bit terms, to 2^-16 of it.  An infinity among values that
+ * are seen may come out as NaN.  All else as in hydra_paged_attn. */
+int hydra_prefix_attn(const void* q, const void* k_pages, const void* v_pages,
+                      const float* k_scales, const float* v_scales, void* out, const int* table,
+                      int64_t table_rs, const int* lengths, const int* shared, int64_t groups,
+                      int64_t N, int64_t Hq, int64_t Hkv, int64_t hd, int64_t P, int64_t page_size,
+                      int64_t pages, const int64_t* q_st, const int64_t* kp_st,
+                      const int64_t* vp_st, const int64_t* ks_st, const int64_t* vs_st,
+                      const int64_t* o_st, float scale, int dtype, int page_dtype, void* workspace,
+                      int64_t workspace_size, void* stream);
+int hydra_prefix_attn_workspace(int64_t groups, int64_t N, int64_t Hq, int64_t Hkv, int64_t hd,
+                                int64_t P, int64_t page_size, int dtype, int page_dtype,
+                                int64_t* bytes);
 
 /* hydra_ccgqa_prep_fwd for the newest token of N requests that are decoded
  * (attention.py:205-266, kernels/fused_conv.py:39-62).  qkv [N, L + 2K] (row

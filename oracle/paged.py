@@ -164,4 +164,27 @@ def _convs(x, w1, w2, groups):
     return causal_conv_seq(x, w1, w2, groups)
 
 
-__all__ = ["plan", "release", "attention", "attention_bound", "decode_bound"]
+
+
+def dequantise(q, scales):
+    """What rows of 8 bits and their scales stand for, fp64."""
+    x = q.view(torch.int8).float() if q.dtype == torch.int8 else q.float()
+    return x.double() * scales.double()[..., None]
+
+
+def two_term_bound(weight, v, lengths, page_dtype, q_dtype):
+    """What the attention over shared prefixes and 8-bit pages adds to
+    attention_bound where its products are of 16-bit operands: a weight p (times its
+    value's scale) is taken as hi + lo, hi off by half a step of the type, lo by half
+    a step of that: 2^-16 of p in bf16 (8-bit pages, bf16), 2^-22 in fp16 (fp16
+    pages), where what is left below fp16's least step, 2^-24, is lost by half: 2^-25
+    of a weight whose largest is 1, for each key."""
+    if q_dtype == torch.float32:
+        return torch.zeros_like(weight)
+    if page_dtype == torch.float16:
+        finite = torch.where(torch.isfinite(v.double()), v.double(), torch.zeros(()).double())
+        return 2.0 ** -22 * weight + 2.0 ** -25 * lengths.double().clamp(min=0).view(-1, 1, 1) * float(finite.abs().max())
+    return 2.0 ** -16 * weight
+
+
+__all__ = ["plan", "release", "attention", "attention_bound", "decode_bound", "dequantise", "two_term_bound"]
