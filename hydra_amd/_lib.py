@@ -70,6 +70,8 @@ SIGNATURES = {
     "hydra_ce_grad_planes": [_P, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P],
     "hydra_token_logprobs": [_P, _I64, _I64, _I64, _P, _F, _I64, _P, _P, _P, _P, _P, _I, _P],
     "hydra_token_logprobs_bwd": [_P, _I64, _I64, _I64, _P, _F, _I64, _P, _P, _P, _P, _P, _P, _P, _I, _P],
+    "hydra_beam_select": [_P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64, _P],
+    "hydra_beam_select_workspace": [_I64, _I64, _I64, _I64, _I, _I64P],
     "hydra_page_plan": [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P],
     "hydra_pool_plan": [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P],
     "hydra_page_plan_in_place": [_I64, _I64],
@@ -77,6 +79,14 @@ SIGNATURES = {
     "hydra_pool_release": [_P, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P],
     "hydra_page_store": [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
                          _I64P, _I, _P],
+    "hydra_page_store8": [_P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P,
+                          _I64P, _I64P, _I64P, _I64P, _I, _I, _P],
+    "hydra_page_read": [_P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
+                        _I64P, _I64P, _I64P, _I, _I, _P],
+    "hydra_page_fork": [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "hydra_page_fork_workspace": [_I64, _I64, _I64, _I64P],
+    "hydra_page_copy": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I, _P],
+    "hydra_rows_take": [_P, _I64, _I64, _P, _I64, _P],
     "hydra_paged_attn": [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                          _I64P, _I64P, _I64P, _I64P, _F, _I, _P, _I64, _P],
     "hydra_paged_attn_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I, _I64P],

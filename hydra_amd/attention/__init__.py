@@ -8,7 +8,8 @@ from .registry import (
 )
 from .backends.ccgqa.attention import CCGQAAttention, CCGQACache
 from .factory import build_hybrid_attention_module
-from .paged import PagePlan, PagePool, paged_attention, plan_pages, release_pages, store_pages
+from .paged import (PageFork, PagePlan, PagePool, copy_pages, fork_pages, paged_attention, plan_pages, read_pages,
+                    release_pages, store_pages, take_rows)
 
 __all__ = [
     "HybridAttentionBackend",
@@ -18,10 +19,15 @@ __all__ = [
     "CCGQAAttention",
     "CCGQACache",
     "build_hybrid_attention_module",
+    "PageFork",
     "PagePlan",
     "PagePool",
+    "copy_pages",
+    "fork_pages",
     "paged_attention",
     "plan_pages",
+    "read_pages",
     "release_pages",
     "store_pages",
+    "take_rows",
 ]

@@ -1,11 +1,14 @@
 """A paged key-value cache: page tables planned on the GPU, key and value rows
-stored into their pages, and the attention of one new token per request over
-them.
+stored into their pages and read back, the attention of one new token per
+request over them, and requests that go on from what others hold.
 
 A pool holds `k_pages` and `v_pages` [pages, Hkv, page_size, hd] (any strides
 with a unit last one); position t of request i lies in page
 `table[i, t // page_size]` at row `t % page_size`, and its *slot* is
 `page * page_size + row`.  `page_size` is a power of two in [16, 4096].
+
+Pages may be of 8 bits (torch.int8, torch.float8_e4m3fn), with a scale for
+each row, fp32 [pages, Hkv, page_size]: a row stands for its values times it.
 
 Nothing here synchronises with the host, so what only the device knows is
 settled there: a request that finds no room is refused by the plan
@@ -17,7 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -171,34 +174,85 @@ def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
                   free_count.data_ptr(), N, table.shape[1], int(page_size), *within, _lib.stream(lengths))
 
 
+def _rows_of_slots(name, N, S, slots, rows):
+    if slots.dtype != torch.int64 or slots.dim() != 2 or slots.shape[1] != S or (rows is None and slots.shape[0] != N):
+        raise ValueError(f"{name}: slots must be int64 [{'R' if rows is not None else N}, {S}], got {slots.dtype} "
+                         f"{tuple(slots.shape)}")
+    return slots.contiguous(), None if rows is None else _vector(name, "rows", rows, torch.int64, N).contiguous()
+
+
 def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                slots: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
+                slots: torch.Tensor, rows: Optional[torch.Tensor] = None, scales=None) -> None:
     """Writes the rows k, v [N, Hkv, S, hd] to their slots in the pool:
     prompt n's are `slots[n]`, or `slots[rows[n]]`, of int64 [R, S] (distinct;
     -1, or any outside the pool, for rows that are not kept).  rows: int64 [N],
     distinct; a row outside the slots stores nothing.  The pages are none of
-    k's and v's memory.  Inference only: no gradient."""
+    k's and v's memory.  Inference only: no gradient.
+
+    `scales`: (k_scales, v_scales) of pages of 8 bits, which get the rows'
+    scales.  int8: a row's largest value over 127 (at least 2^-126), e4m3: the
+    least power of two that brings it to 448; values are rounded to nearest
+    even.  A row with an infinity or NaN gets the scale NaN.  hd up to 256."""
     name = "store_pages"
     _lib.require_gpu(name, k, v, k_pages, v_pages, slots, rows)
     check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
     if k.dim() != 4 or k.shape[1] != K or k.shape[3] != hd or v.shape != k.shape:
         raise ValueError(f"{name}: k and v must be [N, {K}, S, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if not k.dtype == v.dtype == k_pages.dtype:
+    scales = check_scales(name, k_pages, scales)
+    if k.dtype != v.dtype or (scales is None and k.dtype != k_pages.dtype):
         raise ValueError(f"{name}: k, v and the pages must share a dtype")
     check_no_gradient(name, k, v, k_pages, v_pages)
     N, S = k.shape[0], k.shape[2]
-    if slots.dtype != torch.int64 or slots.dim() != 2 or slots.shape[1] != S or (rows is None and slots.shape[0] != N):
-        raise ValueError(f"{name}: slots must be int64 [{'R' if rows is not None else N}, {S}], got {slots.dtype} "
-                         f"{tuple(slots.shape)}")
-    if rows is not None:
-        rows = _vector(name, "rows", rows, torch.int64, N).contiguous()
+    slots, rows = _rows_of_slots(name, N, S, slots, rows)
     k, v = (t if t.stride(-1) == 1 or hd == 1 else t.contiguous() for t in (k, v))
-    slots = slots.contiguous()
     with _lib.on_device(k):
+        if scales is not None:
+            ks, vs = scales
+            _lib.call("hydra_page_store8", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                      ks.data_ptr(), vs.data_ptr(), slots.data_ptr(), slots.shape[0], _lib.ptr(rows), N, K, S, hd,
+                      pages, page, _strides(k), _strides(v), _strides(k_pages), _strides(v_pages), _strides(ks),
+                      _strides(vs), _lib.dtype_code(k), _lib.PAGE_CODE[k_pages.dtype], _lib.stream(k))
+            return
         _lib.call("hydra_page_store", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                   slots.data_ptr(), slots.shape[0], _lib.ptr(rows), N, K, S, hd, pages, page, _strides(k), _strides(v),
                   _strides(k_pages), _strides(v_pages), _lib.dtype_code(k), _lib.stream(k))
+
+
+def read_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor,
+               rows: Optional[torch.Tensor] = None, scales=None,
+               dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """k, v [N, Hkv, S, hd] out of their slots, the way store_pages put them
+    there: prompt n's are `slots[n]` of int64 [N, S], or `slots[rows[n]]`.  Zeros
+    where a slot or a row is none.  Pages of 8 bits need their `scales` and the
+    `dtype` wanted (bf16, fp16 or fp32; each value is rounded once); others
+    are read as they are.  hd up to 256.  Inference only: no gradient."""
+    name = "read_pages"
+    _lib.require_gpu(name, k_pages, v_pages, slots, rows)
+    check_pages(name, k_pages, v_pages)
+    pages, K, page, hd = k_pages.shape
+    scales = check_scales(name, k_pages, scales)
+    if scales is None:
+        if dtype not in (None, k_pages.dtype):
+            raise ValueError(f"{name}: pages of {str(k_pages.dtype)[6:]} are read as they are, not as {str(dtype)[6:]}")
+        dtype = k_pages.dtype
+    elif dtype is None:
+        raise ValueError(f"{name}: say which dtype (pages of {str(k_pages.dtype)[6:]})")
+    check_no_gradient(name, k_pages, v_pages)
+    if slots.dim() != 2:
+        raise ValueError(f"{name}: slots must be int64 [N, S], got {slots.dtype} {tuple(slots.shape)}")
+    N, S = (slots if rows is None else rows).shape[0], slots.shape[1]
+    slots, rows = _rows_of_slots(name, N, S, slots, rows)
+    k, v = (torch.empty((N, K, S, hd), dtype=dtype, device=k_pages.device) for _ in range(2))
+    code = _lib.dtype_code(k)
+    ks, vs = scales or (None, None)
+    with _lib.on_device(k):
+        _lib.call("hydra_page_read", k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks), _lib.ptr(vs), k.data_ptr(),
+                  v.data_ptr(), slots.data_ptr(), slots.shape[0], _lib.ptr(rows), N, K, S, hd, pages, page,
+                  _strides(k_pages), _strides(v_pages), None if ks is None else _strides(ks),
+                  None if vs is None else _strides(vs), _strides(k), _strides(v), code,
+                  code if scales is None else _lib.PAGE_CODE[k_pages.dtype], _lib.stream(k))
+    return k, v
 
 
 def check_scales(name: str, pages: torch.Tensor, scales):
@@ -315,6 +369,111 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
+class PageFork(NamedTuple):
+    """What fork_pages did: `parents` int32 [N], the row that each row goes on
+    from (-1: it holds nothing); `sources`, `copies` int32 [N], the page to copy
+    for a row and where to (-1: none; copy_pages); `granted` bool [N]."""
+    parents: torch.Tensor
+    sources: torch.Tensor
+    copies: torch.Tensor
+    granted: torch.Tensor
+
+
+@functools.lru_cache(maxsize=1024)
+def _fork_workspace(*sizes) -> int:
+    need = ctypes.c_int64(0)
+    _lib.call("hydra_page_fork_workspace", *sizes, ctypes.byref(need))
+    return need.value
+
+
+def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
+               free_count: torch.Tensor, extra: torch.Tensor, page_size: int) -> PageFork:
+    """Row i goes on from what row parents[i] (int32 [N]; any outside [0, N):
+    from nothing) held: its length, and its pages of `table`, all rows at once and
+    in place.
+
+    Pages that are full are held in common; `extra` (int32, one for each page of
+    the pool) counts a page's holders beyond the first.  The page that a row was
+    still filling stays with the first row that goes on from it; the others get
+    copies, taken from the stack in their order, which copy_pages fills.  Pages that
+    nobody holds any more go on the stack before that, in the order of rows and
+    columns.  A row that finds no page for its copy is refused (`granted`) and
+    holds nothing: where every row's last page is begun and each goes on from one
+    of them, there are always enough.  At most 8192 rows."""
+    name = "fork_pages"
+    _lib.require_gpu(name, parents, lengths, table, free_pages, free_count, extra)
+    N = _vector(name, "lengths", lengths, torch.int32).shape[0]
+    _vector(name, "parents", parents, torch.int32, N)
+    _vector(name, "free_pages", free_pages, torch.int32)
+    _vector(name, "free_count", free_count, torch.int32, 1)
+    pages = _vector(name, "extra", extra, torch.int32).shape[0]
+    _check_table(name, table, N)
+    if N == 0 or table.shape[1] == 0 or pages == 0:
+        raise ValueError(f"{name}: {N} rows of {table.shape[1]} pages in a pool of {pages}")
+    _in_place(name, "lengths", lengths)
+    _in_place(name, "free_pages", free_pages)
+    _in_place(name, "extra", extra)
+    parents = parents.contiguous()
+    sources, copies, taken = lengths.new_empty((3, N)).unbind(0)
+    granted = lengths.new_empty((N,), dtype=torch.bool)
+    P = table.shape[1]
+    need = _fork_workspace(N, P, pages)
+    ws = _lib.scratch(need, lengths)
+    with _lib.on_device(lengths):
+        _lib.call("hydra_page_fork", parents.data_ptr(), lengths.data_ptr(), table.data_ptr(), _row_stride(table),
+                  free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), extra.data_ptr(),
+                  sources.data_ptr(), copies.data_ptr(), taken.data_ptr(), granted.data_ptr(), N, P, int(page_size),
+                  pages, ws.data_ptr(), need, _lib.stream(lengths))
+    return PageFork(taken, sources, copies, granted)
+
+
+def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, sources: torch.Tensor, copies: torch.Tensor,
+               scales=None) -> None:
+    """Pages copies[i] become what pages sources[i] are (int32 [N]), in keys,
+    values and `scales`.  Pairs with a page outside the pool are left out; copies
+    are distinct and none is a source.  Inference only: no gradient."""
+    name = "copy_pages"
+    _lib.require_gpu(name, k_pages, v_pages, sources, copies)
+    check_pages(name, k_pages, v_pages)
+    pages, K, page, hd = k_pages.shape
+    N = _vector(name, "sources", sources, torch.int32).shape[0]
+    _vector(name, "copies", copies, torch.int32, N)
+    scales = check_scales(name, k_pages, scales)
+    if scales is None:
+        _lib.dtype_code(k_pages)
+    check_no_gradient(name, k_pages, v_pages)
+    ks, vs = scales or (None, None)
+    sources, copies = sources.contiguous(), copies.contiguous()
+    with _lib.on_device(k_pages):
+        _lib.call("hydra_page_copy", k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks), _lib.ptr(vs),
+                  sources.data_ptr(), copies.data_ptr(), N, K, hd, pages, page, _strides(k_pages), _strides(v_pages),
+                  None if ks is None else _strides(ks), None if vs is None else _strides(vs), k_pages.element_size(),
+                  _lib.stream(k_pages))
+
+
+def take_rows(x: torch.Tensor, parents: torch.Tensor) -> None:
+    """x[i] = x[parents[i]] in place, all rows at once (int32 [N], N = len(x)
+    up to 8192); a parent outside [0, N) leaves its row as it is.  Any dtype; rows
+    are contiguous and do not overlap.  Inference only: no gradient."""
+    name = "take_rows"
+    _lib.require_gpu(name, x, parents)
+    if x.dim() == 0:
+        raise ValueError(f"{name}: x must have rows")
+    N = x.shape[0]
+    _vector(name, "parents", parents, torch.int32, N)
+    check_no_gradient(name, x)
+    if N == 0 or x.numel() == 0:
+        return
+    row = x.numel() // N
+    if not x[0].is_contiguous() or (N > 1 and x.stride(0) < row):
+        raise ValueError(f"{name}: rows of strides {x.stride()} are not contiguous")
+    e = x.element_size()
+    parents = parents.contiguous()
+    with _lib.on_device(x):
+        _lib.call("hydra_rows_take", x.data_ptr(), (x.stride(0) if N > 1 else row) * e, row * e, parents.data_ptr(), N,
+                  _lib.stream(x))
+
+
 class PagePool:
     """The pages of up to `requests` requests of up to `max_length` tokens
     (whatever the page size: a plan refuses what goes past it): which pages each
@@ -322,15 +481,19 @@ class PagePool:
     `pages` pages of their own and share this.
 
     `plan(new_tokens, width)` takes a step's pages and moves the lengths on;
-    `release(done)` returns finished requests' pages.  All of it runs on the
-    device, on the current stream; a captured step replays with the lengths
-    that it finds."""
+    `release(done)` returns finished requests' pages.  With `sharing`,
+    `fork(parents)` makes requests go on from what others hold, with the full
+    pages in common (up to 8192 requests).  All of it runs on the device, on the
+    current stream; a captured step replays with the lengths that it finds."""
 
-    def __init__(self, requests: int, max_length: int, pages: int, page_size: int = 64, device="cuda"):
+    def __init__(self, requests: int, max_length: int, pages: int, page_size: int = 64, device="cuda",
+                 sharing: bool = False):
         if requests < 1 or max_length < 1 or pages < 1:
             raise ValueError(f"PagePool: {requests} requests of up to {max_length} tokens in {pages} pages")
         if page_size not in (16, 32, 64, 128, 256, 512, 1024, 2048, 4096):
             raise ValueError(f"PagePool: page_size {page_size} is no power of two in [16, 4096]")
+        if sharing and requests > 8192:
+            raise ValueError(f"PagePool: pages are shared among up to 8192 requests, not {requests}")
         self.requests, self.pages, self.page_size = int(requests), int(pages), int(page_size)
         self.max_length = int(max_length)
         self.lengths = torch.zeros(self.requests, dtype=torch.int32, device=device)
@@ -338,6 +501,9 @@ class PagePool:
                                 device=device)
         self.free_pages = torch.arange(self.pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), self.pages, dtype=torch.int32, device=device)
+        # a page's holders beyond the first, and every request as its own continuation
+        self.extra = torch.zeros(self.pages, dtype=torch.int32, device=device) if sharing else None
+        self._rows = torch.arange(self.requests, dtype=torch.int32, device=device) if sharing else None
 
     def plan(self, new_tokens: torch.Tensor, width: int = 1, from_empty: bool = False) -> PagePlan:
         """plan_pages of these requests, taken: the pool's lengths and free
@@ -352,5 +518,18 @@ class PagePool:
             plan = plan._replace(lengths=self.lengths, free_count=self.free_count)
         return plan
 
+    def fork(self, parents: torch.Tensor) -> PageFork:
+        """fork_pages of these requests: request i goes on from what request
+        parents[i] holds.  Every layer's cache follows (CCGQACache.fork)."""
+        if self.extra is None:
+            raise RuntimeError("PagePool.fork: the pool shares no pages (sharing=True)")
+        return fork_pages(parents, self.lengths, self.table, self.free_pages, self.free_count, self.extra,
+                          self.page_size)
+
     def release(self, done: torch.Tensor) -> None:
+        if self.extra is not None:  # a page comes back with its last holder
+            _vector("PagePool.release", "done", done, torch.bool, self.requests)
+            _lib.require_gpu("PagePool.release", done, self.lengths)
+            self.fork(torch.where(done, -1, self._rows))
+            return
         release_pages(done, self.lengths, self.table, self.free_pages, self.free_count, self.page_size, self.pages)

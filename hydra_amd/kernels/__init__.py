@@ -21,6 +21,7 @@ from .fused_ops import (
     get_kernel_status,
     set_use_triton_kernels,
 )
+from .beam import BeamChoice, beam_select
 from .logprobs import TokenLogprobs, token_logprobs
 
 __all__ = [
@@ -42,6 +43,8 @@ __all__ = [
     "USE_FUSED_RMS_NORM",
     "set_use_triton_kernels",
     "get_kernel_status",
+    "BeamChoice",
+    "beam_select",
     "TokenLogprobs",
     "token_logprobs",
 ]

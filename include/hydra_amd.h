@@ -475,6 +475,22 @@ int hydra_token_logprobs_bwd(const void* logits, int64_t rows, int64_t vocab, in
                              const float* g_logprobs, const float* g_entropy, const float* g_top,
                              void* grad, int dtype, void* stream);
 
+/* A step of beam search: of each of B texts the n best continuations of its W beams,
+ *   scores[b, w] + logits[b W + w, v] - ln sum_u exp(logits[b W + w, u]),
+ * best first, the lowest w V + v first among equals (compared in fp64, with fp32 sums of
+ * exponentials).  logits: [B W, V], rows logits_rs apart; scores: fp32 [B, W]; out_scores
+ * fp32, beams (w), tokens (v) int64 and parents (b W + w) int32 [B, n].  NaN counts as
+ * larger than any number, and a row with NaN or +inf is NaN throughout; of a beam whose
+ * continuations are all alike (its score or its row not finite) the first tokens are
+ * meant.  W <= 1024, n <= 128, n <= W V < 2^31.  Needs hydra_beam_select_workspace bytes
+ * of device scratch (16-byte aligned). */
+int hydra_beam_select(const void* logits, int64_t logits_rs, const float* scores, int64_t B,
+                      int64_t W, int64_t V, int64_t n, float* out_scores, int64_t* beams,
+                      int64_t* tokens, int* parents, int dtype, void* workspace,
+                      int64_t workspace_size, void* stream);
+int hydra_beam_select_workspace(int64_t B, int64_t W, int64_t V, int64_t n, int dtype,
+                                int64_t* bytes);
+
 /* ---- pages of a key-value cache (no counterpart in the reference, which
  *      recomputes the whole sequence for every token) ---------------------- */
 
@@ -535,6 +551,61 @@ int hydra_page_store(const void* k, const void* v, void* k_pages, void* v_pages,
                      int64_t S, int64_t hd, int64_t pages, int64_t page_size, const int64_t* k_st,
                      const int64_t* v_st, const int64_t* kp_st, const int64_t* vp_st, int dtype,
                      void* stream);
+
+/* hydra_page_store into pages of 8 bits (page_dtype HYDRA_PAGE_I8 or HYDRA_PAGE_E4M3)
+ * with a scale for each row in k_scales, v_scales [pages, Hkv, page_size] (fp32,
+ * element strides ks_st[3], vs_st[3], unit last).  int8: the scale is max(amax / 127,
+ * 2^-126) in fp32, e4m3: the least power of two from 2^-126 on that brings amax to at
+ * most 448; a value is the quotient x / scale rounded to nearest even.  A row with an
+ * infinity or NaN gets the scale NaN.  hd <= 256. */
+int hydra_page_store8(const void* k, const void* v, void* k_pages, void* v_pages, float* k_scales,
+                      float* v_scales, const int64_t* slots, int64_t R, const int64_t* rows,
+                      int64_t N, int64_t Hkv, int64_t S, int64_t hd, int64_t pages,
+                      int64_t page_size, const int64_t* k_st, const int64_t* v_st,
+                      const int64_t* kp_st, const int64_t* vp_st, const int64_t* ks_st,
+                      const int64_t* vs_st, int dtype, int page_dtype, void* stream);
+
+/* The other way: the rows at the slots out of pages of page_dtype (dtype itself, or 8
+ * bits times their scales, rounded once) into k, v [N, Hkv, S, hd] of `dtype` (element
+ * strides k_st[4], v_st[4]; unit last).  Slots outside the pool, and rows outside [0, R),
+ * read zeros.  hd <= 256. */
+int hydra_page_read(const void* k_pages, const void* v_pages, const float* k_scales,
+                    const float* v_scales, void* k, void* v, const int64_t* slots, int64_t R,
+                    const int64_t* rows, int64_t N, int64_t Hkv, int64_t S, int64_t hd,
+                    int64_t pages, int64_t page_size, const int64_t* kp_st, const int64_t* vp_st,
+                    const int64_t* ks_st, const int64_t* vs_st, const int64_t* k_st,
+                    const int64_t* v_st, int dtype, int page_dtype, void* stream);
+
+/* Row i goes on from what row parents[i] held (int32 [N], N <= 8192; any outside [0, N):
+ * from nothing), in place: lengths [N], table [N, P] (row stride table_rs), the stack
+ * free_pages[0 .. free_count) and extra [pages], the holders of a page beyond the first.
+ * Filled pages are held in common; the page that a row was still filling stays with the
+ * first row that goes on from it, and each other one gets a page from the top of the
+ * stack, rows in order, which the caller fills: copies[i] from sources[i] (else both -1).
+ * Pages that nobody holds any more go on the stack first, in the order of rows and
+ * columns, each from the first row among those that held it.  A row that finds no page
+ * is refused (granted 0) and holds nothing.  Entries past what a row holds become
+ * -1.  taken[i]: parents[i], or -1 where the row holds nothing of it.  Needs
+ * hydra_page_fork_workspace bytes of device scratch. */
+int hydra_page_fork(const int* parents, int* lengths, int* table, int64_t table_rs,
+                    int* free_pages, int64_t free_capacity, int* free_count, int* extra,
+                    int* sources, int* copies, int* taken, void* granted, int64_t N, int64_t P,
+                    int64_t page_size, int64_t pages, void* workspace, int64_t workspace_size,
+                    void* stream);
+int hydra_page_fork_workspace(int64_t N, int64_t P, int64_t pages, int64_t* bytes);
+
+/* Pages copies[i] = sources[i] (int32 [N]; pairs with either outside the pool are left
+ * out) of k_pages, v_pages [pages, Hkv, page_size, hd] of elements of element_size bytes
+ * (1, 2, 4), and of their scales (or NULL).  Copies are distinct, and none is a source. */
+int hydra_page_copy(void* k_pages, void* v_pages, float* k_scales, float* v_scales,
+                    const int* sources, const int* copies, int64_t N, int64_t Hkv, int64_t hd,
+                    int64_t pages, int64_t page_size, const int64_t* kp_st, const int64_t* vp_st,
+                    const int64_t* ks_st, const int64_t* vs_st, int element_size, void* stream);
+
+/* x[i] = x[parents[i]] in place, all at once: N <= 8192 rows of row_bytes,
+ * row_stride_bytes apart; a parent outside [0, N) leaves its row as it is. */
+int hydra_rows_take(void* x, int64_t row_stride_bytes, int64_t row_bytes, const int* parents,
+                    int64_t N, void* stream);
 
 /* Attention of one token per request over its pages:
  *   out[n,h] = softmax_t(scale * q[n,h] . k[t]) v[t], t < lengths[n],

@@ -187,4 +187,87 @@ def two_term_bound(weight, v, lengths, page_dtype, q_dtype):
     return 2.0 ** -16 * weight
 
 
-__all__ = ["plan", "release", "attention", "attention_bound", "decode_bound", "dequantise", "two_term_bound"]
+def quantise(x, page_dtype):
+    """Rows x [..., hd] in 8 bits: (values fp64 [..., hd], scales fp32 [...]), from
+    the definition; fp64 holds the quotients apart from the middles between two
+    values (a quotient of two 24-bit numbers is off such a middle by 2^-25 of it
+    or not at all)."""
+    x = x.double()
+    top = x.abs().amax(-1)
+    least = torch.tensor(2.0 ** -126, dtype=torch.float64)
+    if page_dtype == torch.int8:
+        scales = torch.maximum((top / 127).float().double(), least)
+        q = torch.round(x / scales[..., None])
+    else:
+        scales = torch.full_like(top, 2.0 ** -126)
+        finite = torch.where(torch.isfinite(top), top, torch.zeros_like(top))
+        while bool((large := finite / scales > 448).any()):
+            scales[large] *= 2
+        y = x / scales[..., None]
+        _, e = torch.frexp(y)  # y in [2^(e-1), 2^e): steps of 2^(e-4), of 2^-9 at least
+        step = torch.ldexp(torch.ones_like(y), (e - 4).clamp(min=-9))
+        q = torch.round(y / step) * step
+    wrong = ~torch.isfinite(top)
+    q[wrong] = 0.0
+    scales[wrong] = float("nan")
+    return q, scales.float()
+
+
+def fork(parents, lengths, table, free_pages, free_count, extra, page_size):
+    """Lists in, lists out: (lengths, table, free_pages, free_count, extra,
+    sources, copies, taken, granted), by sets of holders."""
+    N, P, pages = len(lengths), len(table[0]), len(extra)
+    stack = list(free_pages)
+    top = max(0, min(free_count, len(stack)))
+    parents = [p if 0 <= p < N else -1 for p in parents]
+    full = [max(0, min(n // page_size, P)) for n in lengths]
+    held = [min(P, -(-n // page_size)) if n > 0 else 0 for n in lengths]
+    kids = [[i for i in range(N) if parents[i] == j] for j in range(N)]
+    count = {}  # holders of a page that is given up or shared
+    for j in range(N):
+        for c in range(held[j]):
+            p = table[j][c]
+            if 0 <= p < pages:
+                count[p] = count.get(p, extra[p] + 1) + (len(kids[j]) - 1 if c < full[j] else -(not kids[j]))
+    done = set()
+    for j in range(N):
+        for c in range(held[j]) if not kids[j] else ():
+            p = table[j][c]
+            if 0 <= p < pages and count[p] == 0 and p not in done:
+                done.add(p)
+                if top < len(stack):
+                    stack[top] = p
+                    top += 1
+    free, rank = top, 0
+    after, rows, sources, copies, taken, granted = [], [], [], [], [], []
+    for i, j in enumerate(parents):
+        row, length, source, copy, ok = [-1] * P, 0, -1, -1, True
+        if j >= 0:
+            last = full[j]
+            if held[j] > last and kids[j][0] != i and 0 <= table[j][last] < pages:
+                ok = rank < free
+                if ok:
+                    source, copy = table[j][last], stack[free - 1 - rank]
+                    top -= 1
+                rank += 1
+            if ok:
+                row[:held[j]] = table[j][:held[j]]
+                length = lengths[j]
+                if copy >= 0:
+                    row[last] = copy
+            else:
+                for p in table[j][:last]:
+                    if 0 <= p < pages:
+                        count[p] -= 1
+        after.append(length)
+        rows.append(row)
+        sources.append(source)
+        copies.append(copy)
+        taken.append(j if ok else -1)
+        granted.append(ok)
+    extra = [max(0, count[p] - 1) if p in count else extra[p] for p in range(pages)]
+    return after, rows, stack, top, extra, sources, copies, taken, granted
+
+
+__all__ = ["plan", "release", "attention", "attention_bound", "decode_bound", "dequantise", "two_term_bound",
+           "quantise", "fork"]
