@@ -40,7 +40,7 @@ from ...._lib import CCGQA_V_TRANSPOSED, CCGQA_W_TILED, MASK_KEY_PADDING, MASK_R
 from .autograd import ccgqa_prep_train
 from .kernels.fused_attention import CCGQAAttentionFused, MaskedAttentionFunction
 from .kernels.fused_conv import OptimizedConvSequence
-from ...paged import PagePlan, PagePool, paged_attention, store_pages
+from ...paged import PageFork, PagePlan, PagePool, copy_pages, paged_attention, store_pages, take_rows
 from .ops import (PackedWeights, attention_forward, ccgqa_decode_prep, ccgqa_prep, ccgqa_ring_fill, decode_reach,
                   linear_weight_ok, output_projection, pack_conv_weight, pack_conv_weights_tiled, pack_linear_weight,
                   prep_flags, tiled_weights_ok)
@@ -96,21 +96,38 @@ class _EvalRecompute(torch.autograd.Function):
 
 
 class CCGQACache:
-    """A layer's keys and values in pages ([pages, Hkv, page_size, head_dim])
-    and the projected rows of each request's last tokens, which its next token
-    needs (ccgqa_decode_prep's ring).  The pool's table says which pages are
-    whose."""
+    """A layer's keys and values in pages ([pages, Hkv, page_size, head_dim]; of
+    8 bits with `scales`) and the projected rows of each request's last tokens,
+    which its next token needs (ccgqa_decode_prep's ring).  The pool's table says
+    which pages are whose."""
 
-    def __init__(self, layer: "CCGQAAttention", pool: PagePool, dtype: torch.dtype):
+    def __init__(self, layer: "CCGQAAttention", pool: PagePool, dtype: torch.dtype,
+                 page_dtype: Optional[torch.dtype] = None):
         device = pool.table.device
         shape = (pool.pages, layer.n_kv_heads, pool.page_size, layer.head_dim)
-        self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
-        self.v_pages = torch.zeros(shape, dtype=dtype, device=device)
+        eight = page_dtype in _lib.PAGE_CODE
+        self.k_pages = torch.zeros(shape, dtype=page_dtype or dtype, device=device)
+        self.v_pages = torch.zeros(shape, dtype=page_dtype or dtype, device=device)
+        self.scales = tuple(torch.zeros(shape[:3], device=device) for _ in range(2)) if eight else None
+        # a new token's key and value rows on their way into pages of 8 bits, as pages of 16
+        # rows, row i request i's
+        self._new = self._new_rows = None
+        if eight:
+            rows = torch.zeros((2, -(-pool.requests // 16) * 16, *shape[1::2]), dtype=dtype, device=device)
+            self._new = rows
+            self._new_rows = torch.arange(pool.requests, device=device)
         reach = decode_reach(layer._prep_args()[0], layer.conv_kernel_size)
         self.ring = torch.zeros((pool.requests, reach + 1, layer.latent_dim + 2 * layer.kv_dim), dtype=dtype,
                                 device=device)
         self.table = pool.table
         self.max_length = pool.max_length
+
+    @torch.no_grad()
+    def fork(self, fork: PageFork) -> None:
+        """Follows the requests of pool.fork(parents): copies of pages, and the
+        projected rows of the requests that they go on from."""
+        copy_pages(self.k_pages, self.v_pages, fork.sources, fork.copies, scales=self.scales)
+        take_rows(self.ring, fork.parents)
 
 
 class CCGQAAttention(nn.Module):
@@ -234,10 +251,14 @@ class CCGQAAttention(nn.Module):
         return out
 
     # ------------------------------------------------------------- serving
-    def new_cache(self, pool: PagePool, dtype: Optional[torch.dtype] = None) -> "CCGQACache":
+    def new_cache(self, pool: PagePool, dtype: Optional[torch.dtype] = None,
+                  page_dtype: Optional[torch.dtype] = None) -> "CCGQACache":
         """This layer's part of a paged cache for the requests of `pool` (which
-        all layers share), in the weights' dtype by default."""
+        all layers share), in the weights' dtype by default.  page_dtype:
+        torch.int8 or torch.float8_e4m3fn for keys and values of 8 bits."""
         w = self.qkv_proj.weight
+        if page_dtype is not None and page_dtype not in _lib.PAGE_CODE:
+            raise ValueError(f"CCGQAAttention: page_dtype must be torch.int8 or torch.float8_e4m3fn, not {page_dtype}")
         if self.use_rope and pool.max_length > self.cos_cached.shape[2]:
             raise ValueError(f"CCGQAAttention: requests of up to {pool.max_length} tokens exceed the RoPE cache "
                              f"({self.cos_cached.shape[2]})")
@@ -258,7 +279,7 @@ class CCGQAAttention(nn.Module):
                              f"to look back at ({ring} bytes)")
         if pool.table.device != w.device:
             raise RuntimeError(f"CCGQAAttention: the pool is on {pool.table.device}, the layer on {w.device}")
-        return CCGQACache(self, pool, dtype)
+        return CCGQACache(self, pool, dtype, page_dtype)
 
     def _check_cache(self, name: str, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan) -> None:
         if _lib.forward_ad._current_level >= 0:
@@ -266,8 +287,8 @@ class CCGQAAttention(nn.Module):
         if cache.k_pages.shape[1] != self.n_kv_heads or cache.k_pages.shape[3] != self.head_dim or \
                 cache.ring.shape[2] != self.latent_dim + 2 * self.kv_dim:
             raise ValueError(f"{name}: the cache is another layer's")
-        if x.dtype != cache.k_pages.dtype:
-            raise ValueError(f"{name}: x is {x.dtype}, the cache {cache.k_pages.dtype}")
+        if x.dtype != cache.ring.dtype:
+            raise ValueError(f"{name}: x is {x.dtype}, the cache {cache.ring.dtype}")
         if plan.slots.shape[0] != cache.ring.shape[0]:
             raise ValueError(f"{name}: a plan of {plan.slots.shape[0]} requests, a cache of {cache.ring.shape[0]}")
         if self.use_rope and cache.max_length > self.cos_cached.shape[2]:
@@ -301,14 +322,17 @@ class CCGQAAttention(nn.Module):
         # padding may hold anything, and the attention's tiles would take it up
         ccgqa_ring_fill(qkv, cache.ring, plan.seen, decode_reach(flags, self.conv_kernel_size), rows, clear=True)
         return self._forward_infer(x, qkv, flags, convw, None,
-                                   keep=lambda k, v: store_pages(k, v, cache.k_pages, cache.v_pages, plan.slots, rows))
+                                   keep=lambda k, v: store_pages(k, v, cache.k_pages, cache.v_pages, plan.slots, rows,
+                                                              scales=cache.scales))
 
     @torch.no_grad()
-    def decode(self, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan) -> torch.Tensor:
+    def decode(self, x: torch.Tensor, cache: "CCGQACache", plan: PagePlan,
+               shared: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward() of each request's newest token, x [N, dim] or [N, 1, dim],
         on what the cache holds of it.  `plan`: pool.plan(new_tokens) of width
         1; a request without a token (0 new, or refused) gets zeros and its
-        cache stays."""
+        cache stays.  `shared`: int32 [groups], the positions that the requests of
+        each group hold in common, which are read once (paged_attention)."""
         name = "CCGQAAttention.decode"
         self._check_cache(name, x, cache, plan)
         N = cache.ring.shape[0]
@@ -320,14 +344,22 @@ class CCGQAAttention(nn.Module):
         tiled = self._tiled(x.dtype)
         w_o = self.o_proj.weight
         packed, packed_o = self._packed(convw, w_o, x.dtype, tiled)
+        slots, k_pages, v_pages = plan.slots, cache.k_pages, cache.v_pages
+        if cache.scales is not None:  # as 16 bits beside the pages first
+            slots = torch.where(slots[:, 0] < 0, slots[:, 0], cache._new_rows)
+            k_pages, v_pages = cache._new.view(2, -1, 16, self.n_kv_heads, self.head_dim).transpose(2, 3).unbind(0)
         q = ccgqa_decode_prep(
-            F.linear(x.reshape(N, self.dim), self.qkv_proj.weight), cache.ring, plan.positions, plan.slots,
-            cache.k_pages, cache.v_pages, self.n_heads, self.n_kv_heads, self.head_dim,
+            F.linear(x.reshape(N, self.dim), self.qkv_proj.weight), cache.ring, plan.positions, slots,
+            k_pages, v_pages, self.n_heads, self.n_kv_heads, self.head_dim,
             flags | (CCGQA_W_TILED if tiled else 0), *packed,
             temperature=self.key_temperature if self.use_qk_norm else None,
             cos=self.cos_cached if self.use_rope else None, sin=self.sin_cached if self.use_rope else None,
             packed=True, conv_ks=self.conv_kernel_size)
-        o = paged_attention(q, cache.k_pages, cache.v_pages, cache.table, plan.seen, scale=self.scale)
+        if cache.scales is not None:
+            k, v = cache._new[:, :N, :, None].unbind(0)
+            store_pages(k, v, cache.k_pages, cache.v_pages, plan.slots, scales=cache.scales)
+        o = paged_attention(q, cache.k_pages, cache.v_pages, cache.table, plan.seen, scale=self.scale,
+                            scales=cache.scales, shared=shared)
         out = output_projection(o.view(N, self.latent_dim), w_o, packed_o).view(x.shape)
         if self.output_scale != 1.0:
             out = out * self.output_scale

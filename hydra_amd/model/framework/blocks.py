@@ -78,9 +78,10 @@ class HydraBlock(nn.Module):
                              norm=_lib.NORM_RMS, want_h=True)
         return _mlp_residual(self.mlp, h, y)
 
-    def new_cache(self, pool: PagePool, dtype: Optional[torch.dtype] = None):
+    def new_cache(self, pool: PagePool, dtype: Optional[torch.dtype] = None,
+                  page_dtype: Optional[torch.dtype] = None):
         """The attention's cache for the requests of `pool`."""
-        return self.attention.new_cache(pool, dtype)
+        return self.attention.new_cache(pool, dtype, page_dtype)
 
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, cache, plan: PagePlan, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -89,12 +90,12 @@ class HydraBlock(nn.Module):
         return self._rest(x, self.attention.prefill(self.norm1(x), cache, plan, rows))
 
     @torch.no_grad()
-    def decode(self, x: torch.Tensor, cache, plan: PagePlan) -> torch.Tensor:
+    def decode(self, x: torch.Tensor, cache, plan: PagePlan, shared: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward() of each request's newest token, x [N, dim] or [N, 1, dim]
-        (CCGQAAttention.decode).  The row of a request without a token
+        (CCGQAAttention.decode, also `shared`).  The row of a request without a token
         (plan.seen 0) holds no result: it is x and the MLP's part of it, without
         attention."""
-        return self._rest(x, self.attention.decode(self.norm1(x), cache, plan))
+        return self._rest(x, self.attention.decode(self.norm1(x), cache, plan, shared))
 
 
 class HydraMoRBlock(nn.Module):
