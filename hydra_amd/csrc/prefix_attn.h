@@ -32,14 +32,15 @@
 //    costs a second matrix instruction where the softmax's arithmetic is the
 //    longer part.  In fp32 all operands are fp32.
 //
-// Split: the rounds (128 keys) of all A items and of all B items are laid end to
-// end and dealt out evenly, A's to the first workgroups and B's to the others in
-// the ratio of their numbers, whatever the lengths.  What a workgroup leaves of an item is
-// (max, sum, unscaled output) per row in the workspace; a second kernel joins each
-// row's parts in their order.  No atomics on results: the same inputs give the
-// same bits.
+// Split: A items are cut into pieces of whole rounds (128 keys), one to a workgroup
+// where they suffice; the rounds of all B items are laid end to end and dealt out
+// evenly to the other workgroups, whatever the lengths.  How many workgroups each gets
+// goes by their rounds' cost.  What a workgroup leaves of an item is (max, sum, unscaled
+// output) per row in the workspace; a second kernel joins each row's parts in their
+// order.  No atomics on results: the same inputs give the same bits.
 #pragma once
 #include "common.h"
+#include "lds_dma.h"
 #include "mod_keys.h"
 
 #include <algorithm>
@@ -78,13 +79,13 @@ struct PrefixArgs {
   bool split;                   // else one workgroup takes one B item, `first` and on
   int first, wgs, cus;
   int* plan;                    // see kPlan
-  float* part;                  // [wgs][2] slots, then (with groups) whole A and B items
-  int64_t slot_a, slot_b, whole_a, whole_b;  // floats of a slot, offsets in part
+  float* part;                  // slots: pieces of A, then [wgs][2] of B, then (with groups) whole B items
+  int64_t slot_a, slot_b, part_b, whole_b;  // floats of a slot, offsets in part
 };
 
-// The plan's whole numbers: workgroups of A, rounds of each and of the others,
-// then prefix sums of the groups' and of the requests' rounds.
-enum { kWgsA, kPerA, kPerB, kPlan };
+// The plan's whole numbers: workgroups of A, rounds of each of the others, then prefix
+// sums of the groups' pieces and of the requests' rounds.
+enum { kWgsA, kPerB, kPlan };
 
 // What depends on the type of the pages and of the queries.
 template <typename C, typename KV> struct Types {
@@ -160,6 +161,23 @@ __device__ __forceinline__ uint4 row_piece(const char* row, int piece, int hd) {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+
+// The weights of 8 keys as two operands of a 16-bit type: rounded, and what that leaves.
+template <typename T>
+__device__ __forceinline__ void two_terms(const f32x4_t& a, const f32x4_t& b, uint4& hi, uint4& lo) {
+  uint32_t h[4], x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float p0 = i < 2 ? a[2 * i] : b[2 * i - 4], p1 = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+    h[i] = pack2<T>(p0, p1);
+    T w0, w1;
+    w0.bits = static_cast<uint16_t>(h[i] & 0xffffu);
+    w1.bits = static_cast<uint16_t>(h[i] >> 16);
+    x[i] = pack2<T>(p0 - to_f32(w0), p1 - to_f32(w1));
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // Four scales of neighbouring rows.
@@ -427,23 +445,7 @@ __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& it, c
           st.l[t] += p;
           s[b][t][r] = EIGHT ? p * vs[b][r] : p;
         }
-      if constexpr (!F32) {
-        uint32_t h[4] = {0, 0, 0, 0}, x[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; r += 2) {
-            const float p0 = s[b][t][r], p1 = s[b][t][r + 1];
-            const uint32_t w = pack2<VT>(p0, p1);
-            VT w0, w1;
-            w0.bits = static_cast<uint16_t>(w & 0xffffu);
-            w1.bits = static_cast<uint16_t>(w >> 16);
-            h[2 * b + r / 2] = w;
-            x[2 * b + r / 2] = pack2<VT>(p0 - to_f32(w0), p1 - to_f32(w1));
-          }
-        hi[t] = make_uint4(h[0], h[1], h[2], h[3]);
-        lo[t] = make_uint4(x[0], x[1], x[2], x[3]);
-      }
+      if constexpr (!F32) two_terms<VT>(s[0][t], s[1][t], hi[t], lo[t]);
     }
     if constexpr (RW == 1) {  // the tile is this wave's alone; its LDS operations keep their order
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -525,6 +527,175 @@ __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& it, c
   __syncthreads();  // the LDS is free
 }
 
+// An A item of more rows than a wave takes, over pages of the queries' 16-bit type:
+// the same product, with keys and values both staged in LDS by direct loads, 64 keys
+// (of more than 128 channels 32) at a time and the next tile's in flight meanwhile.
+// The loads write 16 bytes a lane one after the other, so it is the lanes' sources that
+// are permuted: piece c of row r lies at c ^ f(r), which spreads both the rows' 16-byte
+// reads (16 rows at once) and the transposing ones (8 rows of 32 bytes) over all banks.
+// An item's keys end at a whole 16, so what is not seen are whole blocks of 16: their
+// loads' descriptors are empty, which gives zeros.
+constexpr int rows_tile(int hdp) { return hdp == 256 ? 32 : 64; }
+
+template <typename C, int HDP, int NT>
+__device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, char* lds, State<HDP, NT>& st) {
+  constexpr int KT = rows_tile(HDP), NB = KT / 16, PPR = HDP / 8, RPI = 64 / PPR, NJ = KT * PPR / 256;
+  constexpr int NC = HDP / 32, NO = HDP / 16, TILE = KT * HDP * 2;
+  constexpr int RPB = PPR < 16 ? 16 / PPR : 1, PX = PPR < 16 ? PPR : 16;  // rows of 256 bytes; pieces to permute
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g4 = lane >> 4, rmask = (1 << a.shift) - 1;
+  const int* trow = a.table + it.trow * a.table_rs;
+  const char *kbase = a.k + it.h * a.k_st[1], *vbase = a.v + it.h * a.v_st[1];
+  auto fk = [](int r) { return r / RPB % PX; };
+  auto fv = [](int r) { return r / RPB % (PX / 2) * 2; };
+
+  // q times the scale's sign: the score's product with |scale| is then monotone
+  const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+  const float scale = fabsf(a.scale);
+  uint4 qf[NT][NC];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = wave * 16 * NT + 16 * t + col;
+    const bool there = r < it.rows;
+    const int at = it.row0 + (there ? r : 0), n = it.n0 + at / a.G, head = it.h * a.G + at % a.G;
+    const char* qrow = a.q + n * a.q_st[0] + static_cast<int64_t>(head) * a.q_st[1];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint4 x = row_piece<C, true>(qrow, 4 * c + g4, a.hd);
+      x = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+      qf[t][c] = there ? x : make_uint4(0, 0, 0, 0);
+    }
+    st.m[t] = -INFINITY;
+    st.l[t] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NO; ++i) st.o[t][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  float ms[NT];  // m times the scale, 0 before the first key
+#pragma unroll
+  for (int t = 0; t < NT; ++t) ms[t] = 0.f;
+
+  // this lane's piece of each direct load, in a block of 16 rows
+  uint32_t koff[NJ], voff[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int r = (j * 4 + wave) * RPI + lane / PPR, c = lane % PPR;
+    const uint32_t ck = c ^ fk(r), cv = c ^ fv(r), none = 0x7ffffff0u;
+    koff[j] = static_cast<int>(ck) * 8 < a.hd ? (r & 15) * static_cast<uint32_t>(a.k_st[2]) + 16 * ck : none;
+    voff[j] = static_cast<int>(cv) * 8 < a.hd ? (r & 15) * static_cast<uint32_t>(a.v_st[2]) + 16 * cv : none;
+  }
+  const int kbytes = 15 * static_cast<int>(a.k_st[2]) + 2 * a.hd, vbytes = 15 * static_cast<int>(a.v_st[2]) + 2 * a.hd;
+  const uint32_t base = lds_addr(lds);
+  auto issue = [&](const int (&pg)[NB], int k0, int buf) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int b = (j * 4 + wave) * RPI >> 4;
+      int p = pg[0];
+#pragma unroll
+      for (int x = 1; x < NB; ++x) p = b == x ? pg[x] : p;
+      const int64_t r = (k0 + 16 * b) & rmask, at = max(p, 0);
+      const uint32_t to = base + buf * 2 * TILE + (j * 4 + wave) * 1024;
+      load16_to_lds(raw_rsrc(kbase + at * a.k_st[0] + r * a.k_st[2], p < 0 ? 0 : kbytes), to, koff[j]);
+      load16_to_lds(raw_rsrc(vbase + at * a.v_st[0] + r * a.v_st[2], p < 0 ? 0 : vbytes), to + TILE, voff[j]);
+    }
+  };
+  const uint32_t kread = col * HDP * 2 + ((g4 ^ fk(col)) << 4);
+  const int vr = 4 * g4 + (col >> 2);
+  const uint32_t vread = vr * HDP * 2 + ((((col & 3) >> 1) ^ fv(vr)) << 4) + (col & 1) * 8;
+
+  int page[NB], next[NB];
+  tile_pages<NB>(a, trow, it.begin, it.end, page);
+  tile_pages<NB>(a, trow, it.begin + KT, it.end, next);
+  __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): q is here, only direct loads are counted below
+  issue(page, it.begin, 0);
+  int buf = 0;
+  for (int key0 = it.begin; key0 < it.end; key0 += KT, buf ^= 1) {
+    __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): this wave's part of the tile
+    __syncthreads();                     // everybody's, and the other tile is read
+    if (key0 + KT < it.end) issue(next, key0 + KT, buf ^ 1);
+    int after[NB];
+    tile_pages<NB>(a, trow, key0 + 2 * KT, it.end, after);
+    const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
+    f32x4_t s[NB][NT];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[b][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const uint4 kk = *reinterpret_cast<const uint4*>(kt + b * 16 * HDP * 2 + (kread ^ (c << 6)));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[b][t] = mfma32<C>(kk, qf[t][c], s[b][t]);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (page[b] < 0) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[b][t] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[b][t][r]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = halves_max(top);
+      if (__any(top > st.m[t])) {
+        const float mn = fmaxf(st.m[t], top), mns = mn == -INFINITY ? 0.f : mn * scale;
+        const float alpha = st.m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[t] - mns);
+        st.m[t] = mn;
+        ms[t] = mns;
+        st.l[t] *= alpha;
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st.o[t][i][r] *= alpha;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[b][t][r] = __builtin_amdgcn_exp2f(fmaf(s[b][t][r], scale, -ms[t]));
+          if (page[b] < 0) s[b][t][r] = 0.f;  // also where the scale is 0
+          st.l[t] += s[b][t][r];
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b += 2) {
+      uint4 hi[NT], lo[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) two_terms<C>(s[b][t], s[b + 1][t], hi[t], lo[t]);
+#pragma unroll
+      for (int i = 0; i < NO; ++i) {
+        typedef __attribute__((address_space(3))) s16x4_t* lds_t;
+        const char* p = vt + b * 16 * HDP * 2 + (vread ^ (i << 5));
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p)));
+        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 16 * HDP * 2)));
+        const uint4 vv = make_uint4(x.x, x.y, y.x, y.y);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          st.o[t][i] = mfma32<C>(vv, hi[t], st.o[t][i]);
+          st.o[t][i] = mfma32<C>(vv, lo[t], st.o[t][i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      page[b] = next[b];
+      next[b] = after[b];
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    st.l[t] += __shfl_xor(st.l[t], 16);
+    st.l[t] = halves_sum(st.l[t]);
+    if (st.m[t] != -INFINITY) st.m[t] = ms[t];
+  }
+  __syncthreads();  // the LDS is free
+}
+
 __device__ __host__ __forceinline__ int row4(int hd) { return (hd + 3) & ~3; }
 // Rows of a B slot: an even number, so that its outputs begin at 16 bytes.
 __device__ __host__ __forceinline__ int cap_b(int G) { return G < 16 ? (G + 1) & ~1 : 16; }
@@ -585,17 +756,22 @@ __device__ __forceinline__ Parts parts_of(int u, int r, int per) {
   return p;
 }
 
+// Whether A items of many rows go through item_rows.
+template <typename C, typename KV>
+constexpr bool by_rows(bool vec) { return std::is_same<C, KV>::value && sizeof(C) == 2 && vec; }
+
 template <typename C, typename KV, int HDP>
-constexpr int lds_bytes(int nt, int rw) {
+constexpr int lds_bytes(int nt, int rw, bool vec) {
   const bool f32 = sizeof(C) == 4;
   const int tile = tile_keys(HDP, f32) * pitch_of(HDP, f32) * (f32 ? 4 : 2);
+  if (rw == 4 && by_rows<C, KV>(vec)) return 4 * rows_tile(HDP) * HDP * 2;
   return rw == 1 ? std::max(4 * tile, 2 * 64 * nt * (2 + HDP / 4) * 4) : 2 * tile;
 }
 
 // One workgroup per B item, no split.
 template <typename C, typename KV, int HDP, bool VEC>
 __global__ __launch_bounds__(kThreads, 2) void prefix_whole_kernel(PrefixArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[lds_bytes<C, KV, HDP>(1, 1)];
+  __shared__ __attribute__((aligned(16))) char lds[lds_bytes<C, KV, HDP>(1, 1, VEC)];
   const int item = a.first + blockIdx.x, gb = item % a.GB, h = item / a.GB % a.Hkv, n = item / a.GB / a.Hkv;
   Item it{n, h, 16 * gb, min(16, a.G - 16 * gb), n, 0, clamp_len(a, a.lengths[n])};
   State<HDP, 1> st;
@@ -607,9 +783,10 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_whole_kernel(PrefixArgs a)
 template <typename C, typename KV, int HDP, int RW, bool VEC>
 __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a) {
   constexpr int NT = tiles_a(HDP, sizeof(C) == 4), RA = RW == 0 ? 1 : RW, ROWS = 16 * NT * RA;
-  constexpr int LDS_A = RW == 0 ? 0 : lds_bytes<C, KV, HDP>(NT, RA), LDS_B = lds_bytes<C, KV, HDP>(1, 1);
+  constexpr int LDS_A = RW == 0 ? 0 : lds_bytes<C, KV, HDP>(NT, RA, VEC), LDS_B = lds_bytes<C, KV, HDP>(1, 1, VEC);
   __shared__ __attribute__((aligned(16))) char lds[LDS_A > LDS_B ? LDS_A : LDS_B];
-  __shared__ int pre_a[RW == 0 ? 1 : kRequests + 1], lead[RW == 0 ? 1 : kRequests], pre_b[kRequests + 1];
+  // prefix sums of the groups' rounds and pieces, and of the requests' own rounds
+  __shared__ int units[RW == 0 ? 1 : kRequests + 1], lead[RW == 0 ? 1 : kRequests], pre_b[kRequests + 1];
   __shared__ int wsum[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto scan = [&](int n, int* pre, auto&& value) {  // pre[i + 1] = value(0) + .. + value(i)
@@ -638,8 +815,23 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
       if (clamp_len(a, a.lengths[n]) >= clamp_len(a, a.shared[g])) atomicMin(&lead[g], n);
     }
     __syncthreads();
-    scan(a.groups, pre_a, [&](int g) { return lead[g] < a.N ? rounds_of(shared_keys(a, g)) : 0; });
   }
+  auto rounds_of_group = [&](int g) { return lead[g] < a.N ? rounds_of(shared_keys(a, g)) : 0; };
+  int rounds_a = 0;
+  if constexpr (RW != 0) {
+    scan(a.groups, units, rounds_of_group);
+    rounds_a = units[a.groups];
+    __syncthreads();  // read before it is written again
+  }
+  // the last x with pre[x] <= u
+  auto find = [](const int* pre, int n, int u) {
+    int x = 0;
+    for (int hi = n; hi - x > 1;) {
+      const int mid = (x + hi) >> 1;
+      if (pre[mid] <= u) x = mid; else hi = mid;
+    }
+    return x;
+  };
   auto own_begin = [&](int n) {  // where request n's own keys begin
     if constexpr (RW == 0) return 0;
     const int g = n / a.W;
@@ -647,69 +839,81 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
   };
   scan(a.N, pre_b, [&](int n) { return rounds_of(clamp_len(a, a.lengths[n]) - own_begin(n)); });
   const int HA = a.Hkv * a.RB, HB = a.Hkv * a.GB;
-  const int total_a = RW == 0 ? 0 : pre_a[a.groups] * HA, total_b = pre_b[a.N] * HB;
-  int wgs_a = 0;
-  if (total_a > 0) {
-    wgs_a = total_b == 0 ? a.wgs
-                         : max(1, min(a.wgs - 1, static_cast<int>(static_cast<int64_t>(a.wgs) * total_a /
-                                                                  (static_cast<int64_t>(total_a) + total_b))));
+  const int total_b = pre_b[a.N] * HB;
+  int wgs_a = 0, units_a = 0;
+  if constexpr (RW != 0) {
+    if (rounds_a > 0) {
+      // a round of 128 keys is four tiles of a workgroup whose waves have rows of their own
+      const int64_t cost = static_cast<int64_t>(rounds_a) * HA * RW;
+      wgs_a = total_b == 0 ? a.wgs : max(1, min(a.wgs - 1, static_cast<int>(a.wgs * cost / (cost + total_b))));
+      // The least piece for which the pieces are no more than the workgroups, so that each
+      // has one, if all items are not more than that already.
+      int per = max(1, static_cast<int>((static_cast<int64_t>(rounds_a) * HA + wgs_a - 1) / wgs_a));
+      for (int turn = 0; turn < 16; ++turn) {
+        scan(a.groups, units, [&](int g) { return (rounds_of_group(g) + per - 1) / per; });
+        const int64_t all = static_cast<int64_t>(units[a.groups]) * HA;
+        __syncthreads();
+        if (all <= wgs_a || static_cast<int64_t>(a.groups) * HA > wgs_a) break;
+        per = max(per + 1, static_cast<int>((per * all + wgs_a - 1) / wgs_a));
+      }
+      units_a = units[a.groups] * HA;
+      wgs_a = min(wgs_a, units_a);
+    }
   }
-  const int per_a = wgs_a == 0 ? 1 : (total_a + wgs_a - 1) / wgs_a;
   const int wgs_b = a.wgs - wgs_a;
   const int per_b = wgs_b == 0 ? 1 : max(1, (total_b + wgs_b - 1) / wgs_b);
   if (blockIdx.x == 0) {  // for the joining kernel
     if (tid == 0) {
       a.plan[kWgsA] = wgs_a;
-      a.plan[kPerA] = per_a;
       a.plan[kPerB] = per_b;
     }
     if constexpr (RW != 0)
-      for (int i = tid; i <= a.groups; i += kThreads) a.plan[kPlan + i] = pre_a[i];
+      for (int i = tid; i <= a.groups; i += kThreads) a.plan[kPlan + i] = units_a > 0 ? units[i] : 0;
     for (int i = tid; i <= a.N; i += kThreads) a.plan[kPlan + a.groups + 1 + i] = pre_b[i];
   }
-  const bool is_a = static_cast<int>(blockIdx.x) < wgs_a;
-  const int per = is_a ? per_a : per_b, total = is_a ? total_a : total_b, HG = is_a ? HA : HB;
-  const int count = is_a ? a.groups : a.N;
-  const int* pre = is_a ? pre_a : pre_b;
-  const int64_t from = static_cast<int64_t>(static_cast<int>(blockIdx.x) - (is_a ? 0 : wgs_a)) * per;
-  const int begin = min(from, static_cast<int64_t>(total)), end = min(from + per, static_cast<int64_t>(total));
-  // the last x with pre[x] HG <= begin
-  int x = 0;
-  for (int hi = count; begin < end && hi - x > 1;) {
-    const int mid = (x + hi) >> 1;
-    if (pre[mid] * HG <= begin) x = mid; else hi = mid;
+  if constexpr (RW != 0) {
+    if (static_cast<int>(blockIdx.x) < wgs_a) {
+      // Pieces in the order (group, key head, piece, block of rows), each XCD (workgroups go
+      // to them in turn) a run of them: the blocks of rows read the same keys from its L2.
+      const int w = blockIdx.x, xcds = min(8, wgs_a), x = w % xcds, at = w / xcds, beside = (wgs_a - x + xcds - 1) / xcds;
+      const int first = static_cast<int>(static_cast<int64_t>(units_a) * x / xcds);
+      const int last = static_cast<int>(static_cast<int64_t>(units_a) * (x + 1) / xcds);
+      for (int u = first + at; u < last; u += beside) {
+        const int g = find(units, a.groups, u / HA);
+        const int pieces = units[g + 1] - units[g], r = rounds_of_group(g), v = u - units[g] * HA;
+        const int h = v / (pieces * a.RB), y = v - h * pieces * a.RB, piece = y / a.RB, rb = y - piece * a.RB;
+        const int t0 = static_cast<int>(static_cast<int64_t>(r) * piece / pieces);
+        const int t1 = static_cast<int>(static_cast<int64_t>(r) * (piece + 1) / pieces);
+        Item it{g * a.W, h, rb * ROWS, min(ROWS, a.W * a.G - rb * ROWS), lead[g], t0 * kRound,
+                t1 == r ? shared_keys(a, g) : t1 * kRound};
+        State<HDP, NT> st;
+        if constexpr (RW == 4 && by_rows<C, KV>(VEC)) item_rows<C, HDP, NT>(a, it, lds, st);
+        else item_keys<C, KV, HDP, NT, RA, VEC>(a, it, lds, st);
+        write_slot<HDP, NT, RA>(a, it, st, a.part + u * a.slot_a, ROWS);
+      }
+      return;
+    }
   }
-  const int64_t slot = RW != 0 && a.slot_a > a.slot_b ? a.slot_a : a.slot_b;
+  const int64_t from = static_cast<int64_t>(static_cast<int>(blockIdx.x) - wgs_a) * per_b;
+  const int begin = min(from, static_cast<int64_t>(total_b)), end = min(from + per_b, static_cast<int64_t>(total_b));
+  int n = begin < end ? find(pre_b, a.N, begin / HB) : 0;
   for (int u = begin; u < end;) {
-    while (pre[x + 1] * HG <= u) ++x;
-    const int r = pre[x + 1] - pre[x], at = u - pre[x] * HG, hg = at / r, t0 = at - hg * r;
+    while (pre_b[n + 1] * HB <= u) ++n;
+    const int r = pre_b[n + 1] - pre_b[n], at = u - pre_b[n] * HB, hg = at / r, t0 = at - hg * r;
     const int take = min(r - t0, end - u);
     const bool all = take == r;
-    float* to = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * slot;
-    if constexpr (RW != 0) {
-      if (is_a) {
-        const int h = hg / a.RB, rb = hg - h * a.RB;
-        Item it{x * a.W, h, rb * ROWS, min(ROWS, a.W * a.G - rb * ROWS), lead[x], t0 * kRound,
-                min(shared_keys(a, x), (t0 + take) * kRound)};
-        State<HDP, NT> st;
-        item_keys<C, KV, HDP, NT, RA, VEC>(a, it, lds, st);
-        if (all) to = a.part + a.whole_a + (static_cast<int64_t>(x) * HA + hg) * a.slot_a;
-        write_slot<HDP, NT, RA>(a, it, st, to, ROWS);
-      }
-    }
-    if (!is_a) {
-      const int h = hg / a.GB, gb = hg - h * a.GB, len = clamp_len(a, a.lengths[x]), own = own_begin(x);
-      // a long context's last round may end past an int
-      const int last = len - own - t0 * kRound > take * kRound ? own + (t0 + take) * kRound : len;
-      Item it{x, h, 16 * gb, min(16, a.G - 16 * gb), x, own + t0 * kRound, last};
-      State<HDP, 1> st;
-      item_keys<C, KV, HDP, 1, 1, VEC>(a, it, lds, st);
-      if (RW == 0 && all) {
-        write_out<C, HDP>(a, it, st);
-      } else {
-        if (all) to = a.part + a.whole_b + (static_cast<int64_t>(x) * HB + hg) * a.slot_b;
-        write_slot<HDP, 1, 1>(a, it, st, to, cap_b(a.G));
-      }
+    const int h = hg / a.GB, gb = hg - h * a.GB, len = clamp_len(a, a.lengths[n]), own = own_begin(n);
+    // a long context's last round may end past an int
+    const int last = len - own - t0 * kRound > take * kRound ? own + (t0 + take) * kRound : len;
+    Item it{n, h, 16 * gb, min(16, a.G - 16 * gb), n, own + t0 * kRound, last};
+    State<HDP, 1> st;
+    item_keys<C, KV, HDP, 1, 1, VEC>(a, it, lds, st);
+    if (RW == 0 && all) {
+      write_out<C, HDP>(a, it, st);
+    } else {
+      float* to = a.part + (all ? a.whole_b + (static_cast<int64_t>(n) * HB + hg) * a.slot_b
+                                : a.part_b + (static_cast<int64_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * a.slot_b);
+      write_slot<HDP, 1, 1>(a, it, st, to, cap_b(a.G));
     }
     u += take;
   }
@@ -728,18 +932,16 @@ __global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void prefix_join_k
   if (row >= a.N * a.H) return;  // whole waves; where threads meet, ROWS is 1
   const int n = row / a.H, head = row - n * a.H, h = head / a.G, g = head - h * a.G;
   const int HA = a.Hkv * a.RB, HB = a.Hkv * a.GB;
-  const int wgs_a = a.plan[kWgsA], per_a = a.plan[kPerA], per_b = a.plan[kPerB];
-  const int64_t slot = a.groups != 0 && a.slot_a > a.slot_b ? a.slot_a : a.slot_b;
-  Parts pa{0, 0, false};
-  const float* whole_a = nullptr;
-  int at_a = 0;
+  const int wgs_a = a.plan[kWgsA], per_b = a.plan[kPerB];
+  int pieces = 0, at_a = 0;
+  const float* part_a = nullptr;
   if (a.groups != 0) {
-    const int x = n / a.W, p0 = a.plan[kPlan + x], r = a.plan[kPlan + x + 1] - p0;
+    const int x = n / a.W, u0 = a.plan[kPlan + x];
     if (clamp_len(a, a.lengths[n]) >= clamp_len(a, a.shared[x])) {
-      const int m = (n - x * a.W) * a.G + g, rb = m / rows_a, hg = h * a.RB + rb;
+      const int m = (n - x * a.W) * a.G + g, rb = m / rows_a;
       at_a = m - rb * rows_a;
-      pa = parts_of(p0 * HA + hg * r, r, per_a);
-      if (pa.count == 1) whole_a = a.part + a.whole_a + (static_cast<int64_t>(x) * HA + hg) * a.slot_a;
+      pieces = a.plan[kPlan + x + 1] - u0;
+      part_a = a.part + (static_cast<int64_t>(u0) * HA + static_cast<int64_t>(h) * pieces * a.RB + rb) * a.slot_a;
     }
   }
   const int* pre_b = a.plan + kPlan + a.groups + 1;
@@ -747,14 +949,15 @@ __global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void prefix_join_k
   const Parts pb = parts_of(pre_b[n] * HB + hg * r, r, per_b);
   if (a.groups == 0 && pb.count == 1) return;
   const float* whole_b = pb.count == 1 ? a.part + a.whole_b + (static_cast<int64_t>(n) * HB + hg) * a.slot_b : nullptr;
-  const int parts = pa.count + pb.count, r4 = row4(a.hd);
+  const int parts = pieces + pb.count, r4 = row4(a.hd);
   struct At { const float *m, *l, *o; };
   auto part = [&](int p) {
-    const bool is_a = p < pa.count;
-    const Parts& q = is_a ? pa : pb;
-    const int i = is_a ? p : p - pa.count;
-    const float* s = is_a ? whole_a : whole_b;
-    if (!s) s = a.part + (static_cast<int64_t>(q.first + i + (is_a ? 0 : wgs_a)) * 2 + (i == 0 && q.inside ? 1 : 0)) * slot;
+    const bool is_a = p < pieces;
+    const int i = p - pieces;
+    const float* s = is_a ? part_a + static_cast<int64_t>(p) * a.RB * a.slot_a
+                     : whole_b ? whole_b
+                               : a.part + a.part_b +
+                                     (static_cast<int64_t>(pb.first + i + wgs_a) * 2 + (i == 0 && pb.inside ? 1 : 0)) * a.slot_b;
     const int cap = is_a ? rows_a : cap_b(a.G), at = is_a ? at_a : at_b;
     return At{s + at, s + cap + at, s + 2 * cap + at * r4};
   };

@@ -11,7 +11,7 @@ struct Pieces {
   Shape s;
   bool split;
   int64_t GB, requests, wgs;
-  int64_t slot_a, slot_b, whole_a, whole_b;  // floats; of the largest piece
+  int64_t slot_a, slot_b, part_b, whole_b;  // floats; of the largest piece
 };
 
 int check_prefix(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, int64_t P, int64_t page_size, int dtype,
@@ -51,9 +51,9 @@ int pieces_of(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, int
   if (groups > 0) {
     p.slot_a = p.s.rows_a * (2 + r4);
     const int64_t w = std::min(W, p.requests), g = std::min(groups, std::max<int64_t>(1, p.requests / W));
-    p.whole_a = p.wgs * 2 * std::max(p.slot_a, p.slot_b);
-    p.whole_b = p.whole_a + g * Hkv * ((w * G + p.s.rows_a - 1) / p.s.rows_a) * p.slot_a;
+    p.part_b = (p.wgs + g * Hkv * ((w * G + p.s.rows_a - 1) / p.s.rows_a)) * p.slot_a;
   }
+  p.whole_b = p.part_b + p.wgs * 2 * p.slot_b;
   return HYDRA_OK;
 }
 
@@ -61,7 +61,7 @@ int64_t plan_ints() { return kPlan + 2 * kRequests + 2 + 3; }  // whole 16 bytes
 
 int64_t workspace_bytes(const Pieces& p, int64_t groups, int64_t N, int64_t Hkv) {
   if (!p.split) return 0;
-  const int64_t floats = groups > 0 ? p.whole_b + std::min(N, p.requests) * Hkv * p.GB * p.slot_b : p.wgs * 2 * p.slot_b;
+  const int64_t floats = p.whole_b + (groups > 0 ? std::min(N, p.requests) * Hkv * p.GB * p.slot_b : 0);
   return 4 * (plan_ints() / 4 * 4 + floats);
 }
 
@@ -160,7 +160,7 @@ extern "C" int hydra_prefix_attn(const void* q, const void* k_pages, const void*
   a.part = static_cast<float*>(workspace) + plan_ints() / 4 * 4;
   a.slot_a = p.slot_a;
   a.slot_b = p.slot_b;
-  a.whole_a = p.whole_a;
+  a.part_b = p.part_b;
   a.whole_b = p.whole_b;
   auto st = static_cast<hipStream_t>(stream);
   auto launch = [&](const PrefixArgs& x) -> int {
