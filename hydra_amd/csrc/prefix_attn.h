@@ -33,9 +33,8 @@
 //    longer part.  In fp32 all operands are fp32.
 //
 // Split: A items are cut into pieces of whole rounds (128 keys), one to a workgroup
-// where they suffice; the rounds of all B items are laid end to end and dealt out
-// evenly to the other workgroups, whatever the lengths.  How many workgroups each gets
-// goes by their rounds' cost.  What a workgroup leaves of an item is (max, sum, unscaled
+// where they suffice; the rounds of all B items are laid end to end and dealt out to
+// all workgroups so that each has as much to do, whatever the lengths.  What a workgroup leaves of an item is (max, sum, unscaled
 // output) per row in the workspace; a second kernel joins each row's parts in their
 // order.  No atomics on results: the same inputs give the same bits.
 #pragma once
@@ -44,6 +43,7 @@
 #include "mod_keys.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace hydra {
 namespace prefix {
@@ -83,9 +83,9 @@ struct PrefixArgs {
   int64_t slot_a, slot_b, part_b, whole_b;  // floats of a slot, offsets in part
 };
 
-// The plan's whole numbers: workgroups of A, rounds of each of the others, then prefix
-// sums of the groups' pieces and of the requests' rounds.
-enum { kWgsA, kPerB, kPlan };
+// The plan's whole numbers: how B is dealt out (Deal), then prefix sums of the groups'
+// pieces and of the requests' rounds.
+enum { kWgsA, kBeside, kPer, kPlan };
 
 // What depends on the type of the pages and of the queries.
 template <typename C, typename KV> struct Types {
@@ -171,10 +171,13 @@ __device__ __forceinline__ void two_terms(const f32x4_t& a, const f32x4_t& b, ui
   for (int i = 0; i < 4; ++i) {
     const float p0 = i < 2 ? a[2 * i] : b[2 * i - 4], p1 = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
     h[i] = pack2<T>(p0, p1);
-    T w0, w1;
-    w0.bits = static_cast<uint16_t>(h[i] & 0xffffu);
-    w1.bits = static_cast<uint16_t>(h[i] >> 16);
-    x[i] = pack2<T>(p0 - to_f32(w0), p1 - to_f32(w1));
+    if constexpr (std::is_same<T, bf16>::value) {
+      asm("" : "+v"(h[i]));  // one conversion of the pair: the compiler would make three of it
+      x[i] = pack2<T>(p0 - __uint_as_float(h[i] << 16), p1 - __uint_as_float(h[i] & 0xffff0000u));
+    } else {
+      const f16x2_t w = __builtin_bit_cast(f16x2_t, h[i]);
+      x[i] = pack2<T>(p0 - static_cast<float>(w[0]), p1 - static_cast<float>(w[1]));
+    }
   }
   hi = make_uint4(h[0], h[1], h[2], h[3]);
   lo = make_uint4(x[0], x[1], x[2], x[3]);
@@ -200,27 +203,39 @@ struct Item {
   int trow, begin, end;
 };
 
+// The same in scalar registers: what prefix sums in LDS gave counts as different in
+// each lane, and pages would be looked up by vector loads in line with the keys'.
+__device__ __forceinline__ Item uniform(const Item& i) {
+  auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return Item{u(i.n0), u(i.h), u(i.row0), u(i.rows), u(i.trow), u(i.begin), u(i.end)};
+}
+
 // A wave's state of NT tiles of 16 rows: lane = column (row of the item) and group of four.
 template <int HDP, int NT> struct State {
   f32x4_t o[NT][HDP / 16];
   float m[NT], l[NT];
 };
 
-// Pages of a tile, one for each 16 keys, wave-uniform; -1: not there.
+// Pages of a tile, one for each 16 keys, wave-uniform (scalar loads: nothing in the
+// launch writes the table); -1: not there.
+__device__ __forceinline__ int page_of(const PrefixArgs& a, const int* row, int key0, int end) {
+  typedef const __attribute__((address_space(4))) int* const_t;
+  const const_t at = (const_t)(reinterpret_cast<uintptr_t>(row));
+  const int key = __builtin_amdgcn_readfirstlane(key0);
+  const int p = key < end ? at[key >> a.shift] : -1;
+  return static_cast<unsigned>(p) < static_cast<unsigned>(a.pages) ? p : -1;
+}
 template <int NB>
 __device__ __forceinline__ void tile_pages(const PrefixArgs& a, const int* row, int key0, int end, int (&page)[NB]) {
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int key = __builtin_amdgcn_readfirstlane(key0 + 16 * b);
-    const int p = key < end ? row[key >> a.shift] : -1;
-    page[b] = static_cast<unsigned>(p) < static_cast<unsigned>(a.pages) ? p : -1;
-  }
+  for (int b = 0; b < NB; ++b) page[b] = page_of(a, row, key0 + 16 * b, end);
 }
 
 // An item's keys.  RW = 1: four waves take tiles in turn, and wave 0 ends up with
 // all of their sums; RW = 4: each wave has rows of its own.
 template <typename C, typename KV, int HDP, int NT, int RW, bool VEC>
-__device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& it, char* lds, State<HDP, NT>& st) {
+__device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& item, char* lds, State<HDP, NT>& st) {
+  const Item it = uniform(item);
   using Ty = Types<C, KV>;
   using VT = typename Ty::VT;
   constexpr bool F32 = Ty::f32, EIGHT = Ty::eight;
@@ -538,7 +553,8 @@ __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& it, c
 constexpr int rows_tile(int hdp) { return hdp == 256 ? 32 : 64; }
 
 template <typename C, int HDP, int NT>
-__device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, char* lds, State<HDP, NT>& st) {
+__device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& item, char* lds, State<HDP, NT>& st) {
+  const Item it = uniform(item);
   constexpr int KT = rows_tile(HDP), NB = KT / 16, PPR = HDP / 8, RPI = 64 / PPR, NJ = KT * PPR / 256;
   constexpr int NC = HDP / 32, NO = HDP / 16, TILE = KT * HDP * 2;
   constexpr int RPB = PPR < 16 ? 16 / PPR : 1, PX = PPR < 16 ? PPR : 16;  // rows of 256 bytes; pieces to permute
@@ -551,7 +567,8 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, c
 
   // q times the scale's sign: the score's product with |scale| is then monotone
   const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
-  const float scale = fabsf(a.scale);
+  // a scale of 0 as the least there is: scores of 0, and -inf where a key is not seen
+  const float scale = fmaxf(fabsf(a.scale), 0x1p-126f);
   uint4 qf[NT][NC];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -585,14 +602,17 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, c
   }
   const int kbytes = 15 * static_cast<int>(a.k_st[2]) + 2 * a.hd, vbytes = 15 * static_cast<int>(a.v_st[2]) + 2 * a.hd;
   const uint32_t base = lds_addr(lds);
-  auto issue = [&](const int (&pg)[NB], int k0, int buf) {
+  // the pages that this wave loads from are looked up by themselves: chosen from the
+  // tile's by an index they would go through memory
+  auto load_pages = [&](int k0, int (&pg)[NJ]) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) pg[j] = page_of(a, trow, k0 + ((j * 4 + wave) * RPI & ~15), it.end);
+  };
+  auto issue = [&](const int (&pg)[NJ], int k0, int buf) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int b = (j * 4 + wave) * RPI >> 4;
-      int p = pg[0];
-#pragma unroll
-      for (int x = 1; x < NB; ++x) p = b == x ? pg[x] : p;
-      const int64_t r = (k0 + 16 * b) & rmask, at = max(p, 0);
+      const int p = pg[j];
+      const int64_t r = (k0 + ((j * 4 + wave) * RPI & ~15)) & rmask, at = max(p, 0);
       const uint32_t to = base + buf * 2 * TILE + (j * 4 + wave) * 1024;
       load16_to_lds(raw_rsrc(kbase + at * a.k_st[0] + r * a.k_st[2], p < 0 ? 0 : kbytes), to, koff[j]);
       load16_to_lds(raw_rsrc(vbase + at * a.v_st[0] + r * a.v_st[2], p < 0 ? 0 : vbytes), to + TILE, voff[j]);
@@ -602,37 +622,60 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, c
   const int vr = 4 * g4 + (col >> 2);
   const uint32_t vread = vr * HDP * 2 + ((((col & 3) >> 1) ^ fv(vr)) << 4) + (col & 1) * 8;
 
-  int page[NB], next[NB];
-  tile_pages<NB>(a, trow, it.begin, it.end, page);
-  tile_pages<NB>(a, trow, it.begin + KT, it.end, next);
+  int page[NB], from[NJ];
+  load_pages(it.begin, from);
   __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): q is here, only direct loads are counted below
-  issue(page, it.begin, 0);
+  issue(from, it.begin, 0);
+  tile_pages<NB>(a, trow, it.begin, it.end, page);
+  load_pages(it.begin + KT, from);
   int buf = 0;
   for (int key0 = it.begin; key0 < it.end; key0 += KT, buf ^= 1) {
     __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): this wave's part of the tile
     __syncthreads();                     // everybody's, and the other tile is read
-    if (key0 + KT < it.end) issue(next, key0 + KT, buf ^ 1);
+    if (key0 + KT < it.end) issue(from, key0 + KT, buf ^ 1);
     int after[NB];
-    tile_pages<NB>(a, trow, key0 + 2 * KT, it.end, after);
+    tile_pages<NB>(a, trow, key0 + KT, it.end, after);
+    load_pages(key0 + 2 * KT, from);
     const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
+    // Operands are read a phase ahead of the products that take them, which the barriers
+    // below keep in place: read where they are needed, LDS's latency would be waited for
+    // again and again with two waves to a SIMD.
+    uint4 kk[NB][NC];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) kk[b][c] = *reinterpret_cast<const uint4*>(kt + b * 16 * HDP * 2 + (kread ^ (c << 6)));
+    __builtin_amdgcn_sched_barrier(0);
+    // each sum's next product comes as late as possible: one waits for the other's result
+    __builtin_amdgcn_s_setprio(1);
     f32x4_t s[NB][NT];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      // a block that is not seen (its keys read as zeros): -inf
+      const float none = page[b] < 0 ? -INFINITY : 0.f;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[b][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const uint4 kk = *reinterpret_cast<const uint4*>(kt + b * 16 * HDP * 2 + (kread ^ (c << 6)));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[b][t] = mfma32<C>(kk, qf[t][c], s[b][t]);
-      }
+      for (int t = 0; t < NT; ++t) s[b][t] = f32x4_t{none, none, none, none};
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (page[b] < 0) {
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[b][t] = f32x4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[b][t] = mfma32<C>(kk[b][c], qf[t][c], s[b][t]);
+    uint4 vv[NO];
+    auto read_v = [&](int b) {
+#pragma unroll
+      for (int i = 0; i < NO; ++i) {
+        typedef __attribute__((address_space(3))) s16x4_t* lds_t;
+        const char* p = vt + b * 16 * HDP * 2 + (vread ^ (i << 5));
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p)));
+        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 16 * HDP * 2)));
+        vv[i] = make_uint4(x.x, x.y, y.x, y.y);
       }
+    };
+    read_v(0);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float top = -INFINITY;
@@ -642,7 +685,9 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, c
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[b][t][r]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = halves_max(top);
-      if (__any(top > st.m[t])) {
+      // the reference moves where it has fallen behind by more than 2^8 alone: weights up to
+      // that are as exact, and most tiles raise some row's maximum by a little
+      if (__any(top * scale > ms[t] + 8.f || st.m[t] == -INFINITY)) {
         const float mn = fmaxf(st.m[t], top), mns = mn == -INFINITY ? 0.f : mn * scale;
         const float alpha = st.m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[t] - mns);
         st.m[t] = mn;
@@ -658,7 +703,6 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, c
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           s[b][t][r] = __builtin_amdgcn_exp2f(fmaf(s[b][t][r], scale, -ms[t]));
-          if (page[b] < 0) s[b][t][r] = 0.f;  // also where the scale is 0
           st.l[t] += s[b][t][r];
         }
     }
@@ -667,25 +711,23 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& it, c
       uint4 hi[NT], lo[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) two_terms<C>(s[b][t], s[b + 1][t], hi[t], lo[t]);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int i = 0; i < NO; ++i) {
-        typedef __attribute__((address_space(3))) s16x4_t* lds_t;
-        const char* p = vt + b * 16 * HDP * 2 + (vread ^ (i << 5));
-        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p)));
-        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 16 * HDP * 2)));
-        const uint4 vv = make_uint4(x.x, x.y, y.x, y.y);
+      for (int i = 0; i < NO; ++i)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          st.o[t][i] = mfma32<C>(vv, hi[t], st.o[t][i]);
-          st.o[t][i] = mfma32<C>(vv, lo[t], st.o[t][i]);
-        }
+        for (int t = 0; t < NT; ++t) st.o[t][i] = mfma32<C>(vv[i], hi[t], st.o[t][i]);
+#pragma unroll
+      for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) st.o[t][i] = mfma32<C>(vv[i], lo[t], st.o[t][i]);
+      __builtin_amdgcn_s_setprio(0);
+      if (b + 2 < NB) {
+        read_v(b + 2);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      page[b] = next[b];
-      next[b] = after[b];
-    }
+    for (int b = 0; b < NB; ++b) page[b] = after[b];
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -743,16 +785,28 @@ __device__ __forceinline__ void write_out(const PrefixArgs& a, const Item& it, c
 
 __device__ __forceinline__ int rounds_of(int keys) { return keys / kRound + (keys % kRound != 0); }
 
-// First and last part of an item of r rounds that begins at u: the workgroups
-// that worked on it, `per` rounds each.
+// How B's rounds are dealt out: `beside` to each workgroup that has pieces of A, `per` to
+// the others.
+struct Deal {
+  int wgs_a, beside, per;
+  __device__ __forceinline__ int64_t first(int w) const {
+    return static_cast<int64_t>(min(w, wgs_a)) * beside + static_cast<int64_t>(max(w - wgs_a, 0)) * per;
+  }
+  __device__ __forceinline__ int of(int u) const {
+    const int64_t a = static_cast<int64_t>(wgs_a) * beside;
+    return u < a ? u / beside : wgs_a + static_cast<int>((u - a) / per);
+  }
+};
+
+// The workgroups that worked on an item of r rounds that begins at u.
 struct Parts {
   int first, count;
   bool inside;  // the first one begins inside its workgroup's range
 };
-__device__ __forceinline__ Parts parts_of(int u, int r, int per) {
-  Parts p{u / per, 0, false};
-  p.count = r == 0 ? 0 : (u + r - 1) / per - p.first + 1;
-  p.inside = u != p.first * per;
+__device__ __forceinline__ Parts parts_of(int u, int r, const Deal& d) {
+  Parts p{d.of(u), 0, false};
+  p.count = r == 0 ? 0 : d.of(u + r - 1) - p.first + 1;
+  p.inside = u != d.first(p.first);
   return p;
 }
 
@@ -840,38 +894,49 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
   scan(a.N, pre_b, [&](int n) { return rounds_of(clamp_len(a, a.lengths[n]) - own_begin(n)); });
   const int HA = a.Hkv * a.RB, HB = a.Hkv * a.GB;
   const int total_b = pre_b[a.N] * HB;
-  int wgs_a = 0, units_a = 0;
+  Deal deal{0, 0, 1};
+  int units_a = 0;
   if constexpr (RW != 0) {
     if (rounds_a > 0) {
-      // a round of 128 keys is four tiles of a workgroup whose waves have rows of their own
-      const int64_t cost = static_cast<int64_t>(rounds_a) * HA * RW;
-      wgs_a = total_b == 0 ? a.wgs : max(1, min(a.wgs - 1, static_cast<int>(a.wgs * cost / (cost + total_b))));
       // The least piece for which the pieces are no more than the workgroups, so that each
       // has one, if all items are not more than that already.
-      int per = max(1, static_cast<int>((static_cast<int64_t>(rounds_a) * HA + wgs_a - 1) / wgs_a));
+      const int64_t all_rounds = static_cast<int64_t>(rounds_a) * HA;
+      const bool fit = static_cast<int64_t>(a.groups) * HA <= a.wgs;
+      int per = static_cast<int>((all_rounds + a.wgs - 1) / a.wgs);
       for (int turn = 0; turn < 16; ++turn) {
         scan(a.groups, units, [&](int g) { return (rounds_of_group(g) + per - 1) / per; });
         const int64_t all = static_cast<int64_t>(units[a.groups]) * HA;
         __syncthreads();
-        if (all <= wgs_a || static_cast<int64_t>(a.groups) * HA > wgs_a) break;
-        per = max(per + 1, static_cast<int>((per * all + wgs_a - 1) / wgs_a));
+        if (all <= a.wgs || !fit) break;
+        per = max(per + 1, static_cast<int>((per * all + a.wgs - 1) / a.wgs));
       }
       units_a = units[a.groups] * HA;
-      wgs_a = min(wgs_a, units_a);
+      deal.wgs_a = min(a.wgs, units_a);
+      // B rounds that take a workgroup as long as its pieces: a round of A is RW tiles
+      // of a wave, one of B a single one
+      const int64_t busy = min(all_rounds * RW / deal.wgs_a, int64_t(1) << 30), rest = a.wgs - deal.wgs_a;
+      if (total_b <= busy * rest) {
+        deal.per = static_cast<int>((total_b + rest - 1) / rest);
+      } else {
+        deal.beside = static_cast<int>((total_b - busy * rest + a.wgs - 1) / a.wgs);
+        deal.per = static_cast<int>(busy) + deal.beside;
+      }
     }
   }
-  const int wgs_b = a.wgs - wgs_a;
-  const int per_b = wgs_b == 0 ? 1 : max(1, (total_b + wgs_b - 1) / wgs_b);
+  if (units_a == 0) deal.per = (total_b + a.wgs - 1) / a.wgs;
+  deal.per = max(deal.per, 1);
   if (blockIdx.x == 0) {  // for the joining kernel
     if (tid == 0) {
-      a.plan[kWgsA] = wgs_a;
-      a.plan[kPerB] = per_b;
+      a.plan[kWgsA] = deal.wgs_a;
+      a.plan[kBeside] = deal.beside;
+      a.plan[kPer] = deal.per;
     }
     if constexpr (RW != 0)
       for (int i = tid; i <= a.groups; i += kThreads) a.plan[kPlan + i] = units_a > 0 ? units[i] : 0;
     for (int i = tid; i <= a.N; i += kThreads) a.plan[kPlan + a.groups + 1 + i] = pre_b[i];
   }
   if constexpr (RW != 0) {
+    const int wgs_a = deal.wgs_a;
     if (static_cast<int>(blockIdx.x) < wgs_a) {
       // Pieces in the order (group, key head, piece, block of rows), each XCD (workgroups go
       // to them in turn) a run of them: the blocks of rows read the same keys from its L2.
@@ -891,11 +956,10 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
         else item_keys<C, KV, HDP, NT, RA, VEC>(a, it, lds, st);
         write_slot<HDP, NT, RA>(a, it, st, a.part + u * a.slot_a, ROWS);
       }
-      return;
     }
   }
-  const int64_t from = static_cast<int64_t>(static_cast<int>(blockIdx.x) - wgs_a) * per_b;
-  const int begin = min(from, static_cast<int64_t>(total_b)), end = min(from + per_b, static_cast<int64_t>(total_b));
+  const int begin = min(deal.first(blockIdx.x), static_cast<int64_t>(total_b));
+  const int end = min(deal.first(blockIdx.x + 1), static_cast<int64_t>(total_b));
   int n = begin < end ? find(pre_b, a.N, begin / HB) : 0;
   for (int u = begin; u < end;) {
     while (pre_b[n + 1] * HB <= u) ++n;
@@ -932,7 +996,7 @@ __global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void prefix_join_k
   if (row >= a.N * a.H) return;  // whole waves; where threads meet, ROWS is 1
   const int n = row / a.H, head = row - n * a.H, h = head / a.G, g = head - h * a.G;
   const int HA = a.Hkv * a.RB, HB = a.Hkv * a.GB;
-  const int wgs_a = a.plan[kWgsA], per_b = a.plan[kPerB];
+  const Deal deal{a.plan[kWgsA], a.plan[kBeside], a.plan[kPer]};
   int pieces = 0, at_a = 0;
   const float* part_a = nullptr;
   if (a.groups != 0) {
@@ -946,7 +1010,7 @@ __global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void prefix_join_k
   }
   const int* pre_b = a.plan + kPlan + a.groups + 1;
   const int gb = g >> 4, at_b = g & 15, hg = h * a.GB + gb, r = pre_b[n + 1] - pre_b[n];
-  const Parts pb = parts_of(pre_b[n] * HB + hg * r, r, per_b);
+  const Parts pb = parts_of(pre_b[n] * HB + hg * r, r, deal);
   if (a.groups == 0 && pb.count == 1) return;
   const float* whole_b = pb.count == 1 ? a.part + a.whole_b + (static_cast<int64_t>(n) * HB + hg) * a.slot_b : nullptr;
   const int parts = pieces + pb.count, r4 = row4(a.hd);
@@ -957,7 +1021,7 @@ __global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void prefix_join_k
     const float* s = is_a ? part_a + static_cast<int64_t>(p) * a.RB * a.slot_a
                      : whole_b ? whole_b
                                : a.part + a.part_b +
-                                     (static_cast<int64_t>(pb.first + i + wgs_a) * 2 + (i == 0 && pb.inside ? 1 : 0)) * a.slot_b;
+                                     (static_cast<int64_t>(pb.first + i) * 2 + (i == 0 && pb.inside ? 1 : 0)) * a.slot_b;
     const int cap = is_a ? rows_a : cap_b(a.G), at = is_a ? at_a : at_b;
     return At{s + at, s + cap + at, s + 2 * cap + at * r4};
   };
