@@ -247,11 +247,22 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream_of)
 _HERE = contextlib.nullcontext()
 
 
+# torch.cuda.current_device() without its check that CUDA is initialised, which it is
+# where there is a tensor on a GPU
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def on_device(t: torch.Tensor):
     """Context with t's device current: nothing to do when it already is,
     which is every launch of a one-GPU process (switching costs ~4 us)."""
     index = t.device.index
-    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _HERE if _current_device() == index else torch.cuda.device(index)
+
+
+def layout(t):
+    """What checks and launch parameters of a call go by: they are made once for
+    equal layouts."""
+    return None if t is None else (t.get_device(), t.dtype, t.shape, t.stride())
 
 
 def require_gpu(name: str, *tensors) -> None:

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -174,11 +175,45 @@ def release_pages(done: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
                   free_count.data_ptr(), N, table.shape[1], int(page_size), *within, _lib.stream(lengths))
 
 
-def _rows_of_slots(name, N, S, slots, rows):
+class _Like(NamedTuple):
+    """A tensor's layout (_lib.layout) with as much of a tensor's face as the checks
+    look at."""
+    index: int
+    dtype: torch.dtype
+    shape: torch.Size
+    strides: tuple
+
+    is_cuda = property(lambda t: t.index >= 0)
+    device = property(lambda t: torch.device("cuda", t.index) if t.index >= 0 else torch.device("cpu"))
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def stride(self, i=None):
+        return self.strides if i is None else self.strides[i]
+
+    def is_contiguous(self):
+        expect = 1
+        for size, stride in zip(reversed(self.shape), reversed(self.strides)):
+            if size != 1 and stride != expect:
+                return 0 in self.shape
+            expect *= size
+        return True
+
+
+def _like(layout):
+    return None if layout is None else _Like(*layout)
+
+
+def _check_rows_of_slots(name, N, S, slots, rows):
     if slots.dtype != torch.int64 or slots.dim() != 2 or slots.shape[1] != S or (rows is None and slots.shape[0] != N):
         raise ValueError(f"{name}: slots must be int64 [{'R' if rows is not None else N}, {S}], got {slots.dtype} "
                          f"{tuple(slots.shape)}")
-    return slots.contiguous(), None if rows is None else _vector(name, "rows", rows, torch.int64, N).contiguous()
+    if rows is not None:
+        _vector(name, "rows", rows, torch.int64, N)
 
 
 def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -194,29 +229,90 @@ def store_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     least power of two that brings it to 448; values are rounded to nearest
     even.  A row with an infinity or NaN gets the scale NaN.  hd up to 256."""
     name = "store_pages"
+    if scales is not None:
+        _store_eight(name, k, v, k_pages, v_pages, slots, rows, scales)
+        return
     _lib.require_gpu(name, k, v, k_pages, v_pages, slots, rows)
     check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
     if k.dim() != 4 or k.shape[1] != K or k.shape[3] != hd or v.shape != k.shape:
         raise ValueError(f"{name}: k and v must be [N, {K}, S, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    scales = check_scales(name, k_pages, scales)
-    if k.dtype != v.dtype or (scales is None and k.dtype != k_pages.dtype):
+    check_scales(name, k_pages, None, None)
+    if not k.dtype == v.dtype == k_pages.dtype:
         raise ValueError(f"{name}: k, v and the pages must share a dtype")
     check_no_gradient(name, k, v, k_pages, v_pages)
     N, S = k.shape[0], k.shape[2]
-    slots, rows = _rows_of_slots(name, N, S, slots, rows)
+    _check_rows_of_slots(name, N, S, slots, rows)
     k, v = (t if t.stride(-1) == 1 or hd == 1 else t.contiguous() for t in (k, v))
+    slots, rows = slots.contiguous(), None if rows is None else rows.contiguous()
     with _lib.on_device(k):
-        if scales is not None:
-            ks, vs = scales
-            _lib.call("hydra_page_store8", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                      ks.data_ptr(), vs.data_ptr(), slots.data_ptr(), slots.shape[0], _lib.ptr(rows), N, K, S, hd,
-                      pages, page, _strides(k), _strides(v), _strides(k_pages), _strides(v_pages), _strides(ks),
-                      _strides(vs), _lib.dtype_code(k), _lib.PAGE_CODE[k_pages.dtype], _lib.stream(k))
-            return
         _lib.call("hydra_page_store", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                   slots.data_ptr(), slots.shape[0], _lib.ptr(rows), N, K, S, hd, pages, page, _strides(k), _strides(v),
                   _strides(k_pages), _strides(v_pages), _lib.dtype_code(k), _lib.stream(k))
+
+
+@functools.lru_cache(maxsize=1024)
+def _store_eight_call(name, *layouts):
+    """The checks of a call of these layouts, once; what it is launched with beside
+    addresses."""
+    k, v, kp, vp, slots, rows, ks, vs = map(_like, layouts)
+    _lib.require_gpu(name, k, v, kp, vp, slots, rows)
+    check_pages(name, kp, vp)
+    pages, K, page, hd = kp.shape
+    if k.dim() != 4 or k.shape[1] != K or k.shape[3] != hd or v.shape != k.shape:
+        raise ValueError(f"{name}: k and v must be [N, {K}, S, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    check_scales(name, kp, ks, vs)
+    if k.dtype != v.dtype:
+        raise ValueError(f"{name}: k and v must share a dtype")
+    N, S = k.shape[0], k.shape[2]
+    _check_rows_of_slots(name, N, S, slots, rows)
+    copies = (hd > 1 and (k.stride(-1) != 1 or v.stride(-1) != 1)) or not slots.is_contiguous() or \
+        not (rows is None or rows.is_contiguous())
+    return (copies, slots.shape[0], (N, K, S, hd, pages, page, *map(_strides, (k, v, kp, vp, ks, vs)), _lib.dtype_code(k),
+                                     _lib.PAGE_CODE[kp.dtype]), _lib.load().hydra_page_store8)
+
+
+def _store_eight(name, k, v, k_pages, v_pages, slots, rows, scales):
+    ks, vs = scales
+    layout = _lib.layout
+    copies, R, sizes, entry = _store_eight_call(name, layout(k), layout(v), layout(k_pages), layout(v_pages), layout(slots),
+                                                layout(rows), layout(ks), layout(vs))
+    check_no_gradient(name, k, v, k_pages, v_pages)
+    if copies:
+        _store_eight(name, k.contiguous(), v.contiguous(), k_pages, v_pages, slots.contiguous(),
+                     None if rows is None else rows.contiguous(), scales)
+        return
+    with _lib.on_device(k):
+        rc = entry(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+                   slots.data_ptr(), R, None if rows is None else rows.data_ptr(), *sizes, _lib.stream(k))
+    _lib.check(rc, "hydra_page_store8")
+
+
+@functools.lru_cache(maxsize=1024)
+def _read_call(name, dtype, *layouts):
+    """As _store_eight_call."""
+    kp, vp, slots, rows, ks, vs = map(_like, layouts)
+    _lib.require_gpu(name, kp, vp, slots, rows)
+    check_pages(name, kp, vp)
+    pages, K, page, hd = kp.shape
+    check_scales(name, kp, ks, vs)
+    if ks is None:
+        if dtype not in (None, kp.dtype):
+            raise ValueError(f"{name}: pages of {str(kp.dtype)[6:]} are read as they are, not as {str(dtype)[6:]}")
+        dtype = kp.dtype
+    elif dtype is None:
+        raise ValueError(f"{name}: say which dtype (pages of {str(kp.dtype)[6:]})")
+    if slots.dim() != 2 or (rows is not None and rows.dim() != 1):
+        raise ValueError(f"{name}: slots must be int64 [N, S], got {slots.dtype} {tuple(slots.shape)}")
+    N, S = (slots if rows is None else rows).shape[0], slots.shape[1]
+    _check_rows_of_slots(name, N, S, slots, rows)
+    shape = (N, K, S, hd)
+    out = _Like(0, dtype, torch.Size(shape), (K * S * hd, S * hd, hd, 1))
+    code = _lib.dtype_code(out)
+    return (dtype, (2, *shape), (*shape, pages, page, _strides(kp), _strides(vp),
+                                 *((None, None) if ks is None else (_strides(ks), _strides(vs))), _strides(out),
+                                 _strides(out), code, code if ks is None else _lib.PAGE_CODE[kp.dtype]),
+            _lib.load().hydra_page_read)
 
 
 def read_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor,
@@ -228,58 +324,36 @@ def read_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor
     `dtype` wanted (bf16, fp16 or fp32; each value is rounded once); others
     are read as they are.  hd up to 256.  Inference only: no gradient."""
     name = "read_pages"
-    _lib.require_gpu(name, k_pages, v_pages, slots, rows)
-    check_pages(name, k_pages, v_pages)
-    pages, K, page, hd = k_pages.shape
-    scales = check_scales(name, k_pages, scales)
-    if scales is None:
-        if dtype not in (None, k_pages.dtype):
-            raise ValueError(f"{name}: pages of {str(k_pages.dtype)[6:]} are read as they are, not as {str(dtype)[6:]}")
-        dtype = k_pages.dtype
-    elif dtype is None:
-        raise ValueError(f"{name}: say which dtype (pages of {str(k_pages.dtype)[6:]})")
+    ks, vs = (None, None) if scales is None else scales
+    layout = _lib.layout
+    dtype, shape, sizes, entry = _read_call(name, dtype, layout(k_pages), layout(v_pages), layout(slots), layout(rows),
+                                            layout(ks), layout(vs))
     check_no_gradient(name, k_pages, v_pages)
-    if slots.dim() != 2:
-        raise ValueError(f"{name}: slots must be int64 [N, S], got {slots.dtype} {tuple(slots.shape)}")
-    N, S = (slots if rows is None else rows).shape[0], slots.shape[1]
-    slots, rows = _rows_of_slots(name, N, S, slots, rows)
-    k, v = (torch.empty((N, K, S, hd), dtype=dtype, device=k_pages.device) for _ in range(2))
-    code = _lib.dtype_code(k)
-    ks, vs = scales or (None, None)
+    slots, rows = slots.contiguous(), None if rows is None else rows.contiguous()
+    out = torch.empty(shape, dtype=dtype, device=k_pages.device)
+    k, v = out.unbind(0)
     with _lib.on_device(k):
-        _lib.call("hydra_page_read", k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks), _lib.ptr(vs), k.data_ptr(),
-                  v.data_ptr(), slots.data_ptr(), slots.shape[0], _lib.ptr(rows), N, K, S, hd, pages, page,
-                  _strides(k_pages), _strides(v_pages), None if ks is None else _strides(ks),
-                  None if vs is None else _strides(vs), _strides(k), _strides(v), code,
-                  code if scales is None else _lib.PAGE_CODE[k_pages.dtype], _lib.stream(k))
+        rc = entry(k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks), _lib.ptr(vs), k.data_ptr(), v.data_ptr(),
+                   slots.data_ptr(), slots.shape[0], _lib.ptr(rows), *sizes, _lib.stream(k))
+    _lib.check(rc, "hydra_page_read")
     return k, v
 
 
-def check_scales(name: str, pages: torch.Tensor, scales):
-    """(k_scales, v_scales) of pages of 8 bits; None for others, which have none."""
+def check_scales(name: str, pages, k_scales, v_scales) -> None:
+    """Scales go with pages of 8 bits, and with no others."""
     eight = pages.dtype in _lib.PAGE_CODE
-    if scales is None:
+    if k_scales is None or v_scales is None:
         if eight:
             raise ValueError(f"{name}: pages of {str(pages.dtype)[6:]} need scales")
-        return None
-    k, v = scales
+        return
     if not eight:
         raise ValueError(f"{name}: scales are of pages of 8 bits, these are {str(pages.dtype)[6:]}")
-    _lib.require_gpu(name, pages, k, v)
-    for t in (k, v):
+    _lib.require_gpu(name, pages, k_scales, v_scales)
+    for t in (k_scales, v_scales):
         if t.dtype != torch.float32 or t.shape != pages.shape[:3]:
             raise ValueError(f"{name}: scales must be float32 {list(pages.shape[:3])}, got {t.dtype} {tuple(t.shape)}")
         if not t.is_contiguous():
             check_distinct(name, "scales", t)
-    return k, v
-
-
-@functools.lru_cache(maxsize=1024)
-def _prefix_workspace(device: int, *sizes) -> int:
-    """Scratch bytes of these sizes on a device, which is current."""
-    need = ctypes.c_int64(0)
-    _lib.call("hydra_prefix_attn_workspace", *sizes, ctypes.byref(need))
-    return need.value
 
 
 @functools.lru_cache(maxsize=1024)
@@ -312,7 +386,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     request that sees none (or whose scores are all -inf) gets zeros.  Inference
     only: no gradient."""
     name = "paged_attention"
-    _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out, shared)
+    if scales is not None or shared is not None:
+        return _prefix_attention(name, q, k_pages, v_pages, table, lengths, scale, out, scales, shared)
+    _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out)
     check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
     if q.dim() != 3 or q.shape[2] != hd:
@@ -320,8 +396,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     N, H, _ = q.shape
     if H == 0 or H % K != 0:
         raise ValueError(f"{name}: {H} query heads are no multiple of {K} key heads")
-    scales = check_scales(name, k_pages, scales)
-    if scales is None and q.dtype != k_pages.dtype:
+    check_scales(name, k_pages, None, None)
+    if q.dtype != k_pages.dtype:
         raise ValueError(f"{name}: q and the pages must share a dtype")
     check_no_gradient(name, q, k_pages, v_pages, out)
     _vector(name, "lengths", lengths, torch.int32, N)
@@ -338,7 +414,42 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         check_distinct(name, "rows of out", out)
     lengths = lengths.contiguous()
     P, code = table.shape[1], _lib.dtype_code(q)
-    scale = hd ** -0.5 if scale is None else float(scale)
+    with _lib.on_device(q):
+        need = _attention_workspace(q.device.index, N, H, K, hd, P, page, code)
+        ws = _lib.scratch(need, q) if need else None
+        _lib.call("hydra_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
+                  table.data_ptr(), _row_stride(table), lengths.data_ptr(), N, H, K, hd, P, page, pages, _strides(q),
+                  _strides(k_pages), _strides(v_pages), _strides(out), hd ** -0.5 if scale is None else float(scale),
+                  code, _lib.ptr(ws), need, _lib.stream(q))
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefix_call(name, scale, *layouts):
+    """The checks of a call of these layouts, once; what it is launched with beside
+    addresses, and the bytes of scratch.  On the tensors' device, which is current."""
+    q, kp, vp, table, lengths, out, ks, vs, shared = map(_like, layouts)
+    _lib.require_gpu(name, q, kp, vp, table, lengths, out, shared)
+    check_pages(name, kp, vp)
+    pages, K, page, hd = kp.shape
+    if q.dim() != 3 or q.shape[2] != hd:
+        raise ValueError(f"{name}: q must be [N, Hq, {hd}], got {tuple(q.shape)}")
+    N, H, _ = q.shape
+    if H == 0 or H % K != 0:
+        raise ValueError(f"{name}: {H} query heads are no multiple of {K} key heads")
+    check_scales(name, kp, ks, vs)
+    if ks is None and q.dtype != kp.dtype:
+        raise ValueError(f"{name}: q and the pages must share a dtype")
+    _vector(name, "lengths", lengths, torch.int32, N)
+    _check_table(name, table, N)
+    if table.shape[1] == 0:
+        raise ValueError(f"{name}: a table without pages")
+    if out is None:
+        out = q._replace(strides=(H * hd, hd, 1))
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"{name}: out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+    elif not out.is_contiguous():
+        check_distinct(name, "rows of out", out)
     groups = 0
     if shared is not None:
         groups = _vector(name, "shared", shared, torch.int32).shape[0]
@@ -346,26 +457,42 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             raise ValueError(f"{name}: {N} requests are no multiple of {groups} groups")
         if groups == N:  # nobody shares anything
             groups = 0
-        shared = shared.contiguous()
+    P, code = table.shape[1], _lib.dtype_code(q)
+    copies = (hd > 1 and q.stride(-1) != 1) or not lengths.is_contiguous() or not (shared is None or shared.is_contiguous())
+    if groups == 0 and ks is None:
+        return copies, None, 0, 0, None, None
+    of = code if ks is None else _lib.PAGE_CODE[kp.dtype]
+    need = ctypes.c_int64(0)
+    _lib.call("hydra_prefix_attn_workspace", groups, N, H, K, hd, P, page, code, of, ctypes.byref(need))
+    return (copies, (groups, N, H, K, hd, P, page, pages, _strides(q), _strides(kp), _strides(vp),
+                     *((None, None) if ks is None else (_strides(ks), _strides(vs))), _strides(out),
+                     hd ** -0.5 if scale is None else float(scale), code, of), groups, need.value, _row_stride(table),
+            _lib.load().hydra_prefix_attn)
+
+
+def _prefix_attention(name, q, k_pages, v_pages, table, lengths, scale, out, scales, shared):
+    """paged_attention with scales, groups or both."""
+    ks, vs = (None, None) if scales is None else scales
+    layout = _lib.layout
+    _lib.require_gpu(name, q)
     with _lib.on_device(q):
-        if groups or scales is not None:
-            of = code if scales is None else _lib.PAGE_CODE[k_pages.dtype]
-            ks, vs = scales or (None, None)
-            need = _prefix_workspace(q.device.index, groups, N, H, K, hd, P, page, code, of)
-            ws = _lib.scratch(need, q) if need else None
-            _lib.call("hydra_prefix_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks),
-                      _lib.ptr(vs), out.data_ptr(), table.data_ptr(), _row_stride(table), lengths.data_ptr(),
-                      shared.data_ptr() if groups else None, groups, N, H, K, hd, P, page, pages, _strides(q),
-                      _strides(k_pages), _strides(v_pages), None if ks is None else _strides(ks),
-                      None if vs is None else _strides(vs), _strides(out), scale, code, of, _lib.ptr(ws), need,
-                      _lib.stream(q))
-            return out
-        need = _attention_workspace(q.device.index, N, H, K, hd, P, page, code)
+        copies, sizes, groups, need, table_rs, entry = _prefix_call(
+            name, scale, layout(q), layout(k_pages), layout(v_pages), layout(table), layout(lengths), layout(out),
+            layout(ks), layout(vs), layout(shared))
+        check_no_gradient(name, q, k_pages, v_pages, out)
+        if copies:
+            return _prefix_attention(name, q.contiguous(), k_pages, v_pages, table, lengths.contiguous(), scale, out, scales,
+                                     None if shared is None else shared.contiguous())
+        if sizes is None:
+            return paged_attention(q, k_pages, v_pages, table, lengths, scale, out)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         ws = _lib.scratch(need, q) if need else None
-        _lib.call("hydra_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
-                  table.data_ptr(), _row_stride(table), lengths.data_ptr(), N, H, K, hd, P, page, pages, _strides(q),
-                  _strides(k_pages), _strides(v_pages), _strides(out), scale,
-                  code, _lib.ptr(ws), need, _lib.stream(q))
+        rc = entry(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), None if ks is None else ks.data_ptr(),
+                   None if vs is None else vs.data_ptr(), out.data_ptr(), table.data_ptr(), table_rs, lengths.data_ptr(),
+                   shared.data_ptr() if groups else None, *sizes, None if ws is None else ws.data_ptr(), need,
+                   _lib.stream(q))
+    _lib.check(rc, "hydra_prefix_attn")
     return out
 
 
@@ -380,10 +507,26 @@ class PageFork(NamedTuple):
 
 
 @functools.lru_cache(maxsize=1024)
-def _fork_workspace(*sizes) -> int:
+def _fork_call(name, *layouts):
+    """The checks of a call of these layouts, once; what it is launched with beside
+    addresses."""
+    parents, lengths, table, free_pages, free_count, extra = map(_like, layouts)
+    _lib.require_gpu(name, parents, lengths, table, free_pages, free_count, extra)
+    N = _vector(name, "lengths", lengths, torch.int32).shape[0]
+    _vector(name, "parents", parents, torch.int32, N)
+    _vector(name, "free_pages", free_pages, torch.int32)
+    _vector(name, "free_count", free_count, torch.int32, 1)
+    pages = _vector(name, "extra", extra, torch.int32).shape[0]
+    _check_table(name, table, N)
+    P = table.shape[1]
+    if N == 0 or P == 0 or pages == 0:
+        raise ValueError(f"{name}: {N} rows of {P} pages in a pool of {pages}")
+    _in_place(name, "lengths", lengths)
+    _in_place(name, "free_pages", free_pages)
+    _in_place(name, "extra", extra)
     need = ctypes.c_int64(0)
-    _lib.call("hydra_page_fork_workspace", *sizes, ctypes.byref(need))
-    return need.value
+    _lib.call("hydra_page_fork_workspace", N, P, pages, ctypes.byref(need))
+    return N, P, pages, need.value, _row_stride(table), free_pages.numel(), _lib.load().hydra_page_fork
 
 
 def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
@@ -401,30 +544,35 @@ def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     holds nothing: where every row's last page is begun and each goes on from one
     of them, there are always enough.  At most 8192 rows."""
     name = "fork_pages"
-    _lib.require_gpu(name, parents, lengths, table, free_pages, free_count, extra)
-    N = _vector(name, "lengths", lengths, torch.int32).shape[0]
-    _vector(name, "parents", parents, torch.int32, N)
-    _vector(name, "free_pages", free_pages, torch.int32)
-    _vector(name, "free_count", free_count, torch.int32, 1)
-    pages = _vector(name, "extra", extra, torch.int32).shape[0]
-    _check_table(name, table, N)
-    if N == 0 or table.shape[1] == 0 or pages == 0:
-        raise ValueError(f"{name}: {N} rows of {table.shape[1]} pages in a pool of {pages}")
-    _in_place(name, "lengths", lengths)
-    _in_place(name, "free_pages", free_pages)
-    _in_place(name, "extra", extra)
+    layout = _lib.layout
+    N, P, pages, need, table_rs, stack, entry = _fork_call(name, layout(parents), layout(lengths), layout(table), layout(free_pages),
+                                                    layout(free_count), layout(extra))
     parents = parents.contiguous()
     sources, copies, taken = lengths.new_empty((3, N)).unbind(0)
     granted = lengths.new_empty((N,), dtype=torch.bool)
-    P = table.shape[1]
-    need = _fork_workspace(N, P, pages)
     ws = _lib.scratch(need, lengths)
     with _lib.on_device(lengths):
-        _lib.call("hydra_page_fork", parents.data_ptr(), lengths.data_ptr(), table.data_ptr(), _row_stride(table),
-                  free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), extra.data_ptr(),
-                  sources.data_ptr(), copies.data_ptr(), taken.data_ptr(), granted.data_ptr(), N, P, int(page_size),
-                  pages, ws.data_ptr(), need, _lib.stream(lengths))
+        rc = entry(parents.data_ptr(), lengths.data_ptr(), table.data_ptr(), table_rs, free_pages.data_ptr(), stack,
+                   free_count.data_ptr(), extra.data_ptr(), sources.data_ptr(), copies.data_ptr(), taken.data_ptr(),
+                   granted.data_ptr(), N, P, int(page_size), pages, ws.data_ptr(), need, _lib.stream(lengths))
+    _lib.check(rc, "hydra_page_fork")
     return PageFork(taken, sources, copies, granted)
+
+
+@functools.lru_cache(maxsize=1024)
+def _copy_call(name, *layouts):
+    """As _fork_call."""
+    kp, vp, sources, copies, ks, vs = map(_like, layouts)
+    _lib.require_gpu(name, kp, vp, sources, copies)
+    check_pages(name, kp, vp)
+    pages, K, page, hd = kp.shape
+    N = _vector(name, "sources", sources, torch.int32).shape[0]
+    _vector(name, "copies", copies, torch.int32, N)
+    check_scales(name, kp, ks, vs)
+    if ks is None:
+        _lib.dtype_code(kp)
+    return ((N, K, hd, pages, page, _strides(kp), _strides(vp),
+             *((None, None) if ks is None else (_strides(ks), _strides(vs))), kp.dtype.itemsize), _lib.load().hydra_page_copy)
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, sources: torch.Tensor, copies: torch.Tensor,
@@ -433,22 +581,33 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, sources: torch.Tens
     values and `scales`.  Pairs with a page outside the pool are left out; copies
     are distinct and none is a source.  Inference only: no gradient."""
     name = "copy_pages"
-    _lib.require_gpu(name, k_pages, v_pages, sources, copies)
-    check_pages(name, k_pages, v_pages)
-    pages, K, page, hd = k_pages.shape
-    N = _vector(name, "sources", sources, torch.int32).shape[0]
-    _vector(name, "copies", copies, torch.int32, N)
-    scales = check_scales(name, k_pages, scales)
-    if scales is None:
-        _lib.dtype_code(k_pages)
+    ks, vs = (None, None) if scales is None else scales
+    layout = _lib.layout
+    sizes, entry = _copy_call(name, layout(k_pages), layout(v_pages), layout(sources), layout(copies), layout(ks), layout(vs))
     check_no_gradient(name, k_pages, v_pages)
-    ks, vs = scales or (None, None)
     sources, copies = sources.contiguous(), copies.contiguous()
     with _lib.on_device(k_pages):
-        _lib.call("hydra_page_copy", k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks), _lib.ptr(vs),
-                  sources.data_ptr(), copies.data_ptr(), N, K, hd, pages, page, _strides(k_pages), _strides(v_pages),
-                  None if ks is None else _strides(ks), None if vs is None else _strides(vs), k_pages.element_size(),
-                  _lib.stream(k_pages))
+        rc = entry(k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks), _lib.ptr(vs), sources.data_ptr(),
+                   copies.data_ptr(), *sizes, _lib.stream(k_pages))
+    _lib.check(rc, "hydra_page_copy")
+
+
+@functools.lru_cache(maxsize=1024)
+def _take_call(name, *layouts):
+    """As _fork_call."""
+    x, parents = map(_like, layouts)
+    _lib.require_gpu(name, x, parents)
+    if x.dim() == 0:
+        raise ValueError(f"{name}: x must have rows")
+    N = x.shape[0]
+    _vector(name, "parents", parents, torch.int32, N)
+    if x.numel() == 0:
+        return 0, 0, 0, None
+    row, e = x.numel() // N, x.dtype.itemsize
+    inner = x._replace(shape=x.shape[1:], strides=x.strides[1:])
+    if not inner.is_contiguous() or (N > 1 and x.stride(0) < row):
+        raise ValueError(f"{name}: rows of strides {x.stride()} are not contiguous")
+    return (x.stride(0) if N > 1 else row) * e, row * e, N, _lib.load().hydra_rows_take
 
 
 def take_rows(x: torch.Tensor, parents: torch.Tensor) -> None:
@@ -456,22 +615,14 @@ def take_rows(x: torch.Tensor, parents: torch.Tensor) -> None:
     up to 8192); a parent outside [0, N) leaves its row as it is.  Any dtype; rows
     are contiguous and do not overlap.  Inference only: no gradient."""
     name = "take_rows"
-    _lib.require_gpu(name, x, parents)
-    if x.dim() == 0:
-        raise ValueError(f"{name}: x must have rows")
-    N = x.shape[0]
-    _vector(name, "parents", parents, torch.int32, N)
+    stride, row, N, entry = _take_call(name, _lib.layout(x), _lib.layout(parents))
     check_no_gradient(name, x)
-    if N == 0 or x.numel() == 0:
+    if N == 0:
         return
-    row = x.numel() // N
-    if not x[0].is_contiguous() or (N > 1 and x.stride(0) < row):
-        raise ValueError(f"{name}: rows of strides {x.stride()} are not contiguous")
-    e = x.element_size()
     parents = parents.contiguous()
     with _lib.on_device(x):
-        _lib.call("hydra_rows_take", x.data_ptr(), (x.stride(0) if N > 1 else row) * e, row * e, parents.data_ptr(), N,
-                  _lib.stream(x))
+        rc = entry(x.data_ptr(), stride, row, parents.data_ptr(), N, _lib.stream(x))
+    _lib.check(rc, "hydra_rows_take")
 
 
 class PagePool:
