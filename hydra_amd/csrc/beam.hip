@@ -48,96 +48,134 @@ __device__ __forceinline__ Key2 shuffled(const Key2& k, int off) {
 }
 
 template <typename Key> struct Lists {
-  Key list[2][kCap];
-  Key part[kThreads / 64];
-  int count[2];
+  Key list[kCap];
+  Key part[kThreads];
+  int count;
 };
 
 // The least of the maxima of n' >= n groups of threads (all 256 take part): at
-// least n elements reach it, if there are as many as groups.
+// least n elements reach it, if there are as many as groups.  Thread t is in group t mod
+// n': neighbours hold neighbouring elements, of one beam or one end of a row, and groups
+// of such would be of very different size.
 template <typename Key>
 __device__ __forceinline__ Key bound_of(Key mine, int n, Key* part) {
-  int size = 64;  // of a group
-  while (size > 1 && kThreads / size < n) size >>= 1;
-  for (int off = 1; off < size; off <<= 1) {
+  int groups = 1;
+  while (groups < n) groups <<= 1;
+  const int tid = threadIdx.x, lane = tid & 63;
+  for (int off = 32; off >= groups; off >>= 1) {
     const Key o = shuffled(mine, off);
     if (better(o, mine)) mine = o;
   }
-  for (int off = size; off < 64; off <<= 1) {
+  __syncthreads();  // the last use of `part` is over
+  part[tid] = mine;
+  __syncthreads();
+  const int step = groups < 64 ? 64 : groups;  // threads of one group in other waves
+  for (int o = (tid + step) & (kThreads - 1); o != tid; o = (o + step) & (kThreads - 1))
+    if (better(part[o], mine)) mine = part[o];
+  for (int off = 1; off < groups && off < 64; off <<= 1) {
     const Key o = shuffled(mine, off);
     if (better(mine, o)) mine = o;
   }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mine;
-  __syncthreads();
-  for (int w = 0; w < kThreads / 64; ++w)
-    if (better(mine, part[w])) mine = part[w];
+  if (groups > 64) {  // 128: two waves' groups
+    __syncthreads();
+    if (lane == 0) part[tid >> 6] = mine;
+    __syncthreads();
+    if (better(mine, part[(tid >> 6) ^ 1])) mine = part[(tid >> 6) ^ 1];
+  }
   return mine;
 }
 
-// The n best of the elements that each thread's `each` goes over, best first, to
-// put(rank, key); `best` is the thread's own best.  Ranks without an element get none.
-template <typename Key, typename Each, typename Put>
-__device__ __forceinline__ void top_n(int n, const Key& best, Lists<Key>& L, Each&& each, Put&& put) {
+// A place in the list for each lane with `in`: one count for the wave.
+__device__ __forceinline__ int place(bool in, int* count) {
+  const uint64_t who = __ballot(in);
+  if (who == 0) return 0;
+  int base = 0;
+  if ((threadIdx.x & 63) == __ffsll(static_cast<unsigned long long>(who)) - 1) base = atomicAdd(count, __popcll(who));
+  base = __shfl(base, __ffsll(static_cast<unsigned long long>(who)) - 1);
+  return base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
+}
+
+// The n best of the list's c elements, best first, to put(rank, key); ranks without an
+// element get none.
+template <typename Key, typename Put>
+__device__ __forceinline__ void ranked(int n, int c, Lists<Key>& L, Put&& put) {
+  constexpr int U = kCap / kThreads;
   const int tid = threadIdx.x;
-  const Key none{};
-  const Key bound = bound_of(best, n, L.part);
-  if (tid == 0) L.count[0] = 0;
+  // many: those that reach a bound of the list's own elements move to its front
+  for (int i = 0; i < 4 && c > 128 && c > 2 * n; ++i) {
+    Key mine[U], k{};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      mine[u] = Key{};
+      if (u * kThreads + tid < c) mine[u] = L.list[u * kThreads + tid];
+      if (better(mine[u], k)) k = mine[u];
+    }
+    if (tid == 0) L.count = 0;
+    const Key tight = bound_of(k, n, L.part);  // everybody has read
+    const int trips = (c + kThreads - 1) / kThreads;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u >= trips) continue;
+      const bool in = mine[u].a != 0 && !better(tight, mine[u]);
+      const int at = place(in, &L.count);
+      if (in) L.list[at] = mine[u];
+    }
+    __syncthreads();
+    c = L.count;
+    __syncthreads();
+  }
+  // four lanes to an element, a quarter of the list each
+  const int q = tid & 3, i0 = c * q / 4, i1 = c * (q + 1) / 4;
+  for (int j0 = 0; j0 < c; j0 += kThreads / 4) {
+    const int j = j0 + (tid >> 2);
+    const Key k = L.list[min(j, c - 1)];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) rank += better(L.list[i], k);
+    rank += __shfl_xor(rank, 1);
+    rank += __shfl_xor(rank, 2);
+    if (q == 0 && j < c && k.a != 0 && rank < n) put(rank, k);
+  }
+  for (int j = c + tid; j < n; j += kThreads) put(j, Key{});
+}
+
+// The n best of the elements that each thread's `each` goes over, one after the other: the
+// best below the last.
+template <typename Key, typename Each, typename Put>
+__device__ __forceinline__ void one_by_one(int n, Lists<Key>& L, Each&& each, Put&& put) {
+  Key last{};
+  for (int i = 0; i < n; ++i) {
+    Key k{};
+    each([&](const Key& x) {
+      if ((i == 0 || better(last, x)) && better(x, k)) k = x;
+    });
+    for (int off = 1; off < 64; off <<= 1) {
+      const Key o = shuffled(k, off);
+      if (better(o, k)) k = o;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) L.part[threadIdx.x >> 6] = k;
+    __syncthreads();
+    for (int w = 0; w < kThreads / 64; ++w)
+      if (better(L.part[w], k)) k = L.part[w];
+    if (threadIdx.x == 0) put(i, k);
+    last = k;
+  }
+}
+
+// Those of all elements that reach `bound`, which at least n do, into the list; their
+// number, which may be more than the list holds.
+template <typename Key, typename Each>
+__device__ __forceinline__ int collected(const Key& bound, Lists<Key>& L, Each&& each) {
+  if (threadIdx.x == 0) L.count = 0;
   __syncthreads();
   each([&](const Key& k) {
     if (k.a == 0 || better(bound, k)) return;
-    const int at = atomicAdd(&L.count[0], 1);
-    if (at < kCap) L.list[0][at] = k;
+    const int at = atomicAdd(&L.count, 1);
+    if (at < kCap) L.list[at] = k;
   });
   __syncthreads();
-  int c = L.count[0];
-  if (c > kCap) {  // one after the other: the best below the last
-    Key last = none;
-    for (int i = 0; i < n; ++i) {
-      Key k = none;
-      each([&](const Key& x) {
-        if ((i == 0 || better(last, x)) && better(x, k)) k = x;
-      });
-      for (int off = 1; off < 64; off <<= 1) {
-        const Key o = shuffled(k, off);
-        if (better(o, k)) k = o;
-      }
-      __syncthreads();
-      if ((tid & 63) == 0) L.part[tid >> 6] = k;
-      __syncthreads();
-      for (int w = 0; w < kThreads / 64; ++w)
-        if (better(L.part[w], k)) k = L.part[w];
-      if (tid == 0) put(i, k);
-      last = k;
-    }
-    return;
-  }
-  Key *from = L.list[0], *to = L.list[1];
-  int turn = 0;
-  // many: a tighter bound, of the list's own elements
-  for (int i = 0; i < 4 && c > kThreads && c > 4 * n; ++i) {
-    Key k = none;
-    for (int j = tid; j < c; j += kThreads)
-      if (better(from[j], k)) k = from[j];
-    const Key tight = bound_of(k, n, L.part);
-    turn ^= 1;
-    if (tid == 0) L.count[turn] = 0;
-    __syncthreads();
-    for (int j = tid; j < c; j += kThreads)
-      if (!better(tight, from[j])) to[atomicAdd(&L.count[turn], 1)] = from[j];
-    __syncthreads();
-    c = L.count[turn];
-    Key* const x = from;
-    from = to;
-    to = x;
-  }
-  for (int j = tid; j < c; j += kThreads) {
-    const Key k = from[j];
-    int rank = 0;
-    for (int i = 0; i < c; ++i) rank += better(from[i], k);
-    if (rank < n) put(rank, k);
-  }
-  for (int j = c + tid; j < n; j += kThreads) put(j, none);
+  return L.count;
 }
 
 // A chunk's results: maximum, sum of e^(x - maximum), and pairs (key of the value, ~index).
@@ -153,6 +191,10 @@ struct BeamArgs {
   int B, W, V, n, chunks;
   int first;          // row (text) of the launch's first workgroup
 };
+
+__device__ __forceinline__ Key1 key_of(float v, int i) {
+  return Key1{(static_cast<uint64_t>(score_key_asc(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(i))};
+}
 
 template <typename T, int E>
 __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(BeamArgs a) {
@@ -178,10 +220,11 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(BeamArgs a) {
 #pragma unroll
     for (int e = 0; e < N; ++e) top = fmaxf(top, v[j * N + e]);
   }
+  const float mine = top;
   top = wave_max(top);
   if (lane == 0) red[wave] = top;
   __syncthreads();
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, red[w]);
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float ts = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
@@ -201,18 +244,53 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(BeamArgs a) {
       const int i = c0 + (j * kThreads + tid) * N - off;
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (i + e >= 0 && i + e < a.V)
-          f(Key1{(static_cast<uint64_t>(score_key_asc(v[j * N + e])) << 32) | (0xffffffffu - static_cast<uint32_t>(i + e))});
+        if (i + e >= 0 && i + e < a.V) f(key_of(v[j * N + e], i + e));
     }
   };
+  uint2* out = a.pairs + at * a.n;
+  auto put = [&](int rank, const Key1& k) {
+    out[rank] = make_uint2(static_cast<uint32_t>(k.a >> 32), static_cast<uint32_t>(k.a));
+  };
+  // By the values alone first, which is a comparison for each element.  (A NaN is below
+  // everything here: its row counts as NaN throughout.)
+  float bound = mine;
+  {
+    int size = 64;
+    while (size > 1 && kThreads / size < a.n) size >>= 1;
+    for (int o = 1; o < size; o <<= 1) bound = fmaxf(bound, __shfl_xor(bound, o));
+    for (int o = size; o < 64; o <<= 1) bound = fminf(bound, __shfl_xor(bound, o));
+    __syncthreads();  // red is read
+    if (lane == 0) red[wave] = bound;
+    if (tid == 0) lists.count = 0;
+    __syncthreads();
+    bound = fminf(fminf(red[0], red[1]), fminf(red[2], red[3]));
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int i = c0 + (j * kThreads + tid) * N - off;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (v[j * N + e] >= bound) {  // few; what lies outside the row is -inf
+        if (i + e >= 0 && i + e < a.V) {
+          const int to = atomicAdd(&lists.count, 1);
+          if (to < kCap) lists.list[to] = key_of(v[j * N + e], i + e);
+        }
+      }
+  }
+  __syncthreads();
+  int c = lists.count;
+  if (c <= kCap) {
+    ranked(a.n, c, lists, put);
+    return;
+  }
+  // more equal ones than the list holds (masked rows): by value and index
   Key1 best{0};
   each([&](const Key1& k) {
     if (better(k, best)) best = k;
   });
-  uint2* out = a.pairs + at * a.n;
-  top_n(a.n, best, lists, each, [&](int rank, const Key1& k) {
-    out[rank] = make_uint2(static_cast<uint32_t>(k.a >> 32), static_cast<uint32_t>(k.a));
-  });
+  c = collected(bound_of(best, a.n, lists.part), lists, each);
+  if (c <= kCap) ranked(a.n, c, lists, put);
+  else one_by_one(a.n, lists, each, put);
 }
 
 __device__ __forceinline__ uint64_t double_key(double v) {  // ascending; NaN above all, -0 as 0
@@ -233,22 +311,25 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   // x - top first: a row whose tokens are all masked by the type's lowest value is even
   __shared__ double shift[kMaxBeams];  // score - ln sum e^(x - top)
   __shared__ float tops[kMaxBeams];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = a.first + blockIdx.x;
-  for (int w = wave; w < a.W; w += kThreads / 64) {
-    const float* st = a.stats + 2 * (static_cast<int64_t>(b) * a.W + w) * a.chunks;
+  const int tid = threadIdx.x, b = a.first + blockIdx.x;
+  // as many lanes to a row as it has chunks
+  int lanes = 1;
+  while (lanes < 64 && lanes < a.chunks) lanes *= 2;
+  const int sub = tid & (lanes - 1);
+  for (int w0 = 0; w0 < a.W; w0 += kThreads / lanes) {
+    const int w = min(w0 + tid / lanes, a.W - 1);
+    const float2* st = reinterpret_cast<const float2*>(a.stats) + (static_cast<int64_t>(b) * a.W + w) * a.chunks;
     float top = -INFINITY;
-    for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, st[2 * c]);
-    top = wave_max(top);
+    for (int c = sub; c < a.chunks; c += lanes) top = fmaxf(top, st[c].x);
+    for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
     const double ts = top == -INFINITY ? 0.0 : top;
     double sum = 0.0;
-    for (int c = lane; c < a.chunks; c += 64) {
-      const float m = st[2 * c], l = st[2 * c + 1];
-      sum += m == -INFINITY && l == 0.f ? 0.0 : l * exp(m - ts);
+    for (int c = sub; c < a.chunks; c += lanes) {
+      const float2 s = st[c];
+      sum += s.x == -INFINITY && s.y == 0.f ? 0.0 : s.y * exp(s.x - ts);
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-    if (lane == 0) {  // a row of -inf alone has log probabilities -inf
+    for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o);
+    if (sub == 0) {  // a row of -inf alone has log probabilities -inf
       shift[w] = sum == 0.0 && top == -INFINITY ? -INFINITY : a.scores[static_cast<int64_t>(b) * a.W + w] - log(sum);
       tops[w] = static_cast<float>(ts);
     }
@@ -256,33 +337,40 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   __syncthreads();
   const int per = a.chunks * a.n, all = a.W * per;
   const uint2* pairs = a.pairs + static_cast<int64_t>(b) * all;
-  auto each = [&](auto&& f) {
-    for (int i = tid; i < all; i += kThreads) {
-      const int w = i / per, j = i - w * per;
-      const double s = shift[w];
-      if (!(fabs(s) < INFINITY)) {
-        // all of the beam's continuations are equal: its first ones
-        if (j < a.n && j < a.V) f(Key2{double_key(s), 0xffffffffu - static_cast<uint32_t>(w * a.V + j)});
-        continue;
-      }
-      const uint2 p = pairs[i];
-      if (p.x == 0) continue;
-      f(Key2{double_key(static_cast<double>(key_float(p.x)) - static_cast<double>(tops[w]) + s),
-            0xffffffffu - static_cast<uint32_t>(w * a.V + static_cast<int>(0xffffffffu - p.y))});
-    }
+  auto key_at = [&](int i) {
+    const int w = i / per, j = i - w * per;
+    const double s = shift[w];
+    if (!(fabs(s) < INFINITY))  // all of the beam's continuations are equal: its first ones
+      return j < a.n && j < a.V ? Key2{double_key(s), 0xffffffffu - static_cast<uint32_t>(w * a.V + j)} : Key2{0, 0};
+    const uint2 p = pairs[i];
+    if (p.x == 0) return Key2{0, 0};
+    return Key2{double_key(static_cast<double>(key_float(p.x)) - static_cast<double>(tops[w]) + s),
+                0xffffffffu - static_cast<uint32_t>(w * a.V + static_cast<int>(0xffffffffu - p.y))};
   };
-  Key2 best{0, 0};
-  each([&](const Key2& k) {
-    if (better(k, best)) best = k;
-  });
-  top_n(a.n, best, lists, each, [&](int rank, const Key2& k) {
+  auto each = [&](auto&& f) {
+    for (int i = tid; i < all; i += kThreads) f(key_at(i));
+  };
+  auto put = [&](int rank, const Key2& k) {
     const int flat = static_cast<int>(0xffffffffu - k.b), w = flat / a.V;
     const int64_t at = static_cast<int64_t>(b) * a.n + rank;
     a.out_scores[at] = static_cast<float>(key_double(k.a));
     a.beams[at] = w;
     a.tokens[at] = flat - w * a.V;
     a.parents[at] = b * a.W + w;
+  };
+  if (all <= kCap) {
+    for (int i = tid; i < all; i += kThreads) lists.list[i] = key_at(i);
+    __syncthreads();
+    ranked(a.n, all, lists, put);
+    return;
+  }
+  Key2 best{0, 0};
+  each([&](const Key2& k) {
+    if (better(k, best)) best = k;
   });
+  const int c = collected(bound_of(best, a.n, lists.part), lists, each);
+  if (c <= kCap) ranked(a.n, c, lists, put);
+  else one_by_one(a.n, lists, each, put);
 }
 
 // Elements of a thread: the longest chunks that leave every CU two workgroups.

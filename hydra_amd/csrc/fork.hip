@@ -199,6 +199,114 @@ __global__ __launch_bounds__(kThreads) void fork_take_kernel(ForkArgs a) {
   }
 }
 
+// All of it by one workgroup, where rows and their tables are few: 5 us instead of the
+// five launches' 14.  What its threads hand each other through memory is written, fenced
+// and read past the first-level cache.
+constexpr int kSmallRows = 256, kSmallEntries = 8192;
+
+__device__ __forceinline__ int seen(const int* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Inclusive sum over 1024 threads; `total` gets the whole sum.
+__device__ __forceinline__ int wide_incl_sum(int x, int* part, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = wave_incl_sum(x);
+  __syncthreads();
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < kWide / 64; ++w) {
+    if (w < wave) s += part[w];
+    all += part[w];
+  }
+  total = all;
+  return s;
+}
+
+__global__ __launch_bounds__(kWide) void fork_small_kernel(ForkArgs a) {
+  __shared__ int par[kSmallRows], len[kSmallRows], kids[kSmallRows], first[kSmallRows], copy[kSmallRows];
+  __shared__ int old[kSmallEntries];
+  __shared__ int part[kWide / 64];
+  __shared__ bool ok[kSmallRows];
+  const int tid = threadIdx.x, all = a.N * a.P;
+  int free = *a.free_count;
+  free = free < 0 ? 0 : (free > a.F ? a.F : free);
+  if (tid < a.N) {
+    par[tid] = parent_of(a, tid);
+    len[tid] = a.lengths[tid];
+    kids[tid] = 0;
+    first[tid] = a.N;
+  }
+  __syncthreads();
+  if (tid < a.N && par[tid] >= 0) {
+    atomicAdd(&kids[par[tid]], 1);
+    atomicMin(&first[par[tid]], tid);
+  }
+  for (int e = tid; e < all; e += kWide) {
+    const int j = e / a.P, c = e - j * a.P;
+    if (c >= held_of(a, len[j])) continue;
+    old[e] = a.table[j * a.table_rs + c];
+    if (is_page(a, old[e])) a.owner[old[e]] = a.N;
+  }
+  __threadfence();
+  __syncthreads();
+  for (int e = tid; e < all; e += kWide) {
+    const int j = e / a.P, c = e - j * a.P;
+    if (c >= held_of(a, len[j]) || !is_page(a, old[e])) continue;
+    if (c < full_of(a, len[j]) && kids[j] > 1) atomicAdd(&a.extra[old[e]], kids[j] - 1);
+    if (kids[j] == 0) {
+      atomicAdd(&a.extra[old[e]], -1);
+      atomicMin(&a.owner[old[e]], j);
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  for (int e0 = 0; e0 < all; e0 += kWide) {
+    const int e = e0 + tid, j = e < all ? e / a.P : 0, c = e - j * a.P;
+    const bool mine = e < all && kids[j] == 0 && c < held_of(a, len[j]) && is_page(a, old[e]);
+    const bool back = mine && seen(&a.owner[old[e]]) == j && seen(&a.extra[old[e]]) < 0;
+    int count;
+    const int to = free + wide_incl_sum(back, part, count) - 1;
+    if (back) {
+      a.extra[old[e]] = 0;
+      if (to < a.F) a.free_pages[to] = old[e];
+    }
+    free = min(a.F, free + count);
+  }
+  __threadfence();
+  __syncthreads();
+  {
+    int source = -1;
+    if (tid < a.N && par[tid] >= 0 && first[par[tid]] != tid) {
+      const int full = full_of(a, len[par[tid]]);
+      if (held_of(a, len[par[tid]]) > full) source = old[par[tid] * a.P + full];
+    }
+    const bool need = is_page(a, source);
+    int count;
+    const int rank = wide_incl_sum(need, part, count) - 1;
+    if (tid < a.N) {
+      const bool granted = !need || rank < free;
+      ok[tid] = granted;
+      copy[tid] = need && granted ? seen(&a.free_pages[free - 1 - rank]) : -1;
+      a.lengths[tid] = granted && par[tid] >= 0 ? len[par[tid]] : 0;
+      a.granted[tid] = granted;
+      a.sources[tid] = need && granted ? source : -1;
+      a.copies[tid] = copy[tid];
+      a.taken[tid] = granted ? par[tid] : -1;
+    }
+    if (tid == 0) *a.free_count = free - min(count, free);
+  }
+  __syncthreads();
+  for (int e = tid; e < all; e += kWide) {
+    const int i = e / a.P, c = e - i * a.P, p = par[i], n = p >= 0 ? len[p] : 0, full = full_of(a, n);
+    const int held = held_of(a, n), from = c < held ? old[p * a.P + c] : -1;
+    if (!ok[i] && c < full && is_page(a, from)) atomicAdd(&a.extra[from], -1);  // its share of the filled pages
+    a.table[i * a.table_rs + c] = !ok[i] ? -1 : (c == full && copy[i] >= 0 ? copy[i] : from);
+  }
+}
+
 // Whole pages, sources[i] to copies[i], keys and values (and scales): pieces of V.
 struct CopyArgs {
   const int *sources, *copies;
@@ -353,6 +461,10 @@ extern "C" int hydra_page_fork(const int* parents, int* lengths, int* table, int
   a.pages = static_cast<int>(pages);
   a.shift = shift;
   auto st = static_cast<hipStream_t>(stream);
+  if (N <= kSmallRows && N * P <= kSmallEntries) {
+    fork_small_kernel<<<1, kWide, 0, st>>>(a);
+    return check_launch("page_fork");
+  }
   const int64_t wide = (pages + kWide - 1) / kWide;
   const unsigned rows = static_cast<unsigned>(N);
   fork_count_kernel<<<static_cast<unsigned>(1 + (wide < 1024 ? wide : 1024)), kWide, 0, st>>>(a);
