@@ -76,8 +76,8 @@ struct PrefixArgs {
   int N, H, Hkv, hd, G, W, groups, P, shift, pages;
   int GB, RB;                   // blocks of 16 heads, of A rows
   float scale;                  // times log2(e)
-  bool split;                   // else one workgroup takes one B item, `first` and on
-  int first, wgs, cus;
+  bool split;                   // else one workgroup of `waves` takes one B item, `first` and on
+  int waves, first, wgs, cus;
   int* plan;                    // see kPlan
   float* part;                  // slots: pieces of A, then [wgs][2] of B, then (with groups) whole B items
   int64_t slot_a, slot_b, part_b, whole_b;  // floats of a slot, offsets in part
@@ -231,15 +231,15 @@ __device__ __forceinline__ void tile_pages(const PrefixArgs& a, const int* row, 
   for (int b = 0; b < NB; ++b) page[b] = page_of(a, row, key0 + 16 * b, end);
 }
 
-// An item's keys.  RW = 1: four waves take tiles in turn, and wave 0 ends up with
+// An item's keys.  RW = 1: the NW waves take tiles in turn, and wave 0 ends up with
 // all of their sums; RW = 4: each wave has rows of its own.
-template <typename C, typename KV, int HDP, int NT, int RW, bool VEC>
+template <typename C, typename KV, int HDP, int NT, int RW, bool VEC, int NW = 4>
 __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& item, char* lds, State<HDP, NT>& st) {
   const Item it = uniform(item);
   using Ty = Types<C, KV>;
   using VT = typename Ty::VT;
   constexpr bool F32 = Ty::f32, EIGHT = Ty::eight;
-  constexpr int KT = tile_keys(HDP, F32), NB = KT / 16, KW = 4 / RW, TT = 64 * RW;
+  constexpr int KT = tile_keys(HDP, F32), NB = KT / 16, KW = NW / RW, TT = 64 * RW;
   constexpr int E = 16 / sizeof(KV);                       // elements of a piece
   constexpr int PPR = HDP / E > 0 ? HDP / E : 1;           // pieces of a row
   constexpr int NC = PPR < 4 ? 1 : PPR / 4;                // pieces of a lane
@@ -503,11 +503,11 @@ __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& item,
     st.l[t] += __shfl_xor(st.l[t], 16);
     st.l[t] = halves_sum(st.l[t]);
   }
-  if constexpr (RW == 1) {  // waves 2 and 3 into 0 and 1, then 1 into 0: all hold the same layout
+  if constexpr (RW == 1) {  // the upper half of the waves into the lower one, until one is left: all hold the same layout
     float* sm = reinterpret_cast<float*>(lds);
     constexpr int ROW = NT * (2 + 4 * NO);
 #pragma unroll
-    for (int half = 2; half > 0; half >>= 1) {
+    for (int half = NW / 2; half > 0; half >>= 1) {
       __syncthreads();
       if (wave >= half && wave < 2 * half) {
         float* to = sm + (wave - half) * ROW * 64 + lane;
@@ -794,7 +794,7 @@ struct Deal {
   }
   __device__ __forceinline__ int of(int u) const {
     const int64_t a = static_cast<int64_t>(wgs_a) * beside;
-    return u < a ? u / beside : wgs_a + static_cast<int>((u - a) / per);
+    return u < a ? u / beside : wgs_a + (u - static_cast<int>(a)) / per;
   }
 };
 
@@ -815,21 +815,24 @@ template <typename C, typename KV>
 constexpr bool by_rows(bool vec) { return std::is_same<C, KV>::value && sizeof(C) == 2 && vec; }
 
 template <typename C, typename KV, int HDP>
-constexpr int lds_bytes(int nt, int rw, bool vec) {
+constexpr int lds_bytes(int nt, int rw, bool vec, int nw = 4) {
   const bool f32 = sizeof(C) == 4;
   const int tile = tile_keys(HDP, f32) * pitch_of(HDP, f32) * (f32 ? 4 : 2);
   if (rw == 4 && by_rows<C, KV>(vec)) return 4 * rows_tile(HDP) * HDP * 2;
-  return rw == 1 ? std::max(4 * tile, 2 * 64 * nt * (2 + HDP / 4) * 4) : 2 * tile;
+  return rw == 1 ? std::max(nw * tile, nw / 2 * 64 * nt * (2 + HDP / 4) * 4) : 2 * tile;
 }
 
-// One workgroup per B item, no split.
-template <typename C, typename KV, int HDP, bool VEC>
-__global__ __launch_bounds__(kThreads, 2) void prefix_whole_kernel(PrefixArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[lds_bytes<C, KV, HDP>(1, 1, VEC)];
+// One workgroup per B item, no split.  Few items get as many waves as registers and LDS
+// let one have.
+constexpr int whole_waves(int hdp) { return hdp <= 64 ? 16 : hdp == 128 ? 8 : 4; }
+
+template <typename C, typename KV, int HDP, bool VEC, int NW>
+__global__ __launch_bounds__(64 * NW) void prefix_whole_kernel(PrefixArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[lds_bytes<C, KV, HDP>(1, 1, VEC, NW)];
   const int item = a.first + blockIdx.x, gb = item % a.GB, h = item / a.GB % a.Hkv, n = item / a.GB / a.Hkv;
   Item it{n, h, 16 * gb, min(16, a.G - 16 * gb), n, 0, clamp_len(a, a.lengths[n])};
   State<HDP, 1> st;
-  item_keys<C, KV, HDP, 1, 1, VEC>(a, it, lds, st);
+  item_keys<C, KV, HDP, 1, 1, VEC, NW>(a, it, lds, st);
   write_out<C, HDP>(a, it, st);
 }
 
@@ -840,7 +843,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
   constexpr int LDS_A = RW == 0 ? 0 : lds_bytes<C, KV, HDP>(NT, RA, VEC), LDS_B = lds_bytes<C, KV, HDP>(1, 1, VEC);
   __shared__ __attribute__((aligned(16))) char lds[LDS_A > LDS_B ? LDS_A : LDS_B];
   // prefix sums of the groups' rounds and pieces, and of the requests' own rounds
-  __shared__ int units[RW == 0 ? 1 : kRequests + 1], lead[RW == 0 ? 1 : kRequests], pre_b[kRequests + 1];
+  __shared__ int units[RW == 0 ? 1 : kRequests + 1], pre_b[kRequests + 1];
+  // the first request of a group that has the whole prefix, and the keys read once (0: nobody has it)
+  __shared__ uint16_t lead[RW == 0 ? 1 : kRequests];
+  __shared__ int keys[RW == 0 ? 1 : kRequests];
+  __shared__ Deal s_deal;
   __shared__ int wsum[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto scan = [&](int n, int* pre, auto&& value) {  // pre[i + 1] = value(0) + .. + value(i)
@@ -861,22 +868,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
       __syncthreads();
     }
   };
-  if constexpr (RW != 0) {
-    for (int g = tid; g < a.groups; g += kThreads) lead[g] = a.N;
-    __syncthreads();
-    for (int n = tid; n < a.N; n += kThreads) {  // the first request that has the whole prefix
-      const int g = n / a.W;
-      if (clamp_len(a, a.lengths[n]) >= clamp_len(a, a.shared[g])) atomicMin(&lead[g], n);
-    }
-    __syncthreads();
-  }
-  auto rounds_of_group = [&](int g) { return lead[g] < a.N ? rounds_of(shared_keys(a, g)) : 0; };
-  int rounds_a = 0;
-  if constexpr (RW != 0) {
-    scan(a.groups, units, rounds_of_group);
-    rounds_a = units[a.groups];
-    __syncthreads();  // read before it is written again
-  }
+  const int HA = a.Hkv * a.RB, HB = a.Hkv * a.GB;
   // the last x with pre[x] <= u
   auto find = [](const int* pre, int n, int u) {
     int x = 0;
@@ -891,40 +883,105 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
     const int g = n / a.W;
     return clamp_len(a, a.lengths[n]) >= clamp_len(a, a.shared[g]) ? shared_keys(a, g) : 0;
   };
-  scan(a.N, pre_b, [&](int n) { return rounds_of(clamp_len(a, a.lengths[n]) - own_begin(n)); });
-  const int HA = a.Hkv * a.RB, HB = a.Hkv * a.GB;
-  const int total_b = pre_b[a.N] * HB;
-  Deal deal{0, 0, 1};
-  int units_a = 0;
-  if constexpr (RW != 0) {
+  // How long the pieces are, and how B is dealt out; next_units(per) makes `units` for
+  // pieces of up to `per` rounds and returns their number.  (All of these counts stay below
+  // 2^31, which the host sees to: a 64-bit division here and there took longer than the keys.)
+  auto deal_out = [&](int rounds_a, int total_b, auto&& next_units) {
+    Deal d{0, 0, 1};
     if (rounds_a > 0) {
       // The least piece for which the pieces are no more than the workgroups, so that each
       // has one, if all items are not more than that already.
-      const int64_t all_rounds = static_cast<int64_t>(rounds_a) * HA;
-      const bool fit = static_cast<int64_t>(a.groups) * HA <= a.wgs;
-      int per = static_cast<int>((all_rounds + a.wgs - 1) / a.wgs);
+      const unsigned all_rounds = rounds_a * HA;
+      const bool fit = a.groups * HA <= a.wgs;
+      int per = (all_rounds + a.wgs - 1) / a.wgs, all = 0;
       for (int turn = 0; turn < 16; ++turn) {
-        scan(a.groups, units, [&](int g) { return (rounds_of_group(g) + per - 1) / per; });
-        const int64_t all = static_cast<int64_t>(units[a.groups]) * HA;
-        __syncthreads();
+        all = next_units(per) * HA;
         if (all <= a.wgs || !fit) break;
-        per = max(per + 1, static_cast<int>((per * all + a.wgs - 1) / a.wgs));
+        per = max(per + 1, static_cast<int>(static_cast<float>(per) * static_cast<float>(all) / static_cast<float>(a.wgs)));
       }
-      units_a = units[a.groups] * HA;
-      deal.wgs_a = min(a.wgs, units_a);
+      d.wgs_a = min(a.wgs, all);
       // B rounds that take a workgroup as long as its pieces: a round of A is RW tiles
       // of a wave, one of B a single one
-      const int64_t busy = min(all_rounds * RW / deal.wgs_a, int64_t(1) << 30), rest = a.wgs - deal.wgs_a;
-      if (total_b <= busy * rest) {
-        deal.per = static_cast<int>((total_b + rest - 1) / rest);
+      const int busy = all_rounds * RW / d.wgs_a, rest = a.wgs - d.wgs_a;
+      const int64_t filled = static_cast<int64_t>(busy) * rest;
+      if (total_b <= filled) {
+        d.per = rest == 0 ? 1 : (total_b + rest - 1) / rest;
       } else {
-        deal.beside = static_cast<int>((total_b - busy * rest + a.wgs - 1) / a.wgs);
-        deal.per = static_cast<int>(busy) + deal.beside;
+        d.beside = (total_b - static_cast<int>(filled) + a.wgs - 1) / a.wgs;
+        d.per = busy + d.beside;
       }
+    } else {
+      d.per = (total_b + a.wgs - 1) / a.wgs;
     }
+    d.per = max(d.per, 1);
+    return d;
+  };
+  if (a.N <= 64) {  // in the lanes of one wave
+    if (wave == 0) {
+      const int len = lane < a.N ? clamp_len(a, a.lengths[lane]) : 0;
+      int begin = 0, rounds_a = 0, rounds = 0;
+      if constexpr (RW != 0) {
+        const int own = lane < a.N ? clamp_len(a, a.shared[lane / a.W]) : 0, mine = lane < a.groups ? clamp_len(a, a.shared[lane]) : 0;
+        const bool has = lane < a.N && len >= own;
+        begin = has ? own & ~15 : 0;
+        const uint64_t who = __ballot(has);
+        const uint64_t of_group = lane < a.groups ? who >> (lane * a.W) & (~0ull >> (64 - a.W)) : 0;
+        const int first = of_group ? lane * a.W + __ffsll(static_cast<unsigned long long>(of_group)) - 1 : a.N;
+        const int seen = of_group ? mine & ~15 : 0;
+        if (lane < a.groups) {
+          lead[lane] = static_cast<uint16_t>(first);
+          keys[lane] = seen;
+        }
+        rounds = rounds_of(seen);
+        rounds_a = __builtin_amdgcn_readlane(wave_incl_sum(rounds), 63);
+      }
+      const int upto = wave_incl_sum(lane < a.N ? rounds_of(len - begin) : 0);
+      if (lane < a.N) pre_b[lane + 1] = upto;
+      if (lane == 0) pre_b[0] = 0;
+      const Deal d = deal_out(rounds_a, __builtin_amdgcn_readlane(upto, 63) * HB, [&](int per) {
+        const int s = wave_incl_sum((rounds + per - 1) / per);
+        if (RW != 0 && lane < a.groups) units[lane + 1] = s;
+        return static_cast<int>(__builtin_amdgcn_readlane(s, 63));
+      });
+      if (lane == 0) {
+        s_deal = d;
+        if constexpr (RW != 0) units[0] = 0;
+      }
+      if (RW != 0 && rounds_a == 0 && lane < a.groups) units[lane + 1] = 0;
+    }
+    __syncthreads();
+  } else {
+    int rounds_a = 0;
+    if constexpr (RW != 0) {
+      for (int g = tid; g < a.groups; g += kThreads) keys[g] = a.N;
+      __syncthreads();
+      for (int n = tid; n < a.N; n += kThreads) {
+        const int g = n / a.W;
+        if (clamp_len(a, a.lengths[n]) >= clamp_len(a, a.shared[g])) atomicMin(&keys[g], n);
+      }
+      __syncthreads();
+      for (int g = tid; g < a.groups; g += kThreads) {
+        const int first = keys[g];
+        lead[g] = static_cast<uint16_t>(first);
+        keys[g] = first < a.N ? shared_keys(a, g) : 0;
+      }
+      __syncthreads();
+      scan(a.groups, units, [&](int g) { return rounds_of(keys[g]); });
+      rounds_a = units[a.groups];
+      __syncthreads();  // read before it is written again
+    }
+    scan(a.N, pre_b, [&](int n) { return rounds_of(clamp_len(a, a.lengths[n]) - own_begin(n)); });
+    const Deal d = deal_out(rounds_a, pre_b[a.N] * HB, [&](int per) {
+      scan(a.groups, units, [&](int g) { return (rounds_of(keys[g]) + per - 1) / per; });
+      const int all = units[a.groups];
+      __syncthreads();
+      return all;
+    });
+    if (tid == 0) s_deal = d;
+    __syncthreads();
   }
-  if (units_a == 0) deal.per = (total_b + a.wgs - 1) / a.wgs;
-  deal.per = max(deal.per, 1);
+  const Deal deal = s_deal;
+  const int total_b = pre_b[a.N] * HB, units_a = RW == 0 ? 0 : units[a.groups] * HA;
   if (blockIdx.x == 0) {  // for the joining kernel
     if (tid == 0) {
       a.plan[kWgsA] = deal.wgs_a;
@@ -932,7 +989,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
       a.plan[kPer] = deal.per;
     }
     if constexpr (RW != 0)
-      for (int i = tid; i <= a.groups; i += kThreads) a.plan[kPlan + i] = units_a > 0 ? units[i] : 0;
+      for (int i = tid; i <= a.groups; i += kThreads) a.plan[kPlan + i] = units[i];
     for (int i = tid; i <= a.N; i += kThreads) a.plan[kPlan + a.groups + 1 + i] = pre_b[i];
   }
   if constexpr (RW != 0) {
@@ -941,16 +998,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
       // Pieces in the order (group, key head, piece, block of rows), each XCD (workgroups go
       // to them in turn) a run of them: the blocks of rows read the same keys from its L2.
       const int w = blockIdx.x, xcds = min(8, wgs_a), x = w % xcds, at = w / xcds, beside = (wgs_a - x + xcds - 1) / xcds;
-      const int first = static_cast<int>(static_cast<int64_t>(units_a) * x / xcds);
-      const int last = static_cast<int>(static_cast<int64_t>(units_a) * (x + 1) / xcds);
+      const int some = units_a / xcds, more = units_a - some * xcds;
+      const int first = some * x + min(x, more), last = some * (x + 1) + min(x + 1, more);
       for (int u = first + at; u < last; u += beside) {
         const int g = find(units, a.groups, u / HA);
-        const int pieces = units[g + 1] - units[g], r = rounds_of_group(g), v = u - units[g] * HA;
+        const int pieces = units[g + 1] - units[g], r = rounds_of(keys[g]), v = u - units[g] * HA;
         const int h = v / (pieces * a.RB), y = v - h * pieces * a.RB, piece = y / a.RB, rb = y - piece * a.RB;
-        const int t0 = static_cast<int>(static_cast<int64_t>(r) * piece / pieces);
-        const int t1 = static_cast<int>(static_cast<int64_t>(r) * (piece + 1) / pieces);
+        const int each = r / pieces, over = r - each * pieces;
+        const int t0 = each * piece + min(piece, over), t1 = each * (piece + 1) + min(piece + 1, over);
         Item it{g * a.W, h, rb * ROWS, min(ROWS, a.W * a.G - rb * ROWS), lead[g], t0 * kRound,
-                t1 == r ? shared_keys(a, g) : t1 * kRound};
+                t1 == r ? keys[g] : t1 * kRound};
         State<HDP, NT> st;
         if constexpr (RW == 4 && by_rows<C, KV>(VEC)) item_rows<C, HDP, NT>(a, it, lds, st);
         else item_keys<C, KV, HDP, NT, RA, VEC>(a, it, lds, st);
@@ -1107,7 +1164,7 @@ int launch_split(PrefixArgs a, int rows_a, hipStream_t st) {
   a.wgs = std::min(a.wgs, a.cus * blocks_per_cu(reinterpret_cast<const void*>(kernel), kThreads));
   kernel<<<a.wgs, kThreads, 0, st>>>(a);
   const int64_t rows = static_cast<int64_t>(a.N) * a.H;
-  if (rows <= 256) prefix_join_kernel<C, 1024><<<static_cast<unsigned>(rows), 1024, 0, st>>>(a, rows_a);
+  if (rows <= 32) prefix_join_kernel<C, 1024><<<static_cast<unsigned>(rows), 1024, 0, st>>>(a, rows_a);
   else if (rows <= 2048) prefix_join_kernel<C, 256><<<static_cast<unsigned>(rows), 256, 0, st>>>(a, rows_a);
   else prefix_join_kernel<C, 64><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(a, rows_a);
   return check_launch("prefix_attn");
@@ -1124,7 +1181,9 @@ int launch_form(const PrefixArgs& a, const Shape& s, hipStream_t st) {
     constexpr int64_t most = int64_t(1) << 22;  // HIP counts a launch's threads in 32 bits
     for (int64_t first = 0; first < items; first += most) {
       b.first = static_cast<int>(first);
-      prefix_whole_kernel<C, KV, HDP, VEC><<<static_cast<unsigned>(std::min(most, items - first)), kThreads, 0, st>>>(b);
+      const unsigned wgs = static_cast<unsigned>(std::min(most, items - first));
+      if (a.waves == 4) prefix_whole_kernel<C, KV, HDP, VEC, 4><<<wgs, kThreads, 0, st>>>(b);
+      else prefix_whole_kernel<C, KV, HDP, VEC, whole_waves(HDP)><<<wgs, 64 * whole_waves(HDP), 0, st>>>(b);
     }
     return check_launch("prefix_attn");
   }

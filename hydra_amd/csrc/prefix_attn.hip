@@ -11,6 +11,7 @@ struct Pieces {
   Shape s;
   bool split;
   int64_t GB, requests, wgs;
+  int waves;  // of a workgroup where it takes a whole item
   int64_t slot_a, slot_b, part_b, whole_b;  // floats; of the largest piece
 };
 
@@ -42,8 +43,10 @@ int pieces_of(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, int
   p.s = shape_of(hd, G, W, groups > 0, dtype_size(dtype), vec);
   p.GB = (G + 15) / 16;
   const int64_t rounds = (cap + kRound - 1) / kRound;
-  p.requests = std::min<int64_t>(kRequests, (int64_t(1) << 30) / (rounds * Hkv * (p.GB + 1)));
-  p.split = groups > 0 || (N <= p.requests && N * Hkv * p.GB < 8 * device_cus() && cap > 8 * kRound);
+  p.requests = std::min<int64_t>(kRequests, (int64_t(1) << 29) / (rounds * Hkv * (p.GB + 1)));
+  const int64_t items = N * Hkv * p.GB;
+  p.waves = items > device_cus() || cap <= kRound ? 4 : whole_waves(p.s.hdp);
+  p.split = groups > 0 || (N <= p.requests && items < 8 * device_cus() && cap > (p.waves == 16 ? 16 : 8) * kRound);
   HYDRA_REQUIRE(p.requests >= 1 || !p.split, "prefix_attn: too large");
   p.wgs = static_cast<int64_t>(groups > 0 ? 2 : 4) * device_cus();
   const int64_t r4 = row4(static_cast<int>(hd));
@@ -154,6 +157,7 @@ extern "C" int hydra_prefix_attn(const void* q, const void* k_pages, const void*
   a.pages = static_cast<int>(pages);
   a.scale = scale * kLog2e;
   a.split = p.split;
+  a.waves = p.waves;
   a.wgs = static_cast<int>(p.wgs);
   a.cus = device_cus();
   a.plan = static_cast<int*>(workspace);
