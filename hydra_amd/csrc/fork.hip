@@ -199,9 +199,10 @@ __global__ __launch_bounds__(kThreads) void fork_take_kernel(ForkArgs a) {
   }
 }
 
-// All of it by one workgroup, where rows and their tables are few: 5 us instead of the
-// five launches' 14.  What its threads hand each other through memory is written, fenced
-// and read past the first-level cache.
+// All of it by one workgroup, where rows and their tables are few: 12.8 us on the device,
+// about what the five launches take there (4 rows of 12 pages), but one launch of the
+// host's instead of five.  What its threads hand each other through memory is written,
+// fenced and read past the first-level cache.
 constexpr int kSmallRows = 256, kSmallEntries = 8192;
 
 __device__ __forceinline__ int seen(const int* p) {
@@ -545,6 +546,8 @@ extern "C" int hydra_rows_take(void* x, int64_t row_stride_bytes, int64_t row_by
   a.N = static_cast<int>(N);
   a.log = 0;
   while ((int64_t(2) << a.log) * N <= kTakeThreads * kTakePieces) ++a.log;
+  // narrower ranges where there would be few workgroups, of 64 bytes at least
+  while (a.log > 2 && (a.pieces >> a.log) < device_cus()) --a.log;
   a.cols = 1 << a.log;
   const int64_t wgs = (a.pieces + a.cols - 1) / a.cols;
   HYDRA_REQUIRE(grid_fits(wgs, kTakeThreads), "rows_take: too large");

@@ -591,51 +591,71 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& item,
 #pragma unroll
   for (int t = 0; t < NT; ++t) ms[t] = 0.f;
 
-  // this lane's piece of each direct load, in a block of 16 rows
+  // A tile lies in one page, or its blocks of 16 may lie in several: a descriptor for the
+  // tile, or for each load (which none goes beyond).
+  const bool one = (KT - 1) >> a.shift == 0;
+  // this lane's piece of each direct load, in the tile or in its block
   uint32_t koff[NJ], voff[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    const int r = (j * 4 + wave) * RPI + lane / PPR, c = lane % PPR;
+    const int r = (j * 4 + wave) * RPI + lane / PPR, c = lane % PPR, in = one ? r : r & 15;
     const uint32_t ck = c ^ fk(r), cv = c ^ fv(r), none = 0x7ffffff0u;
-    koff[j] = static_cast<int>(ck) * 8 < a.hd ? (r & 15) * static_cast<uint32_t>(a.k_st[2]) + 16 * ck : none;
-    voff[j] = static_cast<int>(cv) * 8 < a.hd ? (r & 15) * static_cast<uint32_t>(a.v_st[2]) + 16 * cv : none;
+    koff[j] = static_cast<int>(ck) * 8 < a.hd ? in * static_cast<uint32_t>(a.k_st[2]) + 16 * ck : none;
+    voff[j] = static_cast<int>(cv) * 8 < a.hd ? in * static_cast<uint32_t>(a.v_st[2]) + 16 * cv : none;
   }
-  const int kbytes = 15 * static_cast<int>(a.k_st[2]) + 2 * a.hd, vbytes = 15 * static_cast<int>(a.v_st[2]) + 2 * a.hd;
+  const int krow = static_cast<int>(a.k_st[2]), vrow = static_cast<int>(a.v_st[2]);
   const uint32_t base = lds_addr(lds);
-  // the pages that this wave loads from are looked up by themselves: chosen from the
-  // tile's by an index they would go through memory
-  auto load_pages = [&](int k0, int (&pg)[NJ]) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) pg[j] = page_of(a, trow, k0 + ((j * 4 + wave) * RPI & ~15), it.end);
+  // Pages of 64 blocks of 16 keys at a time, one to a lane: looked up tile by tile they
+  // would be waited for together with the operands from LDS.
+  constexpr int TPB = 64 / NB;  // tiles of such a batch
+  auto batch = [&](int first) {
+    const int key = first + 16 * lane;
+    const int p = key < it.end ? trow[key >> a.shift] : -1;
+    return static_cast<unsigned>(p) < static_cast<unsigned>(a.pages) ? p : -1;
   };
-  auto issue = [&](const int (&pg)[NJ], int k0, int buf) {
+  auto page_at = [](int pages, int i) { return __builtin_amdgcn_readlane(pages, i); };
+  auto issue = [&](int pages, int at, int k0, int buf) {  // the batch's blocks from `at` on
+    const uint32_t to = base + buf * 2 * TILE + wave * 1024;
+    if (one) {
+      const int p = page_at(pages, at), rows = min(KT, it.end - k0);
+      const int64_t r = k0 & rmask, pg = max(p, 0);
+      const i32x4_t ks = raw_rsrc(kbase + pg * a.k_st[0] + r * krow, p < 0 ? 0 : (rows - 1) * krow + 2 * a.hd);
+      const i32x4_t vs = raw_rsrc(vbase + pg * a.v_st[0] + r * vrow, p < 0 ? 0 : (rows - 1) * vrow + 2 * a.hd);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int p = pg[j];
-      const int64_t r = (k0 + ((j * 4 + wave) * RPI & ~15)) & rmask, at = max(p, 0);
-      const uint32_t to = base + buf * 2 * TILE + (j * 4 + wave) * 1024;
-      load16_to_lds(raw_rsrc(kbase + at * a.k_st[0] + r * a.k_st[2], p < 0 ? 0 : kbytes), to, koff[j]);
-      load16_to_lds(raw_rsrc(vbase + at * a.v_st[0] + r * a.v_st[2], p < 0 ? 0 : vbytes), to + TILE, voff[j]);
+      for (int j = 0; j < NJ; ++j) {
+        load16_to_lds(ks, to + j * 4096, koff[j]);
+        load16_to_lds(vs, to + j * 4096 + TILE, voff[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int b = (j * 4 + wave) * RPI >> 4, p = page_at(pages, at + b);
+        const int64_t r = (k0 + 16 * b) & rmask, pg = max(p, 0);
+        load16_to_lds(raw_rsrc(kbase + pg * a.k_st[0] + r * krow, p < 0 ? 0 : 15 * krow + 2 * a.hd), to + j * 4096, koff[j]);
+        load16_to_lds(raw_rsrc(vbase + pg * a.v_st[0] + r * vrow, p < 0 ? 0 : 15 * vrow + 2 * a.hd), to + j * 4096 + TILE,
+                      voff[j]);
+      }
     }
   };
   const uint32_t kread = col * HDP * 2 + ((g4 ^ fk(col)) << 4);
   const int vr = 4 * g4 + (col >> 2);
   const uint32_t vread = vr * HDP * 2 + ((((col & 3) >> 1) ^ fv(vr)) << 4) + (col & 1) * 8;
 
-  int page[NB], from[NJ];
-  load_pages(it.begin, from);
-  __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): q is here, only direct loads are counted below
-  issue(from, it.begin, 0);
-  tile_pages<NB>(a, trow, it.begin, it.end, page);
-  load_pages(it.begin + KT, from);
-  int buf = 0;
+  int pages = batch(it.begin), next = -1;
+  __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): q and the pages are here
+  issue(pages, 0, it.begin, 0);
+  int buf = 0, at = 0;  // at: the tile's first block in its batch
   for (int key0 = it.begin; key0 < it.end; key0 += KT, buf ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): this wave's part of the tile
+    __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): this wave's part of the tile, and the next pages
     __syncthreads();                     // everybody's, and the other tile is read
-    if (key0 + KT < it.end) issue(from, key0 + KT, buf ^ 1);
-    int after[NB];
-    tile_pages<NB>(a, trow, key0 + KT, it.end, after);
-    load_pages(key0 + 2 * KT, from);
+    const bool last = at == 64 - NB;     // of the batch
+    if (key0 + KT < it.end) issue(last ? next : pages, last ? 0 : at + NB, key0 + KT, buf ^ 1);
+    if (at == 64 - 2 * NB) next = batch(key0 + 2 * KT);
+    int page[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) page[b] = page_at(pages, at + b);
+    if (last) pages = next;
+    at = last ? 0 : at + NB;
     const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
     // Operands are read a phase ahead of the products that take them, which the barriers
     // below keep in place: read where they are needed, LDS's latency would be waited for
@@ -726,8 +746,6 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& item,
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) page[b] = after[b];
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
