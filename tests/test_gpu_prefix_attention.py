@@ -360,3 +360,53 @@ def test_refusals(cuda):
             (RuntimeError, "no gradient", (q.clone().requires_grad_(), kb, vb, table, lengths), dict(shared=shared))):
         with pytest.raises(error, match=text):
             call(*args, **kw)
+
+
+@pytest.mark.parametrize("form", ["shared few", "shared many", "shared many, pages of 16", "8 bits", "fp32"])
+def test_pools_past_32_bits(cuda, form):
+    """Pages more than 2^32 bytes into the pool, of every kernel that walks them."""
+    from hydra_amd.attention import copy_pages, paged_attention, read_pages, store_pages
+
+    page = 16 if "16" in form else 4096
+    K, hd = 1, 256
+    dtype = torch.float32 if form == "fp32" else torch.bfloat16
+    e = 1 if form == "8 bits" else dtype.itemsize
+    pages = (1 << 32) // (page * hd * e) + 40
+    free, _ = torch.cuda.mem_get_info()
+    if free < 3 * pages * page * hd * e:
+        pytest.skip("too little memory")
+    g = torch.Generator().manual_seed(1)
+    W = 2 if form in ("shared few", "8 bits", "fp32") else 70
+    n = 150
+    P = -(-n // page)
+    # each request its own page behind the prefix's; a small pool with the same rows to compare with
+    case = Case([[n] * W], [n // 2 // page * page if page == 16 else n // 2], 1, K, hd, page, dtype,
+                torch.int8 if form == "8 bits" else None, seed=2)
+    used = case.kp.shape[0]
+    far = torch.arange(pages - used, pages)
+    table = torch.where((case.table >= 0) & (case.table < used), far[case.table.long().clamp(0, used - 1)].to(torch.int32), -1)
+    kp, vp = (torch.empty((pages, K, page, hd), dtype=t.dtype, device=cuda) for t in (case.kp, case.vp))
+    kp[-used:], vp[-used:] = case.kp.to(cuda), case.vp.to(cuda)
+    scales = small = None
+    if case.scales is not None:
+        scales = [torch.empty((pages, K, page), device=cuda) for _ in range(2)]
+        for s, c in zip(scales, case.scales):
+            s[-used:] = c.to(cuda)
+        small = [s.to(cuda) for s in case.scales]
+    shared = None if form == "8 bits" else case.shared.to(cuda)
+    q, lengths = case.q.to(cuda), case.lengths.to(cuda)
+    want = paged_attention(q, case.kp.to(cuda), case.vp.to(cuda), case.table.to(cuda), lengths, scales=small, shared=shared)
+    assert torch.equal(paged_attention(q, kp, vp, table.to(cuda), lengths, scales=scales, shared=shared), want)
+    # rows written, read and copied there
+    slots = ((pages - 1) * page + torch.tensor([[3, 9]])).to(cuda)
+    rows = torch.randn(1, K, 2, hd, generator=g).to(torch.bfloat16 if scales else dtype).to(cuda)
+    store_pages(rows, rows, kp, vp, slots, scales=scales)
+    copy_pages(kp, vp, *(torch.tensor([p], dtype=torch.int32, device=cuda) for p in (pages - 1, pages - 2)), scales=scales)
+    a, _ = read_pages(kp, vp, slots, scales=scales, dtype=dtype)
+    b, _ = read_pages(kp, vp, slots - page, scales=scales, dtype=dtype)
+    assert torch.equal(a, b)
+    if scales is None:
+        assert torch.equal(a, rows)
+    else:
+        x, s = op.quantise(rows.cpu(), torch.int8)
+        assert (a.cpu().double() - x * s.double()[..., None]).abs().max() <= 2.0 ** -8 * rows.abs().max()
