@@ -13,10 +13,10 @@
 // themselves.
 //
 // The n best of a workgroup's elements, without sorting them: the threads fall
-// into at least n groups, and the least of the groups' maxima is a bound that n
-// elements reach; those that do (of 4000 even ones, and n = 16, some 50) are
-// collected and ranked by counting.  Keys are unique (an index is part of them),
-// so the order in which they are collected does not matter.
+// into four n groups or so, and the n-th largest of the groups' maxima is a bound that
+// n elements reach; those that do (a few more than n, whatever the order of the
+// elements) are collected and ranked by counting.  Keys are unique (an index is part of
+// them), so the order in which they are collected does not matter.
 #include "common.h"
 #include "mod_keys.h"
 
@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCap = 2048;       // collected elements
+constexpr int kFew = 64;         // elements that are ranked as they are
 constexpr int kMaxCount = 128;   // n
 constexpr int kMaxBeams = 1024;  // W
 
@@ -39,50 +40,42 @@ struct Key2 {
 };
 __device__ __forceinline__ bool better(const Key1& x, const Key1& y) { return x.a > y.a; }
 __device__ __forceinline__ bool better(const Key2& x, const Key2& y) { return x.a > y.a || (x.a == y.a && x.b > y.b); }
-__device__ __forceinline__ Key1 shuffled(const Key1& k, int off) {
-  return Key1{static_cast<uint64_t>(__shfl_xor(static_cast<long long>(k.a), off))};
-}
-__device__ __forceinline__ Key2 shuffled(const Key2& k, int off) {
-  return Key2{static_cast<uint64_t>(__shfl_xor(static_cast<long long>(k.a), off)),
-              static_cast<uint32_t>(__shfl_xor(static_cast<int>(k.b), off))};
+// In the keys' order, equal ones in any.
+template <typename Key>
+__device__ __forceinline__ uint32_t rough(const Key& k) {
+  return static_cast<uint32_t>(k.a >> 32);
 }
 
 template <typename Key> struct Lists {
   Key list[kCap];
-  Key part[kThreads];
+  alignas(16) uint32_t part[kThreads];
+  Key nth;
+  uint32_t bound;
   int count;
 };
 
-// The least of the maxima of n' >= n groups of threads (all 256 take part): at
-// least n elements reach it, if there are as many as groups.  Thread t is in group t mod
-// n': neighbours hold neighbouring elements, of one beam or one end of a row, and groups
-// of such would be of very different size.
+// A bound that n threads' `mine` reach, and few more (all 256 take part).
 template <typename Key>
-__device__ __forceinline__ Key bound_of(Key mine, int n, Key* part) {
-  int groups = 1;
-  while (groups < n) groups <<= 1;
-  const int tid = threadIdx.x, lane = tid & 63;
-  for (int off = 32; off >= groups; off >>= 1) {
-    const Key o = shuffled(mine, off);
-    if (better(o, mine)) mine = o;
-  }
-  __syncthreads();  // the last use of `part` is over
-  part[tid] = mine;
+__device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n, Lists<Key>& L) {
+  int size = 64;  // threads of a group
+  while (size > 1 && kThreads / size < 4 * n) size >>= 1;
+  for (int o = 1; o < size; o <<= 1) mine = max(mine, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine), o)));
+  const int groups = kThreads / size;
+  if (threadIdx.x % size == 0) L.part[threadIdx.x / size] = mine;
+  if (threadIdx.x == 0) L.bound = 0xffffffffu;
   __syncthreads();
-  const int step = groups < 64 ? 64 : groups;  // threads of one group in other waves
-  for (int o = (tid + step) & (kThreads - 1); o != tid; o = (o + step) & (kThreads - 1))
-    if (better(part[o], mine)) mine = part[o];
-  for (int off = 1; off < groups && off < 64; off <<= 1) {
-    const Key o = shuffled(mine, off);
-    if (better(mine, o)) mine = o;
+  if (threadIdx.x < groups) {
+    const uint4* part = reinterpret_cast<const uint4*>(L.part);
+    mine = L.part[threadIdx.x];
+    int above = 0;
+    for (int i = 0; i < groups / 4; ++i) {
+      const uint4 p = part[i];
+      above += (p.x > mine) + (p.y > mine) + (p.z > mine) + (p.w > mine);
+    }
+    if (above < n) atomicMin(&L.bound, mine);
   }
-  if (groups > 64) {  // 128: two waves' groups
-    __syncthreads();
-    if (lane == 0) part[tid >> 6] = mine;
-    __syncthreads();
-    if (better(mine, part[(tid >> 6) ^ 1])) mine = part[(tid >> 6) ^ 1];
-  }
-  return mine;
+  __syncthreads();
+  return L.bound;
 }
 
 // A place in the list for each lane with `in`: one count for the wave.
@@ -95,37 +88,11 @@ __device__ __forceinline__ int place(bool in, int* count) {
   return base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
 }
 
-// The n best of the list's c elements, best first, to put(rank, key); ranks without an
-// element get none.
+// The list's c elements by ranks, to put(rank, key), as far as the ranks are below n.
 template <typename Key, typename Put>
-__device__ __forceinline__ void ranked(int n, int c, Lists<Key>& L, Put&& put) {
-  constexpr int U = kCap / kThreads;
-  const int tid = threadIdx.x;
-  // many: those that reach a bound of the list's own elements move to its front
-  for (int i = 0; i < 4 && c > 128 && c > 2 * n; ++i) {
-    Key mine[U], k{};
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      mine[u] = Key{};
-      if (u * kThreads + tid < c) mine[u] = L.list[u * kThreads + tid];
-      if (better(mine[u], k)) k = mine[u];
-    }
-    if (tid == 0) L.count = 0;
-    const Key tight = bound_of(k, n, L.part);  // everybody has read
-    const int trips = (c + kThreads - 1) / kThreads;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u >= trips) continue;
-      const bool in = mine[u].a != 0 && !better(tight, mine[u]);
-      const int at = place(in, &L.count);
-      if (in) L.list[at] = mine[u];
-    }
-    __syncthreads();
-    c = L.count;
-    __syncthreads();
-  }
+__device__ __forceinline__ void counted(int n, int c, Lists<Key>& L, Put&& put) {
   // four lanes to an element, a quarter of the list each
-  const int q = tid & 3, i0 = c * q / 4, i1 = c * (q + 1) / 4;
+  const int tid = threadIdx.x, q = tid & 3, i0 = c * q / 4, i1 = c * (q + 1) / 4;
   for (int j0 = 0; j0 < c; j0 += kThreads / 4) {
     const int j = j0 + (tid >> 2);
     const Key k = L.list[min(j, c - 1)];
@@ -136,46 +103,74 @@ __device__ __forceinline__ void ranked(int n, int c, Lists<Key>& L, Put&& put) {
     rank += __shfl_xor(rank, 2);
     if (q == 0 && j < c && k.a != 0 && rank < n) put(rank, k);
   }
+}
+
+// The n best of the list's c elements, best first, to put(rank, key); ranks without an
+// element get none.
+template <typename Key, typename Put>
+__device__ __forceinline__ void ranked(int n, int c, Lists<Key>& L, Put&& put) {
+  constexpr int U = kCap / kThreads;
+  const int tid = threadIdx.x;
+  // many: those that reach a bound of the list's own elements move to its front
+  for (int i = 0; i < 2 && c > 128 && c > 2 * n; ++i) {
+    Key mine[U];
+    uint32_t top = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      mine[u] = Key{};
+      if (u * kThreads + tid < c) mine[u] = L.list[u * kThreads + tid];
+      top = max(top, rough(mine[u]));
+    }
+    const uint32_t bound = bound_of(top, n, L);  // everybody has read
+    if (tid == 0) L.count = 0;
+    __syncthreads();
+    const int trips = (c + kThreads - 1) / kThreads;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u >= trips) continue;
+      const bool in = mine[u].a != 0 && rough(mine[u]) >= bound;
+      const int at = place(in, &L.count);
+      if (in) L.list[at] = mine[u];
+    }
+    __syncthreads();
+    c = L.count;
+    __syncthreads();
+  }
+  counted(n, c, L, put);
   for (int j = c + tid; j < n; j += kThreads) put(j, Key{});
 }
 
-// The n best of the elements that each thread's `each` goes over, one after the other: the
-// best below the last.
-template <typename Key, typename Each, typename Put>
-__device__ __forceinline__ void one_by_one(int n, Lists<Key>& L, Each&& each, Put&& put) {
-  Key last{};
-  for (int i = 0; i < n; ++i) {
-    Key k{};
-    each([&](const Key& x) {
-      if ((i == 0 || better(last, x)) && better(x, k)) k = x;
-    });
-    for (int off = 1; off < 64; off <<= 1) {
-      const Key o = shuffled(k, off);
-      if (better(o, k)) k = o;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) L.part[threadIdx.x >> 6] = k;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w)
-      if (better(L.part[w], k)) k = L.part[w];
-    if (threadIdx.x == 0) put(i, k);
-    last = k;
-  }
-}
-
-// Those of all elements that reach `bound`, which at least n do, into the list; their
-// number, which may be more than the list holds.
+// At least the n best of all elements into the list; their number.  Any n elements give a
+// bound: first the threads' best ones, then those of a list that was too short.
 template <typename Key, typename Each>
-__device__ __forceinline__ int collected(const Key& bound, Lists<Key>& L, Each&& each) {
-  if (threadIdx.x == 0) L.count = 0;
-  __syncthreads();
+__device__ __forceinline__ int collected(int n, Lists<Key>& L, Each&& each) {
+  Key best{};
   each([&](const Key& k) {
-    if (k.a == 0 || better(bound, k)) return;
-    const int at = atomicAdd(&L.count, 1);
-    if (at < kCap) L.list[at] = k;
+    if (better(k, best)) best = k;
   });
   __syncthreads();
-  return L.count;
+  L.list[threadIdx.x] = best;
+  for (int c = kThreads;; c = kCap) {
+    if (threadIdx.x == 0) {
+      L.nth = Key{};
+      L.count = 0;
+    }
+    __syncthreads();
+    counted(n, c, L, [&](int rank, const Key& k) {
+      if (rank == n - 1) L.nth = k;
+    });
+    __syncthreads();
+    const Key nth = L.nth;
+    each([&](const Key& k) {
+      if (k.a == 0 || better(nth, k)) return;
+      const int at = atomicAdd(&L.count, 1);
+      if (at < kCap) L.list[at] = k;
+    });
+    __syncthreads();
+    const int count = L.count;
+    if (count <= kCap) return count;
+    __syncthreads();
+  }
 }
 
 // A chunk's results: maximum, sum of e^(x - maximum), and pairs (key of the value, ~index).
@@ -194,6 +189,10 @@ struct BeamArgs {
 
 __device__ __forceinline__ Key1 key_of(float v, int i) {
   return Key1{(static_cast<uint64_t>(score_key_asc(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(i))};
+}
+
+__device__ __forceinline__ float key_float(uint32_t k) {
+  return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
 }
 
 template <typename T, int E>
@@ -220,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(BeamArgs a) {
 #pragma unroll
     for (int e = 0; e < N; ++e) top = fmaxf(top, v[j * N + e]);
   }
-  const float mine = top;
+  const uint32_t mine = score_key_asc(top);
   top = wave_max(top);
   if (lane == 0) red[wave] = top;
   __syncthreads();
@@ -253,18 +252,9 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(BeamArgs a) {
   };
   // By the values alone first, which is a comparison for each element.  (A NaN is below
   // everything here: its row counts as NaN throughout.)
-  float bound = mine;
-  {
-    int size = 64;
-    while (size > 1 && kThreads / size < a.n) size >>= 1;
-    for (int o = 1; o < size; o <<= 1) bound = fmaxf(bound, __shfl_xor(bound, o));
-    for (int o = size; o < 64; o <<= 1) bound = fminf(bound, __shfl_xor(bound, o));
-    __syncthreads();  // red is read
-    if (lane == 0) red[wave] = bound;
-    if (tid == 0) lists.count = 0;
-    __syncthreads();
-    bound = fminf(fminf(red[0], red[1]), fminf(red[2], red[3]));
-  }
+  const float bound = key_float(bound_of(mine, a.n, lists));
+  if (tid == 0) lists.count = 0;
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int i = c0 + (j * kThreads + tid) * N - off;
@@ -279,18 +269,8 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(BeamArgs a) {
   }
   __syncthreads();
   int c = lists.count;
-  if (c <= kCap) {
-    ranked(a.n, c, lists, put);
-    return;
-  }
-  // more equal ones than the list holds (masked rows): by value and index
-  Key1 best{0};
-  each([&](const Key1& k) {
-    if (better(k, best)) best = k;
-  });
-  c = collected(bound_of(best, a.n, lists.part), lists, each);
-  if (c <= kCap) ranked(a.n, c, lists, put);
-  else one_by_one(a.n, lists, each, put);
+  if (c > kCap) c = collected(a.n, lists, each);  // many equal ones (masked rows): by value and index
+  ranked(a.n, c, lists, put);
 }
 
 __device__ __forceinline__ uint64_t double_key(double v) {  // ascending; NaN above all, -0 as 0
@@ -302,9 +282,6 @@ __device__ __forceinline__ double key_double(uint64_t k) {
   if (k == ~0ull) return __longlong_as_double(0x7ff8000000000000ll);
   return __longlong_as_double(static_cast<long long>(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
-__device__ __forceinline__ float key_float(uint32_t k) {
-  return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
-}
 
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   __shared__ Lists<Key2> lists;
@@ -312,6 +289,19 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   __shared__ double shift[kMaxBeams];  // score - ln sum e^(x - top)
   __shared__ float tops[kMaxBeams];
   const int tid = threadIdx.x, b = a.first + blockIdx.x;
+  const int count = a.W * a.chunks, all = count * a.n;  // lists, and what they hold
+  const uint2* pairs = a.pairs + static_cast<int64_t>(b) * all;
+  // The lists by ranks: all lists' best, then all lists' second, so that neighbours, which
+  // are in different groups, are much alike.  A thread's first ones are under way while the
+  // sums are joined.
+  auto pair_at = [&](int i) {
+    const int rank = i / count;
+    return pairs[static_cast<int64_t>(i - rank * count) * a.n + rank];
+  };
+  constexpr int U = 4;
+  uint2 early[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) early[u] = u * kThreads + tid < all ? pair_at(u * kThreads + tid) : make_uint2(0, 0);
   // as many lanes to a row as it has chunks
   int lanes = 1;
   while (lanes < 64 && lanes < a.chunks) lanes *= 2;
@@ -326,7 +316,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     double sum = 0.0;
     for (int c = sub; c < a.chunks; c += lanes) {
       const float2 s = st[c];
-      sum += s.x == -INFINITY && s.y == 0.f ? 0.0 : s.y * exp(s.x - ts);
+      sum += s.x == -INFINITY && s.y == 0.f ? 0.0 : s.y * __expf(s.x - static_cast<float>(ts));
     }
     for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o);
     if (sub == 0) {  // a row of -inf alone has log probabilities -inf
@@ -335,20 +325,21 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     }
   }
   __syncthreads();
-  const int per = a.chunks * a.n, all = a.W * per;
-  const uint2* pairs = a.pairs + static_cast<int64_t>(b) * all;
-  auto key_at = [&](int i) {
-    const int w = i / per, j = i - w * per;
+  auto key_at = [&](int i, uint2 p) {
+    const int rank = i / count, x = i - rank * count, w = x / a.chunks;
     const double s = shift[w];
     if (!(fabs(s) < INFINITY))  // all of the beam's continuations are equal: its first ones
-      return j < a.n && j < a.V ? Key2{double_key(s), 0xffffffffu - static_cast<uint32_t>(w * a.V + j)} : Key2{0, 0};
-    const uint2 p = pairs[i];
+      return x == w * a.chunks && rank < a.V ? Key2{double_key(s), 0xffffffffu - static_cast<uint32_t>(w * a.V + rank)}
+                                             : Key2{0, 0};
     if (p.x == 0) return Key2{0, 0};
     return Key2{double_key(static_cast<double>(key_float(p.x)) - static_cast<double>(tops[w]) + s),
                 0xffffffffu - static_cast<uint32_t>(w * a.V + static_cast<int>(0xffffffffu - p.y))};
   };
   auto each = [&](auto&& f) {
-    for (int i = tid; i < all; i += kThreads) f(key_at(i));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u * kThreads + tid < all) f(key_at(u * kThreads + tid, early[u]));
+    for (int i = U * kThreads + tid; i < all; i += kThreads) f(key_at(i, pair_at(i)));
   };
   auto put = [&](int rank, const Key2& k) {
     const int flat = static_cast<int>(0xffffffffu - k.b), w = flat / a.V;
@@ -358,31 +349,34 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     a.tokens[at] = flat - w * a.V;
     a.parents[at] = b * a.W + w;
   };
-  if (all <= kCap) {
-    for (int i = tid; i < all; i += kThreads) lists.list[i] = key_at(i);
+  if (all <= kFew) {
+    if (tid < all) lists.list[tid] = key_at(tid, early[0]);
     __syncthreads();
     ranked(a.n, all, lists, put);
     return;
   }
-  Key2 best{0, 0};
+  uint32_t mine = 0;
+  each([&](const Key2& k) { mine = max(mine, rough(k)); });
+  const uint32_t bound = bound_of(mine, a.n, lists);
+  if (tid == 0) lists.count = 0;
+  __syncthreads();
   each([&](const Key2& k) {
-    if (better(k, best)) best = k;
+    if (k.a == 0 || rough(k) < bound) return;
+    const int at = atomicAdd(&lists.count, 1);
+    if (at < kCap) lists.list[at] = k;
   });
-  const int c = collected(bound_of(best, a.n, lists.part), lists, each);
-  if (c <= kCap) ranked(a.n, c, lists, put);
-  else one_by_one(a.n, lists, each, put);
+  __syncthreads();
+  int c = lists.count;
+  if (c > kCap) c = collected(a.n, lists, each);
+  ranked(a.n, c, lists, put);
 }
 
-// Elements of a thread: the longest chunks that leave every CU two workgroups.
-int elements_of(int64_t rows, int64_t V) {
-  for (int e = 32; e > 8; e /= 2)
-    if (rows * ((V + e * kThreads - 1) / (e * kThreads)) >= 2 * device_cus()) return e;
-  return 8;
-}
+// Elements of a thread.
+int elements_of(int64_t n) { return n <= 8 ? 16 : 32; }
 
 // A row that begins inside 16 bytes reaches up to 7 elements further.
-int64_t chunks_of(int64_t rows, int64_t V) {
-  const int64_t c = static_cast<int64_t>(elements_of(rows, V)) * kThreads;
+int64_t chunks_of(int64_t V, int64_t n) {
+  const int64_t c = static_cast<int64_t>(elements_of(n)) * kThreads;
   return (V + 7 + c - 1) / c;
 }
 
@@ -392,7 +386,7 @@ int check_beam(int64_t B, int64_t W, int64_t V, int64_t n, int dtype) {
   HYDRA_REQUIRE(V < (int64_t(1) << 31) && W * V < (int64_t(1) << 31) && n <= W * V,
                 "beam_select: continuations must be at most beams x vocabulary, and these below 2^31");
   HYDRA_REQUIRE(dtype_size(dtype) > 0, "beam_select: unknown dtype");
-  HYDRA_REQUIRE(B < (int64_t(1) << 31) / W && W * chunks_of(B * W, V) * n < (int64_t(1) << 31), "beam_select: too large");
+  HYDRA_REQUIRE(B < (int64_t(1) << 31) / W && W * chunks_of(V, n) * n < (int64_t(1) << 31), "beam_select: too large");
   return HYDRA_OK;
 }
 
@@ -405,8 +399,7 @@ int launch_beam(BeamArgs a, int e, hipStream_t st) {
     a.first = static_cast<int>(r);
     const dim3 grid(static_cast<unsigned>(a.chunks), static_cast<unsigned>(rows - r < 65535 ? rows - r : 65535));
     if (e == 32) beam_chunk_kernel<T, 32><<<grid, kThreads, 0, st>>>(a);
-    else if (e == 16) beam_chunk_kernel<T, 16><<<grid, kThreads, 0, st>>>(a);
-    else beam_chunk_kernel<T, 8><<<grid, kThreads, 0, st>>>(a);
+    else beam_chunk_kernel<T, 16><<<grid, kThreads, 0, st>>>(a);
   }
   constexpr int64_t most = int64_t(1) << 22;  // HIP counts a launch's threads in 32 bits
   for (int64_t b = 0; b < a.B; b += most) {
@@ -425,7 +418,7 @@ extern "C" int hydra_beam_select_workspace(int64_t B, int64_t W, int64_t V, int6
   const int rc = check_beam(B, W, V, n, dtype);
   if (rc != HYDRA_OK) return rc;
   HYDRA_REQUIRE(bytes != nullptr, "beam_select_workspace: null pointer");
-  const int64_t rows = B * W, chunks = B == 0 ? 0 : chunks_of(rows, V);
+  const int64_t rows = B * W, chunks = B == 0 ? 0 : chunks_of(V, n);
   *bytes = stats_bytes(rows, chunks) + rows * chunks * n * 8;
   return HYDRA_OK;
 }
@@ -439,7 +432,7 @@ extern "C" int hydra_beam_select(const void* logits, int64_t logits_rs, const fl
   HYDRA_REQUIRE(logits && scores && out_scores && beams && tokens && parents, "beam_select: null pointer");
   HYDRA_REQUIRE(logits_rs >= V || B * W == 1, "beam_select: row stride < vocabulary");
   HYDRA_REQUIRE(reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype) == 0, "beam_select: logits are not aligned to their type");
-  const int64_t rows = B * W, chunks = chunks_of(rows, V);
+  const int64_t rows = B * W, chunks = chunks_of(V, n);
   HYDRA_REQUIRE(workspace && aligned16(workspace) && workspace_size >= stats_bytes(rows, chunks) + rows * chunks * n * 8,
                 "beam_select: workspace too small");
   BeamArgs a{};
@@ -458,5 +451,5 @@ extern "C" int hydra_beam_select(const void* logits, int64_t logits_rs, const fl
   a.n = static_cast<int>(n);
   a.chunks = static_cast<int>(chunks);
   auto st = static_cast<hipStream_t>(stream);
-  return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int { return launch_beam<T>(a, elements_of(rows, V), st); });
+  return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int { return launch_beam<T>(a, elements_of(n), st); });
 }

@@ -201,12 +201,18 @@ __global__ __launch_bounds__(kThreads) void fork_take_kernel(ForkArgs a) {
 
 // All of it by one workgroup, where rows and their tables are few: 12.8 us on the device,
 // about what the five launches take there (4 rows of 12 pages), but one launch of the
-// host's instead of five.  What its threads hand each other through memory is written,
-// fenced and read past the first-level cache.
+// host's instead of five.  What its threads hand each other through memory need not leave
+// the XCD's L2: atomics, loads and fences are of the workgroup's scope.
 constexpr int kSmallRows = 256, kSmallEntries = 8192;
 
 __device__ __forceinline__ int seen(const int* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ void put(int* p, int v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ void add(int* p, int v) {
+  __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
 // Inclusive sum over 1024 threads; `total` gets the whole sum.
@@ -249,20 +255,20 @@ __global__ __launch_bounds__(kWide) void fork_small_kernel(ForkArgs a) {
     const int j = e / a.P, c = e - j * a.P;
     if (c >= held_of(a, len[j])) continue;
     old[e] = a.table[j * a.table_rs + c];
-    if (is_page(a, old[e])) a.owner[old[e]] = a.N;
+    if (is_page(a, old[e])) put(&a.owner[old[e]], a.N);
   }
-  __threadfence();
+  __threadfence_block();
   __syncthreads();
   for (int e = tid; e < all; e += kWide) {
     const int j = e / a.P, c = e - j * a.P;
     if (c >= held_of(a, len[j]) || !is_page(a, old[e])) continue;
-    if (c < full_of(a, len[j]) && kids[j] > 1) atomicAdd(&a.extra[old[e]], kids[j] - 1);
+    if (c < full_of(a, len[j]) && kids[j] > 1) add(&a.extra[old[e]], kids[j] - 1);
     if (kids[j] == 0) {
-      atomicAdd(&a.extra[old[e]], -1);
-      atomicMin(&a.owner[old[e]], j);
+      add(&a.extra[old[e]], -1);
+      __hip_atomic_fetch_min(&a.owner[old[e]], j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
   }
-  __threadfence();
+  __threadfence_block();
   __syncthreads();
   for (int e0 = 0; e0 < all; e0 += kWide) {
     const int e = e0 + tid, j = e < all ? e / a.P : 0, c = e - j * a.P;
@@ -271,12 +277,12 @@ __global__ __launch_bounds__(kWide) void fork_small_kernel(ForkArgs a) {
     int count;
     const int to = free + wide_incl_sum(back, part, count) - 1;
     if (back) {
-      a.extra[old[e]] = 0;
-      if (to < a.F) a.free_pages[to] = old[e];
+      put(&a.extra[old[e]], 0);
+      if (to < a.F) put(&a.free_pages[to], old[e]);
     }
     free = min(a.F, free + count);
   }
-  __threadfence();
+  __threadfence_block();
   __syncthreads();
   {
     int source = -1;
@@ -303,7 +309,7 @@ __global__ __launch_bounds__(kWide) void fork_small_kernel(ForkArgs a) {
   for (int e = tid; e < all; e += kWide) {
     const int i = e / a.P, c = e - i * a.P, p = par[i], n = p >= 0 ? len[p] : 0, full = full_of(a, n);
     const int held = held_of(a, n), from = c < held ? old[p * a.P + c] : -1;
-    if (!ok[i] && c < full && is_page(a, from)) atomicAdd(&a.extra[from], -1);  // its share of the filled pages
+    if (!ok[i] && c < full && is_page(a, from)) add(&a.extra[from], -1);  // its share of the filled pages
     a.table[i * a.table_rs + c] = !ok[i] ? -1 : (c == full && copy[i] >= 0 ? copy[i] : from);
   }
 }

@@ -119,11 +119,9 @@ __device__ __forceinline__ void put_bytes(char* row, int piece, int hd, const ui
   }
 }
 
-constexpr int kStore8Rows = 2;  // of a group of lanes, a key and a value each
-
 template <typename T, typename KV, bool VEC>
 __global__ __launch_bounds__(256) void store8_kernel(Rows8Args a) {
-  constexpr int U = kStore8Rows, E = Vec<T>::N;
+  constexpr int E = Vec<T>::N;
   const int piece = threadIdx.x & (a.lanes - 1), group = threadIdx.x >> a.log, groups = 256 >> a.log;
   const int h = blockIdx.y;
   for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
@@ -131,42 +129,27 @@ __global__ __launch_bounds__(256) void store8_kernel(Rows8Args a) {
     if (r < 0 || r >= a.R) continue;
     const int64_t* slots = a.slots + r * a.S;
     const char *k = a.k + n * a.k_st[0] + h * a.k_st[1], *v = a.v + n * a.v_st[0] + h * a.v_st[1];
-    int64_t slot[U];
-    float kx[U][E], vx[U][E];
+    const int64_t s = static_cast<int64_t>(blockIdx.x) * groups + group, slot = s < a.S ? slots[s] : -1;
+    if (slot < 0 || slot >= a.limit) continue;  // the lanes of a group together
+    float x[2][E];
+    row_values<T, VEC>(k + s * a.k_st[2], piece, a.hd, x[0]);
+    row_values<T, VEC>(v + s * a.v_st[2], piece, a.hd, x[1]);
+    const int64_t page = slot >> a.shift;
+    const uint32_t row = static_cast<uint32_t>(slot) & ((1u << a.shift) - 1);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t s = (static_cast<int64_t>(blockIdx.x) * U + u) * groups + group;
-      slot[u] = s < a.S ? slots[s] : -1;
-      const bool in = slot[u] >= 0 && slot[u] < a.limit;
-      if (!in) slot[u] = -1;
-      if (in) {  // the lanes of a group together
-        row_values<T, VEC>(k + s * a.k_st[2], piece, a.hd, kx[u]);
-        row_values<T, VEC>(v + s * a.v_st[2], piece, a.hd, vx[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) kx[u][i] = vx[u][i] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      uint32_t kt = top_bits<E>(kx[u]), vt = top_bits<E>(vx[u]);
-      for (int off = a.lanes >> 1; off > 0; off >>= 1) {
-        kt = max(kt, static_cast<uint32_t>(__shfl_xor(static_cast<int>(kt), off)));
-        vt = max(vt, static_cast<uint32_t>(__shfl_xor(static_cast<int>(vt), off)));
-      }
-      if (slot[u] < 0) continue;
-      const int64_t page = slot[u] >> a.shift;
-      const uint32_t row = static_cast<uint32_t>(slot[u]) & ((1u << a.shift) - 1);
-      float s, inv;
+    for (int c = 0; c < 2; ++c) {
+      uint32_t top = top_bits<E>(x[c]);
+      for (int off = a.lanes >> 1; off > 0; off >>= 1)
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off)));
+      float scale, inv;
       uint32_t w[E / 4];
-      scale_of<KV>(kt, s, inv);
-      to_bytes<KV, E>(kx[u], s, inv, w);
-      put_bytes<E, VEC>(a.kp + page * a.kp_st[0] + h * a.kp_st[1] + static_cast<uint64_t>(row) * a.kp_row, piece, a.hd, w);
-      if (piece == 0) a.ks[page * a.ks_st[0] + h * a.ks_st[1] + row] = s;
-      scale_of<KV>(vt, s, inv);
-      to_bytes<KV, E>(vx[u], s, inv, w);
-      put_bytes<E, VEC>(a.vp + page * a.vp_st[0] + h * a.vp_st[1] + static_cast<uint64_t>(row) * a.vp_row, piece, a.hd, w);
-      if (piece == 0) a.vs[page * a.vs_st[0] + h * a.vs_st[1] + row] = s;
+      scale_of<KV>(top, scale, inv);
+      to_bytes<KV, E>(x[c], scale, inv, w);
+      char* to = c ? a.vp + page * a.vp_st[0] + h * a.vp_st[1] + static_cast<uint64_t>(row) * a.vp_row
+                   : a.kp + page * a.kp_st[0] + h * a.kp_st[1] + static_cast<uint64_t>(row) * a.kp_row;
+      put_bytes<E, VEC>(to, piece, a.hd, w);
+      if (piece == 0)
+        (c ? a.vs[page * a.vs_st[0] + h * a.vs_st[1] + row] : a.ks[page * a.ks_st[0] + h * a.ks_st[1] + row]) = scale;
     }
   }
 }
@@ -184,70 +167,60 @@ __device__ __forceinline__ void from_word(uint32_t w, float s, float* x) {
   }
 }
 
-constexpr int kReadRows = 2;
-
 // Rows out of their pages, into k and v.  A lane writes 16 bytes of a row (an
 // element where rows are not made of such).
 template <typename T, typename KV, bool VEC>
 __global__ __launch_bounds__(256) void read_kernel(Rows8Args a) {
-  constexpr int U = kReadRows, E = VEC ? Vec<T>::N : 1;
+  constexpr int E = VEC ? Vec<T>::N : 1;
   constexpr bool EIGHT = sizeof(KV) == 1;
   const int lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x >> a.log, groups = 256 >> a.log;
   const int h = blockIdx.y;
+  const int64_t s = static_cast<int64_t>(blockIdx.x) * groups + group;
+  if (s >= a.S) return;
   for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
     const int64_t r = a.rows ? a.rows[n] : n;
-    const bool known = r >= 0 && r < a.R;
-    const int64_t* slots = a.slots + (known ? r : 0) * a.S;
+    const int64_t slot = r >= 0 && r < a.R ? a.slots[r * a.S + s] : -1;
+    const bool in = slot >= 0 && slot < a.limit;
+    const int64_t page = in ? slot >> a.shift : 0;
+    const uint32_t row = in ? static_cast<uint32_t>(slot) & ((1u << a.shift) - 1) : 0;
+    float scale[2] = {1.f, 1.f};
+    if constexpr (EIGHT) {
+      scale[0] = a.ks[page * a.ks_st[0] + h * a.ks_st[1] + row];
+      scale[1] = a.vs[page * a.vs_st[0] + h * a.vs_st[1] + row];
+    }
     for (int piece = lane; piece * E < a.hd; piece += a.lanes) {
-      float x[U][2][E];
-      int64_t at[U];
+      float x[2][E];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t s = (static_cast<int64_t>(blockIdx.x) * U + u) * groups + group;
-        at[u] = s < a.S ? s : -1;
-        const int64_t slot = s < a.S && known ? slots[s] : -1;
-        const bool in = slot >= 0 && slot < a.limit;
-        const int64_t page = in ? slot >> a.shift : 0;
-        const uint32_t row = in ? static_cast<uint32_t>(slot) & ((1u << a.shift) - 1) : 0;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const char* p = (c ? a.vp + page * a.vp_st[0] + h * a.vp_st[1] + static_cast<uint64_t>(row) * a.vp_row
-                             : a.kp + page * a.kp_st[0] + h * a.kp_st[1] + static_cast<uint64_t>(row) * a.kp_row) +
-                          static_cast<int64_t>(piece) * E * static_cast<int>(sizeof(KV));
-          float s8 = 1.f;
-          if constexpr (EIGHT)
-            s8 = c ? a.vs[page * a.vs_st[0] + h * a.vs_st[1] + row] : a.ks[page * a.ks_st[0] + h * a.ks_st[1] + row];
-          if constexpr (!VEC) {
-            if constexpr (EIGHT) {
-              float f[4];
-              from_word<KV>(*reinterpret_cast<const uint8_t*>(p), s8, f);
-              x[u][c][0] = f[0];
-            } else {
-              x[u][c][0] = to_f32(*reinterpret_cast<const T*>(p));
-            }
-          } else if constexpr (EIGHT) {
-#pragma unroll
-            for (int i = 0; i < E / 4; ++i) from_word<KV>(reinterpret_cast<const uint32_t*>(p)[i], s8, x[u][c] + 4 * i);
+      for (int c = 0; c < 2; ++c) {
+        const char* p = (c ? a.vp + page * a.vp_st[0] + h * a.vp_st[1] + static_cast<uint64_t>(row) * a.vp_row
+                           : a.kp + page * a.kp_st[0] + h * a.kp_st[1] + static_cast<uint64_t>(row) * a.kp_row) +
+                        static_cast<int64_t>(piece) * E * static_cast<int>(sizeof(KV));
+        if constexpr (!VEC) {
+          if constexpr (EIGHT) {
+            float f[4];
+            from_word<KV>(*reinterpret_cast<const uint8_t*>(p), scale[c], f);
+            x[c][0] = f[0];
           } else {
-            load16<T>(reinterpret_cast<const T*>(p), x[u][c]);
+            x[c][0] = to_f32(*reinterpret_cast<const T*>(p));
           }
-          if (!in) {
+        } else if constexpr (EIGHT) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[u][c][i] = 0.f;
-          }
+          for (int i = 0; i < E / 4; ++i) from_word<KV>(reinterpret_cast<const uint32_t*>(p)[i], scale[c], x[c] + 4 * i);
+        } else {
+          load16<T>(reinterpret_cast<const T*>(p), x[c]);
+        }
+        if (!in) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) x[c][i] = 0.f;
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (at[u] < 0) continue;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          T* to = reinterpret_cast<T*>(const_cast<char*>(
-                      c ? a.v + n * a.v_st[0] + h * a.v_st[1] + at[u] * a.v_st[2]
-                        : a.k + n * a.k_st[0] + h * a.k_st[1] + at[u] * a.k_st[2])) + static_cast<int64_t>(piece) * E;
-          if constexpr (VEC) store16<T, true>(to, x[u][c]);
-          else *to = from_f32<T>(x[u][c][0]);
-        }
+      for (int c = 0; c < 2; ++c) {
+        T* to = reinterpret_cast<T*>(const_cast<char*>(c ? a.v + n * a.v_st[0] + h * a.v_st[1] + s * a.v_st[2]
+                                                         : a.k + n * a.k_st[0] + h * a.k_st[1] + s * a.k_st[2])) +
+                static_cast<int64_t>(piece) * E;
+        if constexpr (VEC) store16<T, true>(to, x[c]);
+        else *to = from_f32<T>(x[c][0]);
       }
     }
   }
@@ -330,8 +303,8 @@ void set_lanes(Rows8Args& a, int64_t pieces) {
   a.lanes = 1 << a.log;
 }
 
-dim3 grid_of(const Rows8Args& a, int64_t Hkv, int rows) {
-  const int64_t span = static_cast<int64_t>(256 >> a.log) * rows;
+dim3 grid_of(const Rows8Args& a, int64_t Hkv) {
+  const int64_t span = 256 >> a.log;
   return dim3(static_cast<unsigned>((a.S + span - 1) / span), static_cast<unsigned>(Hkv),
               static_cast<unsigned>(a.N < 65535 ? a.N : 65535));
 }
@@ -354,7 +327,7 @@ extern "C" int hydra_page_store8(const void* k, const void* v, void* k_pages, vo
   if (rc != HYDRA_OK || N == 0 || S == 0) return rc;
   const int e = dtype_size(dtype);
   set_lanes(a, (hd * e + 15) / 16);
-  const dim3 grid = grid_of(a, Hkv, kStore8Rows);
+  const dim3 grid = grid_of(a, Hkv);
   HYDRA_REQUIRE(grid_fits(grid.x, 256), "page_store8: too large");
   auto st = static_cast<hipStream_t>(stream);
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
@@ -381,7 +354,7 @@ extern "C" int hydra_page_read(const void* k_pages, const void* v_pages, const f
   if (rc != HYDRA_OK || N == 0 || S == 0) return rc;
   const int e = dtype_size(dtype);
   set_lanes(a, vec ? hd * e / 16 : hd);
-  const dim3 grid = grid_of(a, Hkv, kReadRows);
+  const dim3 grid = grid_of(a, Hkv);
   HYDRA_REQUIRE(grid_fits(grid.x, 256), "page_read: too large");
   auto st = static_cast<hipStream_t>(stream);
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int {

@@ -1062,8 +1062,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a)
 // four elements each, the parts dealt out over the threads left.  Zeros where no
 // key was seen.  Without groups, items that one workgroup had whole are written.
 template <typename C, int TPR>
-__global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void prefix_join_kernel(PrefixArgs a, int rows_a) {
-  constexpr int ROWS = TPR < kThreads ? kThreads / TPR : 1, WAVES = TPR / 64;
+__global__ __launch_bounds__(kThreads) void prefix_join_kernel(PrefixArgs a, int rows_a) {
+  constexpr int ROWS = kThreads / TPR, WAVES = TPR / 64;
   __shared__ float4 sums[TPR > 64 ? TPR : 1];
   __shared__ float lsum[TPR > 64 ? TPR : 1], tops[WAVES];
   const int tid = threadIdx.x % TPR, lane = threadIdx.x & 63, wave = tid >> 6;
@@ -1182,8 +1182,7 @@ int launch_split(PrefixArgs a, int rows_a, hipStream_t st) {
   a.wgs = std::min(a.wgs, a.cus * blocks_per_cu(reinterpret_cast<const void*>(kernel), kThreads));
   kernel<<<a.wgs, kThreads, 0, st>>>(a);
   const int64_t rows = static_cast<int64_t>(a.N) * a.H;
-  if (rows <= 32) prefix_join_kernel<C, 1024><<<static_cast<unsigned>(rows), 1024, 0, st>>>(a, rows_a);
-  else if (rows <= 2048) prefix_join_kernel<C, 256><<<static_cast<unsigned>(rows), 256, 0, st>>>(a, rows_a);
+  if (rows <= 256) prefix_join_kernel<C, 256><<<static_cast<unsigned>(rows), 256, 0, st>>>(a, rows_a);
   else prefix_join_kernel<C, 64><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(a, rows_a);
   return check_launch("prefix_attn");
 }

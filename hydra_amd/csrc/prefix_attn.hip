@@ -46,7 +46,8 @@ int pieces_of(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, int
   p.requests = std::min<int64_t>(kRequests, (int64_t(1) << 29) / (rounds * Hkv * (p.GB + 1)));
   const int64_t items = N * Hkv * p.GB;
   p.waves = items > device_cus() || cap <= kRound ? 4 : whole_waves(p.s.hdp);
-  p.split = groups > 0 || (N <= p.requests && items < 8 * device_cus() && cap > (p.waves == 16 ? 16 : 8) * kRound);
+  const int64_t whole = 4 * items <= device_cus() ? p.waves / 2 : p.waves == 16 ? 16 : 8;
+  p.split = groups > 0 || (N <= p.requests && items < 8 * device_cus() && rounds > whole);
   HYDRA_REQUIRE(p.requests >= 1 || !p.split, "prefix_attn: too large");
   p.wgs = static_cast<int64_t>(groups > 0 ? 2 : 4) * device_cus();
   const int64_t r4 = row4(static_cast<int>(hd));
