@@ -5,7 +5,9 @@
 //
 // in descending order, the lowest w V + v first among equals.
 //
-// Bound by one pass over the logits.  Each workgroup reads a chunk of a row into
+// Bound by one pass over the logits where texts are many: 32 texts of 8 beams by 32000,
+// bf16 (16 MB), n = 16: 10.0 us, and 7.7 to join; for one text of 4 beams by 50257, n = 4,
+// by latency: 5.6 and 4.9 us.  Each workgroup reads a chunk of a row into
 // registers, takes its maximum and its sum of exponentials (fp32) and leaves the
 // chunk's n best (value, index) pairs; a second kernel joins the chunks' sums,
 // and orders the chunks' pairs by their scores in fp64 (two beams' continuations may be
@@ -25,7 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCap = 2048;       // collected elements
-constexpr int kFew = 64;         // elements that are ranked as they are
+constexpr int kFew = 64;         // elements that are ranked as they are, which takes a comparison for each thread
 constexpr int kMaxCount = 128;   // n
 constexpr int kMaxBeams = 1024;  // W
 
@@ -371,7 +373,11 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   ranked(a.n, c, lists, put);
 }
 
-// Elements of a thread.
+// Elements of a thread.  Longer chunks leave less to join: in a graph, 16 against 32, us,
+//   n = 1, 1 beam by 50257: 8.4 : 9.2        n = 4, 4 beams by 50257: 10.6 : 11.5
+//   n = 4, 32 x 8 by 32000: 13.4 : 13.5      n = 16, 4 x 8 by 32000: 15.3 : 14.2
+//   n = 16, 16 by 32000: 17.6 : 15.6         n = 32, 32 x 16 by 50257: 60 : 49
+// and 8 lost to 16 throughout (n = 4, 4 beams by 50257: equal; n = 16, 16 by 32000: 27 : 21).
 int elements_of(int64_t n) { return n <= 8 ? 16 : 32; }
 
 // A row that begins inside 16 bytes reaches up to 7 elements further.

@@ -13,6 +13,13 @@
 // last place and the difference is at most s).
 //
 // A row with an infinity or NaN gets the scale NaN and zeros: it reads back as NaN.
+//
+// Bound by memory: 16 bytes a lane, the lanes of a row side by side, a key and a value row
+// to each group of lanes, which makes two loads in flight; more rows to a group were
+// slower at every size (four: 14.9 us for both ways of 1003 rows of 4 heads of 16 in a
+// graph, 102 for those below; two: 9.4 and 91; one: 6.4 and 82).  16 prompts of 4096
+// rows of 8 heads of 128, bf16 and int8 (407 MB each way): 82 us for both, 9.9 TB/s, part of it
+// from the last-level cache; 2 heads of 64 to e4m3 and back: 6.7 and 9.1 us.
 #include "common.h"
 
 namespace hydra {

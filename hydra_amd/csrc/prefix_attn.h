@@ -37,6 +37,18 @@
 // all workgroups so that each has as much to do, whatever the lengths.  What a workgroup leaves of an item is (max, sum, unscaled
 // output) per row in the workspace; a second kernel joins each row's parts in their
 // order.  No atomics on results: the same inputs give the same bits.
+//
+// What bounds it, by the kernels' own times:
+//
+//  * B items, many long ones: the reading of the pages.  64 requests of 16384 keys, 8/2
+//    heads of 64 in e4m3 (285 MB) take 53.6 us, 5.3 TB/s, and 4.9 us to join; 256 of
+//    4096, 32/8 heads of 128 in int8 (2.2 GB), 447 us, 4.9 TB/s;
+//  * A items of many rows: the matrix cores and the softmax, in turn.  256 requests that
+//    share 32768 keys, 32/8 heads of 128 (137 GFLOP), with 600 keys of their own each:
+//    235 us.  The instructions alone, with the second terms of P, are 100 us; without the second
+//    terms, and without the loads, it would be 40 us less each, without the softmax 20;
+//  * few requests: the chain of launch, plan, table, keys and join.  8 groups of 4
+//    requests by 1500 keys: 8.4 us and 4.3 to join; one request of 700: 8.6 us.
 #pragma once
 #include "common.h"
 #include "lds_dma.h"
@@ -841,7 +853,9 @@ constexpr int lds_bytes(int nt, int rw, bool vec, int nw = 4) {
 }
 
 // One workgroup per B item, no split.  Few items get as many waves as registers and LDS
-// let one have.
+// let one have: 4/1 heads of 64 by 1024 keys 10.2 us with 16 waves, 12.5 with 4; where
+// items fill the CUs 4 waves waste less (48 requests of 8 key heads of 128 by 512 keys:
+// 18.3 us, with 8 waves 22.3).
 constexpr int whole_waves(int hdp) { return hdp <= 64 ? 16 : hdp == 128 ? 8 : 4; }
 
 template <typename C, typename KV, int HDP, bool VEC, int NW>
@@ -1171,6 +1185,8 @@ inline Shape shape_of(int64_t hd, int64_t G, int64_t W, bool groups, int e, bool
   s.vec = vec;
   s.hdp = !vec ? 256 : hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   const int nt = tiles_a(s.hdp, e == 4);
+  // 16 bits of the queries' own type: as fast either way (8 groups of 16 rows by 1500 keys of 64: 12.6 us);
+  // 8 bits 13.0 : 15.6 there, fp32 15.0 : 21.7
   s.rw = !groups ? 0 : W * G <= 16 * nt ? 1 : 4;
   s.rows_a = 16 * nt * (s.rw == 4 ? 4 : 1);
   return s;
@@ -1182,6 +1198,8 @@ int launch_split(PrefixArgs a, int rows_a, hipStream_t st) {
   a.wgs = std::min(a.wgs, a.cus * blocks_per_cu(reinterpret_cast<const void*>(kernel), kThreads));
   kernel<<<a.wgs, kThreads, 0, st>>>(a);
   const int64_t rows = static_cast<int64_t>(a.N) * a.H;
+  // a workgroup or a wave to a row: 8 rows of 32768 keys 13.6 : 23.0 us (with the split), 256 rows of 8192
+  // 25.7 : 26.8, 384 rows 29.1 : 28.8, 8000 rows 480 : 473
   if (rows <= 256) prefix_join_kernel<C, 256><<<static_cast<unsigned>(rows), 256, 0, st>>>(a, rows_a);
   else prefix_join_kernel<C, 64><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(a, rows_a);
   return check_launch("prefix_attn");

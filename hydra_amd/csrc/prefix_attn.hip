@@ -34,8 +34,20 @@ int check_prefix(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, 
 }
 
 // Split where one workgroup for each item would leave CUs idle and a request may be
-// longer than a few rounds.  The workspace does not depend on how rows are aligned:
-// `vec` false takes the most.
+// longer than a few rounds: than its waves take in two steps of 32 keys each, where items
+// are few.  Measured in a graph, one workgroup an item against split, us, all requests of
+// one length (ragged ones in brackets, up to that length):
+//
+//   4/1 heads of 64, 1 request:     1024 keys 10.3 : 9.5      2048 keys 15.0 : 9.5
+//   32/8 heads of 128, 4 requests:  512 keys 12.0 : 11.6      1024 keys 16.5 : 11.9
+//   4/1 heads of 256, 24 requests:  256 keys 16.6 : 17.6      512 keys 22.3 : 18.1
+//   28/4 heads of 16, 24 requests:  1500 keys 10.8 : 13.0 (10.5 : 10.0)
+//   32/8 heads of 128, 24 requests: 1024 keys 18.8 : 23.7 (16.2 : 16.0)
+//   28/4 heads of 16, 256 requests: 2048 keys 37.6 : 42.2     4096 keys 65.8 : 71.5
+//
+// With many items the split costs up to a quarter where all are equally long, and only
+// lengths that differ (which the host does not know) repay it.  By sizes alone, so that the
+// workspace does not depend on how rows are aligned.
 int pieces_of(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, int64_t P, int64_t page_size, int dtype,
               bool vec, Pieces& p) {
   const int64_t G = H / Hkv, W = groups > 0 ? N / groups : 1, cap = P * page_size;
@@ -46,7 +58,8 @@ int pieces_of(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, int
   p.requests = std::min<int64_t>(kRequests, (int64_t(1) << 29) / (rounds * Hkv * (p.GB + 1)));
   const int64_t items = N * Hkv * p.GB;
   p.waves = items > device_cus() || cap <= kRound ? 4 : whole_waves(p.s.hdp);
-  const int64_t whole = 4 * items <= device_cus() ? p.waves / 2 : p.waves == 16 ? 16 : 8;
+  const int most = whole_waves(shape_of(hd, G, W, groups > 0, dtype_size(dtype), true).hdp);
+  const int64_t whole = 4 * items <= device_cus() ? most / 2 : items <= device_cus() && most == 16 ? 16 : 8;
   p.split = groups > 0 || (N <= p.requests && items < 8 * device_cus() && rounds > whole);
   HYDRA_REQUIRE(p.requests >= 1 || !p.split, "prefix_attn: too large");
   p.wgs = static_cast<int64_t>(groups > 0 ? 2 : 4) * device_cus();
