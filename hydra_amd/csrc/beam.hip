@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     double sum = 0.0;
     for (int c = sub; c < a.chunks; c += lanes) {
       const float2 s = st[c];
-      sum += s.x == -INFINITY && s.y == 0.f ? 0.0 : s.y * __expf(s.x - static_cast<float>(ts));
+      sum += s.x == -INFINITY && s.y == 0.f ? 0.0 : s.y * exp(s.x - ts);
     }
     for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o);
     if (sub == 0) {  // a row of -inf alone has log probabilities -inf

@@ -42,10 +42,10 @@
 //
 //  * B items, many long ones: the reading of the pages.  64 requests of 16384 keys, 8/2
 //    heads of 64 in e4m3 (285 MB) take 53.6 us, 5.3 TB/s, and 4.9 us to join; 256 of
-//    4096, 32/8 heads of 128 in int8 (2.2 GB), 447 us, 4.9 TB/s;
+//    4096, 32/8 heads of 128 in int8 (2.2 GB), 386 us, 5.7 TB/s;
 //  * A items of many rows: the matrix cores and the softmax, in turn.  256 requests that
 //    share 32768 keys, 32/8 heads of 128 (137 GFLOP), with 600 keys of their own each:
-//    235 us.  The instructions alone, with the second terms of P, are 100 us; without the second
+//    235 us (over e4m3 335, int8 375: their general form widens every tile in each wave).  The instructions alone, with the second terms of P, are 100 us; without the second
 //    terms, and without the loads, it would be 40 us less each, without the softmax 20;
 //  * few requests: the chain of launch, plan, table, keys and join.  8 groups of 4
 //    requests by 1500 keys: 8.4 us and 4.3 to join; one request of 700: 8.6 us.
@@ -1179,11 +1179,12 @@ struct Shape {
   bool vec;
 };
 
-// Rows that 16-byte loads cannot take come through the widest form.
+// Rows that 16-byte loads cannot take come element by element, in forms of 64 and 256
+// channels.
 inline Shape shape_of(int64_t hd, int64_t G, int64_t W, bool groups, int e, bool vec) {
   Shape s{};
   s.vec = vec;
-  s.hdp = !vec ? 256 : hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+  s.hdp = !vec ? (hd <= 64 ? 64 : 256) : hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   const int nt = tiles_a(s.hdp, e == 4);
   // 16 bits of the queries' own type: as fast either way (8 groups of 16 rows by 1500 keys of 64: 12.6 us);
   // 8 bits 13.0 : 15.6 there, fp32 15.0 : 21.7
@@ -1227,6 +1228,7 @@ int launch_form(const PrefixArgs& a, const Shape& s, hipStream_t st) {
 
 template <typename C, typename KV>
 int launch_pages(const PrefixArgs& a, const Shape& s, hipStream_t st) {
+  if (!s.vec && s.hdp == 64) return launch_form<C, KV, 64, false>(a, s, st);
   if (!s.vec) return launch_form<C, KV, 256, false>(a, s, st);
   switch (s.hdp) {
     case 32: return launch_form<C, KV, 32, true>(a, s, st);
