@@ -387,7 +387,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     only: no gradient."""
     name = "paged_attention"
     if scales is not None or shared is not None:
-        return _prefix_attention(name, q, k_pages, v_pages, table, lengths, scale, out, scales, shared)
+        return _prefix_attention(name, q, k_pages, v_pages, table, lengths, None if scale is None else float(scale), out,
+                                 scales, shared)
     _lib.require_gpu(name, q, k_pages, v_pages, table, lengths, out)
     check_pages(name, k_pages, v_pages)
     pages, K, page, hd = k_pages.shape
@@ -453,7 +454,7 @@ def _prefix_call(name, scale, *layouts):
     groups = 0
     if shared is not None:
         groups = _vector(name, "shared", shared, torch.int32).shape[0]
-        if groups == 0 or N % groups != 0:
+        if (groups == 0 and N > 0) or (groups > 0 and N % groups != 0):
             raise ValueError(f"{name}: {N} requests are no multiple of {groups} groups")
         if groups == N:  # nobody shares anything
             groups = 0
@@ -466,7 +467,7 @@ def _prefix_call(name, scale, *layouts):
     _lib.call("hydra_prefix_attn_workspace", groups, N, H, K, hd, P, page, code, of, ctypes.byref(need))
     return (copies, (groups, N, H, K, hd, P, page, pages, _strides(q), _strides(kp), _strides(vp),
                      *((None, None) if ks is None else (_strides(ks), _strides(vs))), _strides(out),
-                     hd ** -0.5 if scale is None else float(scale), code, of), groups, need.value, _row_stride(table),
+                     hd ** -0.5 if scale is None else scale, code, of), groups, need.value, _row_stride(table),
             _lib.load().hydra_prefix_attn)
 
 
@@ -613,7 +614,8 @@ def _take_call(name, *layouts):
 def take_rows(x: torch.Tensor, parents: torch.Tensor) -> None:
     """x[i] = x[parents[i]] in place, all rows at once (int32 [N], N = len(x)
     up to 8192); a parent outside [0, N) leaves its row as it is.  Any dtype; rows
-    are contiguous and do not overlap.  Inference only: no gradient."""
+    are contiguous, do not overlap, and are none of the parents' memory.  Inference
+    only: no gradient."""
     name = "take_rows"
     stride, row, N, entry = _take_call(name, _lib.layout(x), _lib.layout(parents))
     check_no_gradient(name, x)

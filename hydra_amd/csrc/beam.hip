@@ -388,11 +388,12 @@ int64_t chunks_of(int64_t V, int64_t n) {
 
 int check_beam(int64_t B, int64_t W, int64_t V, int64_t n, int dtype) {
   HYDRA_REQUIRE(B >= 0 && W >= 1 && V >= 1 && n >= 1, "beam_select: bad size");
+  HYDRA_REQUIRE(V <= (int64_t(1) << 31) - (1 << 14), "beam_select: vocabulary must be at most 2^31 - 2^14");  // a chunk's end in 32 bits
   HYDRA_REQUIRE(W <= kMaxBeams && n <= kMaxCount, "beam_select: at most 1024 beams and 128 continuations of a text");
-  HYDRA_REQUIRE(V < (int64_t(1) << 31) && W * V < (int64_t(1) << 31) && n <= W * V,
+  HYDRA_REQUIRE(W * V < (int64_t(1) << 31) && n <= W * V,
                 "beam_select: continuations must be at most beams x vocabulary, and these below 2^31");
   HYDRA_REQUIRE(dtype_size(dtype) > 0, "beam_select: unknown dtype");
-  HYDRA_REQUIRE(B < (int64_t(1) << 31) / W && W * chunks_of(V, n) * n < (int64_t(1) << 31), "beam_select: too large");
+  HYDRA_REQUIRE(B < (int64_t(1) << 31) / W, "beam_select: too large");
   return HYDRA_OK;
 }
 

@@ -868,9 +868,14 @@ __global__ __launch_bounds__(64 * NW) void prefix_whole_kernel(PrefixArgs a) {
   write_out<C, HDP>(a, it, st);
 }
 
+// Waves of a SIMD that registers are to suffice for.  256 channels without groups: 70.5 us
+// with 1, 81 with 2 (60 dwords spilt; 64 requests of 8192 keys, 4/1 heads in e4m3, pages out
+// of the caches).  64 channels come to 3 by themselves: 68.8 us (64 x 16384 keys), with 4 the same.
+constexpr int split_waves(int hdp, int rw) { return rw == 0 && hdp == 256 ? 1 : 2; }
+
 // Split form; RW 0: without groups.
 template <typename C, typename KV, int HDP, int RW, bool VEC>
-__global__ __launch_bounds__(kThreads, 2) void prefix_split_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(kThreads, split_waves(HDP, RW)) void prefix_split_kernel(PrefixArgs a) {
   constexpr int NT = tiles_a(HDP, sizeof(C) == 4), RA = RW == 0 ? 1 : RW, ROWS = 16 * NT * RA;
   constexpr int LDS_A = RW == 0 ? 0 : lds_bytes<C, KV, HDP>(NT, RA, VEC), LDS_B = lds_bytes<C, KV, HDP>(1, 1, VEC);
   __shared__ __attribute__((aligned(16))) char lds[LDS_A > LDS_B ? LDS_A : LDS_B];

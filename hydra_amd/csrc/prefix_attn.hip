@@ -55,7 +55,8 @@ int pieces_of(int64_t groups, int64_t N, int64_t H, int64_t Hkv, int64_t hd, int
   p.s = shape_of(hd, G, W, groups > 0, dtype_size(dtype), vec);
   p.GB = (G + 15) / 16;
   const int64_t rounds = (cap + kRound - 1) / kRound;
-  p.requests = std::min<int64_t>(kRequests, (int64_t(1) << 29) / (rounds * Hkv * (p.GB + 1)));
+  // rounds and rows of a launch are counted, and its threads launched, in 32 bits
+  p.requests = std::min<int64_t>(std::min<int64_t>(kRequests, (int64_t(1) << 25) / H), (int64_t(1) << 29) / (rounds * Hkv * (p.GB + 1)));
   const int64_t items = N * Hkv * p.GB;
   p.waves = items > device_cus() || cap <= kRound ? 4 : whole_waves(p.s.hdp);
   const int most = whole_waves(shape_of(hd, G, W, groups > 0, dtype_size(dtype), true).hdp);

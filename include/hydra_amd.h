@@ -482,8 +482,8 @@ int hydra_token_logprobs_bwd(const void* logits, int64_t rows, int64_t vocab, in
  * fp32, beams (w), tokens (v) int64 and parents (b W + w) int32 [B, n].  NaN counts as
  * larger than any number, and a row with NaN or +inf is NaN throughout; of a beam whose
  * continuations are all alike (its score or its row not finite) the first tokens are
- * meant.  W <= 1024, n <= 128, n <= W V < 2^31.  Needs hydra_beam_select_workspace bytes
- * of device scratch (16-byte aligned). */
+ * meant.  W <= 1024, n <= 128, n <= W V < 2^31, V <= 2^31 - 2^14.  Needs
+ * hydra_beam_select_workspace bytes of device scratch (16-byte aligned). */
 int hydra_beam_select(const void* logits, int64_t logits_rs, const float* scores, int64_t B,
                       int64_t W, int64_t V, int64_t n, float* out_scores, int64_t* beams,
                       int64_t* tokens, int* parents, int dtype, void* workspace,
