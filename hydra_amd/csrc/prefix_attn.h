@@ -45,9 +45,10 @@
 //    4096, 32/8 heads of 128 in int8 (2.2 GB), 386 us, 5.7 TB/s;
 //  * A items of many rows: the matrix cores and the softmax, in turn.  256 requests that
 //    share 32768 keys, 32/8 heads of 128 (137 GFLOP), with 600 keys of their own each:
-//    235 us (over e4m3 335, int8 375: their general form widens every tile
-//    of keys in each wave; once for all of them, through LDS, it was 336 and 355).  The instructions alone, with the second terms of P, are 100 us; without the second
-//    terms, and without the loads, it would be 40 us less each, without the softmax 20;
+//    235 us (over e4m3 335, int8 375: their general form widens every tile of keys in
+//    each wave; once for all of them, through LDS, it was 336 and 355).  The matrix
+//    instructions alone, with the second terms of P, are 100 us; without the second terms,
+//    and without the loads, it would be 40 us less each, without the softmax 20;
 //  * few requests: the chain of launch, plan, table, keys and join.  8 groups of 4
 //    requests by 1500 keys: 8.4 us and 4.3 to join; one request of 700: 8.6 us.
 #pragma once
