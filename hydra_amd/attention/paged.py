@@ -266,7 +266,8 @@ def _store_eight_call(name, *layouts):
         raise ValueError(f"{name}: k and v must share a dtype")
     N, S = k.shape[0], k.shape[2]
     _check_rows_of_slots(name, N, S, slots, rows)
-    copies = (hd > 1 and (k.stride(-1) != 1 or v.stride(-1) != 1)) or not slots.is_contiguous() or \
+    # (without elements a copy would be the tensor itself, of whatever strides)
+    copies = (N * S > 0 and hd > 1 and (k.stride(-1) != 1 or v.stride(-1) != 1)) or not slots.is_contiguous() or \
         not (rows is None or rows.is_contiguous())
     return (copies, slots.shape[0], (N, K, S, hd, pages, page, *map(_strides, (k, v, kp, vp, ks, vs)), _lib.dtype_code(k),
                                      _lib.PAGE_CODE[kp.dtype]), _lib.load().hydra_page_store8)
@@ -459,7 +460,8 @@ def _prefix_call(name, scale, *layouts):
         if groups == N:  # nobody shares anything
             groups = 0
     P, code = table.shape[1], _lib.dtype_code(q)
-    copies = (hd > 1 and q.stride(-1) != 1) or not lengths.is_contiguous() or not (shared is None or shared.is_contiguous())
+    copies = (N > 0 and hd > 1 and q.stride(-1) != 1) or not lengths.is_contiguous() or \
+        not (shared is None or shared.is_contiguous())  # (an empty q counts as contiguous whatever its strides)
     if groups == 0 and ks is None:
         return copies, None, 0, 0, None, None
     of = code if ks is None else _lib.PAGE_CODE[kp.dtype]

@@ -1,0 +1,34 @@
+"""GPU tests of calls of the operators that continue several texts which their
+documentation allows and the other files pass over."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_prefix_attention import EIGHT, Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("eight", EIGHT)
+def test_nothing_to_do_of_any_strides(cuda, eight):
+    """An empty tensor counts as contiguous whatever its strides are."""
+    from hydra_amd.attention import paged_attention, store_pages
+
+    pages = torch.zeros(2, 2, 16, 8, device=cuda).to(eight)
+    scales = tuple(torch.ones(2, 2, 16, device=cuda) for _ in range(2))
+    before = pages.view(torch.int8).clone()
+    for n, s in ((0, 4), (3, 0), (0, 0)):
+        k = torch.zeros(n, 2, 8, s, device=cuda).transpose(2, 3)
+        assert k.stride(-1) != 1 or s == 0
+        wide = torch.zeros(n, 2, s, 16, device=cuda)[..., ::2]
+        slots = torch.zeros(n, s, dtype=torch.int64, device=cuda)
+        for rows in (k, wide):
+            store_pages(rows, rows, pages, pages.clone(), slots, scales=scales)
+    assert torch.equal(pages.view(torch.int8), before)
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=cuda)  # noqa: E731
+    for q in (torch.zeros(0, 8, 4, device=cuda).transpose(1, 2), torch.zeros(0, 4, 16, device=cuda)[..., ::2]):
+        for kw in (dict(scales=scales), dict(scales=scales, shared=ints(0))):
+            assert paged_attention(q, pages, pages, ints(0, 3), ints(0), **kw).shape == (0, 4, 8)
+        plain = torch.zeros(2, 2, 16, 8, device=cuda)
+        assert paged_attention(q, plain, plain, ints(0, 3), ints(0), shared=ints(0)).shape == (0, 4, 8)
