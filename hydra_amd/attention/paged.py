@@ -278,7 +278,7 @@ def _store_eight(name, k, v, k_pages, v_pages, slots, rows, scales):
     layout = _lib.layout
     copies, R, sizes, entry = _store_eight_call(name, layout(k), layout(v), layout(k_pages), layout(v_pages), layout(slots),
                                                 layout(rows), layout(ks), layout(vs))
-    check_no_gradient(name, k, v, k_pages, v_pages)
+    check_no_gradient(name, k, v, k_pages, v_pages, ks, vs)
     if copies:
         _store_eight(name, k.contiguous(), v.contiguous(), k_pages, v_pages, slots.contiguous(),
                      None if rows is None else rows.contiguous(), scales)
@@ -329,7 +329,7 @@ def read_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor
     layout = _lib.layout
     dtype, shape, sizes, entry = _read_call(name, dtype, layout(k_pages), layout(v_pages), layout(slots), layout(rows),
                                             layout(ks), layout(vs))
-    check_no_gradient(name, k_pages, v_pages)
+    check_no_gradient(name, k_pages, v_pages, ks, vs)
     slots, rows = slots.contiguous(), None if rows is None else rows.contiguous()
     out = torch.empty(shape, dtype=dtype, device=k_pages.device)
     k, v = out.unbind(0)
@@ -482,7 +482,7 @@ def _prefix_attention(name, q, k_pages, v_pages, table, lengths, scale, out, sca
         copies, sizes, groups, need, table_rs, entry = _prefix_call(
             name, scale, layout(q), layout(k_pages), layout(v_pages), layout(table), layout(lengths), layout(out),
             layout(ks), layout(vs), layout(shared))
-        check_no_gradient(name, q, k_pages, v_pages, out)
+        check_no_gradient(name, q, k_pages, v_pages, out, ks, vs)
         if copies:
             return _prefix_attention(name, q.contiguous(), k_pages, v_pages, table, lengths.contiguous(), scale, out, scales,
                                      None if shared is None else shared.contiguous())
@@ -587,7 +587,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, sources: torch.Tens
     ks, vs = (None, None) if scales is None else scales
     layout = _lib.layout
     sizes, entry = _copy_call(name, layout(k_pages), layout(v_pages), layout(sources), layout(copies), layout(ks), layout(vs))
-    check_no_gradient(name, k_pages, v_pages)
+    check_no_gradient(name, k_pages, v_pages, ks, vs)
     sources, copies = sources.contiguous(), copies.contiguous()
     with _lib.on_device(k_pages):
         rc = entry(k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(ks), _lib.ptr(vs), sources.data_ptr(),

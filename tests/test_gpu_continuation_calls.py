@@ -32,3 +32,32 @@ def test_nothing_to_do_of_any_strides(cuda, eight):
             assert paged_attention(q, pages, pages, ints(0, 3), ints(0), **kw).shape == (0, 4, 8)
         plain = torch.zeros(2, 2, 16, 8, device=cuda)
         assert paged_attention(q, plain, plain, ints(0, 3), ints(0), shared=ints(0)).shape == (0, 4, 8)
+
+
+def test_recorded_scales_are_refused(cuda):
+    """As recorded pages are: their gradient would be lost without a word."""
+    from hydra_amd.attention import copy_pages, paged_attention, read_pages, store_pages
+
+    case = Case([[40, 50], [33, 60]], [32, 16], 4, 2, 32, 16, torch.bfloat16, torch.int8, seed=1)
+    q, kp, vp, table, lengths, shared = (t.to(cuda) for t in (case.q, case.kp, case.vp, case.table, case.lengths, case.shared))
+    rows, slots = torch.zeros(1, 2, 3, 32, device=cuda), torch.arange(3, device=cuda)[None]
+    pair = torch.tensor([0], dtype=torch.int32, device=cuda), torch.tensor([1], dtype=torch.int32, device=cuda)
+    for which in (0, 1):
+        scales = [s.to(cuda) for s in case.scales]
+        scales[which].requires_grad_()
+        calls = (lambda: paged_attention(q, kp, vp, table, lengths, scales=scales),
+                 lambda: paged_attention(q, kp, vp, table, lengths, scales=scales, shared=shared),
+                 lambda: store_pages(rows, rows, kp, vp, slots, scales=scales),
+                 lambda: read_pages(kp, vp, slots, scales=scales, dtype=torch.bfloat16),
+                 lambda: copy_pages(kp, vp, *pair, scales=scales))
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+            with torch.no_grad():
+                call()
+        scales[which].requires_grad_(False)
+        with torch.autograd.forward_ad.dual_level():
+            scales[which] = torch.autograd.forward_ad.make_dual(scales[which], torch.ones_like(scales[which]))
+            for call in calls:
+                with pytest.raises(RuntimeError, match="no forward-mode"):
+                    call()
