@@ -81,6 +81,8 @@ class HydraBlock(nn.Module):
     def new_cache(self, pool: PagePool, dtype: Optional[torch.dtype] = None,
                   page_dtype: Optional[torch.dtype] = None):
         """The attention's cache for the requests of `pool`."""
+        if page_dtype is None:  # an attention of the caller's may know of no such pages
+            return self.attention.new_cache(pool, dtype)
         return self.attention.new_cache(pool, dtype, page_dtype)
 
     @torch.no_grad()
@@ -95,6 +97,8 @@ class HydraBlock(nn.Module):
         (CCGQAAttention.decode, also `shared`).  The row of a request without a token
         (plan.seen 0) holds no result: it is x and the MLP's part of it, without
         attention."""
+        if shared is None:  # as in new_cache
+            return self._rest(x, self.attention.decode(self.norm1(x), cache, plan))
         return self._rest(x, self.attention.decode(self.norm1(x), cache, plan, shared))
 
 
