@@ -27,7 +27,8 @@ struct ForkArgs {
   int *sources, *copies, *taken;   // results, [N]; taken: the row that each one continues, -1: none
   uint8_t* granted;
   // scratch: continuations and the first of them, [N]; lengths, tables and stack before;
-  // the first row among those that give a page up, and what each puts back
+  // the first place in the table, j P + c, of those that give a page up, and how many
+  // pages each row puts back
   int *old_free, *kids, *first, *old_len, *back, *old_table, *owner;
   int N, P, F, pages, shift;
 };
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(kWide) void fork_count_kernel(ForkArgs a) {
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     const int step = (gridDim.x - 1) * kWide;
-    for (int64_t i = (blockIdx.x - 1) * kWide + tid; i < a.pages; i += step) a.owner[i] = a.N;
+    for (int64_t i = (blockIdx.x - 1) * kWide + tid; i < a.pages; i += step) a.owner[i] = a.N * a.P;
     return;
   }
   for (int i = tid; i < a.N; i += kWide) {
@@ -105,15 +106,16 @@ __global__ __launch_bounds__(kThreads) void fork_share_kernel(ForkArgs a) {
       if (c < full && kids > 1) atomicAdd(&a.extra[p], kids - 1);
       if (kids == 0) {
         atomicAdd(&a.extra[p], -1);
-        atomicMin(&a.owner[p], j);
+        atomicMin(&a.owner[p], j * a.P + c);
       }
     }
   }
 }
 
-// Whether row j, which has no continuation, is the one to put the page back.
-__device__ __forceinline__ bool gives_back(const ForkArgs& a, int j, int p) {
-  return is_page(a, p) && a.owner[p] == j && a.extra[p] < 0;
+// Whether column c of row j, which has no continuation, is the place to put the page back
+// from.
+__device__ __forceinline__ bool gives_back(const ForkArgs& a, int j, int c, int p) {
+  return is_page(a, p) && a.owner[p] == j * a.P + c && a.extra[p] < 0;
 }
 
 __global__ __launch_bounds__(kThreads) void fork_back_kernel(ForkArgs a) {
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void fork_back_kernel(ForkArgs a) {
   for (int j = blockIdx.x; j < a.N; j += gridDim.x) {
     const int held = a.kids[j] == 0 ? held_of(a, a.old_len[j]) : 0;
     int count = 0, all;
-    for (int c = threadIdx.x; c < held; c += kThreads) count += gives_back(a, j, a.old_table[static_cast<int64_t>(j) * a.P + c]);
+    for (int c = threadIdx.x; c < held; c += kThreads) count += gives_back(a, j, c, a.old_table[static_cast<int64_t>(j) * a.P + c]);
     block_incl_sum(count, part, all);
     if (threadIdx.x == 0) a.back[j] = all;
   }
@@ -144,7 +146,7 @@ __global__ __launch_bounds__(kThreads) void fork_push_kernel(ForkArgs a) {
     const int held = held_of(a, a.old_len[j]);
     for (int c0 = 0; c0 < held; c0 += kThreads) {
       const int c = c0 + threadIdx.x, p = c < held ? a.old_table[static_cast<int64_t>(j) * a.P + c] : -1;
-      const bool back = gives_back(a, j, p);
+      const bool back = gives_back(a, j, c, p);
       int count;
       const int64_t to = top + block_incl_sum(back, part, count) - 1;
       if (back) {
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(kWide) void fork_small_kernel(ForkArgs a) {
     const int j = e / a.P, c = e - j * a.P;
     if (c >= held_of(a, len[j])) continue;
     old[e] = a.table[j * a.table_rs + c];
-    if (is_page(a, old[e])) put(&a.owner[old[e]], a.N);
+    if (is_page(a, old[e])) put(&a.owner[old[e]], all);
   }
   __threadfence_block();
   __syncthreads();
@@ -266,7 +268,7 @@ __global__ __launch_bounds__(kWide) void fork_small_kernel(ForkArgs a) {
     if (c < full_of(a, len[j]) && kids[j] > 1) add(&a.extra[old[e]], kids[j] - 1);
     if (kids[j] == 0) {
       add(&a.extra[old[e]], -1);
-      __hip_atomic_fetch_min(&a.owner[old[e]], j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      __hip_atomic_fetch_min(&a.owner[old[e]], e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
   }
   __threadfence_block();
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(kWide) void fork_small_kernel(ForkArgs a) {
   for (int e0 = 0; e0 < all; e0 += kWide) {
     const int e = e0 + tid, j = e < all ? e / a.P : 0, c = e - j * a.P;
     const bool mine = e < all && kids[j] == 0 && c < held_of(a, len[j]) && is_page(a, old[e]);
-    const bool back = mine && seen(&a.owner[old[e]]) == j && seen(&a.extra[old[e]]) < 0;
+    const bool back = mine && seen(&a.owner[old[e]]) == e && seen(&a.extra[old[e]]) < 0;
     int count;
     const int to = free + wide_incl_sum(back, part, count) - 1;
     if (back) {

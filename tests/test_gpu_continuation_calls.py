@@ -61,3 +61,18 @@ def test_recorded_scales_are_refused(cuda):
             for call in calls:
                 with pytest.raises(RuntimeError, match="no forward-mode"):
                     call()
+
+
+@pytest.mark.parametrize("rows", [4, 300])
+def test_a_page_that_a_row_holds_twice(cuda, rows):
+    """Goes back once."""
+    from hydra_amd.attention import fork_pages
+
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    lengths, extra = [48] + [0] * (rows - 1), [0] * 9
+    table = [[3, 5, 3, -1]] + [[-1] * 4] * (rows - 1)
+    extra[3] = 1
+    t = [i32(lengths), i32(table), i32([8, 0, 0, 0, 0]), i32([1]), i32(extra)]
+    fork = fork_pages(i32([-1] + list(range(1, rows))), *t, 16)
+    assert t[3].item() == 3 and t[2].tolist()[:3] == [8, 3, 5]
+    assert not t[4].any() and not t[0].any() and (t[1] == -1).all() and fork.granted.all()
