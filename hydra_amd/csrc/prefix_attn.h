@@ -581,8 +581,9 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& item,
 
   // q times the scale's sign: the score's product with |scale| is then monotone
   const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
-  // a scale of 0 as the least there is: scores of 0, and -inf where a key is not seen
-  const float scale = fmaxf(fabsf(a.scale), 0x1p-126f);
+  // a scale of 0 as the least normal one: scores of 0, and -inf where a key is not seen (a
+  // maximum would let go of a scale that is NaN)
+  const float scale = fabsf(a.scale) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale);
   uint4 qf[NT][NC];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {

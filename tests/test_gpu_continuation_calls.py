@@ -76,3 +76,14 @@ def test_a_page_that_a_row_holds_twice(cuda, rows):
     fork = fork_pages(i32([-1] + list(range(1, rows))), *t, 16)
     assert t[3].item() == 3 and t[2].tolist()[:3] == [8, 3, 5]
     assert not t[4].any() and not t[0].any() and (t[1] == -1).all() and fork.granted.all()
+
+
+@pytest.mark.parametrize("eight", [None, *EIGHT])
+@pytest.mark.parametrize("W", [2, 40])
+def test_a_scale_that_is_no_number(cuda, eight, W):
+    """Shows in every result, also of requests that end with the prefix, whichever form
+    the rows go through."""
+    case = Case([[192 + i % 3 for i in range(W)]], [192], 4, 2, 64, 16, torch.bfloat16, eight, seed=1)
+    assert case.call(cuda, scale=float("nan")).isnan().all()
+    for scale in (1e-39, -1e-39):  # below fp32's normal numbers
+        case.check(cuda, scale=scale)
