@@ -381,8 +381,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     is answered from its own pages alone.
 
     fp32 scores, softmax and sums, one rounding (with scales or shared a weight
-    enters its product as two 16-bit terms, to 2^-16 of it, and an infinity among
-    the values seen may come out as NaN).  Lengths count within
+    enters its product as two 16-bit terms, to 2^-16 of it, of fp16 pages to 2^-22
+    of it and 2^-38 of the largest one, and an infinity among the values seen may
+    come out as NaN; fp32 queries have fp32 weights).  Lengths count within
     [0, P * page_size]; keys on a page outside the pool are not seen; a
     request that sees none (or whose scores are all -inf) gets zeros.  Inference
     only: no gradient."""

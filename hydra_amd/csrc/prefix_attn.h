@@ -30,7 +30,10 @@
 //    taken as two 16-bit terms, its rounding and what that leaves: 2^-16 of it in
 //    bf16 (2^-22 in fp16), so that the result is rounded once, in effect.  It
 //    costs a second matrix instruction where the softmax's arithmetic is the
-//    longer part.  In fp32 all operands are fp32.
+//    longer part.  fp16's least step is 2^-24, which many light weights beside a heavy
+//    one are all below: they enter times 2^15 (2^13 where the maximum lags behind), so
+//    that of each at most 2^-38 of the largest weight is lost.  In fp32 all operands
+//    are fp32.
 //
 // Split: A items are cut into pieces of whole rounds (128 keys), one to a workgroup
 // where they suffice; the rounds of all B items are laid end to end and dealt out to
@@ -106,6 +109,7 @@ template <typename C, typename KV> struct Types {
   static constexpr bool eight = sizeof(KV) == 1;
   static constexpr bool f32 = sizeof(C) == 4;
   using VT = std::conditional_t<f32, float, std::conditional_t<eight, bf16, C>>;  // V in LDS, and P
+  static constexpr bool f16_p = std::is_same<VT, f16>::value;
 };
 
 constexpr int pitch_of(int hdp, bool f32) { return f32 ? hdp + 4 : (hdp == 32 || hdp == 128 ? hdp + 16 : hdp + 8); }
@@ -253,6 +257,7 @@ __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& item,
   using Ty = Types<C, KV>;
   using VT = typename Ty::VT;
   constexpr bool F32 = Ty::f32, EIGHT = Ty::eight;
+  constexpr float LIFT = Ty::f16_p ? 15.f : 0.f;  // of the weights' exponents, which are at most 0
   constexpr int KT = tile_keys(HDP, F32), NB = KT / 16, KW = NW / RW, TT = 64 * RW;
   constexpr int E = 16 / sizeof(KV);                       // elements of a piece
   constexpr int PPR = HDP / E > 0 ? HDP / E : 1;           // pieces of a row
@@ -465,7 +470,7 @@ __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& item,
 #pragma unroll
           for (int r = 0; r < 4; ++r) st.o[t][i][r] *= alpha;
       }
-      const float ms = st.m[t] == -INFINITY ? 0.f : st.m[t];
+      const float ms = st.m[t] == -INFINITY ? 0.f : st.m[t] - LIFT;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -516,6 +521,7 @@ __device__ __forceinline__ void item_keys(const PrefixArgs& a, const Item& item,
   for (int t = 0; t < NT; ++t) {
     st.l[t] += __shfl_xor(st.l[t], 16);
     st.l[t] = halves_sum(st.l[t]);
+    if (st.m[t] != -INFINITY) st.m[t] -= LIFT;
   }
   if constexpr (RW == 1) {  // the upper half of the waves into the lower one, until one is left: all hold the same layout
     float* sm = reinterpret_cast<float*>(lds);
@@ -602,9 +608,13 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& item,
 #pragma unroll
     for (int i = 0; i < NO; ++i) st.o[t][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  float ms[NT];  // m times the scale, 0 before the first key
+  // The reference of the weights: m times the scale, 0 before the first key, less LIFT.  In
+  // fp16 they are lifted, and the reference lags less behind, so that light ones stay above its
+  // least step and the heaviest, 2^(LIFT + LAG), within its range.
+  constexpr float LIFT = std::is_same<C, f16>::value ? 13.f : 0.f, LAG = std::is_same<C, f16>::value ? 2.f : 8.f;
+  float ms[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) ms[t] = 0.f;
+  for (int t = 0; t < NT; ++t) ms[t] = -LIFT;
 
   // A tile lies in one page, or its blocks of 16 may lie in several: a descriptor for the
   // tile, or for each load (which none goes beyond).
@@ -720,10 +730,10 @@ __device__ __forceinline__ void item_rows(const PrefixArgs& a, const Item& item,
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[b][t][r]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = halves_max(top);
-      // the reference moves where it has fallen behind by more than 2^8 alone: weights up to
+      // the reference moves where it has fallen behind by more than 2^LAG alone: weights up to
       // that are as exact, and most tiles raise some row's maximum by a little
-      if (__any(top * scale > ms[t] + 8.f || st.m[t] == -INFINITY)) {
-        const float mn = fmaxf(st.m[t], top), mns = mn == -INFINITY ? 0.f : mn * scale;
+      if (__any(top * scale > ms[t] + (LIFT + LAG) || st.m[t] == -INFINITY)) {
+        const float mn = fmaxf(st.m[t], top), mns = mn == -INFINITY ? -LIFT : fmaf(mn, scale, -LIFT);
         const float alpha = st.m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[t] - mns);
         st.m[t] = mn;
         ms[t] = mns;

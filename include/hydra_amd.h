@@ -634,8 +634,9 @@ int hydra_paged_attn_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t hd, i
  * from the pages of the first such request's table row, read once for all of them,
  * and the others from their own.  groups 0: shared is not used, and pages are of 8
  * bits.  Scores, softmax and sums are fp32; a weight (times its value's scale) enters
- * the product with v as two 16-bit terms, to 2^-16 of it.  An infinity among values that
- * are seen may come out as NaN.  All else as in hydra_paged_attn. */
+ * the product with v as two 16-bit terms, to 2^-16 of it (in fp16 over its own pages to
+ * 2^-22 of it and 2^-38 of the row's largest).  An infinity among values that are seen may
+ * come out as NaN.  All else as in hydra_paged_attn. */
 int hydra_prefix_attn(const void* q, const void* k_pages, const void* v_pages,
                       const float* k_scales, const float* v_scales, void* out, const int* table,
                       int64_t table_rs, const int* lengths, const int* shared, int64_t groups,

@@ -177,13 +177,15 @@ def two_term_bound(weight, v, lengths, page_dtype, q_dtype):
     attention_bound where its products are of 16-bit operands: a weight p (times its
     value's scale) is taken as hi + lo, hi off by half a step of the type, lo by half
     a step of that: 2^-16 of p in bf16 (8-bit pages, bf16), 2^-22 in fp16 (fp16
-    pages), where what is left below fp16's least step, 2^-24, is lost by half: 2^-25
-    of a weight whose largest is 1, for each key."""
+    pages), where what is left below fp16's least step, 2^-24, is lost by half: under
+    a lift of 2^13 (or 2^15) that is 2^-25 2^-13 of a weight whose largest is 1, for
+    each key.  (The lifted exponents, up to 16, round by 2^-21: 6 u of a weight, which
+    are within the 16 u that attention_bound has beside a score's own.)"""
     if q_dtype == torch.float32:
         return torch.zeros_like(weight)
     if page_dtype == torch.float16:
         finite = torch.where(torch.isfinite(v.double()), v.double(), torch.zeros(()).double())
-        return 2.0 ** -22 * weight + 2.0 ** -25 * lengths.double().clamp(min=0).view(-1, 1, 1) * float(finite.abs().max())
+        return 2.0 ** -22 * weight + 2.0 ** -38 * lengths.double().clamp(min=0).view(-1, 1, 1) * float(finite.abs().max())
     return 2.0 ** -16 * weight
 
 
