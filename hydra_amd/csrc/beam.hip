@@ -186,6 +186,7 @@ struct BeamArgs {
   int* parents;
   int64_t stride;     // bytes of a row
   int B, W, V, n, chunks;
+  int span;           // elements of a chunk
   int first;          // row (text) of the launch's first workgroup
 };
 
@@ -285,11 +286,13 @@ __device__ __forceinline__ double key_double(uint64_t k) {
   return __longlong_as_double(static_cast<long long>(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
 
+template <typename T>
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   __shared__ Lists<Key2> lists;
   // x - top first: a row whose tokens are all masked by the type's lowest value is even
   __shared__ double shift[kMaxBeams];  // score - ln sum e^(x - top)
   __shared__ float tops[kMaxBeams];
+  __shared__ int cut;  // whether a list may end among equals
   const int tid = threadIdx.x, b = a.first + blockIdx.x;
   const int count = a.W * a.chunks, all = count * a.n;  // lists, and what they hold
   const uint2* pairs = a.pairs + static_cast<int64_t>(b) * all;
@@ -304,6 +307,10 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
   uint2 early[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) early[u] = u * kThreads + tid < all ? pair_at(u * kThreads + tid) : make_uint2(0, 0);
+  if (tid == 0) cut = 0;
+  // where a list ends, for the threads' first ones
+  auto last_of = [&](int l) { return pairs[static_cast<int64_t>(l) * a.n + a.n - 1]; };
+  const uint32_t early_last = tid < count ? last_of(tid).x : 0;
   // as many lanes to a row as it has chunks
   int lanes = 1;
   while (lanes < 64 && lanes < a.chunks) lanes *= 2;
@@ -327,6 +334,9 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     }
   }
   __syncthreads();
+  auto key_of_score = [&](int w, uint32_t value) {  // of a beam whose shift is finite
+    return double_key(static_cast<double>(key_float(value)) - static_cast<double>(tops[w]) + shift[w]);
+  };
   auto key_at = [&](int i, uint2 p) {
     const int rank = i / count, x = i - rank * count, w = x / a.chunks;
     const double s = shift[w];
@@ -334,8 +344,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
       return x == w * a.chunks && rank < a.V ? Key2{double_key(s), 0xffffffffu - static_cast<uint32_t>(w * a.V + rank)}
                                              : Key2{0, 0};
     if (p.x == 0) return Key2{0, 0};
-    return Key2{double_key(static_cast<double>(key_float(p.x)) - static_cast<double>(tops[w]) + s),
-                0xffffffffu - static_cast<uint32_t>(w * a.V + static_cast<int>(0xffffffffu - p.y))};
+    return Key2{key_of_score(w, p.x), 0xffffffffu - static_cast<uint32_t>(w * a.V + static_cast<int>(0xffffffffu - p.y))};
   };
   auto each = [&](auto&& f) {
 #pragma unroll
@@ -350,27 +359,65 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
     a.beams[at] = w;
     a.tokens[at] = flat - w * a.V;
     a.parents[at] = b * a.W + w;
+    if (rank == a.n - 1) lists.nth = k;
   };
+  // A list has its chunk's best logits.  Where fp64 does not tell the scores of different
+  // logits apart (a beam's score of -1e30, logits of 1e-30) they are equal, and the lowest
+  // tokens come first, which a list may have left out.
+  auto alike = [&](int l, uint32_t x) {  // x: the key of its last logit
+    const int w = l / a.chunks;
+    const uint64_t k = key_of_score(w, x);
+    return fabs(shift[w]) < INFINITY && x > score_key_asc(-INFINITY) &&
+           (key_of_score(w, x - 1) == k || key_of_score(w, x + 1) == k);
+  };
+  if (tid < count && alike(tid, early_last)) cut = 1;
+  for (int l = kThreads + tid; l < count; l += kThreads)
+    if (alike(l, last_of(l).x)) cut = 1;
+  int c = all;
   if (all <= kFew) {
     if (tid < all) lists.list[tid] = key_at(tid, early[0]);
     __syncthreads();
-    ranked(a.n, all, lists, put);
-    return;
+  } else {
+    uint32_t mine = 0;
+    each([&](const Key2& k) { mine = max(mine, rough(k)); });
+    const uint32_t bound = bound_of(mine, a.n, lists);
+    if (tid == 0) lists.count = 0;
+    __syncthreads();
+    each([&](const Key2& k) {
+      if (k.a == 0 || rough(k) < bound) return;
+      const int at = atomicAdd(&lists.count, 1);
+      if (at < kCap) lists.list[at] = k;
+    });
+    __syncthreads();
+    c = lists.count;
+    if (c > kCap) c = collected(a.n, lists, each);
   }
-  uint32_t mine = 0;
-  each([&](const Key2& k) { mine = max(mine, rough(k)); });
-  const uint32_t bound = bound_of(mine, a.n, lists);
-  if (tid == 0) lists.count = 0;
-  __syncthreads();
-  each([&](const Key2& k) {
-    if (k.a == 0 || rough(k) < bound) return;
-    const int at = atomicAdd(&lists.count, 1);
-    if (at < kCap) lists.list[at] = k;
-  });
-  __syncthreads();
-  int c = lists.count;
-  if (c > kCap) c = collected(a.n, lists, each);
   ranked(a.n, c, lists, put);
+  if (cut == 0) return;
+  // Chunks whose list's last score is the n-th, and that of a logit beside it, are read again.
+  __syncthreads();
+  const uint64_t nth = lists.nth.a;
+  auto is_cut = [&](int l, uint32_t x) { return alike(l, x) && key_of_score(l / a.chunks, x) == nth; };
+  int some = 0;
+  for (int l = tid; l < count; l += kThreads) some |= is_cut(l, last_of(l).x);
+  if (!__syncthreads_or(some)) return;
+  auto with_chunks = [&](auto&& f) {
+    each(f);
+    for (int l = 0; l < count; ++l) {
+      const uint2 last = last_of(l);
+      if (!is_cut(l, last.x)) continue;
+      const int w = l / a.chunks;
+      const Key1 listed{(static_cast<uint64_t>(last.x) << 32) | last.y};  // as far as the list goes
+      const T* x = reinterpret_cast<const T*>(a.logits + (static_cast<int64_t>(b) * a.W + w) * a.stride);
+      const int c0 = (l - w * a.chunks) * a.span - static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+      for (int i = max(c0, 0) + tid; i < min(c0 + a.span, a.V); i += kThreads) {
+        const Key1 k = key_of(to_f32(x[i]), i);
+        if (better(listed, k))
+          f(Key2{key_of_score(w, static_cast<uint32_t>(k.a >> 32)), 0xffffffffu - static_cast<uint32_t>(w * a.V + i)});
+      }
+    }
+  };
+  ranked(a.n, collected(a.n, lists, with_chunks), lists, put);
 }
 
 // Elements of a thread.  Longer chunks leave less to join: in a graph, 16 against 32, us,
@@ -411,7 +458,7 @@ int launch_beam(BeamArgs a, int e, hipStream_t st) {
   constexpr int64_t most = int64_t(1) << 22;  // HIP counts a launch's threads in 32 bits
   for (int64_t b = 0; b < a.B; b += most) {
     a.first = static_cast<int>(b);
-    beam_join_kernel<<<static_cast<unsigned>(a.B - b < most ? a.B - b : most), kThreads, 0, st>>>(a);
+    beam_join_kernel<T><<<static_cast<unsigned>(a.B - b < most ? a.B - b : most), kThreads, 0, st>>>(a);
   }
   return check_launch("beam_select");
 }
@@ -457,6 +504,7 @@ extern "C" int hydra_beam_select(const void* logits, int64_t logits_rs, const fl
   a.V = static_cast<int>(V);
   a.n = static_cast<int>(n);
   a.chunks = static_cast<int>(chunks);
+  a.span = elements_of(n) * kThreads;
   auto st = static_cast<hipStream_t>(stream);
   return HYDRA_DISPATCH_DTYPE(dtype, T, [&]() -> int { return launch_beam<T>(a, elements_of(n), st); });
 }
