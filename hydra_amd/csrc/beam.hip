@@ -6,8 +6,8 @@
 // in descending order, the lowest w V + v first among equals.
 //
 // Bound by one pass over the logits where texts are many: 32 texts of 8 beams by 32000,
-// bf16 (16 MB), n = 16: 10.2 us, and 8.3 to join; for one text of 4 beams by 50257, n = 4,
-// by latency: 5.6 and 5.5 us.  Each workgroup reads a chunk of a row into
+// bf16 (16 MB), n = 16: 10.4 us, and 8.3 to join; for one text of 4 beams by 50257, n = 4,
+// by latency: 5.7 and 5.8 us.  Each workgroup reads a chunk of a row into
 // registers, takes its maximum and its sum of exponentials (fp32) and leaves the
 // chunk's n best (value, index) pairs; a second kernel joins the chunks' sums,
 // and orders the chunks' pairs by their scores in fp64 (two beams' continuations may be
@@ -21,7 +21,7 @@
 // them), so the order in which they are collected does not matter.
 //
 // Chunks that the join reads again, since fp64 tells none of their logits apart, cost it far
-// more: 617 us with all beams of the 32 texts at a score of -1e30, 113 with all logits 0.
+// more: 614 us with all beams of the 32 texts at a score of -1e30, 114 with all logits 0.
 #include "common.h"
 #include "mod_keys.h"
 

@@ -13,7 +13,8 @@
 //
 //   A  (group, key head, block of rows): up to 32 rows a workgroup where the
 //      group has no more (its waves take the keys in turn), else 128 (each wave
-//      32 rows of its own, all waves the same keys);
+//      32 rows of its own, all waves the same keys); in the form of 256 channels,
+//      and in fp32 in that of 128, up to 16, else 64 (16 a wave);
 //   B  (request, key head, block of 16 heads): the waves take the keys in turn.
 //
 // A wave walks its keys 32 at a time, on the matrix cores throughout:
@@ -44,14 +45,19 @@
 // What bounds it, by the kernels' own times:
 //
 //  * B items, many long ones: the reading of the pages.  64 requests of 16384 keys, 8/2
-//    heads of 64 in e4m3 (285 MB) take 53.6 us, 5.3 TB/s, and 4.9 us to join; 256 of
-//    4096, 32/8 heads of 128 in int8 (2.2 GB), 386 us, 5.7 TB/s;
+//    heads of 64 in e4m3 (285 MB) take 53.8 us, 5.3 TB/s, and 4.9 us to join; 256 of
+//    4096, 32/8 heads of 128 in int8 (2.2 GB), 386 us, 5.7 TB/s.  For fp32 queries it is
+//    the fp32 products, of 16 rows of which these heads fill 4: 109 and 786 us;
 //  * A items of many rows: the matrix cores and the softmax, in turn.  256 requests that
 //    share 32768 keys, 32/8 heads of 128 (137 GFLOP), with 600 keys of their own each:
-//    235 us (over e4m3 335, int8 375: their general form widens every tile of keys in
-//    each wave; once for all of them, through LDS, it was 336 and 355).  The matrix
-//    instructions alone, with the second terms of P, are 100 us; without the second terms,
-//    and without the loads, it would be 40 us less each, without the softmax 20;
+//    227 to 251 us, as the clock goes (over e4m3 334, int8 372: their general form widens
+//    every tile of keys in each wave; once for all of them, through LDS, it was 336 and
+//    355).  The products, 206 GFLOP with the second terms of P, and their operands' reads
+//    from LDS take 160 us with all else left out, the rate of a large library product;
+//    without the second terms the whole takes 36 us less, without the softmax 36, without
+//    the loads 16.  With 256 channels 717 us (over e4m3 1056), one workgroup to a CU;
+//  * the same in fp32, 4096 shared keys: the fp32 products, 330 us of 112 at 128 channels,
+//    where one workgroup a CU fits, 895 of 223 at 256, where registers are spilt;
 //  * few requests: the chain of launch, plan, table, keys and join.  8 groups of 4
 //    requests by 1500 keys: 8.4 us and 4.3 to join; one request of 700: 8.6 us.
 #pragma once
@@ -884,6 +890,11 @@ __global__ __launch_bounds__(64 * NW) void prefix_whole_kernel(PrefixArgs a) {
 // Waves of a SIMD that registers are to suffice for.  256 channels without groups: 70.5 us
 // with 1, 81 with 2 (60 dwords spilt; 64 requests of 8192 keys, 4/1 heads in e4m3, pages out
 // of the caches).  64 channels come to 3 by themselves: 68.8 us (64 x 16384 keys), with 4 the same.
+// With groups 2 is not reached where two workgroups do not fit in a CU's LDS: 16-bit queries
+// with 256 channels and fp32 ones with 128 take 81980 bytes each, the plan's arrays among them.
+// What is spilt: fp32 queries with 256 channels and groups 121 and 161 registers over fp32, 9
+// and 16 over 8 bits; in the element-by-element forms of 256 channels with groups 262 to 364 in
+// fp32 and 6 to 57 in 16 bits, 72 and 74 in 16 bits over 8 without groups; at most 5 elsewhere.
 constexpr int split_waves(int hdp, int rw) { return rw == 0 && hdp == 256 ? 1 : 2; }
 
 // Split form; RW 0: without groups.
